@@ -11,6 +11,13 @@
  * KV pool layout (one layer): [num_blocks][num_kv_heads][2: K,V][2: d/64][16 tokens][64] bf16, so
  * K and V of one (block, head) are 8 KiB contiguous.  The layer's "k_cache" pointer is the start
  * of that region and "v_cache" must be k_cache + 4096 bytes; slot = block * 16 + token.
+ *
+ * 8-bit pool layout (one layer, the *_kv8 entry points): [num_blocks][num_kv_heads][4128 bytes]: K's
+ * 16 rows of 128 e4m3 codes, V's 16 rows, K's 16 exponent bytes, V's 16.  Row t's 16-byte chunk i sits
+ * at chunk i ^ (t % 8).  A row with exponent byte b stands for its codes times 2^(b - 127); b - 127 is the
+ * smallest integer in [-100, 120] that brings the row's largest magnitude to at most 448, and b = 255
+ * marks a row that held a NaN or an infinity: it stands for NaN.  `pool` is the layer's first byte,
+ * 16-byte aligned.
  */
 #ifndef MSATTN_H_
 #define MSATTN_H_
@@ -167,6 +174,90 @@ MS_API int ms_paged_attention(const void* q, int64_t q_row_stride, void* out, in
                        const void* v_cache, int32_t num_blocks, const int32_t* plan_dev,
                        const MsPlanInfo* plan, void* workspace, int64_t workspace_bytes,
                        float scale, void* stream);
+
+/* ---- Rows of a pool by slot -------------------------------------------------------------------
+ * No counterpart in the reference.  k_out, v_out [num_tokens, KVH, 128] bf16 (row strides in
+ * elements, multiples of 8, 16-byte aligned) receive rows slots[t] of the pool: draft paths that are
+ * moved after a verify step, sequences handed to another cache.  A slot outside the pool reads as
+ * zeros and sets MS_DEV_BAD_SLOT.  From an 8-bit pool the values are exact (codes times a power of
+ * two are bf16 values), and writing them back stores the same values again. */
+MS_API int ms_kv_gather(const int64_t* slots, int32_t num_tokens, int32_t num_kv_heads,
+                        const void* k_cache, const void* v_cache, int32_t num_blocks, void* k_out,
+                        int64_t k_row_stride, void* v_out, int64_t v_row_stride, void* stream);
+MS_API int ms_kv_gather_kv8(const int64_t* slots, int32_t num_tokens, int32_t num_kv_heads,
+                            const void* pool, int32_t num_blocks, void* k_out,
+                            int64_t k_row_stride, void* v_out, int64_t v_row_stride, void* stream);
+
+/* ---- Writing an 8-bit pool ----------------------------------------------------------------------
+ * ms_kv_scatter and kernel A with rows quantised as they are written.  The arguments are those of
+ * ms_kv_scatter and ms_qk_norm_rope_scatter with `pool` in place of the two cache pointers; the
+ * quantised values are exactly the bf16 rows those would store. */
+MS_API int ms_kv_scatter_kv8(const void* k, int64_t k_row_stride, const void* v,
+                             int64_t v_row_stride, int32_t num_tokens, int32_t num_kv_heads,
+                             const int64_t* slot_mapping, void* pool, int32_t num_blocks,
+                             void* stream);
+MS_API int ms_qk_norm_rope_scatter_kv8(const void* qkv, int64_t qkv_row_stride, int32_t num_tokens,
+                                       int32_t num_heads, int32_t num_kv_heads,
+                                       const void* q_weight, const void* k_weight, float eps,
+                                       const float* cos, const float* sin, int64_t cs_row_stride,
+                                       const int64_t* positions, int64_t max_positions,
+                                       const int64_t* slot_mapping, void* q_out,
+                                       int64_t q_out_row_stride, void* pool, int32_t num_blocks,
+                                       void* stream);
+
+/* ---- Attention through an 8-bit pool --------------------------------------------------------------
+ * Same work and plan as ms_paged_attention.  Rows of up to 64 new tokens read the 8-bit pages in
+ * place; chunks of more than 64 tokens (and the shared prefix of cascade groups) run on the
+ * tensor-core kernel over bf16 copies of their pages, expanded into the workspace first.  What that
+ * needs beside the plan is described by MsKv8Info: ms_kv8_plan_build appends it (host only) to the
+ * packed plan, at int offset plan->total_ints of the same buffer (so one upload brings both; the
+ * buffer holds ms_kv8_plan_capacity ints beyond the plan), and the attention call gets
+ * the uploaded whole.  workspace_bytes >= ms_kv8_workspace_bytes. */
+typedef struct MsKv8Info {
+  int32_t n_pages;    /* pages (per KV head) expanded for the tensor-core kernel */
+  int32_t off_seqs;   /* int offsets in the packed buffer: sequence records whose tables index */
+  int32_t off_map;    /* the expanded pages; the expanded pages' block ids; 0, 1, 2, ... */
+  int32_t off_tables;
+  int32_t total_ints; /* length of the packed buffer with this part */
+  int32_t reserved[3];
+} MsKv8Info;
+
+MS_API int64_t ms_kv8_plan_capacity(const MsPlanInfo* plan, int64_t total_table_entries);
+MS_API int ms_kv8_plan_build(int32_t* packed, int64_t capacity, const MsPlanInfo* plan,
+                             MsKv8Info* info);
+MS_API int64_t ms_kv8_workspace_bytes(const MsPlanInfo* plan, const MsKv8Info* info,
+                                      int32_t num_kv_heads);
+MS_API int ms_paged_attention_kv8(const void* q, int64_t q_row_stride, void* out,
+                                  int64_t out_row_stride, int32_t num_heads, int32_t num_kv_heads,
+                                  const void* pool, int32_t num_blocks, const int32_t* plan_dev,
+                                  const MsPlanInfo* plan, const MsKv8Info* info, void* workspace,
+                                  int64_t workspace_bytes, float scale, void* stream);
+
+/* ---- Attention over trees of drafted tokens ---------------------------------------------------------
+ * No counterpart in the reference (its drafts are chains).  Sequence i's new tokens are drafts: draft
+ * k lies in the cache at position num_cached[i] + k (its slot), and sees the cached tokens, its
+ * ancestors and itself.  parents (concatenated in sequence order, num_new[i] each) holds, for draft
+ * k, an earlier draft of the sequence (0 <= parent < k), -1 for a child of the last cached token, or -2
+ * for an unused position: that draft sees nothing, no draft sees it, and its output is zero whatever
+ * its rows hold (it may not be a parent).  RoPE positions are the caller's: num_cached plus the draft's
+ * depth.
+ *
+ * The plan is a packed int32 buffer described by MsPlanInfo, as ms_plan_build's (masks included);
+ * ms_tree_attention launches it over a bf16 pool, or over an 8-bit pool when v_cache is NULL (k_cache is then
+ * the 8-bit layer).  Sequences of at most MS_MAX_TREE_TOKENS drafts. */
+#define MS_MAX_TREE_TOKENS 1024
+MS_API int64_t ms_tree_plan_capacity(int32_t num_seqs, const int32_t* num_new,
+                                     int64_t total_table_entries);
+MS_API int ms_tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const int32_t* num_new,
+                              const int32_t* num_cached, const int64_t* table_offsets,
+                              const int32_t* tables, const int32_t* parents, int32_t num_tokens,
+                              int32_t block_size, int32_t num_sms, int32_t pages_per_split,
+                              int32_t* out, int64_t out_capacity, MsPlanInfo* info);
+MS_API int ms_tree_attention(const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride,
+                             int32_t num_heads, int32_t num_kv_heads, const void* k_cache,
+                             const void* v_cache, int32_t num_blocks, const int32_t* plan_dev,
+                             const MsPlanInfo* plan, void* workspace, int64_t workspace_bytes,
+                             float scale, void* stream);
 
 /* ---- Attention for callers that cannot allocate device memory -------------------------------
  * No counterpart in the reference (MiniServe allocates everything through PyTorch).

@@ -3,9 +3,10 @@
 Public surface (mirrors src/miniserve/attention/backends.py and model/qwen3.py):
 
 * ``attention``: ``SeqChunk``, ``build_attention_metadata``, ``paged_attention``, ``attend``,
-  ``kv_scatter``, ``SHORT_QUERY``, ``MAX_GATHER_TOKENS``
+  ``kv_scatter``, ``kv_gather``, ``tree_positions``, ``SHORT_QUERY``, ``MAX_GATHER_TOKENS``
 * ``qwen3_attention``: ``Qwen3Attention`` (drop-in module), ``qk_norm_rope_scatter`` (kernel A)
-* ``kv_pool``: ``allocate_kv_cache`` in the pool layout the kernels read
+* ``kv_pool``: ``allocate_kv_cache`` in the pool layout the kernels read (bf16, or 8-bit:
+  ``dtype=torch.float8_e4m3fn``)
 * ``sharding``: sequence sharding over ranks
 
 The compute runs in ``_lib/libmsattn.so`` (C ABI in ``include/msattn.h``); build it with
@@ -19,8 +20,10 @@ from .attention import (
     SeqChunk,
     attend,
     build_attention_metadata,
+    kv_gather,
     kv_scatter,
     paged_attention,
+    tree_positions,
 )
 from .kv_pool import allocate_kv_cache
 
@@ -32,6 +35,8 @@ __all__ = [
     "allocate_kv_cache",
     "attend",
     "build_attention_metadata",
+    "kv_gather",
     "kv_scatter",
     "paged_attention",
+    "tree_positions",
 ]

@@ -36,6 +36,17 @@ EXPORTED = (
     "ms_qk_norm_rope_scatter",
     "ms_qkv_proj_norm_rope_scatter",
     "ms_kv_scatter",
+    "ms_kv_scatter_kv8",
+    "ms_qk_norm_rope_scatter_kv8",
+    "ms_kv_gather",
+    "ms_kv_gather_kv8",
+    "ms_kv8_plan_capacity",
+    "ms_kv8_plan_build",
+    "ms_kv8_workspace_bytes",
+    "ms_paged_attention_kv8",
+    "ms_tree_plan_capacity",
+    "ms_tree_plan_build",
+    "ms_tree_attention",
     "ms_paged_attention",
     "ms_paged_attention_noalloc",
 )
@@ -67,6 +78,17 @@ class MsPlanInfo(C.Structure):
     ]
 
 
+class MsKv8Info(C.Structure):
+    _fields_ = [
+        ("n_pages", C.c_int32),
+        ("off_seqs", C.c_int32),
+        ("off_map", C.c_int32),
+        ("off_tables", C.c_int32),
+        ("total_ints", C.c_int32),
+        ("reserved", C.c_int32 * 3),
+    ]
+
+
 _P = C.c_void_p
 _I32 = C.c_int32
 _I64 = C.c_int64
@@ -92,6 +114,34 @@ _SIGNATURES = {
          _P, _P, _I64, _P, _P, _I32, _P],
     ),
     "ms_kv_scatter": (C.c_int, [_P, _I64, _P, _I64, _I32, _I32, _P, _P, _P, _I32, _P]),
+    "ms_kv_scatter_kv8": (C.c_int, [_P, _I64, _P, _I64, _I32, _I32, _P, _P, _I32, _P]),
+    "ms_qk_norm_rope_scatter_kv8": (
+        C.c_int,
+        [_P, _I64, _I32, _I32, _I32, _P, _P, C.c_float, _P, _P, _I64, _P, _I64, _P, _P, _I64,
+         _P, _I32, _P],
+    ),
+    "ms_kv_gather": (C.c_int, [_P, _I32, _I32, _P, _P, _I32, _P, _I64, _P, _I64, _P]),
+    "ms_kv_gather_kv8": (C.c_int, [_P, _I32, _I32, _P, _I32, _P, _I64, _P, _I64, _P]),
+    "ms_kv8_plan_capacity": (_I64, [C.POINTER(MsPlanInfo), _I64]),
+    "ms_kv8_plan_build": (
+        C.c_int, [_P, _I64, C.POINTER(MsPlanInfo), C.POINTER(MsKv8Info)]),
+    "ms_kv8_workspace_bytes": (
+        _I64, [C.POINTER(MsPlanInfo), C.POINTER(MsKv8Info), _I32]),
+    "ms_paged_attention_kv8": (
+        C.c_int,
+        [_P, _I64, _P, _I64, _I32, _I32, _P, _I32, _P, C.POINTER(MsPlanInfo),
+         C.POINTER(MsKv8Info), _P, _I64, C.c_float, _P],
+    ),
+    "ms_tree_plan_capacity": (_I64, [_I32, _P, _I64]),
+    "ms_tree_plan_build": (
+        C.c_int,
+        [_I32, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _P, _I64, C.POINTER(MsPlanInfo)],
+    ),
+    "ms_tree_attention": (
+        C.c_int,
+        [_P, _I64, _P, _I64, _I32, _I32, _P, _P, _I32, _P, C.POINTER(MsPlanInfo), _P, _I64,
+         C.c_float, _P],
+    ),
     "ms_paged_attention": (
         C.c_int,
         [_P, _I64, _P, _I64, _I32, _I32, _P, _P, _I32, _P, C.POINTER(MsPlanInfo), _P, _I64,

@@ -14,6 +14,11 @@ uploaded with a single pinned, non-blocking copy; the KV pool uses the layout of
 read the pool in place (no gather copy, no padding, no masks in memory).  Everything runs on the
 caller's current CUDA stream and never synchronises; errors surface as ``ValueError`` /
 ``RuntimeError`` like the reference's.
+
+Beyond the reference: the pool may be the 8-bit one (``allocate_kv_cache(...,
+dtype=torch.float8_e4m3fn)``), which ``kv_scatter``, ``attend`` and ``paged_attention`` take like the
+bf16 one; ``kv_gather`` reads rows of either back; and a chunk's new tokens may be a tree of drafted
+tokens (``SeqChunk.parents``).
 """
 
 from __future__ import annotations
@@ -27,7 +32,7 @@ import torch
 from torch import Tensor
 
 from . import _capi
-from .kv_pool import BLOCK_SIZE, HEAD_DIM, check_layer_views
+from .kv_pool import BLOCK_SIZE, HEAD_DIM, check_layer_views, is_kv8
 
 SHORT_QUERY = 8  # rows with at most this many new tokens take the decode kernel
 MAX_GATHER_TOKENS = 16384  # kept for the runner's profiler; nothing is gathered here
@@ -41,10 +46,27 @@ class SeqChunk:
     num_new: int  # new tokens this step (its queries)
     num_cached: int  # tokens already in the KV cache before this step
     block_table: list[int]
+    # A tree of drafts instead of a causal chunk: draft k's parent among the new tokens (an earlier
+    # one), -1 for a child of the last cached token, UNUSED_DRAFT for a position without a draft.
+    # Draft k's K/V lie at position num_cached + k; it sees the cached tokens, its ancestors and
+    # itself.  An unused position sees nothing, is seen by none, and its output row is zero.
+    parents: list[int] | None = None
 
     @property
     def context_len(self) -> int:
         return self.num_cached + self.num_new
+
+
+UNUSED_DRAFT = -2
+
+
+def tree_positions(num_cached: int, parents: list[int]) -> list[int]:
+    """RoPE position of each draft of a tree: ``num_cached`` plus its depth (unused positions get
+    ``num_cached``)."""
+    depth: list[int] = []
+    for p in parents:
+        depth.append(depth[p] + 1 if p >= 0 else 0)
+    return [num_cached + d for d in depth]
 
 
 @dataclass
@@ -58,6 +80,9 @@ class AttentionMetadata:
     _workspace: dict[tuple[int, int], Tensor] = field(default_factory=dict, repr=False)
     _num_sms: int = field(default=148, repr=False)
     _pages_per_split: int = field(default=0, repr=False)
+    kv8: _capi.MsKv8Info = field(default_factory=_capi.MsKv8Info, repr=False)  # 8-bit pool part
+    # The sequences whose new tokens are trees of drafts, planned apart (None: there are none).
+    tree: AttentionMetadata | None = field(default=None, repr=False)
 
     def update(self, chunks: list[SeqChunk], slot_mapping: Tensor | None = None) -> bool:
         """Plan a new step into this metadata's device buffers, for CUDA-graph replay.
@@ -74,21 +99,35 @@ class AttentionMetadata:
         """
         if slot_mapping is not None and tuple(slot_mapping.shape) != tuple(self.slot_mapping.shape):
             return False
-        packed, info = plan_batch(chunks, self.num_tokens, BLOCK_SIZE, self._num_sms,
-                                  self._pages_per_split)
-        if not same_launch_shape(info, self.info):
+        plain, trees = _split_trees(chunks)
+        packed, info, kv8 = _plan_with_kv8(plain, self.num_tokens, self._num_sms,
+                                           self._pages_per_split)
+        if not same_launch_shape(info, self.info) or bytes(kv8) != bytes(self.kv8):
             return False
+        if bool(trees) != (self.tree is not None):
+            return False
+        if self.tree is not None:
+            tpacked, tinfo = plan_tree_batch(trees, self.num_tokens, BLOCK_SIZE, self._num_sms,
+                                             self._pages_per_split)
+            if not same_launch_shape(tinfo, self.tree.info) or tpacked.size != self.tree.plan.numel():
+                return False
+            self.tree.plan.copy_(torch.from_numpy(tpacked).pin_memory(), non_blocking=True)
         self.plan.copy_(torch.from_numpy(packed).pin_memory(), non_blocking=True)
         if slot_mapping is not None and slot_mapping.data_ptr() != self.slot_mapping.data_ptr():
             self.slot_mapping.copy_(slot_mapping, non_blocking=True)
         return True
 
-    def workspace(self, num_kv_heads: int, device: torch.device) -> Tensor | None:
-        """Split-KV scratch for this step (allocated once, reused by every layer)."""
+    def workspace(self, num_kv_heads: int, device: torch.device, kv8: bool = False) -> Tensor | None:
+        """Scratch for this step (allocated once, reused by every layer): split-KV partials and,
+        for an 8-bit pool, the expanded pages of tensor-core items."""
         need = int(self.info.workspace_bytes_per_kv_head) * num_kv_heads
+        if kv8:
+            need = int(_capi.load().ms_kv8_workspace_bytes(C.byref(self.info), C.byref(self.kv8),
+                                                           num_kv_heads))
         if need == 0:
             return None
-        key = (str(device), num_kv_heads)  # a tensor's device always carries its index
+        # A tensor's device always carries its index.
+        key = (str(device), -num_kv_heads if kv8 else num_kv_heads)
         ws = self._workspace.get(key)
         if ws is None:
             ws = torch.empty(need, dtype=torch.uint8, device=device)
@@ -137,6 +176,64 @@ def plan_batch(
     )
     _capi.check(rc, "build_attention_metadata")
     return out[: info.total_ints], info
+
+
+def plan_tree_batch(
+    chunks: list[SeqChunk],
+    num_tokens: int,
+    block_size: int = BLOCK_SIZE,
+    num_sms: int = 148,
+    pages_per_split: int = 0,
+) -> tuple[np.ndarray, _capi.MsPlanInfo]:
+    """Run the native planner of draft trees on the host (every chunk has ``parents``); returns
+    ``(packed int32 plan, info)``."""
+    lib = _capi.load()
+    n = len(chunks)
+    for i, c in enumerate(chunks):
+        if c.parents is None or len(c.parents) != c.num_new:
+            raise ValueError(f"tree sequence {i}: parents must name one parent per new token "
+                             f"({c.num_new})")
+    flat = np.fromiter((c.flat_start for c in chunks), dtype=np.int32, count=n)
+    new = np.fromiter((c.num_new for c in chunks), dtype=np.int32, count=n)
+    cached = np.fromiter((c.num_cached for c in chunks), dtype=np.int32, count=n)
+    lens = np.fromiter((len(c.block_table) for c in chunks), dtype=np.int64, count=n)
+    offsets = np.zeros(n + 1, dtype=np.int64)
+    np.cumsum(lens, out=offsets[1:])
+    total = int(offsets[-1])
+    tables = np.fromiter(chain.from_iterable(c.block_table for c in chunks), dtype=np.int32,
+                         count=total)
+    parents = np.fromiter(chain.from_iterable(c.parents or [] for c in chunks), dtype=np.int32)
+    cap = int(lib.ms_tree_plan_capacity(n, new.ctypes.data, total))
+    out = np.empty(cap, dtype=np.int32)
+    info = _capi.MsPlanInfo()
+    rc = lib.ms_tree_plan_build(
+        n, flat.ctypes.data, new.ctypes.data, cached.ctypes.data, offsets.ctypes.data,
+        tables.ctypes.data if total else None, parents.ctypes.data, num_tokens, block_size,
+        num_sms, pages_per_split, out.ctypes.data, cap, C.byref(info),
+    )
+    _capi.check(rc, "build_attention_metadata")
+    return out[: info.total_ints], info
+
+
+def _split_trees(chunks: list[SeqChunk]) -> tuple[list[SeqChunk], list[SeqChunk]]:
+    trees = [c for c in chunks if c.parents is not None]
+    return ([c for c in chunks if c.parents is None], trees) if trees else (chunks, trees)
+
+
+def _plan_with_kv8(chunks: list[SeqChunk], num_tokens: int, num_sms: int, pages_per_split: int
+                   ) -> tuple[np.ndarray, _capi.MsPlanInfo, _capi.MsKv8Info]:
+    """The plan with the part an 8-bit pool's tensor-core items need behind it, so that one plan
+    (and one upload) serves either kind of pool."""
+    lib = _capi.load()
+    packed, info = plan_batch(chunks, num_tokens, BLOCK_SIZE, num_sms, pages_per_split)
+    kv8 = _capi.MsKv8Info()
+    if not info.n_tc_items:
+        return packed, info, kv8
+    more = int(lib.ms_kv8_plan_capacity(C.byref(info), sum(len(c.block_table) for c in chunks)))
+    packed = np.concatenate([packed, np.empty(more, dtype=np.int32)])
+    _capi.check(lib.ms_kv8_plan_build(packed.ctypes.data, packed.size, C.byref(info),
+                                      C.byref(kv8)), "build_attention_metadata")
+    return packed[: kv8.total_ints], info, kv8
 
 
 def prepare_arrays(num_new: np.ndarray, num_cached: np.ndarray, table_offsets: np.ndarray,
@@ -211,11 +308,18 @@ def build_attention_metadata(
     if block_size != BLOCK_SIZE:
         raise ValueError(f"block_size must be {BLOCK_SIZE}")
     num_tokens = int(slot_mapping.shape[0])
-    packed, info = plan_batch(chunks, num_tokens, block_size, num_sms, pages_per_split)
-    plan = _upload_plan(packed, device)
+    plain, trees = _split_trees(chunks)
+    packed, info, kv8 = _plan_with_kv8(plain, num_tokens, num_sms, pages_per_split)
     slots = slot_mapping if slot_mapping.dtype == torch.int64 else slot_mapping.to(torch.int64)
-    return AttentionMetadata(slots.contiguous(), plan, info, num_tokens,
-                             _num_sms=num_sms, _pages_per_split=pages_per_split)
+    slots = slots.contiguous()
+    tree = None
+    if trees:
+        tpacked, tinfo = plan_tree_batch(trees, num_tokens, block_size, num_sms, pages_per_split)
+        tree = AttentionMetadata(slots, _upload_plan(tpacked, device), tinfo, num_tokens,
+                                 _num_sms=num_sms, _pages_per_split=pages_per_split)
+    return AttentionMetadata(slots, _upload_plan(packed, device), info, num_tokens,
+                             _num_sms=num_sms, _pages_per_split=pages_per_split, kv8=kv8,
+                             tree=tree)
 
 
 def same_launch_shape(a: _capi.MsPlanInfo, b: _capi.MsPlanInfo) -> bool:
@@ -247,29 +351,96 @@ def _rows(t: Tensor, name: str) -> int:
 
 
 def kv_scatter(k: Tensor, v: Tensor, slot_mapping: Tensor, k_cache: Tensor, v_cache: Tensor) -> None:
-    """Write this step's K/V rows into their slots (backends.py:159-160)."""
-    nb, kvh = check_layer_views(k_cache, v_cache)
+    """Write this step's K/V rows into their slots (backends.py:159-160).  Into an 8-bit pool each
+    row is quantised as it is written (see ``kv_pool``)."""
+    nb, kvh = check_layer_views(k_cache, v_cache, kv8=True)
     t = int(k.shape[0])
     lib = _capi.load()
-    rc = lib.ms_kv_scatter(
-        k.data_ptr(), _rows(k, "k"), v.data_ptr(), _rows(v, "v"), t, kvh,
-        slot_mapping.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), nb, _stream(k.device),
-    )
+    if is_kv8(k_cache):
+        _check_rows_args(k, v, slot_mapping, k_cache, kvh)
+        with _on_device(k_cache.device):
+            rc = lib.ms_kv_scatter_kv8(
+                k.data_ptr(), _rows(k, "k"), v.data_ptr(), _rows(v, "v"), t, kvh,
+                slot_mapping.data_ptr(), k_cache.data_ptr(), nb, _stream(k.device),
+            )
+    else:
+        rc = lib.ms_kv_scatter(
+            k.data_ptr(), _rows(k, "k"), v.data_ptr(), _rows(v, "v"), t, kvh,
+            slot_mapping.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), nb, _stream(k.device),
+        )
     _capi.check(rc, "kv_scatter")
+
+
+def _on_device(device: torch.device):
+    """The library launches on the current device: make it the tensors' own."""
+    return torch.cuda.device(device)
+
+
+def _check_rows_args(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, kvh: int) -> None:
+    if k.dim() != 3 or k.shape != v.shape or k.shape[1] != kvh:
+        raise ValueError(f"k and v must both be [T, {kvh}, {HEAD_DIM}]")
+    if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
+        raise ValueError("slots must be a contiguous int64 vector")
+    if slots.shape[0] != k.shape[0]:
+        raise ValueError(f"{k.shape[0]} rows but {slots.shape[0]} slots")
+    if not k_cache.is_cuda:
+        raise RuntimeError("miniserve_b200 attention runs on CUDA only (no CPU fallback)")
+    for t, name in ((k, "k"), (v, "v"), (slots, "slots")):
+        if t.device != k_cache.device:
+            raise ValueError(f"{name} is on {t.device}, the pool on {k_cache.device}")
+
+
+def kv_gather(slots: Tensor, k_cache: Tensor, v_cache: Tensor, k_out: Tensor | None = None,
+              v_out: Tensor | None = None) -> tuple[Tensor, Tensor]:
+    """Rows ``slots`` (int64 vector, any order, repeats allowed) of a layer's pool as bf16
+    ``(k, v)``, each ``[len(slots), kv_heads, 128]``.  No reference counterpart.
+
+    What it is for: after a verify step the accepted drafts' rows are read and written to the
+    positions they take in the sequence (``kv_scatter(*kv_gather(from_slots, ...), to_slots, ...)``; the
+    rows are read before any is written, so the two sets may overlap), or a sequence's rows are handed
+    to another cache.  From an 8-bit pool the values are exact, and writing them back stores the same
+    values again.  A slot outside the pool reads as zeros (and sets the device status bit).
+    """
+    nb, kvh = check_layer_views(k_cache, v_cache, kv8=True)
+    n = int(slots.shape[0]) if slots.dim() == 1 else -1
+    shape = (max(n, 0), kvh, HEAD_DIM)
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=torch.bfloat16, device=slots.device)
+    if v_out is None:
+        v_out = torch.empty(shape, dtype=torch.bfloat16, device=slots.device)
+    _check_rows_args(k_out, v_out, slots, k_cache, kvh)
+    k_stride, v_stride = _rows(k_out, "k_out"), _rows(v_out, "v_out")
+    lib = _capi.load()
+    with _on_device(k_cache.device):
+        stream = _stream(k_cache.device)
+        if is_kv8(k_cache):
+            rc = lib.ms_kv_gather_kv8(slots.data_ptr(), n, kvh, k_cache.data_ptr(), nb,
+                                      k_out.data_ptr(), k_stride, v_out.data_ptr(), v_stride, stream)
+        else:
+            rc = lib.ms_kv_gather(slots.data_ptr(), n, kvh, k_cache.data_ptr(), v_cache.data_ptr(),
+                                  nb, k_out.data_ptr(), k_stride, v_out.data_ptr(), v_stride, stream)
+    _capi.check(rc, "kv_gather")
+    return k_out, v_out
 
 
 def attend(q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: AttentionMetadata, scale: float,
            out: Tensor | None = None) -> Tensor:
-    """Attention of every planned query row through the pool (backends.py:161-197).
+    """Attention of every planned query row through the pool (backends.py:161-197); draft trees
+    and an 8-bit pool included.
 
     Rows not covered by ``meta`` are left untouched (undefined, like ``torch.empty_like``).
     """
-    nb, kvh = check_layer_views(k_cache, v_cache)
+    nb, kvh = check_layer_views(k_cache, v_cache, kv8=True)
     if out is None:
         out = torch.empty_like(q)
     h = int(q.shape[1])
-    ws = meta.workspace(kvh, q.device)
     lib = _capi.load()
+    if is_kv8(k_cache) or meta.tree is not None:
+        _check_attend_args(q, out, k_cache, meta)
+        with _on_device(k_cache.device):
+            _attend_parts(lib, q, k_cache, v_cache, meta, scale, out, nb, kvh)
+        return out
+    ws = meta.workspace(kvh, q.device)
     rc = lib.ms_paged_attention(
         q.data_ptr(), _rows(q, "q"), out.data_ptr(), _rows(out, "out"), h, kvh,
         k_cache.data_ptr(), v_cache.data_ptr(), nb, meta.plan.data_ptr(), C.byref(meta.info),
@@ -278,6 +449,47 @@ def attend(q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: AttentionMetadata,
     )
     _capi.check(rc, "paged_attention")
     return out
+
+
+def _check_attend_args(q: Tensor, out: Tensor, k_cache: Tensor, meta: AttentionMetadata) -> None:
+    if not k_cache.is_cuda:
+        raise RuntimeError("miniserve_b200 attention runs on CUDA only (no CPU fallback)")
+    for t, name in ((q, "q"), (out, "out"), (meta.plan, "meta")):
+        if t.device != k_cache.device:
+            raise ValueError(f"{name} is on {t.device}, the pool on {k_cache.device}")
+    if q.shape[0] < meta.num_tokens or out.shape[0] < meta.num_tokens:
+        raise ValueError(f"q and out must have the step's {meta.num_tokens} rows")
+    if out.shape[1:] != q.shape[1:]:
+        raise ValueError("out must have q's heads")
+
+
+def _attend_parts(lib, q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: AttentionMetadata,
+                  scale: float, out: Tensor, nb: int, kvh: int) -> None:
+    """The causal part and the draft trees of a step, over either kind of pool."""
+    kv8 = is_kv8(k_cache)
+    h, stream = int(q.shape[1]), _stream(q.device)
+    q_args = (q.data_ptr(), _rows(q, "q"), out.data_ptr(), _rows(out, "out"), h, kvh)
+    parts = [meta] if meta.tree is None else [meta, meta.tree]
+    for part in parts:
+        info = part.info
+        if part.tree is not None and not (info.n_decode_items or info.n_tile_items or info.n_tc_items):
+            continue  # every sequence is a tree
+        is_tree = part is meta.tree
+        ws = part.workspace(kvh, q.device, kv8=kv8 and not is_tree)
+        scratch = (ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0)
+        if is_tree:
+            rc = lib.ms_tree_attention(
+                *q_args, k_cache.data_ptr(), None if kv8 else v_cache.data_ptr(), nb,
+                part.plan.data_ptr(), C.byref(info), *scratch, float(scale), stream)
+        elif kv8:
+            rc = lib.ms_paged_attention_kv8(
+                *q_args, k_cache.data_ptr(), nb, part.plan.data_ptr(), C.byref(info),
+                C.byref(part.kv8), *scratch, float(scale), stream)
+        else:
+            rc = lib.ms_paged_attention(
+                *q_args, k_cache.data_ptr(), v_cache.data_ptr(), nb, part.plan.data_ptr(),
+                C.byref(info), *scratch, float(scale), stream)
+        _capi.check(rc, "paged_attention")
 
 
 def paged_attention(

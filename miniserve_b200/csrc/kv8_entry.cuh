@@ -1,0 +1,397 @@
+// C-ABI entry points of the 8-bit pool, of reading rows back, and of attention over drafted token
+// trees (declared in include/msattn.h).  Included at the end of msattn.cu, whose launch helpers and
+// kernels they use.
+
+namespace {
+
+int check_pool8(const char* what, const void* pool, int num_blocks, int num_kv) {
+  if (pool == nullptr || num_blocks <= 0 || num_kv <= 0) {
+    set_error(std::string(what) + ": null pointer or empty pool");
+    return MS_ERR_ARG;
+  }
+  if (!aligned(pool, 16)) {
+    set_error(std::string(what) + ": the 8-bit layer must be 16-byte aligned");
+    return MS_ERR_LAYOUT;
+  }
+  return MS_OK;
+}
+
+// Grid of the row-copy kernels: two rows per warp instruction, kPairs of them per warp.  Enough rows
+// for every SM's warps take four pairs per warp (four loads in flight per lane); fewer take one, so
+// that a decode step's few rows spread over more SMs.
+constexpr int kCopyWarps = 8;
+template <typename Few, typename Many>
+cudaError_t launch_rows(int64_t rows, int sms, Few few, Many many) {
+  const int64_t per4 = kCopyWarps * 8, per1 = kCopyWarps * 2;
+  if ((rows + per4 - 1) / per4 >= 4 * static_cast<int64_t>(sms))
+    return many(static_cast<unsigned>((rows + per4 - 1) / per4));
+  return few(static_cast<unsigned>((rows + per1 - 1) / per1));
+}
+
+int check_attention(const char* what, const void* q, int64_t q_row_stride, const void* out,
+                    int64_t out_row_stride, int num_heads, int num_kv, const int32_t* plan_dev,
+                    const MsPlanInfo* plan, const void* workspace, int64_t workspace_bytes,
+                    int64_t need, float scale) {
+  if (plan == nullptr || num_kv <= 0 || num_heads != ms::kGroup * num_kv) {
+    set_error(std::string(what) + ": need a plan and num_heads == 2 * num_kv_heads > 0");
+    return MS_ERR_ARG;
+  }
+  if (!(scale > 0.f) || scale > 3e38f) {
+    set_error(std::string(what) + ": scale must be positive and finite");
+    return MS_ERR_ARG;
+  }
+  if (!q || !out || !plan_dev || q_row_stride < num_heads * ms::kHeadDim ||
+      out_row_stride < num_heads * ms::kHeadDim || q_row_stride % 8 || out_row_stride % 8 ||
+      !aligned(q, 16) || !aligned(out, 16) || !aligned(plan_dev, 16)) {
+    set_error(std::string(what) + ": null pointer, or q/out rows not 16-byte aligned");
+    return MS_ERR_ARG;
+  }
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16))) {
+    set_error(std::string(what) + ": workspace of " + std::to_string(need) +
+              " bytes (16-byte aligned) required");
+    return MS_ERR_ARG;
+  }
+  const int64_t items = static_cast<int64_t>(plan->n_decode_items) + 2 * plan->n_tile_items +
+                        plan->n_tc_items;
+  if (items * num_kv > 0x7fffffffLL || static_cast<int64_t>(plan->n_combine) * num_kv > 0x7fffffffLL) {
+    set_error(std::string(what) + ": plan too large for one launch");
+    return MS_ERR_ARG;
+  }
+  return MS_OK;
+}
+
+ms::AttnArgs attn_args(const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride,
+                       int num_kv, int num_blocks, const int32_t* plan_dev, const MsPlanInfo* plan,
+                       void* workspace, float scale) {
+  ms::AttnArgs a;
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.q_row_stride = q_row_stride;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.out_row_stride = out_row_stride;
+  a.seqs = plan_dev + plan->off_seqs;
+  a.tables = plan_dev + plan->off_tables;
+  a.items = nullptr;
+  a.n_items = 0;
+  a.num_kv = num_kv;
+  a.num_blocks = num_blocks;
+  float* ws = static_cast<float*>(workspace);
+  a.ws_o = ws;
+  a.ws_lse = ws != nullptr ? ws + plan->part_rows * num_kv * ms::kHeadDim : nullptr;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  return a;
+}
+
+template <typename K, typename... Args>
+cudaError_t launch_plain(K kernel, unsigned grid, unsigned block, size_t smem, cudaStream_t s,
+                         Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+}  // namespace
+
+extern "C" int ms_kv_scatter_kv8(const void* k, int64_t k_row_stride, const void* v,
+                                 int64_t v_row_stride, int32_t num_tokens, int32_t num_kv_heads,
+                                 const int64_t* slot_mapping, void* pool, int32_t num_blocks,
+                                 void* stream) {
+  if (num_tokens < 0 || num_kv_heads <= 0) {
+    set_error("ms_kv_scatter_kv8: bad sizes");
+    return MS_ERR_ARG;
+  }
+  if (num_tokens == 0) return MS_OK;
+  int rc = check_pool8("ms_kv_scatter_kv8", pool, num_blocks, num_kv_heads);
+  if (rc) return rc;
+  const int64_t width = static_cast<int64_t>(num_kv_heads) * ms::kHeadDim;
+  if (!k || !v || !slot_mapping || k_row_stride < width || v_row_stride < width ||
+      k_row_stride % 4 || v_row_stride % 4 || !aligned(k, 8) || !aligned(v, 8)) {
+    set_error("ms_kv_scatter_kv8: null pointer, stride or alignment");
+    return MS_ERR_ARG;
+  }
+  const int64_t rows = static_cast<int64_t>(num_tokens) * 2 * num_kv_heads;
+  if (rows > (int64_t(1) << 33)) {
+    set_error("ms_kv_scatter_kv8: batch too large");
+    return MS_ERR_ARG;
+  }
+  unsigned* st = status_ptr(&rc);
+  if (rc) return rc;
+  int sms = 0;
+  rc = sm_count(&sms);
+  if (rc) return rc;
+  ms::Scatter8Args a;
+  a.k = static_cast<const __nv_bfloat16*>(k);
+  a.k_row_stride = k_row_stride;
+  a.v = static_cast<const __nv_bfloat16*>(v);
+  a.v_row_stride = v_row_stride;
+  a.slots = reinterpret_cast<const long long*>(slot_mapping);
+  a.pool = static_cast<uint8_t*>(pool);
+  a.num_slots = static_cast<long long>(num_blocks) * ms::kBlockTokens;
+  a.num_tokens = num_tokens;
+  a.num_kv = num_kv_heads;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool v16 = aligned(k, 16) && aligned(v, 16) && k_row_stride % 8 == 0 && v_row_stride % 8 == 0;
+  auto go = [&](auto kernel) {
+    return [=](unsigned grid) { return launch(kernel, grid, kCopyWarps * 32, 0, s, a, st); };
+  };
+  const cudaError_t e =
+      v16 ? launch_rows(rows, sms, go(ms::kv_scatter8_kernel<kCopyWarps, 1, true>),
+                        go(ms::kv_scatter8_kernel<kCopyWarps, 4, true>))
+          : launch_rows(rows, sms, go(ms::kv_scatter8_kernel<kCopyWarps, 1, false>),
+                        go(ms::kv_scatter8_kernel<kCopyWarps, 4, false>));
+  if (e != cudaSuccess) return cuda_fail("kv_scatter_kv8 launch", e);
+  return MS_OK;
+}
+
+extern "C" int ms_qk_norm_rope_scatter_kv8(
+    const void* qkv, int64_t qkv_row_stride, int32_t num_tokens, int32_t num_heads,
+    int32_t num_kv_heads, const void* q_weight, const void* k_weight, float eps, const float* cos,
+    const float* sin, int64_t cs_row_stride, const int64_t* positions, int64_t max_positions,
+    const int64_t* slot_mapping, void* q_out, int64_t q_out_row_stride, void* pool,
+    int32_t num_blocks, void* stream) {
+  if (num_tokens < 0 || num_kv_heads <= 0 || num_heads != ms::kGroup * num_kv_heads) {
+    set_error("ms_qk_norm_rope_scatter_kv8: need num_heads == 2 * num_kv_heads > 0, "
+              "num_tokens >= 0");
+    return MS_ERR_ARG;
+  }
+  if (num_tokens == 0) return MS_OK;
+  const int rc = check_pool8("ms_qk_norm_rope_scatter_kv8", pool, num_blocks, num_kv_heads);
+  if (rc) return rc;
+  return norm_rope_scatter<ms::Kv8Rows>(
+      "ms_qk_norm_rope_scatter_kv8", qkv, qkv_row_stride, num_tokens, num_heads, num_kv_heads,
+      q_weight, k_weight, eps, cos, sin, cs_row_stride, positions, max_positions, slot_mapping,
+      q_out, q_out_row_stride, pool, num_blocks, stream);
+}
+
+namespace {
+
+template <bool kKv8>
+int gather(const char* what, const int64_t* slots, int32_t num_tokens, int32_t num_kv_heads,
+           const void* pool, int32_t num_blocks, void* k_out, int64_t k_row_stride, void* v_out,
+           int64_t v_row_stride, void* stream) {
+  const int64_t width = static_cast<int64_t>(num_kv_heads) * ms::kHeadDim;
+  if (!slots || !k_out || !v_out || k_row_stride < width || v_row_stride < width ||
+      k_row_stride % 8 || v_row_stride % 8 || !aligned(k_out, 16) || !aligned(v_out, 16)) {
+    set_error(std::string(what) + ": null pointer, or k/v rows not 16-byte aligned");
+    return MS_ERR_ARG;
+  }
+  const int64_t rows = static_cast<int64_t>(num_tokens) * 2 * num_kv_heads;
+  if (rows > (int64_t(1) << 33)) {
+    set_error(std::string(what) + ": batch too large");
+    return MS_ERR_ARG;
+  }
+  int rc = MS_OK;
+  unsigned* st = status_ptr(&rc);
+  if (rc) return rc;
+  int sms = 0;
+  rc = sm_count(&sms);
+  if (rc) return rc;
+  ms::GatherArgs a;
+  a.slots = reinterpret_cast<const long long*>(slots);
+  a.pool = pool;
+  a.head_stride = ms::kPageKVBytes / 2;
+  a.block_stride = static_cast<long long>(num_kv_heads) * a.head_stride;
+  a.num_slots = static_cast<long long>(num_blocks) * ms::kBlockTokens;
+  a.k = static_cast<__nv_bfloat16*>(k_out);
+  a.k_row_stride = k_row_stride;
+  a.v = static_cast<__nv_bfloat16*>(v_out);
+  a.v_row_stride = v_row_stride;
+  a.num_tokens = num_tokens;
+  a.num_kv = num_kv_heads;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  auto go = [&](auto kernel) {
+    return [=](unsigned grid) { return launch(kernel, grid, kCopyWarps * 32, 0, s, a, st); };
+  };
+  const cudaError_t e = launch_rows(rows, sms, go(ms::kv_gather_kernel<kKv8, kCopyWarps, 1>),
+                                    go(ms::kv_gather_kernel<kKv8, kCopyWarps, 4>));
+  if (e != cudaSuccess) return cuda_fail((std::string(what) + " launch").c_str(), e);
+  return MS_OK;
+}
+
+}  // namespace
+
+extern "C" int ms_kv_gather(const int64_t* slots, int32_t num_tokens, int32_t num_kv_heads,
+                            const void* k_cache, const void* v_cache, int32_t num_blocks,
+                            void* k_out, int64_t k_row_stride, void* v_out, int64_t v_row_stride,
+                            void* stream) {
+  if (num_tokens < 0 || num_kv_heads <= 0) {
+    set_error("ms_kv_gather: bad sizes");
+    return MS_ERR_ARG;
+  }
+  if (num_tokens == 0) return MS_OK;
+  const int rc = check_pool(k_cache, v_cache, num_blocks, num_kv_heads);
+  if (rc) return rc;
+  return gather<false>("ms_kv_gather", slots, num_tokens, num_kv_heads, k_cache, num_blocks, k_out,
+                       k_row_stride, v_out, v_row_stride, stream);
+}
+
+extern "C" int ms_kv_gather_kv8(const int64_t* slots, int32_t num_tokens, int32_t num_kv_heads,
+                                const void* pool, int32_t num_blocks, void* k_out,
+                                int64_t k_row_stride, void* v_out, int64_t v_row_stride,
+                                void* stream) {
+  if (num_tokens < 0 || num_kv_heads <= 0) {
+    set_error("ms_kv_gather_kv8: bad sizes");
+    return MS_ERR_ARG;
+  }
+  if (num_tokens == 0) return MS_OK;
+  const int rc = check_pool8("ms_kv_gather_kv8", pool, num_blocks, num_kv_heads);
+  if (rc) return rc;
+  return gather<true>("ms_kv_gather_kv8", slots, num_tokens, num_kv_heads, pool, num_blocks, k_out,
+                      k_row_stride, v_out, v_row_stride, stream);
+}
+
+extern "C" int ms_paged_attention_kv8(const void* q, int64_t q_row_stride, void* out,
+                                      int64_t out_row_stride, int32_t num_heads,
+                                      int32_t num_kv_heads, const void* pool, int32_t num_blocks,
+                                      const int32_t* plan_dev, const MsPlanInfo* plan,
+                                      const MsKv8Info* info, void* workspace,
+                                      int64_t workspace_bytes, float scale, void* stream) {
+  const char* what = "ms_paged_attention_kv8";
+  if (plan != nullptr &&
+      static_cast<int64_t>(plan->n_decode_items) + plan->n_tile_items + plan->n_tc_items == 0)
+    return MS_OK;
+  if (plan != nullptr && (info == nullptr || (plan->n_tc_items > 0 && info->n_pages <= 0))) {
+    set_error("ms_paged_attention_kv8: the plan has no 8-bit part (ms_kv8_plan_build)");
+    return MS_ERR_ARG;
+  }
+  const int64_t need = plan != nullptr ? ms_kv8_workspace_bytes(plan, info, num_kv_heads) : 0;
+  int rc = check_attention(what, q, q_row_stride, out, out_row_stride, num_heads, num_kv_heads,
+                           plan_dev, plan, workspace, workspace_bytes, need, scale);
+  if (rc) return rc;
+  rc = check_pool8(what, pool, num_blocks, num_kv_heads);
+  if (rc) return rc;
+  rc = ensure_smem_attrs();
+  if (rc) return rc;
+  unsigned* st = status_ptr(&rc);
+  if (rc) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  ms::AttnArgs a = attn_args(q, q_row_stride, out, out_row_stride, num_kv_heads, num_blocks,
+                             plan_dev, plan, workspace, scale);
+
+  // The pages of tensor-core items as a bf16 pool in the workspace, after the partials.
+  void* pages = nullptr;
+  CUtensorMap kmap, vmap;
+  if (plan->n_tc_items > 0) {
+    if (static_cast<int64_t>(info->n_pages) * num_kv_heads > 0x7fffffffLL) {
+      set_error("ms_paged_attention_kv8: plan too large for one launch");
+      return MS_ERR_ARG;
+    }
+    const int64_t part = plan->workspace_bytes_per_kv_head * num_kv_heads;
+    pages = static_cast<char*>(workspace) + (part + 1023) / 1024 * 1024;
+    rc = kv_tensor_map(pages, info->n_pages, num_kv_heads, 1, &kmap);
+    if (rc) return rc;
+    rc = kv_tensor_map(pages, info->n_pages, num_kv_heads, 2, &vmap);
+    if (rc) return rc;
+  }
+
+  // As in ms_paged_attention: beside tensor-core work without cascade groups the bandwidth-bound
+  // rows run on the side stream; with them they follow the kernel that writes the prefix partials.
+  const int n_rows = plan->n_decode_items + plan->n_tile_items;
+  SideStream* side = nullptr;
+  if (plan->n_tc_items > 0 && n_rows > 0 && plan->n_cascade == 0) side = side_stream();
+  cudaStream_t ds = s;
+  if (side != nullptr) {
+    cudaError_t e = cudaEventRecord(side->fork, s);
+    if (e == cudaSuccess) e = cudaStreamWaitEvent(side->stream, side->fork, 0);
+    if (e != cudaSuccess) return cuda_fail("fork to the side stream", e);
+    ds = side->stream;
+  }
+  auto join = [&]() -> cudaError_t {
+    if (side == nullptr) return cudaSuccess;
+    cudaError_t e = cudaEventRecord(side->join, ds);
+    if (e == cudaSuccess) e = cudaStreamWaitEvent(s, side->join, 0);
+    side = nullptr;
+    return e;
+  };
+  if (plan->n_tc_items > 0) {
+    cudaError_t e = launch(ms::kv8_expand_kernel, static_cast<unsigned>(info->n_pages * num_kv_heads),
+                           256, 0, s, static_cast<const uint8_t*>(pool), plan_dev + info->off_map,
+                           num_kv_heads, num_blocks, static_cast<__nv_bfloat16*>(pages), st);
+    if (e == cudaSuccess) {
+      // An ordinary launch: this kernel reads earlier steps' pages before it waits for its
+      // predecessor, and here the predecessor writes them.
+      ms::AttnArgs t = a;
+      t.seqs = plan_dev + info->off_seqs;
+      t.tables = plan_dev + info->off_tables;
+      t.items = plan_dev + plan->off_tc;
+      t.n_items = plan->n_tc_items;
+      t.num_blocks = info->n_pages;
+      e = launch_plain(ms::prefill_tc_kernel, plan->n_tc_items * num_kv_heads, ms::TcCfg::kThreads,
+                       ms::TcCfg::kSmemBytes, s, kmap, vmap, t);
+    }
+    if (e != cudaSuccess) {
+      join();
+      return cuda_fail("8-bit prefill launch", e);
+    }
+  }
+  if (n_rows > 0) {
+    // Decode items (one tile each) and chunk items (two tiles of 32 tokens) in one launch: their
+    // records are adjacent in the plan.
+    ms::RowsArgs r;
+    r.a = a;
+    r.a.items = plan_dev + plan->off_decode;
+    r.a.n_items = n_rows;
+    r.pool = static_cast<const uint8_t*>(pool);
+    r.plan = plan_dev;
+    r.n_single = plan->n_decode_items;
+    CUtensorMap none;
+    std::memset(&none, 0, sizeof(none));
+    const unsigned grid =
+        static_cast<unsigned>((plan->n_decode_items + 2 * plan->n_tile_items) * num_kv_heads);
+    const cudaError_t e = launch(ms::rows_attn_kernel<true, false>, grid, ms::kRowsThreads,
+                                 ms::RowsCfg<true>::kSmemBytes, ds, none, r);
+    if (e != cudaSuccess) {
+      join();
+      return cuda_fail("8-bit rows launch", e);
+    }
+  }
+  {
+    const cudaError_t e = join();
+    if (e != cudaSuccess) return cuda_fail("join of the side stream", e);
+  }
+  return launch_combine(a, plan, plan_dev, s);
+}
+
+extern "C" int ms_tree_attention(const void* q, int64_t q_row_stride, void* out,
+                                 int64_t out_row_stride, int32_t num_heads, int32_t num_kv_heads,
+                                 const void* k_cache, const void* v_cache, int32_t num_blocks,
+                                 const int32_t* plan_dev, const MsPlanInfo* plan, void* workspace,
+                                 int64_t workspace_bytes, float scale, void* stream) {
+  const char* what = "ms_tree_attention";
+  if (plan != nullptr && plan->n_tile_items == 0) return MS_OK;
+  const int64_t need = plan != nullptr ? plan->workspace_bytes_per_kv_head * num_kv_heads : 0;
+  int rc = check_attention(what, q, q_row_stride, out, out_row_stride, num_heads, num_kv_heads,
+                           plan_dev, plan, workspace, workspace_bytes, need, scale);
+  if (rc) return rc;
+  const bool kv8 = v_cache == nullptr;
+  rc = kv8 ? check_pool8(what, k_cache, num_blocks, num_kv_heads)
+           : check_pool(k_cache, v_cache, num_blocks, num_kv_heads);
+  if (rc) return rc;
+  rc = ensure_smem_attrs();
+  if (rc) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  ms::RowsArgs r;
+  r.a = attn_args(q, q_row_stride, out, out_row_stride, num_kv_heads, num_blocks, plan_dev, plan,
+                  workspace, scale);
+  r.a.items = plan_dev + plan->off_tile;
+  r.a.n_items = plan->n_tile_items;
+  r.pool = kv8 ? static_cast<const uint8_t*>(k_cache) : nullptr;
+  r.plan = plan_dev;
+  r.n_single = plan->n_tile_items;
+  CUtensorMap map;
+  std::memset(&map, 0, sizeof(map));
+  if (!kv8) {
+    rc = kv_tensor_map(k_cache, num_blocks, num_kv_heads, 0, &map);
+    if (rc) return rc;
+  }
+  const unsigned grid = static_cast<unsigned>(plan->n_tile_items * num_kv_heads);
+  const cudaError_t e =
+      kv8 ? launch(ms::rows_attn_kernel<true, true>, grid, ms::kRowsThreads,
+                   ms::RowsCfg<true>::kSmemBytes, s, map, r)
+          : launch(ms::rows_attn_kernel<false, true>, grid, ms::kRowsThreads,
+                   ms::RowsCfg<false>::kSmemBytes, s, map, r);
+  if (e != cudaSuccess) return cuda_fail("tree attention launch", e);
+  return launch_combine(r.a, plan, plan_dev, s);
+}

@@ -18,6 +18,7 @@
 #include "paged_attention.cuh"
 #include "prefill_tc.cuh"
 #include "qkv_proj_tc.cuh"
+#include "rows_attention.cuh"
 
 namespace ms_host {
 
@@ -243,6 +244,15 @@ static int ensure_smem_attrs() {
                            cudaFuncAttributeMaxDynamicSharedMemorySize,
                            ms::QkvCfg<1, 2>::kSmemBytes);
   if (e != cudaSuccess) return cuda_fail("cudaFuncSetAttribute(qkv split-K)", e);
+  auto rows_attr = [](auto kernel, int bytes) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  };
+  e = rows_attr(ms::rows_attn_kernel<true, false>, ms::RowsCfg<true>::kSmemBytes);
+  if (e == cudaSuccess)
+    e = rows_attr(ms::rows_attn_kernel<true, true>, ms::RowsCfg<true>::kSmemBytes);
+  if (e == cudaSuccess)
+    e = rows_attr(ms::rows_attn_kernel<false, true>, ms::RowsCfg<false>::kSmemBytes);
+  if (e != cudaSuccess) return cuda_fail("cudaFuncSetAttribute(rows)", e);
   done[dev] = true;
   return MS_OK;
 }
@@ -367,23 +377,18 @@ static unsigned* status_ptr(int* rc) {
   return cached;
 }
 
-extern "C" int ms_qk_norm_rope_scatter(const void* qkv, int64_t qkv_row_stride, int32_t num_tokens,
-                                       int32_t num_heads, int32_t num_kv_heads,
-                                       const void* q_weight, const void* k_weight, float eps,
-                                       const float* cos, const float* sin, int64_t cs_row_stride,
-                                       const int64_t* positions, int64_t max_positions,
-                                       const int64_t* slot_mapping, void* q_out,
-                                       int64_t q_out_row_stride, void* k_cache, void* v_cache,
-                                       int32_t num_blocks, void* stream) {
-  if (num_tokens < 0 || num_kv_heads <= 0 || num_heads != ms::kGroup * num_kv_heads) {
-    set_error("ms_qk_norm_rope_scatter: need num_heads == 2 * num_kv_heads > 0, num_tokens >= 0");
-    return MS_ERR_ARG;
-  }
-  if (num_tokens == 0) return MS_OK;
-  int rc = check_pool(k_cache, v_cache, num_blocks, num_kv_heads);
-  if (rc) return rc;
+// Kernel A over a bf16 pool (Rows = Bf16Rows) or an 8-bit one (Kv8Rows: k_cache is the layer); the
+// caller has checked the pool.
+template <typename Rows>
+static int norm_rope_scatter(const char* what, const void* qkv, int64_t qkv_row_stride,
+                             int32_t num_tokens, int32_t num_heads, int32_t num_kv_heads,
+                             const void* q_weight, const void* k_weight, float eps,
+                             const float* cos, const float* sin, int64_t cs_row_stride,
+                             const int64_t* positions, int64_t max_positions,
+                             const int64_t* slot_mapping, void* q_out, int64_t q_out_row_stride,
+                             void* k_cache, int32_t num_blocks, void* stream) {
   if (!qkv || !q_weight || !k_weight || !cos || !sin || !slot_mapping || !q_out) {
-    set_error("ms_qk_norm_rope_scatter: null pointer argument");
+    set_error(std::string(what) + ": null pointer argument");
     return MS_ERR_ARG;
   }
   const int64_t width = static_cast<int64_t>(num_heads + 2 * num_kv_heads) * ms::kHeadDim;
@@ -391,14 +396,15 @@ extern "C" int ms_qk_norm_rope_scatter(const void* qkv, int64_t qkv_row_stride, 
       cs_row_stride < ms::kHeadDim || qkv_row_stride % 4 || q_out_row_stride % 4 ||
       cs_row_stride % 4 || !aligned(qkv, 8) || !aligned(q_out, 8) || !aligned(cos, 16) ||
       !aligned(sin, 16)) {
-    set_error("ms_qk_norm_rope_scatter: strides/alignment (qkv, q_out rows 8-byte aligned; "
+    set_error(std::string(what) + ": strides/alignment (qkv, q_out rows 8-byte aligned; "
               "cos/sin rows 16-byte aligned)");
     return MS_ERR_ARG;
   }
   if (positions != nullptr && max_positions <= 0) {
-    set_error("ms_qk_norm_rope_scatter: positions given with an empty table");
+    set_error(std::string(what) + ": positions given with an empty table");
     return MS_ERR_ARG;
   }
+  int rc = MS_OK;
   unsigned* st = status_ptr(&rc);
   if (rc) return rc;
   ms::NormRopeArgs a;
@@ -423,7 +429,7 @@ extern "C" int ms_qk_norm_rope_scatter(const void* qkv, int64_t qkv_row_stride, 
   a.num_heads = num_heads;
   a.num_kv = num_kv_heads;
   if (num_kv_heads % ms::kRowsPerWarp != 0) {
-    set_error("ms_qk_norm_rope_scatter: num_kv_heads must be a multiple of 8");
+    set_error(std::string(what) + ": num_kv_heads must be a multiple of 8");
     return MS_ERR_ARG;
   }
   constexpr int kWarps = 8;
@@ -431,7 +437,7 @@ extern "C" int ms_qk_norm_rope_scatter(const void* qkv, int64_t qkv_row_stride, 
       static_cast<long long>(num_tokens) * (num_heads + 2 * num_kv_heads) / ms::kRowsPerWarp;
   const long long blocks = (warps + kWarps - 1) / kWarps;
   if (blocks > 0x7fffffffLL) {
-    set_error("ms_qk_norm_rope_scatter: batch too large");
+    set_error(std::string(what) + ": batch too large");
     return MS_ERR_ARG;
   }
   // The 16-byte form (two whole rows per warp instruction, half the instructions) whenever the
@@ -439,12 +445,33 @@ extern "C" int ms_qk_norm_rope_scatter(const void* qkv, int64_t qkv_row_stride, 
   const bool v16 = aligned(qkv, 16) && aligned(q_out, 16) && qkv_row_stride % 8 == 0 &&
                    q_out_row_stride % 8 == 0 && aligned(q_weight, 16) && aligned(k_weight, 16);
   const cudaError_t e =
-      v16 ? launch(ms::qk_norm_rope_scatter_v16_kernel<kWarps>, static_cast<unsigned>(blocks),
+      v16 ? launch(ms::qk_norm_rope_scatter_v16_kernel<kWarps, Rows>, static_cast<unsigned>(blocks),
                    kWarps * 32, 0, static_cast<cudaStream_t>(stream), a, st)
-          : launch(ms::qk_norm_rope_scatter_kernel<kWarps>, static_cast<unsigned>(blocks),
+          : launch(ms::qk_norm_rope_scatter_kernel<kWarps, Rows>, static_cast<unsigned>(blocks),
                    kWarps * 32, 0, static_cast<cudaStream_t>(stream), a, st);
-  if (e != cudaSuccess) return cuda_fail("qk_norm_rope_scatter launch", e);
+  if (e != cudaSuccess) return cuda_fail((std::string(what) + " launch").c_str(), e);
   return MS_OK;
+}
+
+extern "C" int ms_qk_norm_rope_scatter(const void* qkv, int64_t qkv_row_stride, int32_t num_tokens,
+                                       int32_t num_heads, int32_t num_kv_heads,
+                                       const void* q_weight, const void* k_weight, float eps,
+                                       const float* cos, const float* sin, int64_t cs_row_stride,
+                                       const int64_t* positions, int64_t max_positions,
+                                       const int64_t* slot_mapping, void* q_out,
+                                       int64_t q_out_row_stride, void* k_cache, void* v_cache,
+                                       int32_t num_blocks, void* stream) {
+  if (num_tokens < 0 || num_kv_heads <= 0 || num_heads != ms::kGroup * num_kv_heads) {
+    set_error("ms_qk_norm_rope_scatter: need num_heads == 2 * num_kv_heads > 0, num_tokens >= 0");
+    return MS_ERR_ARG;
+  }
+  if (num_tokens == 0) return MS_OK;
+  int rc = check_pool(k_cache, v_cache, num_blocks, num_kv_heads);
+  if (rc) return rc;
+  return norm_rope_scatter<ms::Bf16Rows>(
+      "ms_qk_norm_rope_scatter", qkv, qkv_row_stride, num_tokens, num_heads, num_kv_heads, q_weight,
+      k_weight, eps, cos, sin, cs_row_stride, positions, max_positions, slot_mapping, q_out,
+      q_out_row_stride, k_cache, num_blocks, stream);
 }
 
 extern "C" int ms_qkv_proj_norm_rope_scatter(
@@ -582,6 +609,30 @@ extern "C" int ms_kv_scatter(const void* k, int64_t k_row_stride, const void* v,
   const cudaError_t e = launch(ms::kv_scatter_kernel<kWarps>, static_cast<unsigned>(blocks),
                                kWarps * 32, 0, static_cast<cudaStream_t>(stream), a, st);
   if (e != cudaSuccess) return cuda_fail("kv_scatter launch", e);
+  return MS_OK;
+}
+
+// Merge of the split items' partials (kernel C), after every launch that writes them.
+static int launch_combine(const ms::AttnArgs& a, const MsPlanInfo* plan, const int32_t* plan_dev,
+                          cudaStream_t s) {
+  if (plan->n_combine == 0) return MS_OK;
+  ms::CombineArgs c;
+  c.out = a.out;
+  c.out_row_stride = a.out_row_stride;
+  c.seqs = plan_dev + plan->off_seqs;
+  c.combines = plan_dev + plan->off_combine;
+  c.n_combine = plan->n_combine;
+  c.num_kv = a.num_kv;
+  c.ws_o = a.ws_o;
+  c.ws_lse = a.ws_lse;
+  // One CTA per (record, KV head, kCombineRows rows): a tensor-core record has 256 rows, and
+  // one CTA walking them all is latency-bound (each row is a few dependent loads).
+  const int64_t rows_max = static_cast<int64_t>(std::max(plan->combine_tokens_max, 1)) * 2;
+  const unsigned row_ctas = static_cast<unsigned>(
+      std::min<int64_t>((rows_max + ms::kCombineRows - 1) / ms::kCombineRows, 65535));
+  const cudaError_t e = launch(ms::combine_kernel, dim3(plan->n_combine * a.num_kv, row_ctas),
+                               ms::kCombineThreads, 0, s, c);
+  if (e != cudaSuccess) return cuda_fail("combine launch", e);
   return MS_OK;
 }
 
@@ -741,24 +792,7 @@ extern "C" int ms_paged_attention(const void* q, int64_t q_row_stride, void* out
     const cudaError_t e = join();
     if (e != cudaSuccess) return cuda_fail("join of the side stream", e);
   }
-  if (plan->n_combine > 0) {
-    ms::CombineArgs c;
-    c.out = a.out;
-    c.out_row_stride = out_row_stride;
-    c.seqs = a.seqs;
-    c.combines = plan_dev + plan->off_combine;
-    c.n_combine = plan->n_combine;
-    c.num_kv = num_kv_heads;
-    c.ws_o = a.ws_o;
-    c.ws_lse = a.ws_lse;
-    // One CTA per (record, KV head, kCombineRows rows): a tensor-core record has 256 rows, and
-    // one CTA walking them all is latency-bound (each row is a few dependent loads).
-    const int64_t rows_max = static_cast<int64_t>(std::max(plan->combine_tokens_max, 1)) * 2;
-    const unsigned row_ctas = static_cast<unsigned>(
-        std::min<int64_t>((rows_max + ms::kCombineRows - 1) / ms::kCombineRows, 65535));
-    const cudaError_t e = launch(ms::combine_kernel, dim3(plan->n_combine * num_kv_heads, row_ctas),
-                                 ms::kCombineThreads, 0, s, c);
-    if (e != cudaSuccess) return cuda_fail("combine launch", e);
-  }
-  return MS_OK;
+  return launch_combine(a, plan, plan_dev, s);
 }
+
+#include "kv8_entry.cuh"

@@ -55,13 +55,29 @@ __device__ __forceinline__ float bf16_round(float x) {
   return __bfloat162float(__float2bfloat16_rn(x));
 }
 
+// Where kernel A puts the K and V rows: the bf16 pool here, the 8-bit pool in kv8.cuh (Kv8Rows).
+// store4: a whole warp holds the row, 4 dims per lane; store8: half a warp, 8 dims per lane (both
+// halves call together, each with its own row).
+struct Bf16Rows {
+  static __device__ __forceinline__ void store4(const NormRopeArgs& a, bool is_v, long long slot,
+                                                int head, int lane, const uint2& x) {
+    __nv_bfloat16* base = a.k_pool + (is_v ? 2 * kBlockTokens * 64 : 0);
+    *reinterpret_cast<uint2*>(base + pool_offset(slot, head, lane * 4, a.block_stride, a.head_stride)) = x;
+  }
+  static __device__ __forceinline__ void store8(const NormRopeArgs& a, bool is_v, long long slot,
+                                                int head, int l16, const uint4& x) {
+    __nv_bfloat16* base = a.k_pool + (is_v ? 2 * kBlockTokens * 64 : 0);
+    *reinterpret_cast<uint4*>(base + pool_offset(slot, head, l16 * 8, a.block_stride, a.head_stride)) = x;
+  }
+};
+
 // One warp handles 8 head rows of one token: warps 0-1 of a token take the 16 query heads, warp 2
 // the 8 key heads, warp 3 the 8 value heads (rows are the 128-column blocks of the fused
 // projection, in order), so every warp does one kind of work.  All 8 row loads are issued before
 // any arithmetic, and the token's cos/sin values are read once per warp.
 constexpr int kRowsPerWarp = 8;
 
-template <int kWarps>
+template <int kWarps, typename Rows = Bf16Rows>
 __global__ void __launch_bounds__(kWarps * 32)
     qk_norm_rope_scatter_kernel(const NormRopeArgs a, unsigned* status) {
   pdl_wait();
@@ -94,10 +110,8 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
   if (is_v) {  // value heads: a pure copy into the pool
     const int h0 = row0 - a.num_heads - a.num_kv;
-    __nv_bfloat16* vbase = a.k_pool + 2 * kBlockTokens * 64;
 #pragma unroll
-    for (int r = 0; r < kRowsPerWarp; ++r)
-      *reinterpret_cast<uint2*>(vbase + pool_offset(slot, h0 + r, d0, a.block_stride, a.head_stride)) = raw[r];
+    for (int r = 0; r < kRowsPerWarp; ++r) Rows::store4(a, true, slot, h0 + r, lane, raw[r]);
     return;
   }
 
@@ -157,8 +171,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     if (is_q) {
       *reinterpret_cast<uint2*>(a.q_out + t * a.q_out_row_stride + (row0 + r) * kHeadDim + d0) = packed;
     } else {
-      *reinterpret_cast<uint2*>(a.k_pool + pool_offset(slot, row0 + r - a.num_heads, d0,
-                                                       a.block_stride, a.head_stride)) = packed;
+      Rows::store4(a, false, slot, row0 + r - a.num_heads, lane, packed);
     }
   }
 }
@@ -191,7 +204,7 @@ __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w 
 // * weight * y, z * cos, rot * sin and p1 + p2 have bf16 operands: bf16x2_mul / bf16x2_add give
 //   the same roundings, two elements per instruction;
 // * rotate_half's partner (dim d +- 64) is lane ^ 8.
-template <int kWarps>
+template <int kWarps, typename Rows = Bf16Rows>
 __global__ void __launch_bounds__(kWarps * 32)
     qk_norm_rope_scatter_v16_kernel(const NormRopeArgs a, unsigned* status) {
   pdl_wait();
@@ -234,11 +247,8 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
   if (is_v) {  // value heads: a pure copy into the pool
     const int h0 = row0 - a.num_heads - a.num_kv + half;
-    __nv_bfloat16* vbase = a.k_pool + 2 * kBlockTokens * 64;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      *reinterpret_cast<uint4*>(vbase + pool_offset(slot, h0 + 2 * k, d0, a.block_stride,
-                                                    a.head_stride)) = raw[k];
+    for (int k = 0; k < 4; ++k) Rows::store8(a, true, slot, h0 + 2 * k, l16, raw[k]);
     return;
   }
 
@@ -318,8 +328,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     if (is_q) {
       *reinterpret_cast<uint4*>(a.q_out + t * a.q_out_row_stride + row * kHeadDim + d0) = packed;
     } else {
-      *reinterpret_cast<uint4*>(a.k_pool + pool_offset(slot, row - a.num_heads, d0,
-                                                       a.block_stride, a.head_stride)) = packed;
+      Rows::store8(a, false, slot, row - a.num_heads, l16, packed);
     }
   }
 }

@@ -1,0 +1,362 @@
+// Host planners of the 8-bit pool and of drafted token trees (declared in include/msattn.h).
+//
+// ms_kv8_plan_build adds to a packed plan what its tensor-core items need over an 8-bit pool: the
+// pages they read are expanded to bf16 in the workspace, numbered densely, so the part holds the
+// expanded pages' block ids, the identity table the kernel walks instead of the block tables, and the
+// sequence records with their tables' places in it.
+//
+// ms_tree_plan_build cuts every sequence of drafts into tiles of at most 32 tokens (64 query rows),
+// each reading the cached context and the drafts up to its own last one (a parent precedes its
+// children), and splits long tiles over their pages as ms_plan_build does.  Masks are bit rows, one per
+// draft, ceil(num_new / 32) words each, at the sequence record's field 6 (length in words in field 7).
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+#include <cstring>
+#include <exception>
+#include <string>
+#include <vector>
+
+#include "../../include/msattn.h"
+
+namespace ms_host {
+void set_error(const std::string& msg);
+}
+
+namespace {
+
+constexpr int kRec = 8;
+constexpr int kTileTokens = 32;
+constexpr int kAssumedKvHeads = 8;  // the planner does not see the head count; only speed depends on it
+// Automatic split (the rule of ms_plan_build): one resident wave of kTreeCtasPerSm CTAs per SM.
+constexpr int kTreeCtasPerSm = 3;
+constexpr int kMinSplitPages = 8;
+constexpr int kMaxSplitPages = 512;
+
+int64_t round4(int64_t x) { return (x + 3) & ~int64_t(3); }
+
+// No C++ exception leaves an extern "C" function: the planners' vectors may fail to allocate.
+template <typename F>
+int guarded(const char* what, F f) {
+  try {
+    return f();
+  } catch (const std::exception& e) {
+    try {
+      ms_host::set_error(std::string(what) + ": " + e.what());
+    } catch (...) {
+    }
+    return MS_ERR_CAPACITY;
+  }
+}
+
+struct TreeItem {
+  int seq, tok0, n_q, pb, pe, part_row;
+};
+
+}  // namespace
+
+extern "C" int64_t ms_kv8_plan_capacity(const MsPlanInfo* plan, int64_t total_table_entries) {
+  if (plan == nullptr || plan->n_tc_items == 0) return 0;
+  return round4(static_cast<int64_t>(plan->num_seqs + plan->n_cascade) * kRec) +
+         2 * round4(total_table_entries);
+}
+
+static int kv8_plan_build(int32_t* packed, int64_t capacity, const MsPlanInfo* plan,
+                          MsKv8Info* info) {
+  if (packed == nullptr || plan == nullptr || info == nullptr) {
+    ms_host::set_error("ms_kv8_plan_build: null argument");
+    return MS_ERR_ARG;
+  }
+  std::memset(info, 0, sizeof(*info));
+  info->total_ints = plan->total_ints;
+  if (plan->n_tc_items == 0) return MS_OK;
+  const int n_rec = plan->num_seqs + plan->n_cascade;
+  const int32_t* seqs = packed + plan->off_seqs;
+  // Pages each record's tensor-core items read (the largest page end).
+  std::vector<int32_t> pages(n_rec, 0);
+  for (int i = 0; i < plan->n_tc_items; ++i) {
+    const int32_t* it = packed + plan->off_tc + static_cast<int64_t>(i) * kRec;
+    pages[it[0]] = std::max(pages[it[0]], it[4]);
+  }
+  int64_t n_pages = 0;
+  for (int p : pages) n_pages += p;
+  const int64_t off_seqs = plan->total_ints;
+  const int64_t off_map = off_seqs + round4(static_cast<int64_t>(n_rec) * kRec);
+  const int64_t off_tables = off_map + round4(n_pages);
+  const int64_t total = off_tables + round4(n_pages);
+  if (total > capacity) {
+    ms_host::set_error("ms_kv8_plan_build: the buffer holds " + std::to_string(capacity) +
+                       " ints, the plan with its 8-bit part needs " + std::to_string(total));
+    return MS_ERR_CAPACITY;
+  }
+  if (total >= INT32_MAX) {
+    ms_host::set_error("ms_kv8_plan_build: plan larger than 2^31 ints");
+    return MS_ERR_PLAN;
+  }
+  std::memset(packed + off_seqs, 0, sizeof(int32_t) * (total - off_seqs));
+  int32_t at = 0;
+  for (int i = 0; i < n_rec; ++i) {
+    int32_t* r = packed + off_seqs + static_cast<int64_t>(i) * kRec;
+    std::memcpy(r, seqs + static_cast<int64_t>(i) * kRec, sizeof(int32_t) * kRec);
+    if (pages[i] == 0) continue;
+    const int32_t* table = packed + plan->off_tables + r[4];
+    for (int p = 0; p < pages[i]; ++p) {
+      packed[off_map + at + p] = table[p];
+      packed[off_tables + at + p] = at + p;
+    }
+    r[4] = at;
+    r[5] = pages[i];
+    at += pages[i];
+  }
+  info->n_pages = static_cast<int32_t>(n_pages);
+  info->off_seqs = static_cast<int32_t>(off_seqs);
+  info->off_map = static_cast<int32_t>(off_map);
+  info->off_tables = static_cast<int32_t>(off_tables);
+  info->total_ints = static_cast<int32_t>(total);
+  return MS_OK;
+}
+
+extern "C" int ms_kv8_plan_build(int32_t* packed, int64_t capacity, const MsPlanInfo* plan,
+                                 MsKv8Info* info) {
+  return guarded("ms_kv8_plan_build",
+                 [&] { return kv8_plan_build(packed, capacity, plan, info); });
+}
+
+extern "C" int64_t ms_kv8_workspace_bytes(const MsPlanInfo* plan, const MsKv8Info* info,
+                                          int32_t num_kv_heads) {
+  if (plan == nullptr || info == nullptr || num_kv_heads <= 0) return 0;
+  // Partials first, then the expanded pages (8 KiB per head) on a 1 KiB boundary.
+  const int64_t part = plan->workspace_bytes_per_kv_head * num_kv_heads;
+  if (info->n_pages == 0) return part;
+  return (part + 1023) / 1024 * 1024 + static_cast<int64_t>(info->n_pages) * num_kv_heads * 8192;
+}
+
+extern "C" int64_t ms_tree_plan_capacity(int32_t num_seqs, const int32_t* num_new,
+                                         int64_t total_table_entries) {
+  if (num_seqs < 0 || (num_seqs > 0 && num_new == nullptr)) return 0;
+  int64_t tiles = 0, masks = 0, tiles_max = 1;
+  for (int i = 0; i < num_seqs; ++i) {
+    const int64_t n = std::max(num_new[i], 0);
+    tiles += (n + kTileTokens - 1) / kTileTokens;
+    tiles_max = std::max(tiles_max, (n + kTileTokens - 1) / kTileTokens);
+    masks += n * ((n + 31) / 32);
+  }
+  // A tile has at most one item per page of its sequence.
+  const int64_t items = tiles + tiles_max * total_table_entries;
+  return round4(static_cast<int64_t>(num_seqs) * kRec) + round4(total_table_entries) +
+         round4(items * kRec) + round4(tiles * kRec) + round4(masks) + 16;
+}
+
+static int tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const int32_t* num_new,
+                           const int32_t* num_cached, const int64_t* table_offsets,
+                           const int32_t* tables, const int32_t* parents, int32_t num_tokens,
+                           int32_t block_size, int32_t num_sms, int32_t pages_per_split,
+                           int32_t* out, int64_t out_capacity, MsPlanInfo* info) {
+  if (info == nullptr || out == nullptr) {
+    ms_host::set_error("ms_tree_plan_build: null output");
+    return MS_ERR_ARG;
+  }
+  std::memset(info, 0, sizeof(*info));
+  if (num_seqs < 0 || num_tokens < 0 || block_size != 16 || num_sms <= 0 || pages_per_split < 0) {
+    ms_host::set_error("ms_tree_plan_build: bad sizes (block_size must be 16, num_sms > 0)");
+    return MS_ERR_ARG;
+  }
+  if (num_seqs > 0 && (flat_start == nullptr || num_new == nullptr || num_cached == nullptr ||
+                       table_offsets == nullptr || parents == nullptr)) {
+    ms_host::set_error("ms_tree_plan_build: null batch arrays");
+    return MS_ERR_ARG;
+  }
+  const int64_t total_entries = num_seqs > 0 ? table_offsets[num_seqs] : 0;
+  if (total_entries > 0 && tables == nullptr) {
+    ms_host::set_error("ms_tree_plan_build: null block tables");
+    return MS_ERR_ARG;
+  }
+  if (total_entries < 0 || total_entries >= (int64_t(1) << 31)) {
+    ms_host::set_error("ms_tree_plan_build: block tables exceed 2^31 entries");
+    return MS_ERR_ARG;
+  }
+
+  std::vector<TreeItem> tiles;
+  int64_t mask_words = 0, total_pages = 0, parent_at = 0;
+  std::vector<int64_t> mask_at(num_seqs, 0);
+  std::vector<int64_t> parents_at(num_seqs, 0);
+  for (int i = 0; i < num_seqs; ++i) {
+    const std::string who = "ms_tree_plan_build: sequence " + std::to_string(i);
+    const int64_t n = num_new[i], c = num_cached[i], f = flat_start[i];
+    const int64_t tlen = table_offsets[i + 1] - table_offsets[i];
+    if (n < 1 || c < 0 || f < 0 || f + n > num_tokens || tlen < 0) {
+      ms_host::set_error(who + " has an invalid flat_start/num_new/num_cached");
+      return MS_ERR_PLAN;
+    }
+    if (n > MS_MAX_TREE_TOKENS) {
+      ms_host::set_error(who + " has " + std::to_string(n) + " drafts, more than " +
+                         std::to_string(MS_MAX_TREE_TOKENS));
+      return MS_ERR_PLAN;
+    }
+    if (c + n >= (int64_t(1) << 30)) {
+      ms_host::set_error("ms_tree_plan_build: context too long");
+      return MS_ERR_PLAN;
+    }
+    if (tlen * block_size < c + n) {
+      ms_host::set_error(who + " needs " + std::to_string((c + n + block_size - 1) / block_size) +
+                         " blocks but its table has " + std::to_string(tlen));
+      return MS_ERR_PLAN;
+    }
+    const int32_t* par = parents + parent_at;
+    for (int64_t k = 0; k < n; ++k) {
+      const int32_t p = par[k];
+      if (p < -2 || p >= k || (p >= 0 && par[p] == -2)) {
+        ms_host::set_error(who + ": draft " + std::to_string(k) + " has parent " +
+                           std::to_string(p) +
+                           " (want an earlier draft in use, -1 for the last cached token, or -2 "
+                           "for an unused position)");
+        return MS_ERR_PLAN;
+      }
+    }
+    parents_at[i] = parent_at;
+    parent_at += n;
+    mask_at[i] = mask_words;
+    mask_words += n * ((n + 31) / 32);
+    for (int64_t t0 = 0; t0 < n; t0 += kTileTokens) {
+      const int nq = static_cast<int>(std::min<int64_t>(kTileTokens, n - t0));
+      const int pages = static_cast<int>((c + t0 + nq + block_size - 1) / block_size);
+      tiles.push_back({i, static_cast<int>(t0), nq, 0, pages, -1});
+      total_pages += pages;
+    }
+  }
+
+  // Split size: the smallest multiple of 8 pages whose items fit one resident wave; when the tiles
+  // alone exceed it, tiles longer than the pages per CTA slot are cut to about that size.
+  int split = pages_per_split;
+  if (split == 0) {
+    const int64_t target = std::max<int64_t>(
+        1, static_cast<int64_t>(num_sms) * kTreeCtasPerSm / kAssumedKvHeads);
+    auto items_at = [&](int64_t p) {
+      int64_t items = 0;
+      for (const TreeItem& t : tiles) items += (t.pe + p - 1) / p;
+      return items;
+    };
+    if (items_at(kMaxSplitPages) > target) {
+      const int64_t per_slot = (total_pages + target - 1) / target;
+      split = static_cast<int>(std::min<int64_t>(
+          kMaxSplitPages, std::max<int64_t>(kMinSplitPages, (per_slot + 7) / 8 * 8)));
+    } else {
+      int lo = kMinSplitPages / 8, hi = kMaxSplitPages / 8;
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (items_at(mid * 8) <= target) hi = mid; else lo = mid + 1;
+      }
+      split = lo * 8;
+    }
+  }
+
+  std::vector<TreeItem> items, comb;
+  int64_t part_rows = 0;
+  for (const TreeItem& t : tiles) {
+    const int ns = (t.pe + split - 1) / split;
+    if (ns <= 1) {
+      items.push_back(t);
+      continue;
+    }
+    const int rows = 2 * t.n_q;
+    if (part_rows + static_cast<int64_t>(ns) * rows >= (int64_t(1) << 31)) {
+      ms_host::set_error("ms_tree_plan_build: too many partial rows");
+      return MS_ERR_PLAN;
+    }
+    const int base = t.pe / ns, rem = t.pe % ns;
+    int pb = 0;
+    for (int s = 0; s < ns; ++s) {
+      const int len = base + (s < rem ? 1 : 0);
+      items.push_back({t.seq, t.tok0, t.n_q, pb, pb + len,
+                       static_cast<int>(part_rows + static_cast<int64_t>(s) * rows)});
+      pb += len;
+    }
+    comb.push_back({t.seq, t.tok0, t.n_q, static_cast<int>(part_rows), ns, 0});
+    part_rows += static_cast<int64_t>(ns) * rows;
+  }
+  std::stable_sort(items.begin(), items.end(), [](const TreeItem& x, const TreeItem& y) {
+    return (x.pe - x.pb) > (y.pe - y.pb);
+  });
+
+  const int64_t off_tables = round4(static_cast<int64_t>(num_seqs) * kRec);
+  const int64_t off_tile = off_tables + round4(total_entries);
+  const int64_t off_combine = off_tile + round4(static_cast<int64_t>(items.size()) * kRec);
+  const int64_t off_masks = off_combine + round4(static_cast<int64_t>(comb.size()) * kRec);
+  const int64_t total = off_masks + round4(mask_words);
+  if (total > out_capacity) {
+    ms_host::set_error("ms_tree_plan_build: output buffer holds " + std::to_string(out_capacity) +
+                       " ints, plan needs " + std::to_string(total));
+    return MS_ERR_CAPACITY;
+  }
+  if (total >= (int64_t(1) << 31)) {
+    ms_host::set_error("ms_tree_plan_build: plan larger than 2^31 ints");
+    return MS_ERR_PLAN;
+  }
+  std::memset(out, 0, sizeof(int32_t) * total);
+  for (int i = 0; i < num_seqs; ++i) {
+    const int n = num_new[i], words = (n + 31) / 32;
+    int32_t* r = out + static_cast<int64_t>(i) * kRec;
+    r[0] = flat_start[i];
+    r[1] = n;
+    r[2] = num_cached[i];
+    r[3] = num_cached[i] + n;
+    r[4] = static_cast<int32_t>(table_offsets[i]);
+    r[5] = static_cast<int32_t>(table_offsets[i + 1] - table_offsets[i]);
+    r[6] = static_cast<int32_t>(off_masks + mask_at[i]);
+    r[7] = words;
+    const int32_t* par = parents + parents_at[i];
+    uint32_t* mask = reinterpret_cast<uint32_t*>(out + off_masks + mask_at[i]);
+    for (int k = 0; k < n; ++k) {
+      if (par[k] == -2) continue;
+      uint32_t* row = mask + static_cast<int64_t>(k) * words;
+      if (par[k] >= 0)
+        std::memcpy(row, mask + static_cast<int64_t>(par[k]) * words, sizeof(uint32_t) * words);
+      row[k >> 5] |= 1u << (k & 31);
+    }
+  }
+  if (total_entries > 0) std::memcpy(out + off_tables, tables, sizeof(int32_t) * total_entries);
+  auto put = [&](int64_t off, const std::vector<TreeItem>& v) {
+    for (size_t k = 0; k < v.size(); ++k) {
+      int32_t* r = out + off + static_cast<int64_t>(k) * kRec;
+      r[0] = v[k].seq;
+      r[1] = v[k].tok0;
+      r[2] = v[k].n_q;
+      r[3] = v[k].pb;
+      r[4] = v[k].pe;
+      r[5] = v[k].part_row;
+    }
+  };
+  put(off_tile, items);
+  put(off_combine, comb);
+
+  info->num_seqs = num_seqs;
+  info->num_tokens = num_tokens;
+  info->n_tile_items = static_cast<int32_t>(items.size());
+  info->n_combine = static_cast<int32_t>(comb.size());
+  info->off_tables = static_cast<int32_t>(off_tables);
+  info->off_decode = static_cast<int32_t>(off_tile);
+  info->off_tile = static_cast<int32_t>(off_tile);
+  info->off_tc = static_cast<int32_t>(off_combine);
+  info->off_combine = static_cast<int32_t>(off_combine);
+  info->total_ints = static_cast<int32_t>(total);
+  info->pages_per_split = split;
+  info->part_rows = part_rows;
+  info->total_pages = total_pages;
+  int combine_tokens_max = 0;
+  for (const TreeItem& c : comb) combine_tokens_max = std::max(combine_tokens_max, c.n_q);
+  info->combine_tokens_max = combine_tokens_max;
+  info->workspace_bytes_per_kv_head = part_rows * (128 + 1) * 4;
+  return MS_OK;
+}
+
+extern "C" int ms_tree_plan_build(int32_t num_seqs, const int32_t* flat_start,
+                                  const int32_t* num_new, const int32_t* num_cached,
+                                  const int64_t* table_offsets, const int32_t* tables,
+                                  const int32_t* parents, int32_t num_tokens, int32_t block_size,
+                                  int32_t num_sms, int32_t pages_per_split, int32_t* out,
+                                  int64_t out_capacity, MsPlanInfo* info) {
+  return guarded("ms_tree_plan_build", [&] {
+    return tree_plan_build(num_seqs, flat_start, num_new, num_cached, table_offsets, tables, parents,
+                           num_tokens, block_size, num_sms, pages_per_split, out, out_capacity, info);
+  });
+}

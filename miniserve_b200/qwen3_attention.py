@@ -17,7 +17,7 @@ from torch import Tensor, nn
 
 from . import _capi
 from .attention import AttentionMetadata, _rows, _stream, attend
-from .kv_pool import HEAD_DIM, check_layer_views
+from .kv_pool import HEAD_DIM, check_layer_views, is_kv8
 
 # Smallest step (tokens) for which ``fused_qkv="auto"`` takes kernel E: measured on a B200 against
 # cuBLAS + kernel A (its 16-byte form) over 28 layers, kernel E is 0.74-0.93x from 64 to 1536
@@ -50,8 +50,9 @@ def qk_norm_rope_scatter(
 ) -> Tensor:
     """Kernel A: returns normalised, rotated q ``[T, H, 128]``; writes k (normalised, rotated)
     and v into their pool slots.  ``cos``/``sin`` are per-token rows ``[T, 128]`` fp32, or the
-    whole table when ``positions`` is given (qwen3.py:94-98 + backends.py:159-160)."""
-    nb, kvh = check_layer_views(k_cache, v_cache)
+    whole table when ``positions`` is given (qwen3.py:94-98 + backends.py:159-160).  Into an 8-bit
+    pool the rows are quantised as they are written."""
+    nb, kvh = check_layer_views(k_cache, v_cache, kv8=True)
     t = int(qkv.shape[0])
     width = (num_heads + 2 * kvh) * HEAD_DIM
     if qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1 or qkv.dtype != torch.bfloat16:
@@ -72,12 +73,17 @@ def qk_norm_rope_scatter(
             raise ValueError("positions must be int64")
         pos_ptr, max_pos = positions.data_ptr(), int(cos.shape[0])
     lib = _capi.load()
-    rc = lib.ms_qk_norm_rope_scatter(
+    args = (
         qkv.data_ptr(), int(qkv.stride(0)), t, num_heads, kvh, q_weight.data_ptr(),
         k_weight.data_ptr(), float(eps), cos.data_ptr(), sin.data_ptr(), int(cos.stride(0)),
         pos_ptr, max_pos, slot_mapping.data_ptr(), q_out.data_ptr(), _rows(q_out, "q_out"),
-        k_cache.data_ptr(), v_cache.data_ptr(), nb, _stream(qkv.device),
     )
+    if is_kv8(k_cache):
+        with torch.cuda.device(k_cache.device):
+            rc = lib.ms_qk_norm_rope_scatter_kv8(*args, k_cache.data_ptr(), nb, _stream(qkv.device))
+    else:
+        rc = lib.ms_qk_norm_rope_scatter(*args, k_cache.data_ptr(), v_cache.data_ptr(), nb,
+                                         _stream(qkv.device))
     _capi.check(rc, "qk_norm_rope_scatter")
     return q_out
 
@@ -174,7 +180,8 @@ class Qwen3Attention(nn.Module):
     ) -> Tensor:
         t = x.shape[0]
         fused = self.fused_qkv is True or (self.fused_qkv == "auto" and t >= FUSED_QKV_MIN_TOKENS)
-        if fused and isinstance(self.qkv_proj, nn.Linear):
+        # Kernel E writes a bf16 pool only; an 8-bit pool takes the projection and kernel A.
+        if fused and isinstance(self.qkv_proj, nn.Linear) and not is_kv8(k_cache):
             q = qkv_proj_norm_rope_scatter(
                 x, self.qkv_proj.weight, self.q_norm.weight, self.k_norm.weight, self.q_norm.eps,
                 cos, sin, meta.slot_mapping, k_cache, v_cache, self.num_heads,

@@ -14,7 +14,7 @@
  *
  * 8-bit pool layout (one layer, the *_kv8 entry points): [num_blocks][num_kv_heads][4128 bytes]: K's
  * 16 rows of 128 e4m3 codes, V's 16 rows, K's 16 exponent bytes, V's 16.  Row t's 16-byte chunk i sits
- * at chunk i ^ (t % 8).  A row with exponent byte b stands for its codes times 2^(b - 127); b - 127 is the
+ * at chunk i ^ (t % 2 + 2 (t / 4)).  A row with exponent byte b stands for its codes times 2^(b - 127); b - 127 is the
  * smallest integer in [-100, 120] that brings the row's largest magnitude to at most 448, and b = 255
  * marks a row that held a NaN or an infinity: it stands for NaN.  `pool` is the layer's first byte,
  * 16-byte aligned.

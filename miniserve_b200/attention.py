@@ -77,7 +77,7 @@ class AttentionMetadata:
     plan: Tensor  # packed int32 plan on the device
     info: _capi.MsPlanInfo  # host-side description of the plan
     num_tokens: int
-    _workspace: dict[tuple[int, int], Tensor] = field(default_factory=dict, repr=False)
+    _workspace: dict[tuple[torch.device, int], Tensor] = field(default_factory=dict, repr=False)
     _num_sms: int = field(default=148, repr=False)
     _pages_per_split: int = field(default=0, repr=False)
     kv8: _capi.MsKv8Info = field(default_factory=_capi.MsKv8Info, repr=False)  # 8-bit pool part
@@ -120,14 +120,14 @@ class AttentionMetadata:
     def workspace(self, num_kv_heads: int, device: torch.device, kv8: bool = False) -> Tensor | None:
         """Scratch for this step (allocated once, reused by every layer): split-KV partials and,
         for an 8-bit pool, the expanded pages of tensor-core items."""
-        need = int(self.info.workspace_bytes_per_kv_head) * num_kv_heads
-        if kv8:
+        if kv8 and self.kv8.n_pages:
             need = int(_capi.load().ms_kv8_workspace_bytes(C.byref(self.info), C.byref(self.kv8),
                                                            num_kv_heads))
+        else:
+            need = int(self.info.workspace_bytes_per_kv_head) * num_kv_heads
         if need == 0:
             return None
-        # A tensor's device always carries its index.
-        key = (str(device), -num_kv_heads if kv8 else num_kv_heads)
+        key = (device, -num_kv_heads if kv8 else num_kv_heads)  # a tensor's device has its index
         ws = self._workspace.get(key)
         if ws is None:
             ws = torch.empty(need, dtype=torch.uint8, device=device)
@@ -338,7 +338,9 @@ def _upload_plan(packed: np.ndarray, device: torch.device) -> Tensor:
 
 
 def _stream(device: torch.device) -> int:
-    return int(torch.cuda.current_stream(device).cuda_stream)
+    """The current stream of a tensor's device, as the library takes it (torch's own accessor of the
+    raw handle: a Stream object per call costs two microseconds)."""
+    return int(torch._C._cuda_getCurrentRawStream(device.index))
 
 
 def _rows(t: Tensor, name: str) -> int:
@@ -357,12 +359,11 @@ def kv_scatter(k: Tensor, v: Tensor, slot_mapping: Tensor, k_cache: Tensor, v_ca
     t = int(k.shape[0])
     lib = _capi.load()
     if is_kv8(k_cache):
-        _check_rows_args(k, v, slot_mapping, k_cache, kvh)
-        with _on_device(k_cache.device):
-            rc = lib.ms_kv_scatter_kv8(
-                k.data_ptr(), _rows(k, "k"), v.data_ptr(), _rows(v, "v"), t, kvh,
-                slot_mapping.data_ptr(), k_cache.data_ptr(), nb, _stream(k.device),
-            )
+        dev = _check_rows_args(k, v, slot_mapping, k_cache, kvh)
+        rc = _on_own_device(
+            lib.ms_kv_scatter_kv8, dev, k.data_ptr(), _rows(k, "k"), v.data_ptr(), _rows(v, "v"), t,
+            kvh, slot_mapping.data_ptr(), k_cache.data_ptr(), nb, _stream(dev),
+        )
     else:
         rc = lib.ms_kv_scatter(
             k.data_ptr(), _rows(k, "k"), v.data_ptr(), _rows(v, "v"), t, kvh,
@@ -371,23 +372,30 @@ def kv_scatter(k: Tensor, v: Tensor, slot_mapping: Tensor, k_cache: Tensor, v_ca
     _capi.check(rc, "kv_scatter")
 
 
-def _on_device(device: torch.device):
-    """The library launches on the current device: make it the tensors' own."""
-    return torch.cuda.device(device)
+def _on_own_device(fn, device: torch.device, *args) -> int:
+    """Call the library, which launches on the current device, with the tensors' own device current."""
+    if torch.cuda.current_device() == device.index:
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
 
 
-def _check_rows_args(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, kvh: int) -> None:
-    if k.dim() != 3 or k.shape != v.shape or k.shape[1] != kvh:
+def _check_rows_args(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, kvh: int) -> torch.device:
+    """Rows and their slots fit each other and the pool; returns the pool's device."""
+    shape = k.shape
+    if len(shape) != 3 or shape != v.shape or shape[1] != kvh:
         raise ValueError(f"k and v must both be [T, {kvh}, {HEAD_DIM}]")
     if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
         raise ValueError("slots must be a contiguous int64 vector")
-    if slots.shape[0] != k.shape[0]:
-        raise ValueError(f"{k.shape[0]} rows but {slots.shape[0]} slots")
-    if not k_cache.is_cuda:
+    if slots.shape[0] != shape[0]:
+        raise ValueError(f"{shape[0]} rows but {slots.shape[0]} slots")
+    dev = k_cache.device
+    if dev.type != "cuda":
         raise RuntimeError("miniserve_b200 attention runs on CUDA only (no CPU fallback)")
-    for t, name in ((k, "k"), (v, "v"), (slots, "slots")):
-        if t.device != k_cache.device:
-            raise ValueError(f"{name} is on {t.device}, the pool on {k_cache.device}")
+    if k.device != dev or v.device != dev or slots.device != dev:
+        raise ValueError(f"k, v and slots are on {k.device}, {v.device} and {slots.device}, "
+                         f"the pool on {dev}")
+    return dev
 
 
 def kv_gather(slots: Tensor, k_cache: Tensor, v_cache: Tensor, k_out: Tensor | None = None,
@@ -402,23 +410,22 @@ def kv_gather(slots: Tensor, k_cache: Tensor, v_cache: Tensor, k_out: Tensor | N
     values again.  A slot outside the pool reads as zeros (and sets the device status bit).
     """
     nb, kvh = check_layer_views(k_cache, v_cache, kv8=True)
-    n = int(slots.shape[0]) if slots.dim() == 1 else -1
-    shape = (max(n, 0), kvh, HEAD_DIM)
+    n = int(slots.shape[0]) if slots.dim() == 1 else 0
+    shape = (n, kvh, HEAD_DIM)
     if k_out is None:
         k_out = torch.empty(shape, dtype=torch.bfloat16, device=slots.device)
     if v_out is None:
         v_out = torch.empty(shape, dtype=torch.bfloat16, device=slots.device)
-    _check_rows_args(k_out, v_out, slots, k_cache, kvh)
-    k_stride, v_stride = _rows(k_out, "k_out"), _rows(v_out, "v_out")
+    dev = _check_rows_args(k_out, v_out, slots, k_cache, kvh)
+    outs = (k_out.data_ptr(), _rows(k_out, "k_out"), v_out.data_ptr(), _rows(v_out, "v_out"),
+            _stream(dev))
     lib = _capi.load()
-    with _on_device(k_cache.device):
-        stream = _stream(k_cache.device)
-        if is_kv8(k_cache):
-            rc = lib.ms_kv_gather_kv8(slots.data_ptr(), n, kvh, k_cache.data_ptr(), nb,
-                                      k_out.data_ptr(), k_stride, v_out.data_ptr(), v_stride, stream)
-        else:
-            rc = lib.ms_kv_gather(slots.data_ptr(), n, kvh, k_cache.data_ptr(), v_cache.data_ptr(),
-                                  nb, k_out.data_ptr(), k_stride, v_out.data_ptr(), v_stride, stream)
+    if is_kv8(k_cache):
+        rc = _on_own_device(lib.ms_kv_gather_kv8, dev, slots.data_ptr(), n, kvh, k_cache.data_ptr(),
+                            nb, *outs)
+    else:
+        rc = _on_own_device(lib.ms_kv_gather, dev, slots.data_ptr(), n, kvh, k_cache.data_ptr(),
+                            v_cache.data_ptr(), nb, *outs)
     _capi.check(rc, "kv_gather")
     return k_out, v_out
 
@@ -436,9 +443,7 @@ def attend(q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: AttentionMetadata,
     h = int(q.shape[1])
     lib = _capi.load()
     if is_kv8(k_cache) or meta.tree is not None:
-        _check_attend_args(q, out, k_cache, meta)
-        with _on_device(k_cache.device):
-            _attend_parts(lib, q, k_cache, v_cache, meta, scale, out, nb, kvh)
+        _attend_parts(lib, q, k_cache, v_cache, meta, float(scale), out, nb, kvh)
         return out
     ws = meta.workspace(kvh, q.device)
     rc = lib.ms_paged_attention(
@@ -451,44 +456,43 @@ def attend(q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: AttentionMetadata,
     return out
 
 
-def _check_attend_args(q: Tensor, out: Tensor, k_cache: Tensor, meta: AttentionMetadata) -> None:
-    if not k_cache.is_cuda:
-        raise RuntimeError("miniserve_b200 attention runs on CUDA only (no CPU fallback)")
-    for t, name in ((q, "q"), (out, "out"), (meta.plan, "meta")):
-        if t.device != k_cache.device:
-            raise ValueError(f"{name} is on {t.device}, the pool on {k_cache.device}")
-    if q.shape[0] < meta.num_tokens or out.shape[0] < meta.num_tokens:
-        raise ValueError(f"q and out must have the step's {meta.num_tokens} rows")
-    if out.shape[1:] != q.shape[1:]:
-        raise ValueError("out must have q's heads")
-
-
 def _attend_parts(lib, q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: AttentionMetadata,
                   scale: float, out: Tensor, nb: int, kvh: int) -> None:
     """The causal part and the draft trees of a step, over either kind of pool."""
+    dev = k_cache.device
+    if dev.type != "cuda":
+        raise RuntimeError("miniserve_b200 attention runs on CUDA only (no CPU fallback)")
+    if q.device != dev or out.device != dev or meta.plan.device != dev:
+        raise ValueError(f"q, out and meta are on {q.device}, {out.device} and {meta.plan.device}, "
+                         f"the pool on {dev}")
+    shape = q.shape
+    if shape != out.shape and shape[1:] != out.shape[1:]:
+        raise ValueError("out must have q's heads")
+    if shape[0] < meta.num_tokens or out.shape[0] < meta.num_tokens:
+        raise ValueError(f"q and out must have the step's {meta.num_tokens} rows")
     kv8 = is_kv8(k_cache)
-    h, stream = int(q.shape[1]), _stream(q.device)
-    q_args = (q.data_ptr(), _rows(q, "q"), out.data_ptr(), _rows(out, "out"), h, kvh)
-    parts = [meta] if meta.tree is None else [meta, meta.tree]
-    for part in parts:
-        info = part.info
-        if part.tree is not None and not (info.n_decode_items or info.n_tile_items or info.n_tc_items):
-            continue  # every sequence is a tree
-        is_tree = part is meta.tree
-        ws = part.workspace(kvh, q.device, kv8=kv8 and not is_tree)
-        scratch = (ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0)
-        if is_tree:
-            rc = lib.ms_tree_attention(
-                *q_args, k_cache.data_ptr(), None if kv8 else v_cache.data_ptr(), nb,
-                part.plan.data_ptr(), C.byref(info), *scratch, float(scale), stream)
-        elif kv8:
-            rc = lib.ms_paged_attention_kv8(
-                *q_args, k_cache.data_ptr(), nb, part.plan.data_ptr(), C.byref(info),
-                C.byref(part.kv8), *scratch, float(scale), stream)
+    stream = _stream(dev)
+    q_args = (q.data_ptr(), _rows(q, "q"), out.data_ptr(), _rows(out, "out"), int(shape[1]), kvh)
+    info, tree = meta.info, meta.tree
+    if tree is None or info.n_decode_items or info.n_tile_items or info.n_tc_items:
+        ws = meta.workspace(kvh, dev, kv8)
+        ws_args = (0, 0) if ws is None else (ws.data_ptr(), ws.numel())
+        if kv8:
+            rc = _on_own_device(
+                lib.ms_paged_attention_kv8, dev, *q_args, k_cache.data_ptr(), nb,
+                meta.plan.data_ptr(), C.byref(info), C.byref(meta.kv8), *ws_args, scale, stream)
         else:
-            rc = lib.ms_paged_attention(
-                *q_args, k_cache.data_ptr(), v_cache.data_ptr(), nb, part.plan.data_ptr(),
-                C.byref(info), *scratch, float(scale), stream)
+            rc = _on_own_device(
+                lib.ms_paged_attention, dev, *q_args, k_cache.data_ptr(), v_cache.data_ptr(), nb,
+                meta.plan.data_ptr(), C.byref(info), *ws_args, scale, stream)
+        _capi.check(rc, "paged_attention")
+    if tree is not None:
+        ws = tree.workspace(kvh, dev)
+        ws_args = (0, 0) if ws is None else (ws.data_ptr(), ws.numel())
+        rc = _on_own_device(
+            lib.ms_tree_attention, dev, *q_args, k_cache.data_ptr(),
+            None if kv8 else v_cache.data_ptr(), nb, tree.plan.data_ptr(), C.byref(tree.info),
+            *ws_args, scale, stream)
         _capi.check(rc, "paged_attention")
 
 

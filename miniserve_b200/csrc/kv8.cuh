@@ -14,9 +14,9 @@
 //
 // Layout of a layer: [num_blocks][kv_heads][4128 bytes]; the 4128 bytes of a (block, head) are K's
 // 16 rows of 128 codes, V's 16 rows, K's 16 exponent bytes, V's 16.  One copy of 4128 contiguous bytes brings
-// everything an attention step needs, and the 16-byte chunks of row t are stored XOR-swizzled
-// (chunk i at position i ^ (t % 8)), so the copy needs no tensor map and ldmatrix reads it without
-// bank conflicts.
+// everything an attention step needs, and the 16-byte chunks of row t are stored XOR-swizzled (chunk
+// i at position i ^ (t % 2 + 2 (t / 4))), so the copy needs no tensor map and ldmatrix reads it
+// without bank conflicts, in the order of tokens that gives a lane four neighbouring ones.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -32,9 +32,13 @@ constexpr int kPage8Bytes = kExp8Off + 2 * kBlockTokens;      // 4128
 constexpr int kExpBias = 127, kExpMin = -100, kExpMax = 120;
 constexpr unsigned kExpNan = 255;
 
+// What the chunk positions of token `tok` are XORed with: distinct over the tokens 0, 1, 4, 5, 8, 9,
+// 12, 13 that one ldmatrix reads, and the same for tok and tok + 2 there.
+__device__ __forceinline__ int code_swizzle8(int tok) { return (tok & 1) | ((tok >> 1) & 6); }
+
 // Byte offset of 16-byte chunk `chunk` of token `tok` inside one K or V code block.
 __device__ __forceinline__ int code_off8(int tok, int chunk) {
-  return tok * kRow8Bytes + ((chunk ^ (tok & 7)) << 4);
+  return tok * kRow8Bytes + ((chunk ^ code_swizzle8(tok)) << 4);
 }
 
 // Exponent byte of a row from the largest magnitude's bf16 bits (NaN and infinity >= 0x7f80).
@@ -166,53 +170,60 @@ struct Scatter8Args {
   int num_kv;
 };
 
-// Rows in order (token, K heads, V heads); a warp takes 2 kPairs consecutive rows, two at a time
-// (half-warp per row).  kVec16: rows are 16-byte aligned; else each lane loads its 8 values as two
-// 8-byte words.
-template <int kWarps, int kPairs, bool kVec16>
+// Which rows a warp of the row-copy kernels moves: rows r = 0 .. 2 KVH - 1 of a token are its K heads,
+// then its V heads; a warp takes the same two neighbouring rows (one per half-warp, 8 values per lane) of
+// kTokens consecutive tokens, so its index is divided once and its kTokens loads are in flight
+// together.
+struct RowPair {
+  long long t0;
+  int h;
+  bool is_v;
+};
+__device__ __forceinline__ RowPair row_pair(unsigned warp, int num_kv, int tokens, int half) {
+  const unsigned tg = warp / static_cast<unsigned>(num_kv);
+  const int r = 2 * static_cast<int>(warp - tg * num_kv) + half;
+  RowPair p;
+  p.t0 = static_cast<long long>(tg) * tokens;
+  p.is_v = r >= num_kv;
+  p.h = p.is_v ? r - num_kv : r;
+  return p;
+}
+
+// kVec16: rows are 16-byte aligned; else each lane loads its 8 values as two 8-byte words.
+template <int kWarps, int kTokens, bool kVec16>
 __global__ void __launch_bounds__(kWarps * 32) kv_scatter8_kernel(const Scatter8Args a,
                                                                   unsigned* status) {
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, l16 = lane & 15;
-  const int rows_per_tok = 2 * a.num_kv;
-  const long long rows = static_cast<long long>(a.num_tokens) * rows_per_tok;
-  const long long row0 =
-      (static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * (2 * kPairs) + (lane >> 4);
-  uint4 x[kPairs];
-  long long slot[kPairs];
-  int r_in[kPairs];
+  const RowPair rp =
+      row_pair(blockIdx.x * kWarps + (threadIdx.x >> 5), a.num_kv, kTokens, lane >> 4);
+  if (rp.t0 >= a.num_tokens) return;
+  const int cnt = static_cast<int>(min(static_cast<long long>(kTokens), a.num_tokens - rp.t0));
+  const long long stride = rp.is_v ? a.v_row_stride : a.k_row_stride;
+  const __nv_bfloat16* src = (rp.is_v ? a.v : a.k) + rp.t0 * stride + rp.h * kHeadDim + l16 * 8;
+  uint4 x[kTokens];
+  long long slot[kTokens];
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) {
-    const long long row = row0 + 2 * i;
+  for (int i = 0; i < kTokens; ++i) {
     x[i] = make_uint4(0u, 0u, 0u, 0u);
     slot[i] = -1;
-    r_in[i] = -1;
-    if (row >= rows) continue;
-    const long long t = row / rows_per_tok;
-    const int r = static_cast<int>(row - t * rows_per_tok);
-    const bool is_v = r >= a.num_kv;
-    const __nv_bfloat16* src = (is_v ? a.v + t * a.v_row_stride + (r - a.num_kv) * kHeadDim
-                                     : a.k + t * a.k_row_stride + r * kHeadDim) +
-                               l16 * 8;
+    if (i >= cnt) continue;
+    slot[i] = a.slots[rp.t0 + i];
     if constexpr (kVec16) {
-      x[i] = *reinterpret_cast<const uint4*>(src);
+      x[i] = *reinterpret_cast<const uint4*>(src + i * stride);
     } else {
-      const uint2 lo = *reinterpret_cast<const uint2*>(src);
-      const uint2 hi = *reinterpret_cast<const uint2*>(src + 4);
+      const uint2 lo = *reinterpret_cast<const uint2*>(src + i * stride);
+      const uint2 hi = *reinterpret_cast<const uint2*>(src + i * stride + 4);
       x[i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
     }
-    slot[i] = a.slots[t];
-    r_in[i] = r;
   }
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) {
+  for (int i = 0; i < kTokens; ++i) {
     const bool ok = slot[i] >= 0 && slot[i] < a.num_slots;
-    if (r_in[i] >= 0 && !ok && l16 == 0) atomicOr(status, kErrSlot);
-    const bool is_v = r_in[i] >= a.num_kv;
-    const int h = is_v ? r_in[i] - a.num_kv : r_in[i];
-    uint8_t* page = ok ? a.pool + page8_off(slot[i], h, a.num_kv) : a.pool;
-    store_row8_l16(page, is_v, static_cast<int>(slot[i] & 15), x[i], l16, ok);
+    if (i < cnt && !ok && l16 == 0) atomicOr(status, kErrSlot);
+    uint8_t* page = ok ? a.pool + page8_off(slot[i], rp.h, a.num_kv) : a.pool;
+    store_row8_l16(page, rp.is_v, static_cast<int>(slot[i] & 15), x[i], l16, ok);
   }
 }
 
@@ -231,68 +242,58 @@ struct GatherArgs {
   int num_kv;
 };
 
-// Rows by slot to [T, KVH, 128] bf16.  Rows in order (token, K heads, V heads), half-warp per row, 8
-// values per lane; a slot outside the pool reads as zeros and sets the status bit.
-template <bool kKv8, int kWarps, int kPairs>
+// Rows by slot to [T, KVH, 128] bf16; a slot outside the pool reads as zeros and sets the status bit.
+template <bool kKv8, int kWarps, int kTokens>
 __global__ void __launch_bounds__(kWarps * 32) kv_gather_kernel(const GatherArgs a,
                                                                 unsigned* status) {
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, l16 = lane & 15;
-  const int rows_per_tok = 2 * a.num_kv;
-  const long long rows = static_cast<long long>(a.num_tokens) * rows_per_tok;
-  const long long row0 =
-      (static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * (2 * kPairs) + (lane >> 4);
-  long long slot[kPairs];
+  const RowPair rp =
+      row_pair(blockIdx.x * kWarps + (threadIdx.x >> 5), a.num_kv, kTokens, lane >> 4);
+  if (rp.t0 >= a.num_tokens) return;
+  const int cnt = static_cast<int>(min(static_cast<long long>(kTokens), a.num_tokens - rp.t0));
+  long long slot[kTokens];
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) {
-    const long long row = row0 + 2 * i;
-    slot[i] = row < rows ? a.slots[row / rows_per_tok] : 0;
-  }
-  uint4 x[kPairs];
-  int b[kPairs];
+  for (int i = 0; i < kTokens; ++i) slot[i] = i < cnt ? a.slots[rp.t0 + i] : 0;
+  uint4 x[kTokens];
+  int b[kTokens];
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) {
-    const long long row = row0 + 2 * i;
+  for (int i = 0; i < kTokens; ++i) {
     x[i] = make_uint4(0u, 0u, 0u, 0u);
     b[i] = 0;
-    if (row >= rows) continue;
+    if (i >= cnt) continue;
     if (slot[i] < 0 || slot[i] >= a.num_slots) {
       if (l16 == 0) atomicOr(status, kErrSlot);
       continue;
     }
-    const int r = static_cast<int>(row % rows_per_tok);
-    const bool is_v = r >= a.num_kv;
-    const int h = is_v ? r - a.num_kv : r;
     if constexpr (kKv8) {
-      const uint8_t* page = static_cast<const uint8_t*>(a.pool) + page8_off(slot[i], h, a.num_kv);
+      const uint8_t* page =
+          static_cast<const uint8_t*>(a.pool) + page8_off(slot[i], rp.h, a.num_kv);
       const int tok = static_cast<int>(slot[i] & 15);
       const uint2 c = *reinterpret_cast<const uint2*>(
-          page + (is_v ? kCodes8Bytes : 0) + code_off8(tok, l16 >> 1) + (l16 & 1) * 8);
+          page + (rp.is_v ? kCodes8Bytes : 0) + code_off8(tok, l16 >> 1) + (l16 & 1) * 8);
       x[i].x = c.x;
       x[i].y = c.y;
-      b[i] = page[kExp8Off + (is_v ? kBlockTokens : 0) + tok];
+      b[i] = page[kExp8Off + (rp.is_v ? kBlockTokens : 0) + tok];
     } else {
       x[i] = *reinterpret_cast<const uint4*>(
-          static_cast<const __nv_bfloat16*>(a.pool) + (is_v ? 2 * kBlockTokens * 64 : 0) +
-          pool_offset(slot[i], h, l16 * 8, a.block_stride, a.head_stride));
+          static_cast<const __nv_bfloat16*>(a.pool) + (rp.is_v ? 2 * kBlockTokens * 64 : 0) +
+          pool_offset(slot[i], rp.h, l16 * 8, a.block_stride, a.head_stride));
     }
   }
+  const long long stride = rp.is_v ? a.v_row_stride : a.k_row_stride;
+  __nv_bfloat16* dst = (rp.is_v ? a.v : a.k) + rp.t0 * stride + rp.h * kHeadDim + l16 * 8;
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) {
-    const long long row = row0 + 2 * i;
-    if (row >= rows) continue;
-    const long long t = row / rows_per_tok;
-    const int r = static_cast<int>(row - t * rows_per_tok);
+  for (int i = 0; i < kTokens; ++i) {
+    if (i >= cnt) break;
     if constexpr (kKv8) {
       const float s = row_scale8(b[i]);
       const uint2 c = make_uint2(x[i].x, x[i].y);
       expand4(c.x, s, x[i].x, x[i].y);
       expand4(c.y, s, x[i].z, x[i].w);
     }
-    __nv_bfloat16* dst = r >= a.num_kv ? a.v + t * a.v_row_stride + (r - a.num_kv) * kHeadDim
-                                       : a.k + t * a.k_row_stride + r * kHeadDim;
-    *reinterpret_cast<uint4*>(dst + l16 * 8) = x[i];
+    *reinterpret_cast<uint4*>(dst + i * stride) = x[i];
   }
 }
 

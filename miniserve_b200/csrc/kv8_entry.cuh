@@ -16,16 +16,16 @@ int check_pool8(const char* what, const void* pool, int num_blocks, int num_kv) 
   return MS_OK;
 }
 
-// Grid of the row-copy kernels: two rows per warp instruction, kPairs of them per warp.  Enough rows
-// for every SM's warps take four pairs per warp (four loads in flight per lane); fewer take one, so
-// that a decode step's few rows spread over more SMs.
+// Grid of the row-copy kernels (see row_pair): a warp takes 4 tokens where that leaves every SM enough
+// warps, else one, so that a decode step's few rows spread over more SMs.
 constexpr int kCopyWarps = 8;
+constexpr int64_t kMaxCopyWarps = int64_t(1) << 31;  // warp indices are 32-bit
 template <typename Few, typename Many>
-cudaError_t launch_rows(int64_t rows, int sms, Few few, Many many) {
-  const int64_t per4 = kCopyWarps * 8, per1 = kCopyWarps * 2;
-  if ((rows + per4 - 1) / per4 >= 4 * static_cast<int64_t>(sms))
-    return many(static_cast<unsigned>((rows + per4 - 1) / per4));
-  return few(static_cast<unsigned>((rows + per1 - 1) / per1));
+cudaError_t launch_rows(int64_t tokens, int num_kv, int sms, Few few, Many many) {
+  const int64_t w4 = (tokens + 3) / 4 * num_kv, w1 = tokens * num_kv;
+  if (w4 >= static_cast<int64_t>(16) * sms)
+    return many(static_cast<unsigned>((w4 + kCopyWarps - 1) / kCopyWarps));
+  return few(static_cast<unsigned>((w1 + kCopyWarps - 1) / kCopyWarps));
 }
 
 int check_attention(const char* what, const void* q, int64_t q_row_stride, const void* out,
@@ -111,8 +111,7 @@ extern "C" int ms_kv_scatter_kv8(const void* k, int64_t k_row_stride, const void
     set_error("ms_kv_scatter_kv8: null pointer, stride or alignment");
     return MS_ERR_ARG;
   }
-  const int64_t rows = static_cast<int64_t>(num_tokens) * 2 * num_kv_heads;
-  if (rows > (int64_t(1) << 33)) {
+  if (static_cast<int64_t>(num_tokens) * num_kv_heads > kMaxCopyWarps) {
     set_error("ms_kv_scatter_kv8: batch too large");
     return MS_ERR_ARG;
   }
@@ -137,9 +136,9 @@ extern "C" int ms_kv_scatter_kv8(const void* k, int64_t k_row_stride, const void
     return [=](unsigned grid) { return launch(kernel, grid, kCopyWarps * 32, 0, s, a, st); };
   };
   const cudaError_t e =
-      v16 ? launch_rows(rows, sms, go(ms::kv_scatter8_kernel<kCopyWarps, 1, true>),
+      v16 ? launch_rows(num_tokens, num_kv_heads, sms, go(ms::kv_scatter8_kernel<kCopyWarps, 1, true>),
                         go(ms::kv_scatter8_kernel<kCopyWarps, 4, true>))
-          : launch_rows(rows, sms, go(ms::kv_scatter8_kernel<kCopyWarps, 1, false>),
+          : launch_rows(num_tokens, num_kv_heads, sms, go(ms::kv_scatter8_kernel<kCopyWarps, 1, false>),
                         go(ms::kv_scatter8_kernel<kCopyWarps, 4, false>));
   if (e != cudaSuccess) return cuda_fail("kv_scatter_kv8 launch", e);
   return MS_OK;
@@ -177,8 +176,7 @@ int gather(const char* what, const int64_t* slots, int32_t num_tokens, int32_t n
     set_error(std::string(what) + ": null pointer, or k/v rows not 16-byte aligned");
     return MS_ERR_ARG;
   }
-  const int64_t rows = static_cast<int64_t>(num_tokens) * 2 * num_kv_heads;
-  if (rows > (int64_t(1) << 33)) {
+  if (static_cast<int64_t>(num_tokens) * num_kv_heads > kMaxCopyWarps) {
     set_error(std::string(what) + ": batch too large");
     return MS_ERR_ARG;
   }
@@ -204,7 +202,7 @@ int gather(const char* what, const int64_t* slots, int32_t num_tokens, int32_t n
   auto go = [&](auto kernel) {
     return [=](unsigned grid) { return launch(kernel, grid, kCopyWarps * 32, 0, s, a, st); };
   };
-  const cudaError_t e = launch_rows(rows, sms, go(ms::kv_gather_kernel<kKv8, kCopyWarps, 1>),
+  const cudaError_t e = launch_rows(num_tokens, num_kv_heads, sms, go(ms::kv_gather_kernel<kKv8, kCopyWarps, 1>),
                                     go(ms::kv_gather_kernel<kKv8, kCopyWarps, 4>));
   if (e != cudaSuccess) return cuda_fail((std::string(what) + " launch").c_str(), e);
   return MS_OK;

@@ -5,7 +5,7 @@
 // a contiguous range of the sequence's pages.  A producer warp streams whole pages (K and V of
 // this head) into a ring; four consumer warps form R row groups of 16 rows (R = 1, 2 or 4, the
 // smallest that holds the rows) times 4 / R page phases, so a short tile still uses every warp: warp
-// w takes row group w % R and the pages j with j % (4 / R) == w / R.  The phases merge through the
+// w takes row group w % R and the page pairs i with i % (4 / R) == w / R.  The phases merge through the
 // idle ring at the end.
 //
 // The mathematics per page (16 keys), in the exp2 domain with an online softmax:
@@ -15,16 +15,15 @@
 //
 // bf16 pool: mma.sync m16n8k16 with bf16 operands, as in kernel B.
 //
-// 8-bit pool.  K needs no conversion: mma.sync m16n8k32 multiplies e4m3 codes directly, so a
-// query row (bf16, 8 significant bits) is written as two e4m3 rows, q 2^-e = hi + lo / 16, each of 4
-// significant bits.  hi is the nearest e4m3 to q 2^-e, the remainder is exact, and lo holds it to
-// 2^-14 against a row maximum of up to 448: S is as exact as fp32 accumulation (2^-23 of the row's
-// largest |q|).  The two products run at four times the rate per multiply of the bf16 form (1.07
-// against 2.0 cycles per SM and warp instruction, twice the depth, measured), and K's page is read
-// once for both query heads as it lies in memory.
-// V's codes become f16 pairs (exact) on the way to the P V product: ldmatrix.trans moves 16-bit
-// units, so a register holds two neighbouring columns of two neighbouring tokens; one byte permute and
-// two conversions give the B operands of two column tiles (even and odd columns).
+// 8-bit pool: mma.sync m16n8k16 with f16 operands.  e4m3 codes are f16 values, so they are converted
+// exactly, two codes per instruction, after ldmatrix has brought them (16-bit units of two codes)
+// to the lanes.  K: a lane's word is four neighbouring dims of one key; the query fragments are
+// loaded in that order of dims, so two conversions give a B operand.  V: ldmatrix.trans
+// leaves two neighbouring columns of two neighbouring tokens in a word; one byte permute and two
+// conversions give the operands of two column tiles (even and odd columns).  The query row (bf16, 8
+// significant bits) is scaled by a power of two into f16's range: exact down to 2^-33 of its
+// largest value.  (mma.sync on e4m3 operands would need no conversion, but it runs at less than
+// half the rate per product here: 256 decode rows took 431 us with K multiplied that way.)
 // The row exponents of K multiply S's columns in fp32; those of V multiply p before it is rounded
 // to f16: p 2^(b - E), with E the largest exponent byte this warp has met (raised only when a page
 // exceeds it by more than 7, as the running maximum is raised only beyond 2^8, so a product stays
@@ -51,9 +50,11 @@ struct RowsArgs {
 template <bool kKv8>
 struct RowsCfg {
   static constexpr int kPage = kKv8 ? kPage8Bytes : kPageKVBytes;
-  // A multiple of 4: a slot's previous fill is then a page of the same phase (the parity waits
+  // A multiple of 8: a slot's previous fill is then a page of the same phase (the parity waits
   // are exact only then).
   static constexpr int kStages = kKv8 ? 16 : 8;
+  static constexpr int kBatch = 4;  // pages the producer's lanes issue side by side
+  static_assert(kStages % kBatch == 0 && kBatch <= 32, "a lane's pages reuse the same slots");
   static constexpr int kStageBytes = kStages * kPage;
   // Merge scratch in the ring: per warp 16 column tiles and (m, l), a float4 per lane each.
   static_assert(kRowsWarps * 17 * 32 * 16 <= kStageBytes, "merge scratch reuses the ring");
@@ -70,15 +71,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
@@ -109,17 +101,29 @@ struct RowsState {
   float o[16][4];
   float m[2], l[2];
   int eb;      // 8-bit pool: the exponent byte E that O is held against
-  float inv_e; // 2^(127 - E)
+  float inv_e;   // 2^(127 - E)
+  uint32_t hot;  // E + 7 in every byte (0 while E is unset)
 };
 
-// Raises the running maxima to the page's (mx, in exp2 units) where they exceed them by 2^8, and,
-// for an 8-bit pool, E to the page's largest exponent byte (vb: this thread's four, invisible keys as
-// 0) where that exceeds it by 7; O and l follow.
+// A warp takes two pages (32 keys) at a time: the products of one page hide the latencies of the
+// other, and one maximum, one vote and one rescale serve both (256 decode rows over an 8-bit pool:
+// 219 us page by page).
+constexpr int kBlockPages = 2;
+
+// Raises the running maxima to the block's (mx, in exp2 units) where they exceed them by 2^8, and,
+// for an 8-bit pool, E to the block's largest exponent byte (vw: this thread's exponent words,
+// invisible keys as 0) where that exceeds it by 7; O and l follow.
 template <bool kKv8>
-__device__ __forceinline__ void raise(RowsState& st, float mx0, float mx1, const int (&vb)[4]) {
+__device__ __forceinline__ void raise(RowsState& st, float mx0, float mx1,
+                                      const uint32_t (&vw)[kBlockPages]) {
   const bool up0 = mx0 > st.m[0] + 8.f, up1 = mx1 > st.m[1] + 8.f;
   bool hot = false;
-  if constexpr (kKv8) hot = max(max(vb[0], vb[1]), max(vb[2], vb[3])) > st.eb + 7;
+  uint32_t top4 = 0;
+  if constexpr (kKv8) {
+    top4 = __vmaxu4(vw[0], vw[1]);
+    // Any byte above E + 7 (E >= 0 once set; an unset E lets everything through).
+    hot = __vcmpgtu4(top4, st.hot) != 0;
+  }
   if (!__any_sync(0xffffffffu, up0 || up1 || hot)) return;
   float al0 = 1.f, al1 = 1.f;
   if (up0) {
@@ -137,7 +141,13 @@ __device__ __forceinline__ void raise(RowsState& st, float mx0, float mx1, const
     // infinite factor, and only on the rows that see it).
     int top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, vb[i] == static_cast<int>(kExpNan) ? 0 : vb[i]);
+    for (int t = 0; t < kBlockPages; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = static_cast<int>(vw[t] >> (8 * i) & 255u);
+        top = max(top, e == static_cast<int>(kExpNan) ? 0 : e);
+      }
+    }
     top = __reduce_max_sync(0xffffffffu, top);
     if (top > st.eb + 7 || st.eb < 0) {
       const int d = st.eb - top + kExpBias;  // 2^(E_old - E_new); O is still zero when E was unset
@@ -146,6 +156,7 @@ __device__ __forceinline__ void raise(RowsState& st, float mx0, float mx1, const
       al1 *= f;
       st.eb = top;
       st.inv_e = __int_as_float((2 * kExpBias - top) << 23);
+      st.hot = static_cast<uint32_t>(min(top + 7, 255)) * 0x01010101u;
     }
   }
 #pragma unroll
@@ -157,225 +168,264 @@ __device__ __forceinline__ void raise(RowsState& st, float mx0, float mx1, const
   }
 }
 
-// Masked scores of a thread's 8 (row, key) pairs: keys 2q, 2q + 1 (s0) and 2q + 8, 2q + 9 (s1).
-__device__ __forceinline__ void mask_scores(float (&s0)[4], float (&s1)[4], uint32_t vis0,
-                                            uint32_t vis1, int q2) {
-  const float ninf = -INFINITY;
+// Row maxima of the block over the quad that holds a row.
+__device__ __forceinline__ void block_max(const float (&s)[2 * kBlockPages][4], float& mx0,
+                                          float& mx1) {
+  mx0 = fmaxf(s[0][0], s[0][1]);
+  mx1 = fmaxf(s[0][2], s[0][3]);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (!(vis0 >> (q2 + i) & 1u)) s0[i] = ninf;
-    if (!(vis1 >> (q2 + i) & 1u)) s0[2 + i] = ninf;
-    if (!(vis0 >> (q2 + 8 + i) & 1u)) s1[i] = ninf;
-    if (!(vis1 >> (q2 + 8 + i) & 1u)) s1[2 + i] = ninf;
+  for (int t = 1; t < 2 * kBlockPages; ++t) {
+    mx0 = fmaxf(mx0, fmaxf(s[t][0], s[t][1]));
+    mx1 = fmaxf(mx1, fmaxf(s[t][2], s[t][3]));
   }
-}
-
-// Row maxima of the page over the quad that holds a row.
-__device__ __forceinline__ void page_max(const float (&s0)[4], const float (&s1)[4], float& mx0,
-                                         float& mx1) {
-  mx0 = fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s1[0], s1[1]));
-  mx1 = fmaxf(fmaxf(s0[2], s0[3]), fmaxf(s1[2], s1[3]));
   mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
   mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
   mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
   mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
 }
 
-// p = 2^(s c - m) for the page, and its sums into l.
-__device__ __forceinline__ void page_exp(const float (&s0)[4], const float (&s1)[4], float c0,
-                                         float c1, RowsState& st, float (&p0)[4], float (&p1)[4]) {
+// p = 2^(s c - m) in place, and its sums into l.
+__device__ __forceinline__ void block_exp(float (&s)[2 * kBlockPages][4], float c0, float c1,
+                                          RowsState& st) {
   const float mu0 = st.m[0] == -INFINITY ? 0.f : st.m[0];
   const float mu1 = st.m[1] == -INFINITY ? 0.f : st.m[1];
-  p0[0] = fast_exp2(__fmaf_rn(s0[0], c0, -mu0));
-  p0[1] = fast_exp2(__fmaf_rn(s0[1], c0, -mu0));
-  p0[2] = fast_exp2(__fmaf_rn(s0[2], c1, -mu1));
-  p0[3] = fast_exp2(__fmaf_rn(s0[3], c1, -mu1));
-  p1[0] = fast_exp2(__fmaf_rn(s1[0], c0, -mu0));
-  p1[1] = fast_exp2(__fmaf_rn(s1[1], c0, -mu0));
-  p1[2] = fast_exp2(__fmaf_rn(s1[2], c1, -mu1));
-  p1[3] = fast_exp2(__fmaf_rn(s1[3], c1, -mu1));
-  st.l[0] += (p0[0] + p0[1]) + (p1[0] + p1[1]);
-  st.l[1] += (p0[2] + p0[3]) + (p1[2] + p1[3]);
+  float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+  for (int t = 0; t < 2 * kBlockPages; ++t) {
+    s[t][0] = fast_exp2(__fmaf_rn(s[t][0], c0, -mu0));
+    s[t][1] = fast_exp2(__fmaf_rn(s[t][1], c0, -mu0));
+    s[t][2] = fast_exp2(__fmaf_rn(s[t][2], c1, -mu1));
+    s[t][3] = fast_exp2(__fmaf_rn(s[t][3], c1, -mu1));
+    l0 += s[t][0] + s[t][1];
+    l1 += s[t][2] + s[t][3];
+  }
+  st.l[0] += l0;
+  st.l[1] += l1;
 }
 
-// ---- one page, 8-bit pool -----------------------------------------------------------------------
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t w;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(addr));
+  return w;
+}
 
-// qh/ql: the query rows' high and low e4m3 parts, [chunk of 16 dims][row r0, r1].  c0, c1: scale
-// log2(e) times the rows' query scale.  Accumulator tile 2u + p holds columns 16u + 2j + p, so a
-// thread's o[2u][0], o[2u + 1][0], o[2u][1], o[2u + 1][1] are four neighbouring columns.
+// 2^(b - 127) of byte i of a word of exponent bytes (infinity for 255, 0 for 0).
+template <int i>
+__device__ __forceinline__ float scale_of_byte(uint32_t w) {
+  const uint32_t m = i == 3 ? w >> 1 : w << (23 - 8 * i);
+  return __uint_as_float(m & 0x7f800000u);
+}
+
+// ---- two pages, 8-bit pool ----------------------------------------------------------------------
+
+// qf: the query rows' fragments, f16, dims 16 ks + 4 (lane % 4) .. + 3 of rows r0, r1.  c0, c1: scale
+// log2(e) times the rows' query scale.  Key column j of tile t (of two per page) is token
+// 4 (j / 2) + j % 2 + 2 t, so a thread's four keys of a page are neighbours (4 (lane % 4) .. + 3) and
+// their exponent bytes one word.  Accumulator tile 2u + p holds columns 16u + 2j + p, so a thread's
+// o[2u][0], o[2u + 1][0], o[2u][1], o[2u + 1][1] are four neighbouring columns.  vis: bit k of page t
+// in vis[t] (kMask only).
 template <bool kMask>
-__device__ __forceinline__ void rows_page8(uint32_t page, const uint32_t (&qh)[8][2],
-                                           const uint32_t (&ql)[8][2], RowsState& st, float c0,
-                                           float c1, uint32_t vis0, uint32_t vis1, int lane) {
-  const int mi = lane >> 3, t8 = lane & 7, q2 = 2 * (lane & 3);
-  float s[2][4], e[2][4];  // hi and lo products of the two key tiles
+__device__ __forceinline__ void rows_block8(const uint32_t (&page)[kBlockPages],
+                                            const uint32_t (&qf)[8][4], RowsState& st, float c0,
+                                            float c1, const uint32_t (&vis0)[kBlockPages],
+                                            const uint32_t (&vis1)[kBlockPages], int lane) {
+  const int mi = lane >> 3, t8 = lane & 7, q4 = 4 * (lane & 3);
+  const int tok = 4 * (t8 >> 1) + (t8 & 1);  // this lane's ldmatrix row in tile 0
+  const int sw = code_swizzle8(tok);         // the same for tok + 2
+  float s[2 * kBlockPages][4];
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < 2 * kBlockPages; ++t) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[t][i] = e[t][i] = 0.f;
+    for (int i = 0; i < 4; ++i) s[t][i] = 0.f;
   }
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      uint32_t b0, b1, b2, b3;
-      ldsm_x4(page + (t * 8 + t8) * kRow8Bytes + (((4 * u + mi) ^ t8) << 4), b0, b1, b2, b3);
-      mma_e4m3(s[t], qh[4 * u][0], qh[4 * u][1], qh[4 * u + 1][0], qh[4 * u + 1][1], b0, b1);
-      mma_e4m3(e[t], ql[4 * u][0], ql[4 * u][1], ql[4 * u + 1][0], ql[4 * u + 1][1], b0, b1);
-      mma_e4m3(s[t], qh[4 * u + 2][0], qh[4 * u + 2][1], qh[4 * u + 3][0], qh[4 * u + 3][1], b2, b3);
-      mma_e4m3(e[t], ql[4 * u + 2][0], ql[4 * u + 2][1], ql[4 * u + 3][0], ql[4 * u + 3][1], b2, b3);
+    for (int t = 0; t < 2 * kBlockPages; ++t) {
+      uint32_t b[4];
+      ldsm_x4(page[t >> 1] + (tok + 2 * (t & 1)) * kRow8Bytes + (((4 * u + mi) ^ sw) << 4), b[0],
+              b[1], b[2], b[3]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        mma_f16(s[t], qf[4 * u + i], e4m3x2_to_f16x2<0>(b[i]), e4m3x2_to_f16x2<1>(b[i]));
     }
   }
-  // Exponent bytes of this thread's four keys (K, then V).
-  uint32_t kb[2], vb16[2];
+  uint32_t vw[kBlockPages], keep[kBlockPages][2];
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    asm volatile("ld.shared.u16 %0, [%1];" : "=r"(kb[t]) : "r"(page + kExp8Off + t * 8 + q2));
-    asm volatile("ld.shared.u16 %0, [%1];"
-                 : "=r"(vb16[t])
-                 : "r"(page + kExp8Off + kBlockTokens + t * 8 + q2));
-  }
-  int vb[4] = {static_cast<int>(vb16[0] & 255u), static_cast<int>(vb16[0] >> 8),
-               static_cast<int>(vb16[1] & 255u), static_cast<int>(vb16[1] >> 8)};
+  for (int t = 0; t < kBlockPages; ++t) {
+    const uint32_t kw = lds32(page[t] + kExp8Off + q4);
+    vw[t] = lds32(page[t] + kExp8Off + kBlockTokens + q4);
+    const float f[4] = {scale_of_byte<0>(kw), scale_of_byte<1>(kw), scale_of_byte<2>(kw),
+                        scale_of_byte<3>(kw)};
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const float fa = scale8(kb[t] & 255u), fb = scale8(kb[t] >> 8);
-    s[t][0] = __fmaf_rn(e[t][0], 0.0625f, s[t][0]) * fa;
-    s[t][1] = __fmaf_rn(e[t][1], 0.0625f, s[t][1]) * fb;
-    s[t][2] = __fmaf_rn(e[t][2], 0.0625f, s[t][2]) * fa;
-    s[t][3] = __fmaf_rn(e[t][3], 0.0625f, s[t][3]) * fb;
-  }
-  uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;  // V words of tokens some row sees
-  if constexpr (kMask) {
-    mask_scores(s[0], s[1], vis0, vis1, q2);
-    // Rows of keys no row here sees may hold anything (pages of a finished sequence, unused drafts).
-    const uint32_t any = __reduce_or_sync(0xffffffffu, vis0 | vis1);
-    keep0 = (any >> q2 & 1u ? 0xffffu : 0u) | (any >> (q2 + 1) & 1u ? 0xffff0000u : 0u);
-    keep1 = (any >> (q2 + 8) & 1u ? 0xffffu : 0u) | (any >> (q2 + 9) & 1u ? 0xffff0000u : 0u);
-    if (!(keep0 & 0xffffu)) vb[0] = 0;
-    if (!(keep0 >> 16)) vb[1] = 0;
-    if (!(keep1 & 0xffffu)) vb[2] = 0;
-    if (!(keep1 >> 16)) vb[3] = 0;
+    for (int i = 0; i < 4; ++i) {
+      s[2 * t][i] *= f[i & 1];
+      s[2 * t + 1][i] *= f[2 + (i & 1)];
+    }
+    if constexpr (kMask) {
+      // Rows of keys no row here sees may hold anything (pages of a finished sequence, unused
+      // drafts, a second page that is not there): their values and exponents become zero.
+      const uint32_t v0 = vis0[t] >> q4, v1 = vis1[t] >> q4;
+      const uint32_t any = __reduce_or_sync(0xffffffffu, vis0[t] | vis1[t]) >> q4;
+      keep[t][0] = (any & 1u ? 0xffffu : 0u) | (any & 2u ? 0xffff0000u : 0u);
+      keep[t][1] = (any & 4u ? 0xffffu : 0u) | (any & 8u ? 0xffff0000u : 0u);
+      vw[t] &= (any & 1u ? 0xffu : 0u) | (any & 2u ? 0xff00u : 0u) | (any & 4u ? 0xff0000u : 0u) |
+               (any & 8u ? 0xff000000u : 0u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t v = (i & 2) ? v1 : v0;
+        if (!(v >> (i & 1) & 1u)) s[2 * t][i] = -INFINITY;
+        if (!(v >> (2 + (i & 1)) & 1u)) s[2 * t + 1][i] = -INFINITY;
+      }
+    }
   }
   float mx0, mx1;
-  page_max(s[0], s[1], mx0, mx1);
-  raise<true>(st, mx0 * c0, mx1 * c1, vb);
-  float p0[4], p1[4];
-  page_exp(s[0], s[1], c0, c1, st, p0, p1);
-  const float f[4] = {scale8(vb[0]) * st.inv_e, scale8(vb[1]) * st.inv_e, scale8(vb[2]) * st.inv_e,
-                      scale8(vb[3]) * st.inv_e};
+  block_max(s, mx0, mx1);
+  raise<true>(st, mx0 * c0, mx1 * c1, vw);
+  block_exp(s, c0, c1, st);
+  const int vtok = tok + 2 * (mi & 1);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    // A key this row does not see contributes nothing, whatever its exponent byte.
-    p0[i] = kMask && s[0][i] == -INFINITY ? 0.f : p0[i] * f[i & 1];
-    p1[i] = kMask && s[1][i] == -INFINITY ? 0.f : p1[i] * f[2 + (i & 1)];
-  }
-  const uint32_t pa[4] = {pack_f16(p0[0], p0[1]), pack_f16(p0[2], p0[3]), pack_f16(p1[0], p1[1]),
-                          pack_f16(p1[2], p1[3])};
-  const uint32_t vrow = page + kCodes8Bytes + (t8 + (mi & 1) * 8) * kRow8Bytes;
+  for (int t = 0; t < kBlockPages; ++t) {
+    const float f[4] = {scale_of_byte<0>(vw[t]) * st.inv_e, scale_of_byte<1>(vw[t]) * st.inv_e,
+                        scale_of_byte<2>(vw[t]) * st.inv_e, scale_of_byte<3>(vw[t]) * st.inv_e};
+    float p[2][4];
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    uint32_t w[4];
-    ldsm_x4_t(vrow + (((2 * u + (mi >> 1)) ^ t8) << 4), w[0], w[1], w[2], w[3]);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t a = w[2 * h], b = w[2 * h + 1];
+    for (int i = 0; i < 4; ++i) {
+      p[0][i] = s[2 * t][i] * f[i & 1];
+      p[1][i] = s[2 * t + 1][i] * f[2 + (i & 1)];
       if constexpr (kMask) {
-        a &= keep0;
-        b &= keep1;
+        // A key this row does not see contributes nothing, whatever its exponent byte.
+        const uint32_t v = ((i & 2) ? vis1[t] : vis0[t]) >> q4;
+        if (!(v >> (i & 1) & 1u)) p[0][i] = 0.f;
+        if (!(v >> (2 + (i & 1)) & 1u)) p[1][i] = 0.f;
       }
-      // Bytes (token t: columns 2j, 2j + 1; token t + 1: the same) -> column 2j of both tokens in
-      // the low half, column 2j + 1 in the high half.
-      a = __byte_perm(a, 0, 0x3120);
-      b = __byte_perm(b, 0, 0x3120);
-      mma_f16(st.o[4 * u + 2 * h], pa, e4m3x2_to_f16x2<0>(a), e4m3x2_to_f16x2<0>(b));
-      mma_f16(st.o[4 * u + 2 * h + 1], pa, e4m3x2_to_f16x2<1>(a), e4m3x2_to_f16x2<1>(b));
+    }
+    const uint32_t pa[4] = {pack_f16(p[0][0], p[0][1]), pack_f16(p[0][2], p[0][3]),
+                            pack_f16(p[1][0], p[1][1]), pack_f16(p[1][2], p[1][3])};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      uint32_t w[4];
+      ldsm_x4_t(page[t] + kCodes8Bytes + vtok * kRow8Bytes + (((2 * u + (mi >> 1)) ^ sw) << 4), w[0],
+                w[1], w[2], w[3]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t a = w[2 * h], b = w[2 * h + 1];
+        if constexpr (kMask) {
+          a &= keep[t][0];
+          b &= keep[t][1];
+        }
+        // Bytes (token t: columns 2j, 2j + 1; token t + 1: the same) -> column 2j of both tokens
+        // in the low half, column 2j + 1 in the high half.
+        a = __byte_perm(a, 0, 0x3120);
+        b = __byte_perm(b, 0, 0x3120);
+        mma_f16(st.o[4 * u + 2 * h], pa, e4m3x2_to_f16x2<0>(a), e4m3x2_to_f16x2<0>(b));
+        mma_f16(st.o[4 * u + 2 * h + 1], pa, e4m3x2_to_f16x2<1>(a), e4m3x2_to_f16x2<1>(b));
+      }
     }
   }
 }
 
-// ---- one page, bf16 pool ------------------------------------------------------------------------
+// ---- two pages, bf16 pool -----------------------------------------------------------------------
 
 __device__ __forceinline__ bool bf16_pair_bad(uint32_t w) {
   return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
 
-// qf: query fragments as in kernel B.  Accumulator tile n holds columns 8n + 2q, 8n + 2q + 1.
+// qf: query fragments as in kernel B; a thread's keys of a page are 2q, 2q + 1, 2q + 8, 2q + 9
+// (q = lane % 4).  Accumulator tile n holds columns 8n + 2q, 8n + 2q + 1.
 template <bool kMask>
-__device__ __forceinline__ void rows_page16(uint32_t page, const uint32_t (&qf)[8][4],
-                                            RowsState& st, float c, uint32_t vis0, uint32_t vis1,
-                                            int lane) {
+__device__ __forceinline__ void rows_block16(const uint32_t (&page)[kBlockPages],
+                                             const uint32_t (&qf)[8][4], RowsState& st, float c,
+                                             const uint32_t (&vis0)[kBlockPages],
+                                             const uint32_t (&vis1)[kBlockPages], int lane) {
   const int mi = lane >> 3, q2 = 2 * (lane & 3);
-  float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-  {
-    const int key = (lane & 7) + (mi >> 1) * 8;
+  float s[2 * kBlockPages][4];
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
+  for (int t = 0; t < 2 * kBlockPages; ++t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[t][i] = 0.f;
+  }
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) {
+#pragma unroll
+    for (int t = 0; t < kBlockPages; ++t) {
       uint32_t b0, b1, b2, b3;
-      ldsm_x4(page + swz_off(key, ks * 16 + (mi & 1) * 8, 16), b0, b1, b2, b3);
-      mma_bf16(s0, qf[ks], b0, b1);
-      mma_bf16(s1, qf[ks], b2, b3);
+      ldsm_x4(page[t] + swz_off((lane & 7) + (mi >> 1) * 8, ks * 16 + (mi & 1) * 8, 16), b0, b1, b2,
+              b3);
+      mma_bf16(s[2 * t], qf[ks], b0, b1);
+      mma_bf16(s[2 * t + 1], qf[ks], b2, b3);
     }
   }
-  uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+  uint32_t keep[kBlockPages][2];
   if constexpr (kMask) {
-    mask_scores(s0, s1, vis0, vis1, q2);
-    const uint32_t any = __reduce_or_sync(0xffffffffu, vis0 | vis1);
-    keep0 = (any >> q2 & 1u ? 0xffffu : 0u) | (any >> (q2 + 1) & 1u ? 0xffff0000u : 0u);
-    keep1 = (any >> (q2 + 8) & 1u ? 0xffffu : 0u) | (any >> (q2 + 9) & 1u ? 0xffff0000u : 0u);
-  }
-  float mx0, mx1;
-  page_max(s0, s1, mx0, mx1);
-  const int none[4] = {0, 0, 0, 0};
-  raise<false>(st, mx0 * c, mx1 * c, none);
-  float p0[4], p1[4];
-  page_exp(s0, s1, c, c, st, p0, p1);
-  // p is rounded to bf16 for the product (half a step of 2^-8), as in kernels B and D.
-  const uint32_t pa[4] = {pack_bf16(p0[0], p0[1]), pack_bf16(p0[2], p0[3]),
-                          pack_bf16(p1[0], p1[1]), pack_bf16(p1[2], p1[3])};
-  const int key = (lane & 7) + (mi & 1) * 8;
-  const uint32_t vbase = page + kPageBytes;
-  bool bad = false;
 #pragma unroll
-  for (int np = 0; np < 8; ++np) {
-    uint32_t b[4];
-    ldsm_x4_t(vbase + swz_off(key, np * 16 + (mi >> 1) * 8, 16), b[0], b[1], b[2], b[3]);
-    if constexpr (kMask) {
-      // Values of keys no row here sees are dropped; infinities and NaN of the others too, and
-      // added below for the rows that do see them (0 times them would reach every row).
+    for (int t = 0; t < kBlockPages; ++t) {
+      const uint32_t any = __reduce_or_sync(0xffffffffu, vis0[t] | vis1[t]) >> q2;
+      keep[t][0] = (any & 1u ? 0xffffu : 0u) | (any & 2u ? 0xffff0000u : 0u);
+      keep[t][1] = (any & 0x100u ? 0xffffu : 0u) | (any & 0x200u ? 0xffff0000u : 0u);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        b[i] &= (i & 1) ? keep1 : keep0;
-        if (bf16_pair_bad(b[i])) {
-          bad = true;
-          if ((b[i] & 0x7f80u) == 0x7f80u) b[i] &= 0xffff0000u;
-          if ((b[i] & 0x7f800000u) == 0x7f800000u) b[i] &= 0xffffu;
-        }
+        const uint32_t v = ((i & 2) ? vis1[t] : vis0[t]) >> q2;
+        if (!(v >> (i & 1) & 1u)) s[2 * t][i] = -INFINITY;
+        if (!(v >> (8 + (i & 1)) & 1u)) s[2 * t + 1][i] = -INFINITY;
       }
     }
-    mma_bf16(st.o[2 * np], pa, b[0], b[1]);
-    mma_bf16(st.o[2 * np + 1], pa, b[2], b[3]);
   }
-  if constexpr (kMask) {
-    if (__any_sync(0xffffffffu, bad)) {
-      for (int k = 0; k < 16; ++k) {
-        const int src = (lane & ~3) | ((k & 7) >> 1);
-        const float a0 = (k & 8) ? ((k & 1) ? p1[1] : p1[0]) : ((k & 1) ? p0[1] : p0[0]);
-        const float a1 = (k & 8) ? ((k & 1) ? p1[3] : p1[2]) : ((k & 1) ? p0[3] : p0[2]);
-        const float w0 = __shfl_sync(0xffffffffu, a0, src);
-        const float w1 = __shfl_sync(0xffffffffu, a1, src);
-        const bool see0 = vis0 >> k & 1u, see1 = vis1 >> k & 1u;
+  float mx0, mx1;
+  block_max(s, mx0, mx1);
+  const uint32_t none[kBlockPages] = {};
+  raise<false>(st, mx0 * c, mx1 * c, none);
+  block_exp(s, c, c, st);
 #pragma unroll
-        for (int n = 0; n < 16; ++n) {
-          uint32_t w;
-          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(vbase + swz_off(k, n * 8 + q2, 16)));
+  for (int t = 0; t < kBlockPages; ++t) {
+    // p is rounded to bf16 for the product (half a step of 2^-8), as in kernels B and D.
+    const float(&p0)[4] = s[2 * t];
+    const float(&p1)[4] = s[2 * t + 1];
+    const uint32_t pa[4] = {pack_bf16(p0[0], p0[1]), pack_bf16(p0[2], p0[3]),
+                            pack_bf16(p1[0], p1[1]), pack_bf16(p1[2], p1[3])};
+    const int key = (lane & 7) + (mi & 1) * 8;
+    const uint32_t vbase = page[t] + kPageBytes;
+    bool bad = false;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t bits = i == 0 ? w << 16 : w & 0xffff0000u;
-            if ((bits & 0x7f800000u) != 0x7f800000u) continue;
-            const float v = __uint_as_float(bits);
-            if (see0) st.o[n][i] += w0 * v;
-            if (see1) st.o[n][2 + i] += w1 * v;
+    for (int np = 0; np < 8; ++np) {
+      uint32_t b[4];
+      ldsm_x4_t(vbase + swz_off(key, np * 16 + (mi >> 1) * 8, 16), b[0], b[1], b[2], b[3]);
+      if constexpr (kMask) {
+        // Values of keys no row here sees are dropped; infinities and NaN of the others too, and
+        // added below for the rows that do see them (0 times them would reach every row).
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          b[i] &= keep[t][i & 1];
+          if (bf16_pair_bad(b[i])) {
+            bad = true;
+            if ((b[i] & 0x7f80u) == 0x7f80u) b[i] &= 0xffff0000u;
+            if ((b[i] & 0x7f800000u) == 0x7f800000u) b[i] &= 0xffffu;
+          }
+        }
+      }
+      mma_bf16(st.o[2 * np], pa, b[0], b[1]);
+      mma_bf16(st.o[2 * np + 1], pa, b[2], b[3]);
+    }
+    if constexpr (kMask) {
+      if (__any_sync(0xffffffffu, bad)) {
+        for (int k = 0; k < 16; ++k) {
+          const int src = (lane & ~3) | ((k & 7) >> 1);
+          const float a0 = (k & 8) ? ((k & 1) ? p1[1] : p1[0]) : ((k & 1) ? p0[1] : p0[0]);
+          const float a1 = (k & 8) ? ((k & 1) ? p1[3] : p1[2]) : ((k & 1) ? p0[3] : p0[2]);
+          const float w0 = __shfl_sync(0xffffffffu, a0, src);
+          const float w1 = __shfl_sync(0xffffffffu, a1, src);
+          const bool see0 = vis0[t] >> k & 1u, see1 = vis1[t] >> k & 1u;
+#pragma unroll
+          for (int n = 0; n < 16; ++n) {
+            const uint32_t w = lds32(vbase + swz_off(k, n * 8 + q2, 16));
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t bits = i == 0 ? w << 16 : w & 0xffff0000u;
+              if ((bits & 0x7f800000u) != 0x7f800000u) continue;
+              const float v = __uint_as_float(bits);
+              if (see0) st.o[n][i] += w0 * v;
+              if (see1) st.o[n][2 + i] += w1 * v;
+            }
           }
         }
       }
@@ -450,10 +500,10 @@ __device__ __forceinline__ void put_cols(const RowOut& o, int d, const float (&x
 }
 
 template <bool kKv8, bool kTree>
-__global__ void __launch_bounds__(kRowsThreads, 3)
+__global__ void __launch_bounds__(kRowsThreads, 2)
     rows_attn_kernel(const __grid_constant__ CUtensorMap kv_map, const RowsArgs ra) {
   using Cfg = RowsCfg<kKv8>;
-  constexpr int kStages = Cfg::kStages;
+  constexpr int kStages = Cfg::kStages, kBatch = Cfg::kBatch;
   const AttnArgs& a = ra.a;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -499,72 +549,67 @@ __global__ void __launch_bounds__(kRowsThreads, 3)
 
   if (warp == kRowsWarps) {
     // ---------------- producer warp ----------------
+    // Lane i of the first kBatch takes the pages j with j % kBatch == i: the lanes wait for their
+    // slots and issue their copies side by side.  (One lane issuing every page takes a chain of
+    // several hundred cycles per page, which three CTAs of 4 KiB pages per SM cannot afford.)
     const uint64_t policy = l2_policy_evict_first();
     const int* table = a.tables + table_off + page_begin;
-    int issued = 0;
+    int issued = 0;  // by this lane
     bool stop = false;
     for (int j0 = 0; j0 < npages && !stop; j0 += 32) {
-      int mine = 0;
-      if (j0 + lane < npages) mine = table[j0 + lane];
-      const int cnt = min(32, npages - j0);
-      for (int jj = 0; jj < cnt; ++jj) {
-        const int blk = __shfl_sync(0xffffffffu, mine, jj);
-        const bool inside = static_cast<unsigned>(blk) < static_cast<unsigned>(a.num_blocks);
-        const int s = (j0 + jj) % kStages;
-        int ok = 1;
-        if (lane == 0) {
-          const int j = j0 + jj;
-          if (*abort_flag) ok = 0;
-          if (ok && j >= kStages && !mbar_wait(&empty[s], ((j / kStages) - 1) & 1)) {
+      const int mine = j0 + lane < npages ? table[j0 + lane] : 0;
+      for (int b = 0; b < 32 && j0 + b < npages; b += kBatch) {
+        const int blk = __shfl_sync(0xffffffffu, mine, b + (lane & (kBatch - 1)));
+        const int j = j0 + b + lane;
+        bool ok = *abort_flag == 0;
+        if (ok && lane < kBatch && j < npages) {
+          const int s = j % kStages;
+          if (j >= kStages && !mbar_wait(&empty[s], ((j / kStages) - 1) & 1)) {
             atomicOr(&g_status_word, kErrTimeout);
             *abort_flag = 1;
-            ok = 0;
-          }
-          if (ok) {
+            ok = false;
+          } else {
+            const bool inside = static_cast<unsigned>(blk) < static_cast<unsigned>(a.num_blocks);
+            uint8_t* dst = ring + s * Cfg::kPage;
             // Block ids outside the pool are flagged and read as zeros (the TMA unit's fill, or
-            // written below).
+            // written here).
             if (!inside) atomicOr(&g_status_word, kErrBlock);
             if constexpr (kKv8) {
               if (inside) {
                 mbar_arrive_expect_tx(&full[s], Cfg::kPage);
                 asm volatile(
                     "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::"
-                    "cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(smem_u32(ring + s * Cfg::kPage)),
+                    "cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(smem_u32(dst)),
                     "l"(ra.pool + (static_cast<long long>(blk) * a.num_kv + kvh) * Cfg::kPage),
                     "r"(Cfg::kPage), "r"(smem_u32(&full[s])), "l"(policy)
                     : "memory");
+              } else {
+                for (int i = 0; i < Cfg::kPage / 16; ++i)
+                  reinterpret_cast<uint4*>(dst)[i] = make_uint4(0u, 0u, 0u, 0u);
+                // Later copies into the slot go through the async proxy.
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(&full[s]);
               }
             } else {
               mbar_arrive_expect_tx(&full[s], Cfg::kPage);
-              tma_load_5d(ring + s * Cfg::kPage, &kv_map, &full[s], 0, 0, 0, kvh, blk, policy);
+              tma_load_5d(dst, &kv_map, &full[s], 0, 0, 0, kvh, blk, policy);
             }
             ++issued;
           }
         }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) {
+        if (!__all_sync(0xffffffffu, ok)) {
           stop = true;
           break;
-        }
-        if constexpr (kKv8) {
-          if (!inside) {
-            for (int i = lane; i < Cfg::kPage / 16; i += 32)
-              reinterpret_cast<uint4*>(ring + s * Cfg::kPage)[i] = make_uint4(0u, 0u, 0u, 0u);
-            // Later copies into the slot go through the async proxy.
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&full[s]);
-          }
         }
       }
     }
     // Drain: never leave the CTA with a copy in flight.
-    if (lane == 0) {
-      for (int j = issued > kStages ? issued - kStages : 0; j < issued; ++j) {
-        if (!mbar_wait(&full[j % kStages], (j / kStages) & 1)) {
-          atomicOr(&g_status_word, kErrTimeout);
-          break;
-        }
+    constexpr int kPerLane = kStages / kBatch;
+    for (int i = issued > kPerLane ? issued - kPerLane : 0; i < issued; ++i) {
+      const int j = i * kBatch + lane;
+      if (!mbar_wait(&full[j % kStages], (j / kStages) & 1)) {
+        atomicOr(&g_status_word, kErrTimeout);
+        break;
       }
     }
     return;
@@ -583,8 +628,7 @@ __global__ void __launch_bounds__(kRowsThreads, 3)
                                (kvh * kGroup + (ra0 & 1)) * kHeadDim;
   const __nv_bfloat16* qrow1 = a.q + static_cast<long long>(flat_start + tok0 + tk1) * a.q_row_stride +
                                (kvh * kGroup + (ra1 & 1)) * kHeadDim;
-  uint32_t qh[8][2], ql[8][2];  // 8-bit pool
-  uint32_t qf[8][4];            // bf16 pool
+  uint32_t qf[8][4];
   float c0 = a.scale_log2, c1 = a.scale_log2;
   if constexpr (kKv8) {
     uint2 x[2][8];
@@ -608,15 +652,8 @@ __global__ void __launch_bounds__(kRowsThreads, 3)
       (r == 0 ? c0 : c1) *= row_scale8(b);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float y[4] = {bf16_lo(x[r][i].x) * inv, bf16_hi(x[r][i].x) * inv,
-                            bf16_lo(x[r][i].y) * inv, bf16_hi(x[r][i].y) * inv};
-        const uint32_t hi = cvt_e4m3x4(y[0], y[1], y[2], y[3]);
-        const uint32_t h0 = e4m3x2_to_f16x2<0>(hi), h1 = e4m3x2_to_f16x2<1>(hi);
-        const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-        const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-        qh[i][r] = hi;
-        ql[i][r] = cvt_e4m3x4((y[0] - f0.x) * 16.f, (y[1] - f0.y) * 16.f, (y[2] - f1.x) * 16.f,
-                              (y[3] - f1.y) * 16.f);
+        qf[i][r] = pack_f16(bf16_lo(x[r][i].x) * inv, bf16_hi(x[r][i].x) * inv);
+        qf[i][2 + r] = pack_f16(bf16_lo(x[r][i].y) * inv, bf16_hi(x[r][i].y) * inv);
       }
     }
   } else {
@@ -655,15 +692,24 @@ __global__ void __launch_bounds__(kRowsThreads, 3)
   st.l[0] = st.l[1] = 0.f;
   st.eb = -1000;
   st.inv_e = 0.f;
+  st.hot = 0;
   const int qpos0 = num_cached + tok0 + tk0, qpos1 = num_cached + tok0 + tk1;
   // First key position that some row of the tile may not see.
   const int first_masked = kTree ? num_cached : num_cached + tok0 + (row_base >> 1) + 1;
   const uint32_t ring_u32 = smem_u32(ring);
-  for (int j = phase; j < npages; j += phases) {
-    const int s = j % kStages;
+  for (int j = phase * kBlockPages; j < npages; j += phases * kBlockPages) {
+    const int cnt = min(kBlockPages, npages - j);
+    uint32_t page[kBlockPages];
+    bool ok = true;
+#pragma unroll
+    for (int t = 0; t < kBlockPages; ++t) {
+      // A second page that is not there is masked out; its slot's leftovers are read.
+      const int s = (j + t) % kStages;
+      page[t] = ring_u32 + s * Cfg::kPage;
+      if (t < cnt) ok = ok && mbar_wait_fast(&full[s], ((j + t) / kStages) & 1, abort_flag);
+    }
     // Leave the loop only as a whole warp: the tensor-core operations are warp-collective.
-    const bool ok = __all_sync(0xffffffffu, mbar_wait_fast(&full[s], (j / kStages) & 1, abort_flag));
-    if (!ok) {
+    if (!__all_sync(0xffffffffu, ok)) {
       if (lane == 0) {
         atomicOr(&g_status_word, kErrTimeout);
         *abort_flag = 1;
@@ -671,30 +717,39 @@ __global__ void __launch_bounds__(kRowsThreads, 3)
       break;
     }
     const int key0 = (page_begin + j) * kBlockTokens;
-    const uint32_t page = ring_u32 + s * Cfg::kPage;
     if (warp_active) {
-      if (key0 + kBlockTokens > first_masked) {
-        uint32_t vis0, vis1;
-        if constexpr (kTree) {
-          vis0 = live0 ? tree_bits(mask0, words, key0 - num_cached) : 0u;
-          vis1 = live1 ? tree_bits(mask1, words, key0 - num_cached) : 0u;
-        } else {
-          vis0 = live0 ? causal_bits(qpos0, key0) : 0u;
-          vis1 = live1 ? causal_bits(qpos1, key0) : 0u;
+      uint32_t vis0[kBlockPages], vis1[kBlockPages];
+      if (cnt < kBlockPages || key0 + kBlockPages * kBlockTokens > first_masked) {
+#pragma unroll
+        for (int t = 0; t < kBlockPages; ++t) {
+          const int k0 = key0 + t * kBlockTokens;
+          if (k0 + kBlockTokens <= first_masked) {
+            vis0[t] = live0 ? 0xffffu : 0u;
+            vis1[t] = live1 ? 0xffffu : 0u;
+          } else if constexpr (kTree) {
+            vis0[t] = live0 ? tree_bits(mask0, words, k0 - num_cached) : 0u;
+            vis1[t] = live1 ? tree_bits(mask1, words, k0 - num_cached) : 0u;
+          } else {
+            vis0[t] = live0 ? causal_bits(qpos0, k0) : 0u;
+            vis1[t] = live1 ? causal_bits(qpos1, k0) : 0u;
+          }
+          if (t >= cnt) vis0[t] = vis1[t] = 0u;
         }
         if constexpr (kKv8)
-          rows_page8<true>(page, qh, ql, st, c0, c1, vis0, vis1, lane);
+          rows_block8<true>(page, qf, st, c0, c1, vis0, vis1, lane);
         else
-          rows_page16<true>(page, qf, st, c0, vis0, vis1, lane);
+          rows_block16<true>(page, qf, st, c0, vis0, vis1, lane);
       } else {
+#pragma unroll
+        for (int t = 0; t < kBlockPages; ++t) vis0[t] = vis1[t] = 0xffffu;
         if constexpr (kKv8)
-          rows_page8<false>(page, qh, ql, st, c0, c1, 0xffffu, 0xffffu, lane);
+          rows_block8<false>(page, qf, st, c0, c1, vis0, vis1, lane);
         else
-          rows_page16<false>(page, qf, st, c0, 0xffffu, 0xffffu, lane);
+          rows_block16<false>(page, qf, st, c0, vis0, vis1, lane);
       }
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[s]);
+    if (lane < cnt) mbar_arrive(&empty[(j + lane) % kStages]);
   }
 
 #pragma unroll

@@ -20,7 +20,7 @@ e4m3 codes and one exponent byte, 129 bytes instead of 256:
 
 A row with exponent byte b stands for its codes times 2^(b - 127); b is chosen when the row is written
 (``kv_scatter``, kernel A), from the row's largest magnitude.  The 16-byte chunks of row t are stored
-at chunk ^ (t % 8), the order the kernels read without bank conflicts; ``layer_as_slots`` gives the
+at chunk ^ (t % 2 + 2 (t // 4)), which the kernels read without bank conflicts; ``layer_as_slots`` gives the
 values a layer stands for.
 """
 
@@ -88,16 +88,17 @@ def is_kv8(k_cache: Tensor) -> bool:
 
 
 def _check_kv8_views(k_cache: Tensor, v_cache: Tensor) -> tuple[int, int]:
-    if k_cache.dim() != 4 or tuple(k_cache.shape[2:]) != (BLOCK_SIZE, HEAD_DIM):
+    shape = k_cache.shape
+    if len(shape) != 4 or shape[2] != BLOCK_SIZE or shape[3] != HEAD_DIM:
         raise ValueError(
             "k_cache must be a layer view of miniserve_b200.kv_pool.allocate_kv_cache "
-            f"([blocks, kv_heads, 16, 128] of an 8-bit pool); got shape {tuple(k_cache.shape)}"
+            f"([blocks, kv_heads, 16, 128] of an 8-bit pool); got shape {tuple(shape)}"
         )
-    nb, kvh = int(k_cache.shape[0]), int(k_cache.shape[1])
+    nb, kvh = int(shape[0]), int(shape[1])
     want = (kvh * KV8_PAGE_BYTES, KV8_PAGE_BYTES, HEAD_DIM, 1)
-    if tuple(k_cache.stride()) != want or tuple(v_cache.stride()) != want:
-        raise ValueError(f"KV pool views have strides {tuple(k_cache.stride())}, expected {want}")
-    if (v_cache.dtype != KV8 or v_cache.shape != k_cache.shape
+    if k_cache.stride() != want or v_cache.stride() != want:
+        raise ValueError(f"KV pool views have strides {k_cache.stride()}, expected {want}")
+    if (v_cache.dtype != KV8 or v_cache.shape != shape
             or v_cache.data_ptr() != k_cache.data_ptr() + KV8_ROWS_BYTES):
         raise ValueError("v_cache must be the V half of the same pool as k_cache")
     return nb, kvh
@@ -140,9 +141,9 @@ def _kv8_parts(view: Tensor) -> tuple[Tensor, Tensor]:
 
 
 def _kv8_order(device: torch.device) -> Tensor:
-    """``[16, 8]``: where row t's chunk i is stored (i ^ (t % 8))."""
-    t = torch.arange(BLOCK_SIZE, device=device)[:, None] % 8
-    return torch.arange(8, device=device)[None, :] ^ t
+    """``[16, 8]``: where row t's chunk i is stored (i ^ (t % 2 + 2 (t // 4)))."""
+    t = torch.arange(BLOCK_SIZE, device=device)[:, None]
+    return torch.arange(8, device=device)[None, :] ^ (t % 2 + 2 * (t // 4))
 
 
 def layer_as_slots(view: Tensor) -> Tensor:

@@ -31,12 +31,12 @@ def test_layout_and_size() -> None:
     assert v.data_ptr() - k.data_ptr() == 2048
     assert kv8_bytes_per_token(28, 8) == 2 * 28 * 8 * 129
     assert bool((layer_as_slots(k) == 0).all())
-    # slot 37 = block 2, token 5; its 16-byte chunk 3 lies at chunk 3 ^ 5, its exponent in byte 5.
+    # slot 37 = block 2, token 5; its 16-byte chunk 6 lies at chunk 6 ^ 3, its exponent in byte 5.
     x = torch.randn(80, 3, 128).bfloat16()
     slots_into_layer(k, x)
     codes, e = quantise_rows(x)
     got, exps = _kv8_parts(k)
-    assert torch.equal(got[2, 1, 5, 3 ^ 5], codes[37, 1, 48:64].view(torch.uint8))
+    assert torch.equal(got[2, 1, 5, 6 ^ 3], codes[37, 1, 96:112].view(torch.uint8))
     assert exps[2, 1, 5] == e[37, 1]
     raw = pool[1, 2, 1].view(torch.uint8)
     assert raw[4096 + 5] == e[37, 1]

@@ -97,7 +97,8 @@ typedef struct MsPlanInfo {
                               describe the groups */
   int32_t decode_pages;    /* pages (per KV head) the decode / verify items read, in total */
   int32_t combine_tokens_max; /* most query tokens of one combine record (sizes its grid) */
-  int32_t reserved[3];
+  int32_t n_tc_combine;       /* combine records of tensor-core items: the last ones */
+  int32_t reserved[2];
 } MsPlanInfo;
 
 /* Upper bound on the packed buffer length (int32 elements) for a batch of this size. */
@@ -212,7 +213,9 @@ MS_API int ms_qk_norm_rope_scatter_kv8(const void* qkv, int64_t qkv_row_stride, 
  * needs beside the plan is described by MsKv8Info: ms_kv8_plan_build appends it (host only) to the
  * packed plan, at int offset plan->total_ints of the same buffer (so one upload brings both; the
  * buffer holds ms_kv8_plan_capacity ints beyond the plan), and the attention call gets
- * the uploaded whole.  workspace_bytes >= ms_kv8_workspace_bytes. */
+ * the uploaded whole.  workspace_bytes >= ms_kv8_workspace_bytes; the workspace is zero-filled before
+ * its first use (it holds arrival counters of split tiles, which every call leaves at zero), and calls
+ * that share one are ordered on the GPU. */
 typedef struct MsKv8Info {
   int32_t n_pages;    /* pages (per KV head) expanded for the tensor-core kernel */
   int32_t off_seqs;   /* int offsets in the packed buffer: sequence records whose tables index */
@@ -244,7 +247,8 @@ MS_API int ms_paged_attention_kv8(const void* q, int64_t q_row_stride, void* out
  *
  * The plan is a packed int32 buffer described by MsPlanInfo, as ms_plan_build's (masks included);
  * ms_tree_attention launches it over a bf16 pool, or over an 8-bit pool when v_cache is NULL (k_cache is then
- * the 8-bit layer).  Sequences of at most MS_MAX_TREE_TOKENS drafts. */
+ * the 8-bit layer).  Its workspace of plan->workspace_bytes_per_kv_head * num_kv_heads bytes is
+ * zero-filled before its first use, as ms_paged_attention_kv8's.  Sequences of at most MS_MAX_TREE_TOKENS drafts. */
 #define MS_MAX_TREE_TOKENS 1024
 MS_API int64_t ms_tree_plan_capacity(int32_t num_seqs, const int32_t* num_new,
                                      int64_t total_table_entries);

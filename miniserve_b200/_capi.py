@@ -74,7 +74,8 @@ class MsPlanInfo(C.Structure):
         ("n_cascade", C.c_int32),
         ("decode_pages", C.c_int32),
         ("combine_tokens_max", C.c_int32),
-        ("reserved", C.c_int32 * 3),
+        ("n_tc_combine", C.c_int32),
+        ("reserved", C.c_int32 * 2),
     ]
 
 

@@ -117,21 +117,27 @@ class AttentionMetadata:
             self.slot_mapping.copy_(slot_mapping, non_blocking=True)
         return True
 
-    def workspace(self, num_kv_heads: int, device: torch.device, kv8: bool = False) -> Tensor | None:
-        """Scratch for this step (allocated once, reused by every layer): split-KV partials and,
-        for an 8-bit pool, the expanded pages of tensor-core items."""
-        if kv8 and self.kv8.n_pages:
+    def workspace(self, num_kv_heads: int, device: torch.device, kv8: bool = False,
+                  counters: bool = False) -> Tensor | None:
+        """Scratch for this step (allocated once, reused by every layer): split-KV partials, with
+        ``counters`` the arrival counters of split tiles behind them (zeroed here, left at zero by
+        every call), and for an 8-bit pool the expanded pages of tensor-core items."""
+        key = (device, -num_kv_heads if kv8 else num_kv_heads)  # a tensor's device has its index
+        ws = self._workspace.get(key)
+        if ws is not None:
+            return ws
+        if kv8:
             need = int(_capi.load().ms_kv8_workspace_bytes(C.byref(self.info), C.byref(self.kv8),
                                                            num_kv_heads))
         else:
             need = int(self.info.workspace_bytes_per_kv_head) * num_kv_heads
         if need == 0:
             return None
-        key = (device, -num_kv_heads if kv8 else num_kv_heads)  # a tensor's device has its index
-        ws = self._workspace.get(key)
-        if ws is None:
-            ws = torch.empty(need, dtype=torch.uint8, device=device)
-            self._workspace[key] = ws
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        if counters:
+            at = int(self.info.part_rows) * (HEAD_DIM + 1) * 4 * num_kv_heads
+            ws[at : at + int(self.info.n_combine) * 8 * num_kv_heads].zero_()
+        self._workspace[key] = ws
         return ws
 
 
@@ -345,11 +351,12 @@ def _stream(device: torch.device) -> int:
 
 def _rows(t: Tensor, name: str) -> int:
     """Row stride (elements) of a [T, heads, 128] tensor whose heads are packed in each row."""
-    if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.stride(2) != 1 or t.stride(1) != HEAD_DIM:
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[2] != HEAD_DIM or stride[2] != 1 or stride[1] != HEAD_DIM:
         raise ValueError(f"{name} must be [T, heads, {HEAD_DIM}] with contiguous heads")
     if t.dtype != torch.bfloat16:
         raise ValueError(f"{name} must be bf16")
-    return int(t.stride(0))
+    return stride[0]
 
 
 def kv_scatter(k: Tensor, v: Tensor, slot_mapping: Tensor, k_cache: Tensor, v_cache: Tensor) -> None:
@@ -411,11 +418,10 @@ def kv_gather(slots: Tensor, k_cache: Tensor, v_cache: Tensor, k_out: Tensor | N
     """
     nb, kvh = check_layer_views(k_cache, v_cache, kv8=True)
     n = int(slots.shape[0]) if slots.dim() == 1 else 0
-    shape = (n, kvh, HEAD_DIM)
     if k_out is None:
-        k_out = torch.empty(shape, dtype=torch.bfloat16, device=slots.device)
+        k_out = torch.empty((n, kvh, HEAD_DIM), dtype=torch.bfloat16, device=slots.device)
     if v_out is None:
-        v_out = torch.empty(shape, dtype=torch.bfloat16, device=slots.device)
+        v_out = torch.empty_like(k_out)
     dev = _check_rows_args(k_out, v_out, slots, k_cache, kvh)
     outs = (k_out.data_ptr(), _rows(k_out, "k_out"), v_out.data_ptr(), _rows(v_out, "v_out"),
             _stream(dev))
@@ -475,7 +481,7 @@ def _attend_parts(lib, q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: Attent
     q_args = (q.data_ptr(), _rows(q, "q"), out.data_ptr(), _rows(out, "out"), int(shape[1]), kvh)
     info, tree = meta.info, meta.tree
     if tree is None or info.n_decode_items or info.n_tile_items or info.n_tc_items:
-        ws = meta.workspace(kvh, dev, kv8)
+        ws = meta.workspace(kvh, dev, kv8, kv8)
         ws_args = (0, 0) if ws is None else (ws.data_ptr(), ws.numel())
         if kv8:
             rc = _on_own_device(
@@ -487,7 +493,7 @@ def _attend_parts(lib, q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: Attent
                 meta.plan.data_ptr(), C.byref(info), *ws_args, scale, stream)
         _capi.check(rc, "paged_attention")
     if tree is not None:
-        ws = tree.workspace(kvh, dev)
+        ws = tree.workspace(kvh, dev, counters=True)
         ws_args = (0, 0) if ws is None else (ws.data_ptr(), ws.numel())
         rc = _on_own_device(
             lib.ms_tree_attention, dev, *q_args, k_cache.data_ptr(),

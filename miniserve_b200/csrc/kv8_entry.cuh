@@ -81,6 +81,41 @@ ms::AttnArgs attn_args(const void* q, int64_t q_row_stride, void* out, int64_t o
   return a;
 }
 
+// Kernel F over the plan's narrow items (decode rows, trees of up to 8 drafts) and its wide ones
+// (chunks of up to 64 tokens as two halves of 32, larger trees).
+template <bool kKv8, bool kTree>
+cudaError_t launch_rows_attention(const ms::AttnArgs& a, const void* pool, const CUtensorMap& map,
+                                  const int32_t* plan_dev, const MsPlanInfo* plan, cudaStream_t s) {
+  ms::RowsArgs r;
+  r.a = a;
+  r.pool = static_cast<const uint8_t*>(pool);
+  r.plan = plan_dev;
+  r.combines = plan_dev + plan->off_combine;
+  // Arrival counters lie behind the partials.
+  r.arrived = a.ws_lse != nullptr ? reinterpret_cast<int*>(a.ws_lse + plan->part_rows * a.num_kv)
+                                  : nullptr;
+  cudaError_t e = cudaSuccess;
+  if (plan->n_decode_items > 0) {
+    using Cfg = ms::RowsCfg<kKv8, 1>;
+    r.halves = 1;
+    r.a.items = plan_dev + plan->off_decode;
+    r.a.n_items = plan->n_decode_items;
+    e = launch(ms::rows_attn_kernel<kKv8, kTree, 1>,
+               static_cast<unsigned>(plan->n_decode_items * a.num_kv), Cfg::kThreads,
+               Cfg::kSmemBytes, s, map, r);
+  }
+  if (e == cudaSuccess && plan->n_tile_items > 0) {
+    using Cfg = ms::RowsCfg<kKv8, 2>;
+    r.halves = kTree ? 1 : 2;
+    r.a.items = plan_dev + plan->off_tile;
+    r.a.n_items = plan->n_tile_items;
+    e = launch(ms::rows_attn_kernel<kKv8, kTree, 2>,
+               static_cast<unsigned>(plan->n_tile_items * r.halves * a.num_kv), Cfg::kThreads,
+               Cfg::kSmemBytes, s, map, r);
+  }
+  return e;
+}
+
 template <typename K, typename... Args>
 cudaError_t launch_plain(K kernel, unsigned grid, unsigned block, size_t smem, cudaStream_t s,
                          Args... args) {
@@ -276,8 +311,8 @@ extern "C" int ms_paged_attention_kv8(const void* q, int64_t q_row_stride, void*
       set_error("ms_paged_attention_kv8: plan too large for one launch");
       return MS_ERR_ARG;
     }
-    const int64_t part = plan->workspace_bytes_per_kv_head * num_kv_heads;
-    pages = static_cast<char*>(workspace) + (part + 1023) / 1024 * 1024;
+    pages = static_cast<char*>(workspace) + need - static_cast<int64_t>(info->n_pages) * num_kv_heads *
+                                                       ms::kPageKVBytes;
     rc = kv_tensor_map(pages, info->n_pages, num_kv_heads, 1, &kmap);
     if (rc) return rc;
     rc = kv_tensor_map(pages, info->n_pages, num_kv_heads, 2, &vmap);
@@ -325,21 +360,9 @@ extern "C" int ms_paged_attention_kv8(const void* q, int64_t q_row_stride, void*
     }
   }
   if (n_rows > 0) {
-    // Decode items (one tile each) and chunk items (two tiles of 32 tokens) in one launch: their
-    // records are adjacent in the plan.
-    ms::RowsArgs r;
-    r.a = a;
-    r.a.items = plan_dev + plan->off_decode;
-    r.a.n_items = n_rows;
-    r.pool = static_cast<const uint8_t*>(pool);
-    r.plan = plan_dev;
-    r.n_single = plan->n_decode_items;
     CUtensorMap none;
     std::memset(&none, 0, sizeof(none));
-    const unsigned grid =
-        static_cast<unsigned>((plan->n_decode_items + 2 * plan->n_tile_items) * num_kv_heads);
-    const cudaError_t e = launch(ms::rows_attn_kernel<true, false>, grid, ms::kRowsThreads,
-                                 ms::RowsCfg<true>::kSmemBytes, ds, none, r);
+    const cudaError_t e = launch_rows_attention<true, false>(a, pool, none, plan_dev, plan, ds);
     if (e != cudaSuccess) {
       join();
       return cuda_fail("8-bit rows launch", e);
@@ -349,7 +372,11 @@ extern "C" int ms_paged_attention_kv8(const void* q, int64_t q_row_stride, void*
     const cudaError_t e = join();
     if (e != cudaSuccess) return cuda_fail("join of the side stream", e);
   }
-  return launch_combine(a, plan, plan_dev, s);
+  // Kernel F merges its own splits; the tensor-core items' records are the last ones.
+  MsPlanInfo tc = *plan;
+  tc.off_combine += (plan->n_combine - plan->n_tc_combine) * 8;
+  tc.n_combine = plan->n_tc_combine;
+  return launch_combine(a, &tc, plan_dev, s);
 }
 
 extern "C" int ms_tree_attention(const void* q, int64_t q_row_stride, void* out,
@@ -358,7 +385,7 @@ extern "C" int ms_tree_attention(const void* q, int64_t q_row_stride, void* out,
                                  const int32_t* plan_dev, const MsPlanInfo* plan, void* workspace,
                                  int64_t workspace_bytes, float scale, void* stream) {
   const char* what = "ms_tree_attention";
-  if (plan != nullptr && plan->n_tile_items == 0) return MS_OK;
+  if (plan != nullptr && plan->n_decode_items + plan->n_tile_items == 0) return MS_OK;
   const int64_t need = plan != nullptr ? plan->workspace_bytes_per_kv_head * num_kv_heads : 0;
   int rc = check_attention(what, q, q_row_stride, out, out_row_stride, num_heads, num_kv_heads,
                            plan_dev, plan, workspace, workspace_bytes, need, scale);
@@ -369,27 +396,18 @@ extern "C" int ms_tree_attention(const void* q, int64_t q_row_stride, void* out,
   if (rc) return rc;
   rc = ensure_smem_attrs();
   if (rc) return rc;
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  ms::RowsArgs r;
-  r.a = attn_args(q, q_row_stride, out, out_row_stride, num_kv_heads, num_blocks, plan_dev, plan,
-                  workspace, scale);
-  r.a.items = plan_dev + plan->off_tile;
-  r.a.n_items = plan->n_tile_items;
-  r.pool = kv8 ? static_cast<const uint8_t*>(k_cache) : nullptr;
-  r.plan = plan_dev;
-  r.n_single = plan->n_tile_items;
   CUtensorMap map;
   std::memset(&map, 0, sizeof(map));
   if (!kv8) {
     rc = kv_tensor_map(k_cache, num_blocks, num_kv_heads, 0, &map);
     if (rc) return rc;
   }
-  const unsigned grid = static_cast<unsigned>(plan->n_tile_items * num_kv_heads);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const ms::AttnArgs a = attn_args(q, q_row_stride, out, out_row_stride, num_kv_heads, num_blocks,
+                                   plan_dev, plan, workspace, scale);
   const cudaError_t e =
-      kv8 ? launch(ms::rows_attn_kernel<true, true>, grid, ms::kRowsThreads,
-                   ms::RowsCfg<true>::kSmemBytes, s, map, r)
-          : launch(ms::rows_attn_kernel<false, true>, grid, ms::kRowsThreads,
-                   ms::RowsCfg<false>::kSmemBytes, s, map, r);
+      kv8 ? launch_rows_attention<true, true>(a, k_cache, map, plan_dev, plan, s)
+          : launch_rows_attention<false, true>(a, nullptr, map, plan_dev, plan, s);
   if (e != cudaSuccess) return cuda_fail("tree attention launch", e);
-  return launch_combine(r.a, plan, plan_dev, s);
+  return MS_OK;
 }

@@ -247,12 +247,29 @@ static int ensure_smem_attrs() {
   auto rows_attr = [](auto kernel, int bytes) {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   };
-  e = rows_attr(ms::rows_attn_kernel<true, false>, ms::RowsCfg<true>::kSmemBytes);
+  e = rows_attr(ms::rows_attn_kernel<true, false, 1>, ms::RowsCfg<true, 1>::kSmemBytes);
   if (e == cudaSuccess)
-    e = rows_attr(ms::rows_attn_kernel<true, true>, ms::RowsCfg<true>::kSmemBytes);
+    e = rows_attr(ms::rows_attn_kernel<true, true, 1>, ms::RowsCfg<true, 1>::kSmemBytes);
   if (e == cudaSuccess)
-    e = rows_attr(ms::rows_attn_kernel<false, true>, ms::RowsCfg<false>::kSmemBytes);
-  if (e != cudaSuccess) return cuda_fail("cudaFuncSetAttribute(rows)", e);
+    e = rows_attr(ms::rows_attn_kernel<false, true, 1>, ms::RowsCfg<false, 1>::kSmemBytes);
+  // The wide forms move registers between their warpgroups (see the tensor-core kernel above).
+  auto wide_attr = [&](auto kernel, int bytes, int need) {
+    cudaFuncAttributes fa{};
+    cudaError_t r = cudaFuncGetAttributes(&fa, kernel);
+    if (r != cudaSuccess) return r;
+    if (fa.numRegs < need) return cudaErrorInvalidKernelImage;
+    return rows_attr(kernel, bytes);
+  };
+  if (e == cudaSuccess)
+    e = wide_attr(ms::rows_attn_kernel<true, false, 2>, ms::RowsCfg<true, 2>::kSmemBytes,
+                  ms::RowsCfg<true, 2>::kLaunchRegs);
+  if (e == cudaSuccess)
+    e = wide_attr(ms::rows_attn_kernel<true, true, 2>, ms::RowsCfg<true, 2>::kSmemBytes,
+                  ms::RowsCfg<true, 2>::kLaunchRegs);
+  if (e == cudaSuccess)
+    e = wide_attr(ms::rows_attn_kernel<false, true, 2>, ms::RowsCfg<false, 2>::kSmemBytes,
+                  ms::RowsCfg<false, 2>::kLaunchRegs);
+  if (e != cudaSuccess) return cuda_fail("attributes of the rows kernel", e);
   done[dev] = true;
   return MS_OK;
 }

@@ -246,7 +246,8 @@ extern "C" int ms_plan_build(int32_t num_seqs, const int32_t* flat_start, const 
     }
   }
 
-  std::vector<Item> dec, til, tcv, comb;
+  // Combine records: those of decode and chunk items first, then the tensor-core items'.
+  std::vector<Item> dec, til, tcv, comb, comb_tc;
   int64_t part_rows = 0;
   int64_t n_tc_tiles = 0, tc_pages = 0;
   for (const Item& t : tiles) {
@@ -344,7 +345,7 @@ extern "C" int ms_plan_build(int32_t num_seqs, const int32_t* flat_start, const 
                      static_cast<int>(part_rows + static_cast<int64_t>(s) * rows), tok_b, n_b});
       pb += len;
     }
-    comb.push_back({t.seq, t.tok0, t.n_q, static_cast<int>(part_rows), ns, 0});
+    (is_tc ? comb_tc : comb).push_back({t.seq, t.tok0, t.n_q, static_cast<int>(part_rows), ns, 0});
     part_rows += static_cast<int64_t>(ns) * rows;
   }
   // Cascade groups.  The shared prefix is attended once by tensor-core items over a virtual
@@ -376,6 +377,8 @@ extern "C" int ms_plan_build(int32_t num_seqs, const int32_t* flat_start, const 
       dec.push_back({k, 0, n, G.pages, pages, -1, static_cast<int>(prefix_row), 1});
     }
   }
+
+  comb.insert(comb.end(), comb_tc.begin(), comb_tc.end());
 
   auto longest_first = [](const Item& x, const Item& y) { return (x.pe - x.pb) > (y.pe - y.pb); };
   std::stable_sort(dec.begin(), dec.end(), longest_first);
@@ -409,6 +412,9 @@ extern "C" int ms_plan_build(int32_t num_seqs, const int32_t* flat_start, const 
     r[4] = static_cast<int32_t>(table_offsets[i]);
     r[5] = static_cast<int32_t>(table_offsets[i + 1] - table_offsets[i]);
   }
+  // Field 6 of a sequence whose one decode or chunk tile is split: its combine record.
+  for (size_t k = 0; k + comb_tc.size() < comb.size(); ++k)
+    out[off_seqs + static_cast<int64_t>(comb[k].seq) * kRec + 6] = static_cast<int32_t>(k);
   for (size_t g = 0; g < groups.size(); ++g) {
     const Group& G = groups[g];
     int32_t* r = out + off_seqs + (static_cast<int64_t>(num_seqs) + static_cast<int64_t>(g)) * kRec;
@@ -463,6 +469,7 @@ extern "C" int ms_plan_build(int32_t num_seqs, const int32_t* flat_start, const 
   int combine_tokens_max = 0;
   for (const Item& c : comb) combine_tokens_max = std::max(combine_tokens_max, c.n_q);
   info->combine_tokens_max = combine_tokens_max;
+  info->n_tc_combine = static_cast<int32_t>(comb_tc.size());
   info->off_tc = static_cast<int32_t>(off_tc);
   info->off_combine = static_cast<int32_t>(off_combine);
   info->total_ints = static_cast<int32_t>(total);

@@ -1,14 +1,14 @@
 // Kernel F: paged attention of up to 32 query tokens per work item, through an 8-bit pool (decode
 // rows, verify rows, chunks of up to 64 tokens) or over a tree of drafted tokens (bf16 or 8-bit pool).
 //
-// One CTA owns (item, KV head): query rows r = token * 2 + head-in-pair, up to 64 of them, against
-// a contiguous range of the sequence's pages.  A producer warp streams whole pages (K and V of
-// this head) into a ring; four consumer warps form R row groups of 16 rows (R = 1, 2 or 4, the
-// smallest that holds the rows) times 4 / R page phases, so a short tile still uses every warp: warp
-// w takes row group w % R and the page pairs i with i % (4 / R) == w / R.  The phases merge through the
-// idle ring at the end.
+// One CTA owns (item, KV head): query rows r = token * 2 + head-in-pair against a contiguous range of
+// the sequence's pages.  A producer warp streams whole pages (K and V of this head) into a ring; four
+// consumer warps, kRG row groups of 16 rows each, form S = 1 or 2 row sets times 4 / S page phases,
+// so a short tile still uses every warp: warp w takes row set w % S and the page pairs i with
+// i % (4 / S) == w / S.  The phases merge through the idle ring at the end; the CTA that finishes last of
+// a tile whose pages are split over several merges their partials (in the order of the splits).
 //
-// The mathematics per page (16 keys), in the exp2 domain with an online softmax:
+// The mathematics per pair of pages (32 keys), in the exp2 domain with an online softmax:
 //   S = Q K^T, p = 2^(S c - m) with c = scale log2(e), l += p, O += p V, out = O / l.
 // A tree token sees the cached context and the drafts its mask names (ancestors and itself); a row
 // that sees nothing writes zeros.
@@ -17,8 +17,8 @@
 //
 // 8-bit pool: mma.sync m16n8k16 with f16 operands.  e4m3 codes are f16 values, so they are converted
 // exactly, two codes per instruction, after ldmatrix has brought them (16-bit units of two codes)
-// to the lanes.  K: a lane's word is four neighbouring dims of one key; the query fragments are
-// loaded in that order of dims, so two conversions give a B operand.  V: ldmatrix.trans
+// to the lanes.  K: a lane's word is four neighbouring dims of one key; the query rows lie in shared
+// memory in that order of dims, so two conversions give a B operand.  V: ldmatrix.trans
 // leaves two neighbouring columns of two neighbouring tokens in a word; one byte permute and two
 // conversions give the operands of two column tiles (even and odd columns).  The query row (bf16, 8
 // significant bits) is scaled by a power of two into f16's range: exact down to 2^-33 of its
@@ -29,37 +29,58 @@
 // exceeds it by more than 7, as the running maximum is raised only beyond 2^8, so a product stays
 // below 2^15).  f16 keeps 11 bits of p, three more than the bf16 form; what it drops lies 2^-40
 // below the largest p 2^b.
+//
+// Why this shape.  A decode row needs its bytes and little else: up to 32 rows per CTA, three CTAs per SM
+// at 128 registers (the query rows stay in shared memory and are read again for every pair of pages).
+// Tiles of more than 16 tokens are bound by the conversions and the products, so a warp holds two row
+// groups (kRG = 2) and uses each converted operand twice; that takes more than 168 registers, which
+// two CTAs of two warpgroups have once the producer's warpgroup hands its share to the consumers.
 #pragma once
 
 #include "kv8.cuh"
 #include "paged_attention.cuh"
+#include "tc_common.cuh"
 
 namespace ms {
 
-constexpr int kRowsWarps = 4;                        // consumer warps
-constexpr int kRowsThreads = (kRowsWarps + 1) * 32;  // and one producer warp
-constexpr int kRowsTokens = 32;                      // query tokens of a work item (64 rows)
+constexpr int kRowsWarps = 4;        // consumer warps
+constexpr int kRowsTokens = 32;      // query tokens of a wide work item (64 rows)
+constexpr int kRowsNarrowTokens = 16;  // of a narrow one (32 rows)
 
 struct RowsArgs {
   AttnArgs a;           // queries, output, plan sections, partials
   const uint8_t* pool;  // 8-bit layer (null for a bf16 pool, which the tensor map describes)
   const int* plan;      // start of the packed plan: tree masks are at sequence record field 6
-  int n_single;         // items of one tile; the items after them are two tiles of 32 tokens
+  const int* combines;  // combine records of split tiles: a tree item names its record in field 6, a
+                        // causal sequence (which has one tile) in its sequence record's field 6
+  int* arrived;         // [record][2 halves][KVH] splits that have finished: zero between calls
+  int halves;           // 2: an item is two tiles of 32 tokens (chunks of up to 64), else 1
 };
 
-template <bool kKv8>
+template <bool kKv8, int kRG>
 struct RowsCfg {
   static constexpr int kPage = kKv8 ? kPage8Bytes : kPageKVBytes;
   // A multiple of 8: a slot's previous fill is then a page of the same phase (the parity waits
   // are exact only then).
   static constexpr int kStages = kKv8 ? 16 : 8;
   static constexpr int kBatch = 4;  // pages the producer's lanes issue side by side
-  static_assert(kStages % kBatch == 0 && kBatch <= 32, "a lane's pages reuse the same slots");
+  static_assert(kStages % 8 == 0 && kStages % kBatch == 0, "slots are reused by the same lane, warp");
   static constexpr int kStageBytes = kStages * kPage;
-  // Merge scratch in the ring: per warp 16 column tiles and (m, l), a float4 per lane each.
+  // Merge scratch in the ring: per warp 16 column tiles and (m, l) of one row group, a float4 per
+  // lane each.
   static_assert(kRowsWarps * 17 * 32 * 16 <= kStageBytes, "merge scratch reuses the ring");
-  static constexpr int kBarOffset = kStageBytes;
+  static constexpr int kRows = kRG == 1 ? 32 : 64;
+  static constexpr int kQOffset = (kStageBytes + 127) / 128 * 128;
+  static constexpr int kScaleOffset = kQOffset + kRows * kHeadDim * 2;  // the rows' query scales
+  static constexpr int kBarOffset = kScaleOffset + kRows * 4;
   static constexpr int kSmemBytes = 1024 + kBarOffset + 2 * kStages * 8 + 16;
+  // kRG == 1: four consumer warps and a producer warp, three CTAs per SM.  kRG == 2: a consumer
+  // warpgroup and a producer warpgroup (one warp of it works), two CTAs per SM launched with 128
+  // registers per thread: 128 x 232 + 128 x 24 = 256 x 128.
+  static constexpr int kThreads = kRG == 1 ? (kRowsWarps + 1) * 32 : 256;
+  static constexpr int kCtasPerSm = kRG == 1 ? 3 : 2;
+  static constexpr int kLaunchRegs = 128, kConsumerRegs = 232, kProducerRegs = 24;
+  static_assert(128 * (kConsumerRegs + kProducerRegs) <= 256 * kLaunchRegs, "register split");
 };
 
 // ---- small pieces -----------------------------------------------------------------------------
@@ -76,6 +97,19 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t w;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(addr));
+  return w;
+}
+
+// 2^(b - 127) of byte i of a word of exponent bytes (infinity for 255, 0 for 0).
+template <int i>
+__device__ __forceinline__ float scale_of_byte(uint32_t w) {
+  const uint32_t m = i == 3 ? w >> 1 : w << (23 - 8 * i);
+  return __uint_as_float(m & 0x7f800000u);
 }
 
 // Which of a page's 16 keys (bit k: key0 + k) the query at position qpos sees: keys 0..qpos.
@@ -96,46 +130,33 @@ __device__ __forceinline__ uint32_t tree_bits(const int* row, int words, int fir
   return bits & 0xffffu;
 }
 
-// Per-thread state of one row group: rows r0 = lane / 4 and r1 = r0 + 8 of the group.
+// A warp takes two pages (32 keys) at a time: the products of one page hide the latencies of the
+// other, and one maximum, one vote and one rescale serve both.
+constexpr int kBlockPages = 2;
+
+// A thread's state: rows lane / 4 and lane / 4 + 8 of each of its warp's row groups.
+template <int kRG>
 struct RowsState {
-  float o[16][4];
-  float m[2], l[2];
-  int eb;      // 8-bit pool: the exponent byte E that O is held against
+  float o[kRG][16][4];
+  float m[kRG][2], l[kRG][2];
+  int eb;        // 8-bit pool: the exponent byte E that O is held against
   float inv_e;   // 2^(127 - E)
   uint32_t hot;  // E + 7 in every byte (0 while E is unset)
 };
 
-// A warp takes two pages (32 keys) at a time: the products of one page hide the latencies of the
-// other, and one maximum, one vote and one rescale serve both (256 decode rows over an 8-bit pool:
-// 219 us page by page).
-constexpr int kBlockPages = 2;
-
 // Raises the running maxima to the block's (mx, in exp2 units) where they exceed them by 2^8, and,
 // for an 8-bit pool, E to the block's largest exponent byte (vw: this thread's exponent words,
 // invisible keys as 0) where that exceeds it by 7; O and l follow.
-template <bool kKv8>
-__device__ __forceinline__ void raise(RowsState& st, float mx0, float mx1,
+template <bool kKv8, int kRG>
+__device__ __forceinline__ void raise(RowsState<kRG>& st, const float (&mx)[kRG][2],
                                       const uint32_t (&vw)[kBlockPages]) {
-  const bool up0 = mx0 > st.m[0] + 8.f, up1 = mx1 > st.m[1] + 8.f;
-  bool hot = false;
-  uint32_t top4 = 0;
-  if constexpr (kKv8) {
-    top4 = __vmaxu4(vw[0], vw[1]);
-    // Any byte above E + 7 (E >= 0 once set; an unset E lets everything through).
-    hot = __vcmpgtu4(top4, st.hot) != 0;
-  }
-  if (!__any_sync(0xffffffffu, up0 || up1 || hot)) return;
-  float al0 = 1.f, al1 = 1.f;
-  if (up0) {
-    al0 = fast_exp2(st.m[0] - mx0);
-    st.m[0] = mx0;
-  }
-  if (up1) {
-    al1 = fast_exp2(st.m[1] - mx1);
-    st.m[1] = mx1;
-  }
-  st.l[0] *= al0;
-  st.l[1] *= al1;
+  bool up = false;
+#pragma unroll
+  for (int g = 0; g < kRG; ++g) up = up || mx[g][0] > st.m[g][0] + 8.f || mx[g][1] > st.m[g][1] + 8.f;
+  // Any byte above E + 7 (an unset E lets everything through).
+  if constexpr (kKv8) up = up || __vcmpgtu4(__vmaxu4(vw[0], vw[1]), st.hot) != 0;
+  if (!__any_sync(0xffffffffu, up)) return;
+  float f = 1.f;
   if constexpr (kKv8) {
     // The largest exponent of a finite row (a NaN row's 255 does not move E: it acts through its
     // infinite factor, and only on the rows that see it).
@@ -151,103 +172,141 @@ __device__ __forceinline__ void raise(RowsState& st, float mx0, float mx1,
     top = __reduce_max_sync(0xffffffffu, top);
     if (top > st.eb + 7 || st.eb < 0) {
       const int d = st.eb - top + kExpBias;  // 2^(E_old - E_new); O is still zero when E was unset
-      const float f = d <= 0 ? 0.f : __int_as_float(d << 23);
-      al0 *= f;
-      al1 *= f;
+      f = d <= 0 ? 0.f : __int_as_float(d << 23);
       st.eb = top;
       st.inv_e = __int_as_float((2 * kExpBias - top) << 23);
       st.hot = static_cast<uint32_t>(min(top + 7, 255)) * 0x01010101u;
     }
   }
 #pragma unroll
-  for (int n = 0; n < 16; ++n) {
-    st.o[n][0] *= al0;
-    st.o[n][1] *= al0;
-    st.o[n][2] *= al1;
-    st.o[n][3] *= al1;
+  for (int g = 0; g < kRG; ++g) {
+    float al[2] = {1.f, 1.f};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (mx[g][h] > st.m[g][h] + 8.f) {
+        al[h] = fast_exp2(st.m[g][h] - mx[g][h]);
+        st.m[g][h] = mx[g][h];
+      }
+      st.l[g][h] *= al[h];
+      al[h] *= f;
+    }
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+      st.o[g][n][0] *= al[0];
+      st.o[g][n][1] *= al[0];
+      st.o[g][n][2] *= al[1];
+      st.o[g][n][3] *= al[1];
+    }
   }
 }
 
-// Row maxima of the block over the quad that holds a row.
-__device__ __forceinline__ void block_max(const float (&s)[2 * kBlockPages][4], float& mx0,
-                                          float& mx1) {
-  mx0 = fmaxf(s[0][0], s[0][1]);
-  mx1 = fmaxf(s[0][2], s[0][3]);
+// Row maxima of a row group's block over the quad that holds a row.
+__device__ __forceinline__ void block_max(const float (&s)[2 * kBlockPages][4], float (&mx)[2]) {
+  mx[0] = fmaxf(s[0][0], s[0][1]);
+  mx[1] = fmaxf(s[0][2], s[0][3]);
 #pragma unroll
   for (int t = 1; t < 2 * kBlockPages; ++t) {
-    mx0 = fmaxf(mx0, fmaxf(s[t][0], s[t][1]));
-    mx1 = fmaxf(mx1, fmaxf(s[t][2], s[t][3]));
+    mx[0] = fmaxf(mx[0], fmaxf(s[t][0], s[t][1]));
+    mx[1] = fmaxf(mx[1], fmaxf(s[t][2], s[t][3]));
   }
-  mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-  mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-  mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-  mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+#pragma unroll
+  for (int off = 1; off <= 2; ++off) {
+    mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], off));
+    mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], off));
+  }
 }
 
 // p = 2^(s c - m) in place, and its sums into l.
-__device__ __forceinline__ void block_exp(float (&s)[2 * kBlockPages][4], float c0, float c1,
-                                          RowsState& st) {
-  const float mu0 = st.m[0] == -INFINITY ? 0.f : st.m[0];
-  const float mu1 = st.m[1] == -INFINITY ? 0.f : st.m[1];
+__device__ __forceinline__ void block_exp(float (&s)[2 * kBlockPages][4], const float (&c)[2],
+                                          const float (&m)[2], float (&l)[2]) {
+  const float mu0 = m[0] == -INFINITY ? 0.f : m[0];
+  const float mu1 = m[1] == -INFINITY ? 0.f : m[1];
   float l0 = 0.f, l1 = 0.f;
 #pragma unroll
   for (int t = 0; t < 2 * kBlockPages; ++t) {
-    s[t][0] = fast_exp2(__fmaf_rn(s[t][0], c0, -mu0));
-    s[t][1] = fast_exp2(__fmaf_rn(s[t][1], c0, -mu0));
-    s[t][2] = fast_exp2(__fmaf_rn(s[t][2], c1, -mu1));
-    s[t][3] = fast_exp2(__fmaf_rn(s[t][3], c1, -mu1));
+    s[t][0] = fast_exp2(__fmaf_rn(s[t][0], c[0], -mu0));
+    s[t][1] = fast_exp2(__fmaf_rn(s[t][1], c[0], -mu0));
+    s[t][2] = fast_exp2(__fmaf_rn(s[t][2], c[1], -mu1));
+    s[t][3] = fast_exp2(__fmaf_rn(s[t][3], c[1], -mu1));
     l0 += s[t][0] + s[t][1];
     l1 += s[t][2] + s[t][3];
   }
-  st.l[0] += l0;
-  st.l[1] += l1;
+  l[0] += l0;
+  l[1] += l1;
 }
 
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-  uint32_t w;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(addr));
-  return w;
+// Scores of key column col (0..15) of page t that a row does not see become -infinity.
+// vis[g][h]: bit 16 t + k: row (g, h) sees key k of page t.  kCol1: the second column tile's first key.
+template <int kCol1>
+__device__ __forceinline__ void mask_block(float (&s)[2 * kBlockPages][4], const uint32_t (&vis)[2],
+                                           int col0) {
+#pragma unroll
+  for (int t = 0; t < kBlockPages; ++t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = vis[i >> 1] >> (16 * t + col0);
+      if (!(v >> (i & 1) & 1u)) s[2 * t][i] = -INFINITY;
+      if (!(v >> (kCol1 + (i & 1)) & 1u)) s[2 * t + 1][i] = -INFINITY;
+    }
+  }
 }
 
-// 2^(b - 127) of byte i of a word of exponent bytes (infinity for 255, 0 for 0).
-template <int i>
-__device__ __forceinline__ float scale_of_byte(uint32_t w) {
-  const uint32_t m = i == 3 ? w >> 1 : w << (23 - 8 * i);
-  return __uint_as_float(m & 0x7f800000u);
+// Keys that some row of the warp sees, both pages.
+template <int kRG>
+__device__ __forceinline__ uint32_t seen_by_any(const uint32_t (&vis)[kRG][2]) {
+  uint32_t v = 0;
+#pragma unroll
+  for (int g = 0; g < kRG; ++g) v |= vis[g][0] | vis[g][1];
+  return __reduce_or_sync(0xffffffffu, v);
 }
 
 // ---- two pages, 8-bit pool ----------------------------------------------------------------------
 
-// qf: the query rows' fragments, f16, dims 16 ks + 4 (lane % 4) .. + 3 of rows r0, r1.  c0, c1: scale
-// log2(e) times the rows' query scale.  Key column j of tile t (of two per page) is token
-// 4 (j / 2) + j % 2 + 2 t, so a thread's four keys of a page are neighbours (4 (lane % 4) .. + 3) and
-// their exponent bytes one word.  Accumulator tile 2u + p holds columns 16u + 2j + p, so a thread's
-// o[2u][0], o[2u + 1][0], o[2u][1], o[2u + 1][1] are four neighbouring columns.  vis: bit k of page t
-// in vis[t] (kMask only).
-template <bool kMask>
-__device__ __forceinline__ void rows_block8(const uint32_t (&page)[kBlockPages],
-                                            const uint32_t (&qf)[8][4], RowsState& st, float c0,
-                                            float c1, const uint32_t (&vis0)[kBlockPages],
-                                            const uint32_t (&vis1)[kBlockPages], int lane) {
+// q: shared address of this lane's ldmatrix row of the warp's first row group (f16, the dims of a
+// 16-dim chunk in the order 0 1 4 5 8 9 12 13 2 3 6 7 10 11 14 15, so that a lane's fragment is the dims
+// 4 (lane % 4) .. + 3 that its word of codes holds).  c: scale log2(e) times the rows' query scale.
+// Key column j of tile t (of two per page) is token 4 (j / 2) + j % 2 + 2 t, so a thread's four
+// keys of a page are neighbours (4 (lane % 4) .. + 3) and their exponent bytes one word.  Accumulator
+// tile 2u + p holds columns 16u + 2j + p, so a thread's o[2u][0], o[2u + 1][0], o[2u][1],
+// o[2u + 1][1] are four neighbouring columns.
+template <int kRG, bool kMask>
+__device__ __forceinline__ void rows_block8(const uint32_t (&page)[kBlockPages], uint32_t q,
+                                            RowsState<kRG>& st, const float (&c)[kRG][2],
+                                            const uint32_t (&vis)[kRG][2], int lane) {
   const int mi = lane >> 3, t8 = lane & 7, q4 = 4 * (lane & 3);
   const int tok = 4 * (t8 >> 1) + (t8 & 1);  // this lane's ldmatrix row in tile 0
   const int sw = code_swizzle8(tok);         // the same for tok + 2
-  float s[2 * kBlockPages][4];
+  float s[kRG][2 * kBlockPages][4];
 #pragma unroll
-  for (int t = 0; t < 2 * kBlockPages; ++t) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[t][i] = 0.f;
-  }
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  for (int g = 0; g < kRG; ++g) {
 #pragma unroll
     for (int t = 0; t < 2 * kBlockPages; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[g][t][i] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {  // 32 dims at a time
+    uint32_t qa[kRG][2][4];
+#pragma unroll
+    for (int g = 0; g < kRG; ++g) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        ldsm_x4(q + g * (16 * kHeadDim * 2) + (((2 * (2 * u + i) + (mi >> 1)) ^ t8) << 4),
+                qa[g][i][0], qa[g][i][1], qa[g][i][2], qa[g][i][3]);
+    }
+#pragma unroll
+    for (int t = 0; t < kBlockPages; ++t) {
+      // Both key tiles of the page, chunks 2u and 2u + 1.
       uint32_t b[4];
-      ldsm_x4(page[t >> 1] + (tok + 2 * (t & 1)) * kRow8Bytes + (((4 * u + mi) ^ sw) << 4), b[0],
+      ldsm_x4(page[t] + (tok + 2 * (mi >> 1)) * kRow8Bytes + (((2 * u + (mi & 1)) ^ sw) << 4), b[0],
               b[1], b[2], b[3]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        mma_f16(s[t], qf[4 * u + i], e4m3x2_to_f16x2<0>(b[i]), e4m3x2_to_f16x2<1>(b[i]));
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t b0 = e4m3x2_to_f16x2<0>(b[i]), b1 = e4m3x2_to_f16x2<1>(b[i]);
+#pragma unroll
+        for (int g = 0; g < kRG; ++g) mma_f16(s[g][2 * t + (i >> 1)], qa[g][i & 1], b0, b1);
+      }
     }
   }
   uint32_t vw[kBlockPages], keep[kBlockPages][2];
@@ -258,50 +317,67 @@ __device__ __forceinline__ void rows_block8(const uint32_t (&page)[kBlockPages],
     const float f[4] = {scale_of_byte<0>(kw), scale_of_byte<1>(kw), scale_of_byte<2>(kw),
                         scale_of_byte<3>(kw)};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[2 * t][i] *= f[i & 1];
-      s[2 * t + 1][i] *= f[2 + (i & 1)];
-    }
-    if constexpr (kMask) {
-      // Rows of keys no row here sees may hold anything (pages of a finished sequence, unused
-      // drafts, a second page that is not there): their values and exponents become zero.
-      const uint32_t v0 = vis0[t] >> q4, v1 = vis1[t] >> q4;
-      const uint32_t any = __reduce_or_sync(0xffffffffu, vis0[t] | vis1[t]) >> q4;
-      keep[t][0] = (any & 1u ? 0xffffu : 0u) | (any & 2u ? 0xffff0000u : 0u);
-      keep[t][1] = (any & 4u ? 0xffffu : 0u) | (any & 8u ? 0xffff0000u : 0u);
-      vw[t] &= (any & 1u ? 0xffu : 0u) | (any & 2u ? 0xff00u : 0u) | (any & 4u ? 0xff0000u : 0u) |
-               (any & 8u ? 0xff000000u : 0u);
+    for (int g = 0; g < kRG; ++g) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t v = (i & 2) ? v1 : v0;
-        if (!(v >> (i & 1) & 1u)) s[2 * t][i] = -INFINITY;
-        if (!(v >> (2 + (i & 1)) & 1u)) s[2 * t + 1][i] = -INFINITY;
+        s[g][2 * t][i] *= f[i & 1];
+        s[g][2 * t + 1][i] *= f[2 + (i & 1)];
       }
     }
   }
-  float mx0, mx1;
-  block_max(s, mx0, mx1);
-  raise<true>(st, mx0 * c0, mx1 * c1, vw);
-  block_exp(s, c0, c1, st);
-  const int vtok = tok + 2 * (mi & 1);
+  if constexpr (kMask) {
+    // Rows of keys no row here sees may hold anything (pages of a finished sequence, unused
+    // drafts, a second page that is not there): their values and exponents become zero.
+    const uint32_t any = seen_by_any<kRG>(vis) >> q4;
+#pragma unroll
+    for (int t = 0; t < kBlockPages; ++t) {
+      const uint32_t a = any >> (16 * t);
+      keep[t][0] = (a & 1u ? 0xffffu : 0u) | (a & 2u ? 0xffff0000u : 0u);
+      keep[t][1] = (a & 4u ? 0xffffu : 0u) | (a & 8u ? 0xffff0000u : 0u);
+      vw[t] &= (a & 1u ? 0xffu : 0u) | (a & 2u ? 0xff00u : 0u) | (a & 4u ? 0xff0000u : 0u) |
+               (a & 8u ? 0xff000000u : 0u);
+    }
+#pragma unroll
+    for (int g = 0; g < kRG; ++g) mask_block<2>(s[g], vis[g], q4);
+  }
+  float mx[kRG][2];
+#pragma unroll
+  for (int g = 0; g < kRG; ++g) {
+    block_max(s[g], mx[g]);
+    mx[g][0] *= c[g][0];
+    mx[g][1] *= c[g][1];
+  }
+  raise<true, kRG>(st, mx, vw);
+  uint32_t pa[kRG][kBlockPages][4];
+#pragma unroll
+  for (int g = 0; g < kRG; ++g) block_exp(s[g], c[g], st.m[g], st.l[g]);
 #pragma unroll
   for (int t = 0; t < kBlockPages; ++t) {
     const float f[4] = {scale_of_byte<0>(vw[t]) * st.inv_e, scale_of_byte<1>(vw[t]) * st.inv_e,
                         scale_of_byte<2>(vw[t]) * st.inv_e, scale_of_byte<3>(vw[t]) * st.inv_e};
-    float p[2][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      p[0][i] = s[2 * t][i] * f[i & 1];
-      p[1][i] = s[2 * t + 1][i] * f[2 + (i & 1)];
-      if constexpr (kMask) {
-        // A key this row does not see contributes nothing, whatever its exponent byte.
-        const uint32_t v = ((i & 2) ? vis1[t] : vis0[t]) >> q4;
-        if (!(v >> (i & 1) & 1u)) p[0][i] = 0.f;
-        if (!(v >> (2 + (i & 1)) & 1u)) p[1][i] = 0.f;
+    for (int g = 0; g < kRG; ++g) {
+      float p[2][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[0][i] = s[g][2 * t][i] * f[i & 1];
+        p[1][i] = s[g][2 * t + 1][i] * f[2 + (i & 1)];
+        if constexpr (kMask) {
+          // A key this row does not see contributes nothing, whatever its exponent byte.
+          const uint32_t v = vis[g][i >> 1] >> (16 * t + q4);
+          if (!(v >> (i & 1) & 1u)) p[0][i] = 0.f;
+          if (!(v >> (2 + (i & 1)) & 1u)) p[1][i] = 0.f;
+        }
       }
+      pa[g][t][0] = pack_f16(p[0][0], p[0][1]);
+      pa[g][t][1] = pack_f16(p[0][2], p[0][3]);
+      pa[g][t][2] = pack_f16(p[1][0], p[1][1]);
+      pa[g][t][3] = pack_f16(p[1][2], p[1][3]);
     }
-    const uint32_t pa[4] = {pack_f16(p[0][0], p[0][1]), pack_f16(p[0][2], p[0][3]),
-                            pack_f16(p[1][0], p[1][1]), pack_f16(p[1][2], p[1][3])};
+  }
+  const int vtok = tok + 2 * (mi & 1);
+#pragma unroll
+  for (int t = 0; t < kBlockPages; ++t) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       uint32_t w[4];
@@ -318,8 +394,13 @@ __device__ __forceinline__ void rows_block8(const uint32_t (&page)[kBlockPages],
         // in the low half, column 2j + 1 in the high half.
         a = __byte_perm(a, 0, 0x3120);
         b = __byte_perm(b, 0, 0x3120);
-        mma_f16(st.o[4 * u + 2 * h], pa, e4m3x2_to_f16x2<0>(a), e4m3x2_to_f16x2<0>(b));
-        mma_f16(st.o[4 * u + 2 * h + 1], pa, e4m3x2_to_f16x2<1>(a), e4m3x2_to_f16x2<1>(b));
+        const uint32_t a0 = e4m3x2_to_f16x2<0>(a), b0 = e4m3x2_to_f16x2<0>(b);
+        const uint32_t a1 = e4m3x2_to_f16x2<1>(a), b1 = e4m3x2_to_f16x2<1>(b);
+#pragma unroll
+        for (int g = 0; g < kRG; ++g) {
+          mma_f16(st.o[g][4 * u + 2 * h], pa[g][t], a0, b0);
+          mma_f16(st.o[g][4 * u + 2 * h + 1], pa[g][t], a1, b1);
+        }
       }
     }
   }
@@ -331,59 +412,74 @@ __device__ __forceinline__ bool bf16_pair_bad(uint32_t w) {
   return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
 
-// qf: query fragments as in kernel B; a thread's keys of a page are 2q, 2q + 1, 2q + 8, 2q + 9
-// (q = lane % 4).  Accumulator tile n holds columns 8n + 2q, 8n + 2q + 1.
-template <bool kMask>
-__device__ __forceinline__ void rows_block16(const uint32_t (&page)[kBlockPages],
-                                             const uint32_t (&qf)[8][4], RowsState& st, float c,
-                                             const uint32_t (&vis0)[kBlockPages],
-                                             const uint32_t (&vis1)[kBlockPages], int lane) {
-  const int mi = lane >> 3, q2 = 2 * (lane & 3);
-  float s[2 * kBlockPages][4];
+// A thread's keys of a page are 2q, 2q + 1, 2q + 8, 2q + 9 (q = lane % 4).  Accumulator tile n holds
+// columns 8n + 2q, 8n + 2q + 1.
+template <int kRG, bool kMask>
+__device__ __forceinline__ void rows_block16(const uint32_t (&page)[kBlockPages], uint32_t q,
+                                             RowsState<kRG>& st, const float (&c)[kRG][2],
+                                             const uint32_t (&vis)[kRG][2], int lane) {
+  const int mi = lane >> 3, t8 = lane & 7, q2 = 2 * (lane & 3);
+  float s[kRG][2 * kBlockPages][4];
 #pragma unroll
-  for (int t = 0; t < 2 * kBlockPages; ++t) {
+  for (int g = 0; g < kRG; ++g) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[t][i] = 0.f;
+    for (int t = 0; t < 2 * kBlockPages; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[g][t][i] = 0.f;
+    }
   }
 #pragma unroll
   for (int ks = 0; ks < 8; ++ks) {
+    uint32_t qa[kRG][4];
+#pragma unroll
+    for (int g = 0; g < kRG; ++g)
+      ldsm_x4(q + g * (16 * kHeadDim * 2) + (((2 * ks + (mi >> 1)) ^ t8) << 4), qa[g][0], qa[g][1],
+              qa[g][2], qa[g][3]);
 #pragma unroll
     for (int t = 0; t < kBlockPages; ++t) {
       uint32_t b0, b1, b2, b3;
-      ldsm_x4(page[t] + swz_off((lane & 7) + (mi >> 1) * 8, ks * 16 + (mi & 1) * 8, 16), b0, b1, b2,
-              b3);
-      mma_bf16(s[2 * t], qf[ks], b0, b1);
-      mma_bf16(s[2 * t + 1], qf[ks], b2, b3);
-    }
-  }
-  uint32_t keep[kBlockPages][2];
-  if constexpr (kMask) {
+      ldsm_x4(page[t] + swz_off(t8 + (mi >> 1) * 8, ks * 16 + (mi & 1) * 8, 16), b0, b1, b2, b3);
 #pragma unroll
-    for (int t = 0; t < kBlockPages; ++t) {
-      const uint32_t any = __reduce_or_sync(0xffffffffu, vis0[t] | vis1[t]) >> q2;
-      keep[t][0] = (any & 1u ? 0xffffu : 0u) | (any & 2u ? 0xffff0000u : 0u);
-      keep[t][1] = (any & 0x100u ? 0xffffu : 0u) | (any & 0x200u ? 0xffff0000u : 0u);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t v = ((i & 2) ? vis1[t] : vis0[t]) >> q2;
-        if (!(v >> (i & 1) & 1u)) s[2 * t][i] = -INFINITY;
-        if (!(v >> (8 + (i & 1)) & 1u)) s[2 * t + 1][i] = -INFINITY;
+      for (int g = 0; g < kRG; ++g) {
+        mma_bf16(s[g][2 * t], qa[g], b0, b1);
+        mma_bf16(s[g][2 * t + 1], qa[g], b2, b3);
       }
     }
   }
-  float mx0, mx1;
-  block_max(s, mx0, mx1);
+  uint32_t any = 0;
+  if constexpr (kMask) {
+    any = seen_by_any<kRG>(vis) >> q2;
+#pragma unroll
+    for (int g = 0; g < kRG; ++g) mask_block<8>(s[g], vis[g], q2);
+  }
+  float mx[kRG][2];
+#pragma unroll
+  for (int g = 0; g < kRG; ++g) {
+    block_max(s[g], mx[g]);
+    mx[g][0] *= c[g][0];
+    mx[g][1] *= c[g][1];
+  }
   const uint32_t none[kBlockPages] = {};
-  raise<false>(st, mx0 * c, mx1 * c, none);
-  block_exp(s, c, c, st);
+  raise<false, kRG>(st, mx, none);
+#pragma unroll
+  for (int g = 0; g < kRG; ++g) block_exp(s[g], c[g], st.m[g], st.l[g]);
 #pragma unroll
   for (int t = 0; t < kBlockPages; ++t) {
     // p is rounded to bf16 for the product (half a step of 2^-8), as in kernels B and D.
-    const float(&p0)[4] = s[2 * t];
-    const float(&p1)[4] = s[2 * t + 1];
-    const uint32_t pa[4] = {pack_bf16(p0[0], p0[1]), pack_bf16(p0[2], p0[3]),
-                            pack_bf16(p1[0], p1[1]), pack_bf16(p1[2], p1[3])};
-    const int key = (lane & 7) + (mi & 1) * 8;
+    uint32_t pa[kRG][4];
+#pragma unroll
+    for (int g = 0; g < kRG; ++g) {
+      const float(&p0)[4] = s[g][2 * t];
+      const float(&p1)[4] = s[g][2 * t + 1];
+      pa[g][0] = pack_bf16(p0[0], p0[1]);
+      pa[g][1] = pack_bf16(p0[2], p0[3]);
+      pa[g][2] = pack_bf16(p1[0], p1[1]);
+      pa[g][3] = pack_bf16(p1[2], p1[3]);
+    }
+    const uint32_t a = any >> (16 * t);
+    const uint32_t keep0 = (a & 1u ? 0xffffu : 0u) | (a & 2u ? 0xffff0000u : 0u);
+    const uint32_t keep1 = (a & 0x100u ? 0xffffu : 0u) | (a & 0x200u ? 0xffff0000u : 0u);
+    const int key = t8 + (mi & 1) * 8;
     const uint32_t vbase = page[t] + kPageBytes;
     bool bad = false;
 #pragma unroll
@@ -395,7 +491,7 @@ __device__ __forceinline__ void rows_block16(const uint32_t (&page)[kBlockPages]
         // added below for the rows that do see them (0 times them would reach every row).
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          b[i] &= keep[t][i & 1];
+          b[i] &= (i & 1) ? keep1 : keep0;
           if (bf16_pair_bad(b[i])) {
             bad = true;
             if ((b[i] & 0x7f80u) == 0x7f80u) b[i] &= 0xffff0000u;
@@ -403,28 +499,37 @@ __device__ __forceinline__ void rows_block16(const uint32_t (&page)[kBlockPages]
           }
         }
       }
-      mma_bf16(st.o[2 * np], pa, b[0], b[1]);
-      mma_bf16(st.o[2 * np + 1], pa, b[2], b[3]);
+#pragma unroll
+      for (int g = 0; g < kRG; ++g) {
+        mma_bf16(st.o[g][2 * np], pa[g], b[0], b[1]);
+        mma_bf16(st.o[g][2 * np + 1], pa[g], b[2], b[3]);
+      }
     }
     if constexpr (kMask) {
       if (__any_sync(0xffffffffu, bad)) {
+#pragma unroll 1
         for (int k = 0; k < 16; ++k) {
           const int src = (lane & ~3) | ((k & 7) >> 1);
-          const float a0 = (k & 8) ? ((k & 1) ? p1[1] : p1[0]) : ((k & 1) ? p0[1] : p0[0]);
-          const float a1 = (k & 8) ? ((k & 1) ? p1[3] : p1[2]) : ((k & 1) ? p0[3] : p0[2]);
-          const float w0 = __shfl_sync(0xffffffffu, a0, src);
-          const float w1 = __shfl_sync(0xffffffffu, a1, src);
-          const bool see0 = vis0[t] >> k & 1u, see1 = vis1[t] >> k & 1u;
 #pragma unroll
-          for (int n = 0; n < 16; ++n) {
-            const uint32_t w = lds32(vbase + swz_off(k, n * 8 + q2, 16));
+          for (int g = 0; g < kRG; ++g) {
+            const float(&p0)[4] = s[g][2 * t];
+            const float(&p1)[4] = s[g][2 * t + 1];
+            const float a0 = (k & 8) ? ((k & 1) ? p1[1] : p1[0]) : ((k & 1) ? p0[1] : p0[0]);
+            const float a1 = (k & 8) ? ((k & 1) ? p1[3] : p1[2]) : ((k & 1) ? p0[3] : p0[2]);
+            const float w0 = __shfl_sync(0xffffffffu, a0, src);
+            const float w1 = __shfl_sync(0xffffffffu, a1, src);
+            const bool see0 = vis[g][0] >> (16 * t + k) & 1u, see1 = vis[g][1] >> (16 * t + k) & 1u;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t bits = i == 0 ? w << 16 : w & 0xffff0000u;
-              if ((bits & 0x7f800000u) != 0x7f800000u) continue;
-              const float v = __uint_as_float(bits);
-              if (see0) st.o[n][i] += w0 * v;
-              if (see1) st.o[n][2 + i] += w1 * v;
+            for (int n = 0; n < 16; ++n) {
+              const uint32_t w = lds32(vbase + swz_off(k, n * 8 + q2, 16));
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t bits = i == 0 ? w << 16 : w & 0xffff0000u;
+                if ((bits & 0x7f800000u) != 0x7f800000u) continue;
+                const float v = __uint_as_float(bits);
+                if (see0) st.o[g][n][i] += w0 * v;
+                if (see1) st.o[g][n][2 + i] += w1 * v;
+              }
             }
           }
         }
@@ -499,65 +604,151 @@ __device__ __forceinline__ void put_cols(const RowOut& o, int d, const float (&x
   }
 }
 
-template <bool kKv8, bool kTree>
-__global__ void __launch_bounds__(kRowsThreads, 2)
+// The last CTA of a split tile merges the splits' partial rows: out = sum_s 2^(lse_s - M) O_s /
+// sum_s 2^(lse_s - M), s in order, so the result does not depend on which CTA came last.  A warp
+// takes kR rows at a time, a lane four columns; kR times kS loads of partial rows are in flight (few rows
+// have many splits, many rows few).
+template <int kR, int kS>
+__device__ __forceinline__ void merge_splits(const AttnArgs& a, int row0, int stride, int n_splits,
+                                             int rows, int kvh, int flat_tok, int warp, int lane) {
+  for (int r0 = warp * kR; r0 < rows; r0 += kRowsWarps * kR) {
+    float M[kR], L[kR];
+    float4 acc[kR];
+#pragma unroll
+    for (int k = 0; k < kR; ++k) {
+      M[k] = -INFINITY;
+      L[k] = 0.f;
+      acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    auto at = [&](int s, int k) {
+      return (static_cast<long long>(row0) + static_cast<long long>(s) * stride +
+              min(r0 + k, rows - 1)) * a.num_kv + kvh;
+    };
+    for (int s = lane; s < n_splits; s += 32) {
+#pragma unroll
+      for (int k = 0; k < kR; ++k) M[k] = fmaxf(M[k], __ldcg(a.ws_lse + at(s, k)));
+    }
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) {
+#pragma unroll
+      for (int k = 0; k < kR; ++k) M[k] = fmaxf(M[k], __shfl_xor_sync(0xffffffffu, M[k], off));
+    }
+    for (int sb = 0; sb < n_splits; sb += 32) {
+      float w[kR];
+#pragma unroll
+      for (int k = 0; k < kR; ++k) {
+        const float lse = sb + lane < n_splits ? __ldcg(a.ws_lse + at(sb + lane, k)) : -INFINITY;
+        w[k] = lse == -INFINITY ? 0.f : fast_exp2(lse - M[k]);
+        L[k] += w[k];
+      }
+      const int cnt = min(32, n_splits - sb);
+      for (int i0 = 0; i0 < cnt; i0 += kS) {
+        float4 v[kS][kR];
+#pragma unroll
+        for (int i = 0; i < kS; ++i) {
+#pragma unroll
+          for (int k = 0; k < kR; ++k)
+            v[i][k] = __ldcg(reinterpret_cast<const float4*>(
+                                 a.ws_o + at(sb + min(i0 + i, cnt - 1), k) * kHeadDim) + lane);
+        }
+#pragma unroll
+        for (int i = 0; i < kS; ++i) {
+#pragma unroll
+          for (int k = 0; k < kR; ++k) {
+            const float wi = i0 + i < cnt ? __shfl_sync(0xffffffffu, w[k], i0 + i) : 0.f;
+            if (i0 + i >= cnt) continue;
+            acc[k].x += wi * v[i][k].x;
+            acc[k].y += wi * v[i][k].y;
+            acc[k].z += wi * v[i][k].z;
+            acc[k].w += wi * v[i][k].w;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) {
+#pragma unroll
+      for (int k = 0; k < kR; ++k) L[k] += __shfl_xor_sync(0xffffffffu, L[k], off);
+    }
+#pragma unroll
+    for (int k = 0; k < kR; ++k) {
+      const int r = r0 + k;
+      if (r >= rows) break;
+      const float inv = L[k] != 0.f ? 1.f / L[k] : 0.f;
+      __nv_bfloat16* dst = a.out + static_cast<long long>(flat_tok + (r >> 1)) * a.out_row_stride +
+                           (kvh * kGroup + (r & 1)) * kHeadDim + lane * 4;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc[k].x * inv, acc[k].y * inv),
+                                                  pack_bf16(acc[k].z * inv, acc[k].w * inv));
+    }
+  }
+}
+
+template <bool kKv8, bool kTree, int kRG>
+__global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kRG>::kCtasPerSm)
     rows_attn_kernel(const __grid_constant__ CUtensorMap kv_map, const RowsArgs ra) {
-  using Cfg = RowsCfg<kKv8>;
+  using Cfg = RowsCfg<kKv8, kRG>;
   constexpr int kStages = Cfg::kStages, kBatch = Cfg::kBatch;
   const AttnArgs& a = ra.a;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* ring = smem;
+  uint8_t* qtile = smem + Cfg::kQOffset;
+  float* qscale = reinterpret_cast<float*>(smem + Cfg::kScaleOffset);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kBarOffset);
   uint64_t* empty = full + kStages;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + kStages);
+  volatile int* last_flag = abort_flag + 1;
+  static_assert(2 * kRowsNarrowTokens == RowsCfg<kKv8, 1>::kRows, "rows of a narrow tile");
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  // Work item: the first n_single items are one tile, the rest two tiles of 32 tokens.
   const int slot = blockIdx.x / a.num_kv;
   const int kvh = blockIdx.x - slot * a.num_kv;
-  const int item_idx = slot < ra.n_single ? slot : ra.n_single + ((slot - ra.n_single) >> 1);
-  const int sub = slot < ra.n_single ? 0 : (slot - ra.n_single) & 1;
+  const int item_idx = slot / ra.halves;
+  const int half = slot - item_idx * ra.halves;
   // The plan was copied in before the previous kernel started, so it is read before the wait.
   const int* it = a.items + static_cast<long long>(item_idx) * kRec;
-  const int seq = it[0], tok0 = it[1] + sub * kRowsTokens, page_begin = it[3];
-  const int n_q = min(it[2] - sub * kRowsTokens, kRowsTokens);
-  const int part_row = it[5] < 0 ? -1 : it[5] + sub * kRowsTokens * kGroup;
+  const int seq = it[0], tok0 = it[1] + half * kRowsTokens, page_begin = it[3];
+  const int n_q = min(it[2] - half * kRowsTokens, kRG == 1 ? kRowsNarrowTokens : kRowsTokens);
+  if (n_q <= 0) return;  // the second half of a chunk of up to 32 tokens
+  const int part_row = it[5] < 0 ? -1 : it[5] + half * kRowsTokens * kGroup;
   const int merge_row = it[7] == 1 ? it[6] : -1;
   const int* sr = a.seqs + static_cast<long long>(seq) * kRec;
   const int flat_start = sr[0], num_cached = sr[2], table_off = sr[4];
   // Keys after the tile's last token are visible to none of its rows.
   const int npages = min(it[4], (num_cached + tok0 + n_q + kBlockTokens - 1) / kBlockTokens) - page_begin;
-  if (n_q <= 0) return;  // the second half of a chunk of up to 32 tokens
 
-  const int groups = n_q * kGroup <= 16 ? 1 : (n_q * kGroup <= 32 ? 2 : 4);
-  const int phases = kRowsWarps / groups;
+  const int sets = n_q * kGroup > 16 * kRG ? 2 : 1;
+  const int phases = kRowsWarps / sets;
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], groups);  // one warp of each row group reads a page
+      mbar_init(&empty[s], sets);  // one warp of each row set reads a page
     }
     *abort_flag = 0;
     fence_barrier_init();
   }
   __syncthreads();
-  pdl_wait();
-  pdl_trigger();
 
-  if (warp == kRowsWarps) {
+  if (warp >= kRowsWarps) {
+    if constexpr (kRG == 2) setmaxnreg_dec<Cfg::kProducerRegs>();
+    const int* table = a.tables + table_off + page_begin;
+    int mine = lane < npages ? table[lane] : 0;
+    pdl_wait();
+    pdl_trigger();
+    if (warp != kRowsWarps) return;
     // ---------------- producer warp ----------------
     // Lane i of the first kBatch takes the pages j with j % kBatch == i: the lanes wait for their
     // slots and issue their copies side by side.  (One lane issuing every page takes a chain of
-    // several hundred cycles per page, which three CTAs of 4 KiB pages per SM cannot afford.)
+    // several hundred cycles per page, which three CTAs of 4 KiB pages per SM cannot afford: 256
+    // decode rows 287 us that way, 219 with four lanes.)
     const uint64_t policy = l2_policy_evict_first();
-    const int* table = a.tables + table_off + page_begin;
     int issued = 0;  // by this lane
     bool stop = false;
     for (int j0 = 0; j0 < npages && !stop; j0 += 32) {
-      const int mine = j0 + lane < npages ? table[j0 + lane] : 0;
+      if (j0 > 0) mine = j0 + lane < npages ? table[j0 + lane] : 0;
       for (int b = 0; b < 32 && j0 + b < npages; b += kBatch) {
         const int blk = __shfl_sync(0xffffffffu, mine, b + (lane & (kBatch - 1)));
         const int j = j0 + b + lane;
@@ -616,87 +807,111 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   }
 
   // ---------------- consumer warps ----------------
-  const int group = warp % groups, phase = warp / groups;
-  const int row_base = group * 16;
-  const int ra0 = row_base + (lane >> 2), ra1 = ra0 + 8;  // this thread's two rows
-  const int tk0 = ra0 >> 1, tk1 = ra1 >> 1;               // and their tokens
+  if constexpr (kRG == 2) setmaxnreg_inc<Cfg::kConsumerRegs>();
+  pdl_wait();
+  pdl_trigger();
+  // Query rows to shared memory, half a warp per row: bf16 as they are; for an 8-bit pool scaled
+  // into f16 and in the order of dims that rows_block8 wants.  Rows without a token are zeros.
+  const uint32_t q_u32 = smem_u32(qtile);
+  {
+    const int l16 = lane & 15;
+    constexpr int kPer = Cfg::kRows / (2 * kRowsWarps);
+    uint4 x[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int r = (i * kRowsWarps + warp) * 2 + (lane >> 4);
+      x[i] = make_uint4(0u, 0u, 0u, 0u);
+      if ((r >> 1) < n_q)
+        x[i] = __ldg(reinterpret_cast<const uint4*>(
+            a.q + static_cast<long long>(flat_start + tok0 + (r >> 1)) * a.q_row_stride +
+            (kvh * kGroup + (r & 1)) * kHeadDim + l16 * 8));
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int r = (i * kRowsWarps + warp) * 2 + (lane >> 4);
+      const uint32_t row = q_u32 + r * (kHeadDim * 2);
+      if constexpr (kKv8) {
+        unsigned top = __vmaxu2(__vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu),
+                                __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu));
+#pragma unroll
+        for (int off = 8; off >= 1; off >>= 1)
+          top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, off));
+        const int b = exp_byte8(max(top & 0xffffu, top >> 16));
+        const float inv = inv_scale8(b);
+        // A row with a NaN or an infinity gets the scale NaN: it scores NaN.
+        if (l16 == 0) qscale[r] = row_scale8(b);
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        uint32_t h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[k] = pack_f16(bf16_lo(w[k]) * inv, bf16_hi(w[k]) * inv);
+        // Dims 8 l .. + 7: words (0, 1), (4, 5) go to the chunk's first half, (2, 3), (6, 7) to
+        // its second.
+        const int chunk = l16 & ~1;
+        const int off = (l16 & 1) * 8;
+        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(row + ((chunk ^ (r & 7)) << 4) + off),
+                     "r"(h[0]), "r"(h[2])
+                     : "memory");
+        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(row + (((chunk + 1) ^ (r & 7)) << 4) + off),
+                     "r"(h[1]), "r"(h[3])
+                     : "memory");
+      } else {
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((l16 ^ (r & 7)) << 4)),
+                     "r"(x[i].x), "r"(x[i].y), "r"(x[i].z), "r"(x[i].w)
+                     : "memory");
+      }
+    }
+    asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
+  }
+
+  const int set = warp % sets, phase = warp / sets;
+  const int row_base = set * 16 * kRG;  // of this warp's rows
   const bool warp_active = (row_base >> 1) < n_q;
   const int q2 = 2 * (lane & 3);
-
-  // Query fragments, straight from memory.
-  const __nv_bfloat16* qrow0 = a.q + static_cast<long long>(flat_start + tok0 + tk0) * a.q_row_stride +
-                               (kvh * kGroup + (ra0 & 1)) * kHeadDim;
-  const __nv_bfloat16* qrow1 = a.q + static_cast<long long>(flat_start + tok0 + tk1) * a.q_row_stride +
-                               (kvh * kGroup + (ra1 & 1)) * kHeadDim;
-  uint32_t qf[8][4];
-  float c0 = a.scale_log2, c1 = a.scale_log2;
-  if constexpr (kKv8) {
-    uint2 x[2][8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[0][i] = x[1][i] = make_uint2(0u, 0u);
-      if (tk0 < n_q) x[0][i] = __ldg(reinterpret_cast<const uint2*>(qrow0 + 16 * i + 2 * q2));
-      if (tk1 < n_q) x[1][i] = __ldg(reinterpret_cast<const uint2*>(qrow1 + 16 * i + 2 * q2));
-    }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      unsigned top = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        top = __vmaxu2(top, __vmaxu2(x[r][i].x & 0x7fff7fffu, x[r][i].y & 0x7fff7fffu));
-      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int b = exp_byte8(max(top & 0xffffu, top >> 16));
-      const float inv = inv_scale8(b);
-      // The row's query scale; a row with a NaN or an infinity scores NaN.
-      (r == 0 ? c0 : c1) *= row_scale8(b);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        qf[i][r] = pack_f16(bf16_lo(x[r][i].x) * inv, bf16_hi(x[r][i].x) * inv);
-        qf[i][2 + r] = pack_f16(bf16_lo(x[r][i].y) * inv, bf16_hi(x[r][i].y) * inv);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      qf[i][0] = qf[i][1] = qf[i][2] = qf[i][3] = 0u;
-      if (tk0 < n_q) {
-        qf[i][0] = __ldg(reinterpret_cast<const uint32_t*>(qrow0 + 16 * i + q2));
-        qf[i][2] = __ldg(reinterpret_cast<const uint32_t*>(qrow0 + 16 * i + 8 + q2));
-      }
-      if (tk1 < n_q) {
-        qf[i][1] = __ldg(reinterpret_cast<const uint32_t*>(qrow1 + 16 * i + q2));
-        qf[i][3] = __ldg(reinterpret_cast<const uint32_t*>(qrow1 + 16 * i + 8 + q2));
-      }
-    }
-  }
-
-  // Tree masks of the two rows' tokens; a token whose mask misses itself sees nothing.
-  const int* mask0 = nullptr;
-  const int* mask1 = nullptr;
+  // This thread's rows row(g, h) = row_base + 16 g + lane / 4 + 8 h and their facts.
+  const int row00 = row_base + (lane >> 2);
+  float c[kRG][2];
+  bool live[kRG][2];
   int words = 0;
-  bool live0 = tk0 < n_q, live1 = tk1 < n_q;
+  const int* masks = nullptr;  // tree: mask rows of the sequence
   if constexpr (kTree) {
     words = sr[7];
-    const int g0 = tok0 + min(tk0, n_q - 1), g1 = tok0 + min(tk1, n_q - 1);
-    mask0 = ra.plan + sr[6] + static_cast<long long>(g0) * words;
-    mask1 = ra.plan + sr[6] + static_cast<long long>(g1) * words;
-    live0 = live0 && (mask0[g0 >> 5] >> (g0 & 31) & 1);
-    live1 = live1 && (mask1[g1 >> 5] >> (g1 & 31) & 1);
+    masks = ra.plan + sr[6];
+  }
+#pragma unroll
+  for (int g = 0; g < kRG; ++g) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = row00 + 16 * g + 8 * h;
+      c[g][h] = a.scale_log2;
+      if constexpr (kKv8) c[g][h] *= qscale[r];
+      live[g][h] = (r >> 1) < n_q;
+      if constexpr (kTree) {
+        // A token whose mask misses itself sees nothing.
+        if (live[g][h]) {
+          const int k = tok0 + (r >> 1);
+          live[g][h] = masks[static_cast<long long>(k) * words + (k >> 5)] >> (k & 31) & 1;
+        }
+      }
+    }
   }
 
-  RowsState st;
+  RowsState<kRG> st;
 #pragma unroll
-  for (int n = 0; n < 16; ++n) st.o[n][0] = st.o[n][1] = st.o[n][2] = st.o[n][3] = 0.f;
-  st.m[0] = st.m[1] = -INFINITY;
-  st.l[0] = st.l[1] = 0.f;
+  for (int g = 0; g < kRG; ++g) {
+#pragma unroll
+    for (int n = 0; n < 16; ++n)
+      st.o[g][n][0] = st.o[g][n][1] = st.o[g][n][2] = st.o[g][n][3] = 0.f;
+    st.m[g][0] = st.m[g][1] = -INFINITY;
+    st.l[g][0] = st.l[g][1] = 0.f;
+  }
   st.eb = -1000;
   st.inv_e = 0.f;
   st.hot = 0;
-  const int qpos0 = num_cached + tok0 + tk0, qpos1 = num_cached + tok0 + tk1;
-  // First key position that some row of the tile may not see.
+  // First key position that some row of the warp may not see.
   const int first_masked = kTree ? num_cached : num_cached + tok0 + (row_base >> 1) + 1;
   const uint32_t ring_u32 = smem_u32(ring);
+  // This lane's ldmatrix row of the query tile.
+  const uint32_t q_row = q_u32 + (row_base + (lane & 7) + ((lane >> 3) & 1) * 8) * (kHeadDim * 2);
   for (int j = phase * kBlockPages; j < npages; j += phases * kBlockPages) {
     const int cnt = min(kBlockPages, npages - j);
     uint32_t page[kBlockPages];
@@ -718,148 +933,155 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     }
     const int key0 = (page_begin + j) * kBlockTokens;
     if (warp_active) {
-      uint32_t vis0[kBlockPages], vis1[kBlockPages];
+      uint32_t vis[kRG][2];
       if (cnt < kBlockPages || key0 + kBlockPages * kBlockTokens > first_masked) {
 #pragma unroll
-        for (int t = 0; t < kBlockPages; ++t) {
-          const int k0 = key0 + t * kBlockTokens;
-          if (k0 + kBlockTokens <= first_masked) {
-            vis0[t] = live0 ? 0xffffu : 0u;
-            vis1[t] = live1 ? 0xffffu : 0u;
-          } else if constexpr (kTree) {
-            vis0[t] = live0 ? tree_bits(mask0, words, k0 - num_cached) : 0u;
-            vis1[t] = live1 ? tree_bits(mask1, words, k0 - num_cached) : 0u;
-          } else {
-            vis0[t] = live0 ? causal_bits(qpos0, k0) : 0u;
-            vis1[t] = live1 ? causal_bits(qpos1, k0) : 0u;
+        for (int g = 0; g < kRG; ++g) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int k = tok0 + ((row00 + 16 * g + 8 * h) >> 1);  // the row's new token
+            uint32_t v = 0;
+            if (live[g][h]) {
+#pragma unroll
+              for (int t = 0; t < kBlockPages; ++t) {
+                const int k0 = key0 + t * kBlockTokens;
+                uint32_t bits;
+                if constexpr (kTree) {
+                  bits = k0 + kBlockTokens <= num_cached
+                             ? 0xffffu
+                             : tree_bits(masks + static_cast<long long>(k) * words, words, k0 - num_cached);
+                } else {
+                  bits = causal_bits(num_cached + k, k0);
+                }
+                if (t < cnt) v |= bits << (16 * t);
+              }
+            }
+            vis[g][h] = v;
           }
-          if (t >= cnt) vis0[t] = vis1[t] = 0u;
         }
         if constexpr (kKv8)
-          rows_block8<true>(page, qf, st, c0, c1, vis0, vis1, lane);
+          rows_block8<kRG, true>(page, q_row, st, c, vis, lane);
         else
-          rows_block16<true>(page, qf, st, c0, vis0, vis1, lane);
+          rows_block16<kRG, true>(page, q_row, st, c, vis, lane);
       } else {
 #pragma unroll
-        for (int t = 0; t < kBlockPages; ++t) vis0[t] = vis1[t] = 0xffffu;
+        for (int g = 0; g < kRG; ++g) vis[g][0] = vis[g][1] = 0xffffffffu;
         if constexpr (kKv8)
-          rows_block8<false>(page, qf, st, c0, c1, vis0, vis1, lane);
+          rows_block8<kRG, false>(page, q_row, st, c, vis, lane);
         else
-          rows_block16<false>(page, qf, st, c0, vis0, vis1, lane);
+          rows_block16<kRG, false>(page, q_row, st, c, vis, lane);
       }
     }
     __syncwarp();
     if (lane < cnt) mbar_arrive(&empty[(j + lane) % kStages]);
   }
 
+  const float fe = st.eb < 0 ? 0.f : scale8(st.eb);  // O back to the values the codes stand for
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 1);
-    st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], 2);
-  }
-  if constexpr (kKv8) {  // O back to the values the codes stand for
-    const float f = st.eb < 0 ? 0.f : scale8(st.eb);
-#pragma unroll
-    for (int n = 0; n < 16; ++n) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) st.o[n][i] *= f;
-    }
-  }
-
-  if (phases == 1) {
-    if (!warp_active) return;
+  for (int g = 0; g < kRG; ++g) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = h == 0 ? ra0 : ra1;
-      const int tok = r >> 1;
-      if (tok >= n_q) continue;
-      const bool live = h == 0 ? live0 : live1;
-      const RowOut out = row_out(a, r, tok, live, st.m[h], st.l[h], kvh, part_row, merge_row,
-                                 flat_start + tok0, q2 == 0);
-      if constexpr (kKv8) {
+      st.l[g][h] += __shfl_xor_sync(0xffffffffu, st.l[g][h], 1);
+      st.l[g][h] += __shfl_xor_sync(0xffffffffu, st.l[g][h], 2);
+    }
+    if constexpr (kKv8) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const float x[4] = {st.o[2 * u][2 * h], st.o[2 * u + 1][2 * h], st.o[2 * u][2 * h + 1],
-                              st.o[2 * u + 1][2 * h + 1]};
-          put_cols<4>(out, 16 * u + 2 * q2, x, live);
-        }
-      } else {
+      for (int n = 0; n < 16; ++n) {
 #pragma unroll
-        for (int n = 0; n < 16; ++n) {
-          const float x[2] = {st.o[n][2 * h], st.o[n][2 * h + 1]};
-          put_cols<2>(out, 8 * n + q2, x, live);
-        }
+        for (int i = 0; i < 4; ++i) st.o[g][n][i] *= fe;
       }
     }
-    return;
   }
 
-  // Merge of the page phases: every warp leaves its (O, m, l) in the idle ring (each page has been
-  // read once all consumer warps reach the barrier; a copy that was abandoned on a timeout is
-  // drained by the producer before the CTA ends), and each warp merges and writes 16 / phases of
-  // its row group's column tiles.
+  // Merge of the page phases, one row group at a time: every warp leaves its (O, m, l) in the idle
+  // ring (each page has been read once all consumer warps reach the barrier; a copy that was
+  // abandoned on a timeout is drained by the producer before the CTA ends), and each warp merges
+  // and writes 16 / phases of its row set's column tiles.
   float4* scratch = reinterpret_cast<float4*>(ring);
-  asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
-#pragma unroll
-  for (int n = 0; n < 16; ++n)
-    scratch[(warp * 17 + n) * 32 + lane] =
-        make_float4(st.o[n][0], st.o[n][1], st.o[n][2], st.o[n][3]);
-  scratch[(warp * 17 + 16) * 32 + lane] = make_float4(st.m[0], st.m[1], st.l[0], st.l[1]);
-  asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
-  if (!warp_active) return;
-  float mx[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f}, wt[kRowsWarps][2];
-#pragma unroll
-  for (int p = 0; p < kRowsWarps; ++p) {
-    if (p < phases) {
-      const float4 ml = scratch[((p * groups + group) * 17 + 16) * 32 + lane];
-      mx[0] = fmaxf(mx[0], ml.x);
-      mx[1] = fmaxf(mx[1], ml.y);
-    }
-  }
-#pragma unroll
-  for (int p = 0; p < kRowsWarps; ++p) {
-    wt[p][0] = wt[p][1] = 0.f;
-    if (p < phases) {
-      const float4 ml = scratch[((p * groups + group) * 17 + 16) * 32 + lane];
-      wt[p][0] = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mx[0]);
-      wt[p][1] = ml.y == -INFINITY ? 0.f : fast_exp2(ml.y - mx[1]);
-      // A phase whose scores were all NaN never raised its maximum: its sum is kept as it is.
-      if (ml.z != ml.z) wt[p][0] = 1.f;
-      if (ml.w != ml.w) wt[p][1] = 1.f;
-      L[0] += ml.z * wt[p][0];
-      L[1] += ml.w * wt[p][1];
-    }
-  }
   const int per = 16 / phases;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = h == 0 ? ra0 : ra1;
-    const int tok = r >> 1;
-    if (tok >= n_q) continue;
-    const bool live = h == 0 ? live0 : live1;
-    const RowOut out = row_out(a, r, tok, live, mx[h], L[h], kvh, part_row, merge_row,
-                               flat_start + tok0, phase == 0 && q2 == 0);
-    for (int n = phase * per; n < (phase + 1) * per; n += 2) {
-      float x0[2] = {0.f, 0.f}, x1[2] = {0.f, 0.f};  // tiles n and n + 1
+  for (int g = 0; g < kRG; ++g) {
+    asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
 #pragma unroll
-      for (int p = 0; p < kRowsWarps; ++p) {
-        if (p < phases) {
-          const float2* base = reinterpret_cast<const float2*>(
-              scratch + ((p * groups + group) * 17 + n) * 32 + lane);
-          const float2 y0 = base[h], y1 = base[64 + h];
-          x0[0] += y0.x * wt[p][h];
-          x0[1] += y0.y * wt[p][h];
-          x1[0] += y1.x * wt[p][h];
-          x1[1] += y1.y * wt[p][h];
+    for (int n = 0; n < 16; ++n)
+      scratch[(warp * 17 + n) * 32 + lane] =
+          make_float4(st.o[g][n][0], st.o[g][n][1], st.o[g][n][2], st.o[g][n][3]);
+    scratch[(warp * 17 + 16) * 32 + lane] =
+        make_float4(st.m[g][0], st.m[g][1], st.l[g][0], st.l[g][1]);
+    asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
+    float mx[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f}, wt[kRowsWarps][2];
+#pragma unroll
+    for (int p = 0; p < kRowsWarps; ++p) {
+      if (p < phases) {
+        const float4 ml = scratch[((p * sets + set) * 17 + 16) * 32 + lane];
+        mx[0] = fmaxf(mx[0], ml.x);
+        mx[1] = fmaxf(mx[1], ml.y);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < kRowsWarps; ++p) {
+      wt[p][0] = wt[p][1] = 0.f;
+      if (p < phases) {
+        const float4 ml = scratch[((p * sets + set) * 17 + 16) * 32 + lane];
+        wt[p][0] = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mx[0]);
+        wt[p][1] = ml.y == -INFINITY ? 0.f : fast_exp2(ml.y - mx[1]);
+        // A phase whose scores were all NaN never raised its maximum: its sum is kept as it is.
+        if (ml.z != ml.z) wt[p][0] = 1.f;
+        if (ml.w != ml.w) wt[p][1] = 1.f;
+        L[0] += ml.z * wt[p][0];
+        L[1] += ml.w * wt[p][1];
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = row00 + 16 * g + 8 * h;
+      const int tok = r >> 1;
+      if (tok >= n_q) continue;
+      const RowOut out = row_out(a, r, tok, live[g][h], mx[h], L[h], kvh, part_row, merge_row,
+                                 flat_start + tok0, phase == 0 && q2 == 0);
+      for (int n = phase * per; n < (phase + 1) * per; n += 2) {
+        float x0[2] = {0.f, 0.f}, x1[2] = {0.f, 0.f};  // tiles n and n + 1
+#pragma unroll
+        for (int p = 0; p < kRowsWarps; ++p) {
+          if (p < phases) {
+            const float2* base = reinterpret_cast<const float2*>(
+                scratch + ((p * sets + set) * 17 + n) * 32 + lane);
+            const float2 y0 = base[h], y1 = base[64 + h];
+            x0[0] += y0.x * wt[p][h];
+            x0[1] += y0.y * wt[p][h];
+            x1[0] += y1.x * wt[p][h];
+            x1[1] += y1.y * wt[p][h];
+          }
+        }
+        if constexpr (kKv8) {
+          const float x[4] = {x0[0], x1[0], x0[1], x1[1]};
+          put_cols<4>(out, 8 * n + 2 * q2, x, live[g][h]);
+        } else {
+          put_cols<2>(out, 8 * n + q2, x0, live[g][h]);
+          put_cols<2>(out, 8 * n + 8 + q2, x1, live[g][h]);
         }
       }
-      if constexpr (kKv8) {
-        const float x[4] = {x0[0], x1[0], x0[1], x1[1]};
-        put_cols<4>(out, 8 * n + 2 * q2, x, live);
-      } else {
-        put_cols<2>(out, 8 * n + q2, x0, live);
-        put_cols<2>(out, 8 * n + 8 + q2, x1, live);
-      }
+    }
+  }
+
+  if (part_row >= 0) {
+    // A split of a tile: the last one to arrive merges them all.
+    __threadfence();
+    asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
+    const int record = kTree ? it[6] : sr[6];
+    const int* cr = ra.combines + static_cast<long long>(record) * kRec;
+    if (threadIdx.x == 0) {
+      int* counter = ra.arrived + (static_cast<long long>(record) * 2 + half) * a.num_kv + kvh;
+      const bool last = atomicAdd(counter, 1) == cr[4] - 1;
+      if (last) *counter = 0;  // ready for the next call
+      *last_flag = last ? 1 : 0;
+    }
+    asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
+    if (*last_flag) {
+      __threadfence();
+      merge_splits<kRG == 1 ? 2 : 8, kRG == 1 ? 8 : 2>(
+          a, cr[3] + half * kRowsTokens * kGroup, cr[5] != 0 ? cr[5] : cr[2] * kGroup, cr[4],
+          n_q * kGroup, kvh, flat_start + tok0, warp, lane);
     }
   }
 }

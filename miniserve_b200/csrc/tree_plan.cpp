@@ -27,9 +27,8 @@ namespace {
 
 constexpr int kRec = 8;
 constexpr int kTileTokens = 32;
-constexpr int kAssumedKvHeads = 8;  // the planner does not see the head count; only speed depends on it
-// Automatic split (the rule of ms_plan_build): one resident wave of kTreeCtasPerSm CTAs per SM.
-constexpr int kTreeCtasPerSm = 3;
+constexpr int kAssumedKvHeads = 4;  // the planner does not see the head count; only speed depends on it
+constexpr int kNarrowTokens = 16;   // tiles of at most 32 query rows run three CTAs per SM, others two
 constexpr int kMinSplitPages = 8;
 constexpr int kMaxSplitPages = 512;
 
@@ -51,6 +50,7 @@ int guarded(const char* what, F f) {
 
 struct TreeItem {
   int seq, tok0, n_q, pb, pe, part_row;
+  int record = 0, flag = 0;  // of a split item: its combine record, and 2
 };
 
 }  // namespace
@@ -125,8 +125,10 @@ extern "C" int ms_kv8_plan_build(int32_t* packed, int64_t capacity, const MsPlan
 extern "C" int64_t ms_kv8_workspace_bytes(const MsPlanInfo* plan, const MsKv8Info* info,
                                           int32_t num_kv_heads) {
   if (plan == nullptr || info == nullptr || num_kv_heads <= 0) return 0;
-  // Partials first, then the expanded pages (8 KiB per head) on a 1 KiB boundary.
-  const int64_t part = plan->workspace_bytes_per_kv_head * num_kv_heads;
+  // Partials, arrival counters (two per combine record and head), then the expanded pages (8 KiB
+  // per head) on a 1 KiB boundary.
+  const int64_t part =
+      (plan->workspace_bytes_per_kv_head + static_cast<int64_t>(plan->n_combine) * 8) * num_kv_heads;
   if (info->n_pages == 0) return part;
   return (part + 1023) / 1024 * 1024 + static_cast<int64_t>(info->n_pages) * num_kv_heads * 8192;
 }
@@ -144,7 +146,7 @@ extern "C" int64_t ms_tree_plan_capacity(int32_t num_seqs, const int32_t* num_ne
   // A tile has at most one item per page of its sequence.
   const int64_t items = tiles + tiles_max * total_table_entries;
   return round4(static_cast<int64_t>(num_seqs) * kRec) + round4(total_table_entries) +
-         round4(items * kRec) + round4(tiles * kRec) + round4(masks) + 16;
+         2 * round4(items * kRec) + round4(tiles * kRec) + round4(masks) + 16;
 }
 
 static int tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const int32_t* num_new,
@@ -225,34 +227,41 @@ static int tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const in
     }
   }
 
-  // Split size: the smallest multiple of 8 pages whose items fit one resident wave; when the tiles
-  // alone exceed it, tiles longer than the pages per CTA slot are cut to about that size.
-  int split = pages_per_split;
-  if (split == 0) {
-    const int64_t target = std::max<int64_t>(
-        1, static_cast<int64_t>(num_sms) * kTreeCtasPerSm / kAssumedKvHeads);
+  // Split size, for the narrow tiles and the wide ones (two launches): the smallest multiple of 8
+  // pages whose items fit one resident wave of CTAs; when the tiles alone exceed it, tiles longer
+  // than the pages per CTA slot are cut to about that size.
+  auto choose = [&](bool narrow) {
+    if (pages_per_split > 0) return pages_per_split;
+    const int64_t target =
+        std::max<int64_t>(1, static_cast<int64_t>(num_sms) * (narrow ? 3 : 2) / kAssumedKvHeads);
+    int64_t all = 0;
+    for (const TreeItem& t : tiles)
+      if ((t.n_q <= kNarrowTokens) == narrow) all += t.pe;
     auto items_at = [&](int64_t p) {
       int64_t items = 0;
-      for (const TreeItem& t : tiles) items += (t.pe + p - 1) / p;
+      for (const TreeItem& t : tiles)
+        if ((t.n_q <= kNarrowTokens) == narrow) items += (t.pe + p - 1) / p;
       return items;
     };
     if (items_at(kMaxSplitPages) > target) {
-      const int64_t per_slot = (total_pages + target - 1) / target;
-      split = static_cast<int>(std::min<int64_t>(
+      const int64_t per_slot = (all + target - 1) / target;
+      return static_cast<int>(std::min<int64_t>(
           kMaxSplitPages, std::max<int64_t>(kMinSplitPages, (per_slot + 7) / 8 * 8)));
-    } else {
-      int lo = kMinSplitPages / 8, hi = kMaxSplitPages / 8;
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (items_at(mid * 8) <= target) hi = mid; else lo = mid + 1;
-      }
-      split = lo * 8;
     }
-  }
+    int lo = kMinSplitPages / 8, hi = kMaxSplitPages / 8;
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (items_at(mid * 8) <= target) hi = mid; else lo = mid + 1;
+    }
+    return lo * 8;
+  };
+  const int split_narrow = choose(true), split_wide = choose(false);
 
-  std::vector<TreeItem> items, comb;
+  std::vector<TreeItem> narrow, wide, comb;
   int64_t part_rows = 0;
   for (const TreeItem& t : tiles) {
+    const int split = t.n_q <= kNarrowTokens ? split_narrow : split_wide;
+    std::vector<TreeItem>& items = t.n_q <= kNarrowTokens ? narrow : wide;
     const int ns = (t.pe + split - 1) / split;
     if (ns <= 1) {
       items.push_back(t);
@@ -268,19 +277,23 @@ static int tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const in
     for (int s = 0; s < ns; ++s) {
       const int len = base + (s < rem ? 1 : 0);
       items.push_back({t.seq, t.tok0, t.n_q, pb, pb + len,
-                       static_cast<int>(part_rows + static_cast<int64_t>(s) * rows)});
+                       static_cast<int>(part_rows + static_cast<int64_t>(s) * rows),
+                       static_cast<int>(comb.size()), 2});
       pb += len;
     }
     comb.push_back({t.seq, t.tok0, t.n_q, static_cast<int>(part_rows), ns, 0});
     part_rows += static_cast<int64_t>(ns) * rows;
   }
-  std::stable_sort(items.begin(), items.end(), [](const TreeItem& x, const TreeItem& y) {
+  auto longest_first = [](const TreeItem& x, const TreeItem& y) {
     return (x.pe - x.pb) > (y.pe - y.pb);
-  });
+  };
+  std::stable_sort(narrow.begin(), narrow.end(), longest_first);
+  std::stable_sort(wide.begin(), wide.end(), longest_first);
 
   const int64_t off_tables = round4(static_cast<int64_t>(num_seqs) * kRec);
-  const int64_t off_tile = off_tables + round4(total_entries);
-  const int64_t off_combine = off_tile + round4(static_cast<int64_t>(items.size()) * kRec);
+  const int64_t off_narrow = off_tables + round4(total_entries);
+  const int64_t off_tile = off_narrow + round4(static_cast<int64_t>(narrow.size()) * kRec);
+  const int64_t off_combine = off_tile + round4(static_cast<int64_t>(wide.size()) * kRec);
   const int64_t off_masks = off_combine + round4(static_cast<int64_t>(comb.size()) * kRec);
   const int64_t total = off_masks + round4(mask_words);
   if (total > out_capacity) {
@@ -324,28 +337,33 @@ static int tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const in
       r[3] = v[k].pb;
       r[4] = v[k].pe;
       r[5] = v[k].part_row;
+      r[6] = v[k].record;
+      r[7] = v[k].flag;
     }
   };
-  put(off_tile, items);
+  put(off_narrow, narrow);
+  put(off_tile, wide);
   put(off_combine, comb);
 
   info->num_seqs = num_seqs;
   info->num_tokens = num_tokens;
-  info->n_tile_items = static_cast<int32_t>(items.size());
+  info->n_decode_items = static_cast<int32_t>(narrow.size());
+  info->n_tile_items = static_cast<int32_t>(wide.size());
   info->n_combine = static_cast<int32_t>(comb.size());
   info->off_tables = static_cast<int32_t>(off_tables);
-  info->off_decode = static_cast<int32_t>(off_tile);
+  info->off_decode = static_cast<int32_t>(off_narrow);
   info->off_tile = static_cast<int32_t>(off_tile);
   info->off_tc = static_cast<int32_t>(off_combine);
   info->off_combine = static_cast<int32_t>(off_combine);
   info->total_ints = static_cast<int32_t>(total);
-  info->pages_per_split = split;
+  info->pages_per_split = narrow.empty() ? split_wide : split_narrow;
   info->part_rows = part_rows;
   info->total_pages = total_pages;
   int combine_tokens_max = 0;
   for (const TreeItem& c : comb) combine_tokens_max = std::max(combine_tokens_max, c.n_q);
   info->combine_tokens_max = combine_tokens_max;
-  info->workspace_bytes_per_kv_head = part_rows * (128 + 1) * 4;
+  // Partials and the arrival counters (two per combine record).
+  info->workspace_bytes_per_kv_head = part_rows * (128 + 1) * 4 + static_cast<int64_t>(comb.size()) * 8;
   return MS_OK;
 }
 

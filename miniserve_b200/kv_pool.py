@@ -84,7 +84,7 @@ def allocate_kv_cache(
 
 def is_kv8(k_cache: Tensor) -> bool:
     """Whether a layer's view belongs to an 8-bit pool."""
-    return isinstance(k_cache, Tensor) and k_cache.dtype == KV8
+    return k_cache is not None and k_cache.dtype == KV8
 
 
 def _check_kv8_views(k_cache: Tensor, v_cache: Tensor) -> tuple[int, int]:

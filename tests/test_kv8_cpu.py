@@ -121,9 +121,17 @@ def test_tree_plan_covers_every_page_once(n: int, split: int) -> None:
     seqs = packed[: 4 * 8].reshape(4, 8)
     pages: dict[tuple[int, int], set[int]] = {}
     parts = set()
-    for it in packed[info.off_tile : info.off_tile + 8 * info.n_tile_items].reshape(-1, 8):
-        s, tok0, nq, pb, pe, part = (int(v) for v in it[:6])
-        assert tok0 % 32 == 0 and 1 <= nq <= 32 and pb < pe
+    narrow = packed[info.off_decode :][: 8 * info.n_decode_items].reshape(-1, 8)
+    wide = packed[info.off_tile :][: 8 * info.n_tile_items].reshape(-1, 8)
+    assert all(it[2] <= 16 for it in narrow) and all(16 < it[2] <= 32 for it in wide)
+    combine = packed[info.off_combine :][: 8 * info.n_combine].reshape(-1, 8)
+    for it in np.concatenate([narrow, wide]):
+        s, tok0, nq, pb, pe, part, rec, flag = (int(v) for v in it)
+        assert tok0 % 32 == 0 and pb < pe
+        if part >= 0:  # its combine record names its tile
+            assert flag == 2 and combine[rec, :3].tolist() == [s, tok0, nq]
+            assert (part - combine[rec, 3]) % (2 * nq) == 0
+            assert 0 <= (part - combine[rec, 3]) // (2 * nq) < combine[rec, 4]
         seen = pages.setdefault((s, tok0), set())
         assert not seen & set(range(pb, pe))
         seen |= set(range(pb, pe))
@@ -162,7 +170,8 @@ def test_tree_plan_refuses_bad_batches() -> None:
         plan_tree_batch([_chunk(1, 2, 4, 0, [-1, 0])], 2)
     with pytest.raises(ValueError, match="more than 1024"):
         plan_tree_batch([_chunk(0, 1025, 0, 0, [-1] * 1025)], 1025)
-    assert plan_tree_batch([], 0)[1].n_tile_items == 0
+    none = plan_tree_batch([], 0)[1]
+    assert none.n_tile_items == 0 and none.n_decode_items == 0
 
 
 def test_tree_plan_reports_a_small_buffer() -> None:
@@ -203,7 +212,7 @@ def test_kv8_part_maps_every_page_of_tensor_core_items() -> None:
             assert np.array_equal(seqs[i], plain[i])
     lib = _capi.load()
     need = lib.ms_kv8_workspace_bytes(C.byref(info), C.byref(kv8), 8)
-    part = info.workspace_bytes_per_kv_head * 8
+    part = (info.workspace_bytes_per_kv_head + 8 * info.n_combine) * 8
     assert need == -(-part // 1024) * 1024 + kv8.n_pages * 8 * 8192
     _, short, none = _plan_with_kv8(chunks[:1], 1, 148, 0)
     assert none.n_pages == 0 and short.n_tc_items == 0

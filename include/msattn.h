@@ -221,13 +221,20 @@ typedef struct MsKv8Info {
   int32_t off_seqs;   /* int offsets in the packed buffer: sequence records whose tables index */
   int32_t off_map;    /* the expanded pages; the expanded pages' block ids; 0, 1, 2, ... */
   int32_t off_tables;
+  int32_t n_narrow;   /* work items of the rows with up to 64 new tokens: tiles of <= 16 tokens, */
+  int32_t off_narrow; /* tiles of 17..32, and the combine records of split tiles */
+  int32_t n_wide;
+  int32_t off_wide;
+  int32_t n_combine;
+  int32_t off_combine;
   int32_t total_ints; /* length of the packed buffer with this part */
-  int32_t reserved[3];
+  int32_t reserved;
+  int64_t part_rows;  /* partial rows beyond the plan's */
 } MsKv8Info;
 
-MS_API int64_t ms_kv8_plan_capacity(const MsPlanInfo* plan, int64_t total_table_entries);
+MS_API int64_t ms_kv8_plan_capacity(int32_t num_seqs, int64_t total_table_entries);
 MS_API int ms_kv8_plan_build(int32_t* packed, int64_t capacity, const MsPlanInfo* plan,
-                             MsKv8Info* info);
+                             int32_t num_sms, int32_t pages_per_split, MsKv8Info* info);
 MS_API int64_t ms_kv8_workspace_bytes(const MsPlanInfo* plan, const MsKv8Info* info,
                                       int32_t num_kv_heads);
 MS_API int ms_paged_attention_kv8(const void* q, int64_t q_row_stride, void* out,

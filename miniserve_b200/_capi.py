@@ -85,8 +85,15 @@ class MsKv8Info(C.Structure):
         ("off_seqs", C.c_int32),
         ("off_map", C.c_int32),
         ("off_tables", C.c_int32),
+        ("n_narrow", C.c_int32),
+        ("off_narrow", C.c_int32),
+        ("n_wide", C.c_int32),
+        ("off_wide", C.c_int32),
+        ("n_combine", C.c_int32),
+        ("off_combine", C.c_int32),
         ("total_ints", C.c_int32),
-        ("reserved", C.c_int32 * 3),
+        ("reserved", C.c_int32),
+        ("part_rows", C.c_int64),
     ]
 
 
@@ -123,9 +130,9 @@ _SIGNATURES = {
     ),
     "ms_kv_gather": (C.c_int, [_P, _I32, _I32, _P, _P, _I32, _P, _I64, _P, _I64, _P]),
     "ms_kv_gather_kv8": (C.c_int, [_P, _I32, _I32, _P, _I32, _P, _I64, _P, _I64, _P]),
-    "ms_kv8_plan_capacity": (_I64, [C.POINTER(MsPlanInfo), _I64]),
+    "ms_kv8_plan_capacity": (_I64, [_I32, _I64]),
     "ms_kv8_plan_build": (
-        C.c_int, [_P, _I64, C.POINTER(MsPlanInfo), C.POINTER(MsKv8Info)]),
+        C.c_int, [_P, _I64, C.POINTER(MsPlanInfo), _I32, _I32, C.POINTER(MsKv8Info)]),
     "ms_kv8_workspace_bytes": (
         _I64, [C.POINTER(MsPlanInfo), C.POINTER(MsKv8Info), _I32]),
     "ms_paged_attention_kv8": (

@@ -135,8 +135,10 @@ class AttentionMetadata:
             return None
         ws = torch.empty(need, dtype=torch.uint8, device=device)
         if counters:
-            at = int(self.info.part_rows) * (HEAD_DIM + 1) * 4 * num_kv_heads
-            ws[at : at + int(self.info.n_combine) * 8 * num_kv_heads].zero_()
+            rows = int(self.info.part_rows) + (int(self.kv8.part_rows) if kv8 else 0)
+            n = int(self.kv8.n_combine if kv8 else self.info.n_combine)
+            at = rows * (HEAD_DIM + 1) * 4 * num_kv_heads
+            ws[at : at + n * 4 * num_kv_heads].zero_()
         self._workspace[key] = ws
         return ws
 
@@ -161,6 +163,20 @@ def plan_batch(
     pages_per_split: int = 0,
 ) -> tuple[np.ndarray, _capi.MsPlanInfo]:
     """Run the native planner on the host; returns ``(packed int32 plan, info)``."""
+    packed, info, _ = _plan(chunks, num_tokens, block_size, num_sms, pages_per_split, None)
+    return packed, info
+
+
+def _plan_with_kv8(chunks: list[SeqChunk], num_tokens: int, num_sms: int, pages_per_split: int
+                   ) -> tuple[np.ndarray, _capi.MsPlanInfo, _capi.MsKv8Info]:
+    """The plan with the part an 8-bit pool needs behind it, so that one plan (and one upload)
+    serves either kind of pool."""
+    kv8 = _capi.MsKv8Info()
+    return _plan(chunks, num_tokens, BLOCK_SIZE, num_sms, pages_per_split, kv8)
+
+
+def _plan(chunks: list[SeqChunk], num_tokens: int, block_size: int, num_sms: int,
+          pages_per_split: int, kv8: _capi.MsKv8Info | None):
     lib = _capi.load()
     n = len(chunks)
     flat = np.fromiter((c.flat_start for c in chunks), dtype=np.int32, count=n)
@@ -173,7 +189,8 @@ def plan_batch(
     tables = np.fromiter(chain.from_iterable(c.block_table for c in chunks), dtype=np.int32,
                          count=total)
     cap = int(lib.ms_plan_capacity(n, num_tokens, total))
-    out = np.empty(cap, dtype=np.int32)
+    out = np.empty(cap + (int(lib.ms_kv8_plan_capacity(n, total)) if kv8 is not None else 0),
+                   dtype=np.int32)
     info = _capi.MsPlanInfo()
     rc = lib.ms_plan_build(
         n, flat.ctypes.data, new.ctypes.data, cached.ctypes.data, offsets.ctypes.data,
@@ -181,7 +198,12 @@ def plan_batch(
         out.ctypes.data, cap, C.byref(info),
     )
     _capi.check(rc, "build_attention_metadata")
-    return out[: info.total_ints], info
+    if kv8 is None:
+        return out[: info.total_ints], info, None
+    rc = lib.ms_kv8_plan_build(out.ctypes.data, out.size, C.byref(info), num_sms, pages_per_split,
+                               C.byref(kv8))
+    _capi.check(rc, "build_attention_metadata")
+    return out[: kv8.total_ints], info, kv8
 
 
 def plan_tree_batch(
@@ -224,22 +246,6 @@ def plan_tree_batch(
 def _split_trees(chunks: list[SeqChunk]) -> tuple[list[SeqChunk], list[SeqChunk]]:
     trees = [c for c in chunks if c.parents is not None]
     return ([c for c in chunks if c.parents is None], trees) if trees else (chunks, trees)
-
-
-def _plan_with_kv8(chunks: list[SeqChunk], num_tokens: int, num_sms: int, pages_per_split: int
-                   ) -> tuple[np.ndarray, _capi.MsPlanInfo, _capi.MsKv8Info]:
-    """The plan with the part an 8-bit pool's tensor-core items need behind it, so that one plan
-    (and one upload) serves either kind of pool."""
-    lib = _capi.load()
-    packed, info = plan_batch(chunks, num_tokens, BLOCK_SIZE, num_sms, pages_per_split)
-    kv8 = _capi.MsKv8Info()
-    if not info.n_tc_items:
-        return packed, info, kv8
-    more = int(lib.ms_kv8_plan_capacity(C.byref(info), sum(len(c.block_table) for c in chunks)))
-    packed = np.concatenate([packed, np.empty(more, dtype=np.int32)])
-    _capi.check(lib.ms_kv8_plan_build(packed.ctypes.data, packed.size, C.byref(info),
-                                      C.byref(kv8)), "build_attention_metadata")
-    return packed[: kv8.total_ints], info, kv8
 
 
 def prepare_arrays(num_new: np.ndarray, num_cached: np.ndarray, table_offsets: np.ndarray,

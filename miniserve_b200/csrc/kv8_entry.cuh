@@ -31,7 +31,7 @@ cudaError_t launch_rows(int64_t tokens, int num_kv, int sms, Few few, Many many)
 int check_attention(const char* what, const void* q, int64_t q_row_stride, const void* out,
                     int64_t out_row_stride, int num_heads, int num_kv, const int32_t* plan_dev,
                     const MsPlanInfo* plan, const void* workspace, int64_t workspace_bytes,
-                    int64_t need, float scale) {
+                    int64_t need, int64_t most_items, float scale) {
   if (plan == nullptr || num_kv <= 0 || num_heads != ms::kGroup * num_kv) {
     set_error(std::string(what) + ": need a plan and num_heads == 2 * num_kv_heads > 0");
     return MS_ERR_ARG;
@@ -51,9 +51,8 @@ int check_attention(const char* what, const void* q, int64_t q_row_stride, const
               " bytes (16-byte aligned) required");
     return MS_ERR_ARG;
   }
-  const int64_t items = static_cast<int64_t>(plan->n_decode_items) + 2 * plan->n_tile_items +
-                        plan->n_tc_items;
-  if (items * num_kv > 0x7fffffffLL || static_cast<int64_t>(plan->n_combine) * num_kv > 0x7fffffffLL) {
+  if (most_items * num_kv > 0x7fffffffLL ||
+      static_cast<int64_t>(plan->n_combine) * num_kv > 0x7fffffffLL) {
     set_error(std::string(what) + ": plan too large for one launch");
     return MS_ERR_ARG;
   }
@@ -62,7 +61,7 @@ int check_attention(const char* what, const void* q, int64_t q_row_stride, const
 
 ms::AttnArgs attn_args(const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride,
                        int num_kv, int num_blocks, const int32_t* plan_dev, const MsPlanInfo* plan,
-                       void* workspace, float scale) {
+                       void* workspace, int64_t part_rows, float scale) {
   ms::AttnArgs a;
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.q_row_stride = q_row_stride;
@@ -76,42 +75,41 @@ ms::AttnArgs attn_args(const void* q, int64_t q_row_stride, void* out, int64_t o
   a.num_blocks = num_blocks;
   float* ws = static_cast<float*>(workspace);
   a.ws_o = ws;
-  a.ws_lse = ws != nullptr ? ws + plan->part_rows * num_kv * ms::kHeadDim : nullptr;
+  a.ws_lse = ws != nullptr ? ws + part_rows * num_kv * ms::kHeadDim : nullptr;
   a.scale_log2 = scale * 1.4426950408889634f;
   return a;
 }
 
-// Kernel F over the plan's narrow items (decode rows, trees of up to 8 drafts) and its wide ones
-// (chunks of up to 64 tokens as two halves of 32, larger trees).
+// Where a packed plan holds kernel F's work.
+struct RowsWork {
+  int32_t n_narrow, off_narrow, n_wide, off_wide, off_combine;
+  int64_t part_rows;  // of all partials in the workspace; the arrival counters lie behind them
+};
+
+// Kernel F over the narrow tiles and the wide ones.
 template <bool kKv8, bool kTree>
 cudaError_t launch_rows_attention(const ms::AttnArgs& a, const void* pool, const CUtensorMap& map,
-                                  const int32_t* plan_dev, const MsPlanInfo* plan, cudaStream_t s) {
+                                  const int32_t* plan_dev, const RowsWork& w, cudaStream_t s) {
   ms::RowsArgs r;
   r.a = a;
   r.pool = static_cast<const uint8_t*>(pool);
   r.plan = plan_dev;
-  r.combines = plan_dev + plan->off_combine;
-  // Arrival counters lie behind the partials.
-  r.arrived = a.ws_lse != nullptr ? reinterpret_cast<int*>(a.ws_lse + plan->part_rows * a.num_kv)
-                                  : nullptr;
+  r.combines = plan_dev + w.off_combine;
+  r.arrived = a.ws_lse != nullptr ? reinterpret_cast<int*>(a.ws_lse + w.part_rows * a.num_kv) : nullptr;
   cudaError_t e = cudaSuccess;
-  if (plan->n_decode_items > 0) {
+  if (w.n_narrow > 0) {
     using Cfg = ms::RowsCfg<kKv8, 1>;
-    r.halves = 1;
-    r.a.items = plan_dev + plan->off_decode;
-    r.a.n_items = plan->n_decode_items;
-    e = launch(ms::rows_attn_kernel<kKv8, kTree, 1>,
-               static_cast<unsigned>(plan->n_decode_items * a.num_kv), Cfg::kThreads,
-               Cfg::kSmemBytes, s, map, r);
+    r.a.items = plan_dev + w.off_narrow;
+    r.a.n_items = w.n_narrow;
+    e = launch(ms::rows_attn_kernel<kKv8, kTree, 1>, static_cast<unsigned>(w.n_narrow * a.num_kv),
+               Cfg::kThreads, Cfg::kSmemBytes, s, map, r);
   }
-  if (e == cudaSuccess && plan->n_tile_items > 0) {
+  if (e == cudaSuccess && w.n_wide > 0) {
     using Cfg = ms::RowsCfg<kKv8, 2>;
-    r.halves = kTree ? 1 : 2;
-    r.a.items = plan_dev + plan->off_tile;
-    r.a.n_items = plan->n_tile_items;
-    e = launch(ms::rows_attn_kernel<kKv8, kTree, 2>,
-               static_cast<unsigned>(plan->n_tile_items * r.halves * a.num_kv), Cfg::kThreads,
-               Cfg::kSmemBytes, s, map, r);
+    r.a.items = plan_dev + w.off_wide;
+    r.a.n_items = w.n_wide;
+    e = launch(ms::rows_attn_kernel<kKv8, kTree, 2>, static_cast<unsigned>(w.n_wide * a.num_kv),
+               Cfg::kThreads, Cfg::kSmemBytes, s, map, r);
   }
   return e;
 }
@@ -285,13 +283,16 @@ extern "C" int ms_paged_attention_kv8(const void* q, int64_t q_row_stride, void*
   if (plan != nullptr &&
       static_cast<int64_t>(plan->n_decode_items) + plan->n_tile_items + plan->n_tc_items == 0)
     return MS_OK;
-  if (plan != nullptr && (info == nullptr || (plan->n_tc_items > 0 && info->n_pages <= 0))) {
+  if (plan != nullptr && (info == nullptr || info->total_ints < plan->total_ints ||
+                          (plan->n_tc_items > 0 && info->n_pages <= 0))) {
     set_error("ms_paged_attention_kv8: the plan has no 8-bit part (ms_kv8_plan_build)");
     return MS_ERR_ARG;
   }
   const int64_t need = plan != nullptr ? ms_kv8_workspace_bytes(plan, info, num_kv_heads) : 0;
   int rc = check_attention(what, q, q_row_stride, out, out_row_stride, num_heads, num_kv_heads,
-                           plan_dev, plan, workspace, workspace_bytes, need, scale);
+                           plan_dev, plan, workspace, workspace_bytes, need,
+                           plan == nullptr ? 0 : std::max(std::max(info->n_narrow, info->n_wide),
+                                                          plan->n_tc_items), scale);
   if (rc) return rc;
   rc = check_pool8(what, pool, num_blocks, num_kv_heads);
   if (rc) return rc;
@@ -300,8 +301,10 @@ extern "C" int ms_paged_attention_kv8(const void* q, int64_t q_row_stride, void*
   unsigned* st = status_ptr(&rc);
   if (rc) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const RowsWork work = {info->n_narrow,    info->off_narrow,  info->n_wide, info->off_wide,
+                         info->off_combine, plan->part_rows + info->part_rows};
   ms::AttnArgs a = attn_args(q, q_row_stride, out, out_row_stride, num_kv_heads, num_blocks,
-                             plan_dev, plan, workspace, scale);
+                             plan_dev, plan, workspace, work.part_rows, scale);
 
   // The pages of tensor-core items as a bf16 pool in the workspace, after the partials.
   void* pages = nullptr;
@@ -321,7 +324,7 @@ extern "C" int ms_paged_attention_kv8(const void* q, int64_t q_row_stride, void*
 
   // As in ms_paged_attention: beside tensor-core work without cascade groups the bandwidth-bound
   // rows run on the side stream; with them they follow the kernel that writes the prefix partials.
-  const int n_rows = plan->n_decode_items + plan->n_tile_items;
+  const int n_rows = work.n_narrow + work.n_wide;
   SideStream* side = nullptr;
   if (plan->n_tc_items > 0 && n_rows > 0 && plan->n_cascade == 0) side = side_stream();
   cudaStream_t ds = s;
@@ -362,7 +365,7 @@ extern "C" int ms_paged_attention_kv8(const void* q, int64_t q_row_stride, void*
   if (n_rows > 0) {
     CUtensorMap none;
     std::memset(&none, 0, sizeof(none));
-    const cudaError_t e = launch_rows_attention<true, false>(a, pool, none, plan_dev, plan, ds);
+    const cudaError_t e = launch_rows_attention<true, false>(a, pool, none, plan_dev, work, ds);
     if (e != cudaSuccess) {
       join();
       return cuda_fail("8-bit rows launch", e);
@@ -388,7 +391,9 @@ extern "C" int ms_tree_attention(const void* q, int64_t q_row_stride, void* out,
   if (plan != nullptr && plan->n_decode_items + plan->n_tile_items == 0) return MS_OK;
   const int64_t need = plan != nullptr ? plan->workspace_bytes_per_kv_head * num_kv_heads : 0;
   int rc = check_attention(what, q, q_row_stride, out, out_row_stride, num_heads, num_kv_heads,
-                           plan_dev, plan, workspace, workspace_bytes, need, scale);
+                           plan_dev, plan, workspace, workspace_bytes, need,
+                           plan == nullptr ? 0 : std::max(plan->n_decode_items, plan->n_tile_items),
+                           scale);
   if (rc) return rc;
   const bool kv8 = v_cache == nullptr;
   rc = kv8 ? check_pool8(what, k_cache, num_blocks, num_kv_heads)
@@ -403,11 +408,13 @@ extern "C" int ms_tree_attention(const void* q, int64_t q_row_stride, void* out,
     if (rc) return rc;
   }
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const RowsWork work = {plan->n_decode_items, plan->off_decode,  plan->n_tile_items,
+                         plan->off_tile,       plan->off_combine, plan->part_rows};
   const ms::AttnArgs a = attn_args(q, q_row_stride, out, out_row_stride, num_kv_heads, num_blocks,
-                                   plan_dev, plan, workspace, scale);
+                                   plan_dev, plan, workspace, work.part_rows, scale);
   const cudaError_t e =
-      kv8 ? launch_rows_attention<true, true>(a, k_cache, map, plan_dev, plan, s)
-          : launch_rows_attention<false, true>(a, nullptr, map, plan_dev, plan, s);
+      kv8 ? launch_rows_attention<true, true>(a, k_cache, map, plan_dev, work, s)
+          : launch_rows_attention<false, true>(a, nullptr, map, plan_dev, work, s);
   if (e != cudaSuccess) return cuda_fail("tree attention launch", e);
   return MS_OK;
 }

@@ -412,9 +412,6 @@ extern "C" int ms_plan_build(int32_t num_seqs, const int32_t* flat_start, const 
     r[4] = static_cast<int32_t>(table_offsets[i]);
     r[5] = static_cast<int32_t>(table_offsets[i + 1] - table_offsets[i]);
   }
-  // Field 6 of a sequence whose one decode or chunk tile is split: its combine record.
-  for (size_t k = 0; k + comb_tc.size() < comb.size(); ++k)
-    out[off_seqs + static_cast<int64_t>(comb[k].seq) * kRec + 6] = static_cast<int32_t>(k);
   for (size_t g = 0; g < groups.size(); ++g) {
     const Group& G = groups[g];
     int32_t* r = out + off_seqs + (static_cast<int64_t>(num_seqs) + static_cast<int64_t>(g)) * kRec;

@@ -51,10 +51,8 @@ struct RowsArgs {
   AttnArgs a;           // queries, output, plan sections, partials
   const uint8_t* pool;  // 8-bit layer (null for a bf16 pool, which the tensor map describes)
   const int* plan;      // start of the packed plan: tree masks are at sequence record field 6
-  const int* combines;  // combine records of split tiles: a tree item names its record in field 6, a
-                        // causal sequence (which has one tile) in its sequence record's field 6
-  int* arrived;         // [record][2 halves][KVH] splits that have finished: zero between calls
-  int halves;           // 2: an item is two tiles of 32 tokens (chunks of up to 64), else 1
+  const int* combines;  // combine records of split tiles (an item names its record in field 6)
+  int* arrived;         // [record][KVH] splits that have finished: zero between calls
 };
 
 template <bool kKv8, int kRG>
@@ -605,81 +603,93 @@ __device__ __forceinline__ void put_cols(const RowOut& o, int d, const float (&x
 }
 
 // The last CTA of a split tile merges the splits' partial rows: out = sum_s 2^(lse_s - M) O_s /
-// sum_s 2^(lse_s - M), s in order, so the result does not depend on which CTA came last.  A warp
-// takes kR rows at a time, a lane four columns; kR times kS loads of partial rows are in flight (few rows
-// have many splits, many rows few).
-template <int kR, int kS>
-__device__ __forceinline__ void merge_splits(const AttnArgs& a, int row0, int stride, int n_splits,
-                                             int rows, int kvh, int flat_tok, int warp, int lane) {
-  for (int r0 = warp * kR; r0 < rows; r0 += kRowsWarps * kR) {
-    float M[kR], L[kR];
-    float4 acc[kR];
+// sum_s 2^(lse_s - M), s in order, so the result does not depend on which CTA came last.  The
+// partial rows come through shared memory (the idle ring, `bytes` of it) by asynchronous copies, as many
+// splits at a time as fit, so that one latency covers them all (through registers the merge took 4-8
+// us of a short call); the rows' M and sums are formed from global memory meanwhile.  A warp
+// takes rows warp, warp + 4, ..., a lane four columns.
+template <int kRows>
+__device__ __forceinline__ void merge_splits(const AttnArgs& a, uint8_t* smem, int bytes, int row0,
+                                             int n_splits, int rows, int kvh, int flat_tok) {
+  constexpr int kT = kRowsWarps * 32, kPer = kRows / kRowsWarps, kLanes = kT / kRows;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  float* top = reinterpret_cast<float*>(smem);  // [kRows] M, then [kRows] 1 / sum
+  float* lse_s = top + 2 * kRows;               // [splits of a chunk][rows], then their O rows
+  const int chunk = max(1, min(n_splits, (bytes - 2 * kRows * 4) / (rows * (kHeadDim + 1) * 4 + 16)));
+  float* o_s = lse_s + (chunk * rows + 3) / 4 * 4;
+  auto at = [&](int s, int r) {
+    return (static_cast<long long>(row0) + static_cast<long long>(s) * rows + r) * a.num_kv + kvh;
+  };
+  float4 acc[kPer];
 #pragma unroll
-    for (int k = 0; k < kR; ++k) {
-      M[k] = -INFINITY;
-      L[k] = 0.f;
-      acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < kPer; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < n_splits; s0 += chunk) {
+    const int cnt = min(chunk, n_splits - s0);
+    if (s0 > 0) asm volatile("bar.sync 1, %0;" ::"r"(kT) : "memory");  // the last chunk was read
+    for (int i = warp; i < cnt * rows; i += kRowsWarps) {
+      const float* src = a.ws_o + at(s0, 0) * kHeadDim +
+                         static_cast<long long>(i) * a.num_kv * kHeadDim + lane * 4;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                       smem_u32(o_s + i * kHeadDim + lane * 4)),
+                   "l"(src)
+                   : "memory");
     }
-    auto at = [&](int s, int k) {
-      return (static_cast<long long>(row0) + static_cast<long long>(s) * stride +
-              min(r0 + k, rows - 1)) * a.num_kv + kvh;
-    };
-    for (int s = lane; s < n_splits; s += 32) {
-#pragma unroll
-      for (int k = 0; k < kR; ++k) M[k] = fmaxf(M[k], __ldcg(a.ws_lse + at(s, k)));
-    }
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) {
-#pragma unroll
-      for (int k = 0; k < kR; ++k) M[k] = fmaxf(M[k], __shfl_xor_sync(0xffffffffu, M[k], off));
-    }
-    for (int sb = 0; sb < n_splits; sb += 32) {
-      float w[kR];
-#pragma unroll
-      for (int k = 0; k < kR; ++k) {
-        const float lse = sb + lane < n_splits ? __ldcg(a.ws_lse + at(sb + lane, k)) : -INFINITY;
-        w[k] = lse == -INFINITY ? 0.f : fast_exp2(lse - M[k]);
-        L[k] += w[k];
-      }
-      const int cnt = min(32, n_splits - sb);
-      for (int i0 = 0; i0 < cnt; i0 += kS) {
-        float4 v[kS][kR];
-#pragma unroll
-        for (int i = 0; i < kS; ++i) {
-#pragma unroll
-          for (int k = 0; k < kR; ++k)
-            v[i][k] = __ldcg(reinterpret_cast<const float4*>(
-                                 a.ws_o + at(sb + min(i0 + i, cnt - 1), k) * kHeadDim) + lane);
-        }
-#pragma unroll
-        for (int i = 0; i < kS; ++i) {
-#pragma unroll
-          for (int k = 0; k < kR; ++k) {
-            const float wi = i0 + i < cnt ? __shfl_sync(0xffffffffu, w[k], i0 + i) : 0.f;
-            if (i0 + i >= cnt) continue;
-            acc[k].x += wi * v[i][k].x;
-            acc[k].y += wi * v[i][k].y;
-            acc[k].z += wi * v[i][k].z;
-            acc[k].w += wi * v[i][k].w;
-          }
+    for (int i = tid; i < cnt * rows; i += kT) lse_s[i] = __ldcg(a.ws_lse + at(s0, 0) + static_cast<long long>(i) * a.num_kv);
+    if (s0 == 0) {
+      // kLanes neighbouring threads per row, over all splits.
+      const int r = tid / kLanes;
+      float m = -INFINITY, l = 0.f;
+      if (r < rows) {
+#pragma unroll 4
+        for (int s = tid % kLanes; s < n_splits; s += kLanes) {
+          const float x = __ldcg(a.ws_lse + at(s, r));
+          if (x == -INFINITY) continue;
+          const float mn = fmaxf(m, x);
+          l = l * fast_exp2(m - mn) + fast_exp2(x - mn);  // a NaN stays in l
+          m = mn;
         }
       }
-    }
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) {
-#pragma unroll
-      for (int k = 0; k < kR; ++k) L[k] += __shfl_xor_sync(0xffffffffu, L[k], off);
+      for (int off = 1; off < kLanes; off <<= 1) {
+        const float mo = __shfl_xor_sync(0xffffffffu, m, off);
+        const float lo = __shfl_xor_sync(0xffffffffu, l, off);
+        const float mn = fmaxf(m, mo);
+        l = (m == -INFINITY ? l : l * fast_exp2(m - mn)) + (mo == -INFINITY ? lo : lo * fast_exp2(mo - mn));
+        m = mn;
+      }
+      if (r < kRows && tid % kLanes == 0) {
+        top[r] = m;
+        top[kRows + r] = l != 0.f ? 1.f / l : 0.f;
+      }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    asm volatile("bar.sync 1, %0;" ::"r"(kT) : "memory");
 #pragma unroll
-    for (int k = 0; k < kR; ++k) {
-      const int r = r0 + k;
-      if (r >= rows) break;
-      const float inv = L[k] != 0.f ? 1.f / L[k] : 0.f;
-      __nv_bfloat16* dst = a.out + static_cast<long long>(flat_tok + (r >> 1)) * a.out_row_stride +
-                           (kvh * kGroup + (r & 1)) * kHeadDim + lane * 4;
-      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc[k].x * inv, acc[k].y * inv),
-                                                  pack_bf16(acc[k].z * inv, acc[k].w * inv));
+    for (int k = 0; k < kPer; ++k) {
+      const int r = warp + k * kRowsWarps;
+      if (r < rows) {
+        const float m = top[r];
+        for (int i = 0; i < cnt; ++i) {
+          const float x = lse_s[i * rows + r];
+          const float w = x == -INFINITY ? 0.f : fast_exp2(x - m);
+          const float4 v = *reinterpret_cast<const float4*>(o_s + (i * rows + r) * kHeadDim + lane * 4);
+          acc[k].x += w * v.x;
+          acc[k].y += w * v.y;
+          acc[k].z += w * v.z;
+          acc[k].w += w * v.w;
+        }
+      }
     }
+  }
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int r = warp + k * kRowsWarps;
+    if (r >= rows) break;
+    const float inv = top[kRows + r];
+    __nv_bfloat16* dst = a.out + static_cast<long long>(flat_tok + (r >> 1)) * a.out_row_stride +
+                         (kvh * kGroup + (r & 1)) * kHeadDim + lane * 4;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc[k].x * inv, acc[k].y * inv),
+                                                pack_bf16(acc[k].z * inv, acc[k].w * inv));
   }
 }
 
@@ -699,25 +709,24 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
   uint64_t* empty = full + kStages;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + kStages);
   volatile int* last_flag = abort_flag + 1;
-  static_assert(2 * kRowsNarrowTokens == RowsCfg<kKv8, 1>::kRows, "rows of a narrow tile");
+  static_assert(2 * (kRG == 1 ? kRowsNarrowTokens : kRowsTokens) == Cfg::kRows, "rows of a tile");
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int slot = blockIdx.x / a.num_kv;
-  const int kvh = blockIdx.x - slot * a.num_kv;
-  const int item_idx = slot / ra.halves;
-  const int half = slot - item_idx * ra.halves;
+  const int item_idx = blockIdx.x / a.num_kv;
+  const int kvh = blockIdx.x - item_idx * a.num_kv;
   // The plan was copied in before the previous kernel started, so it is read before the wait.
   const int* it = a.items + static_cast<long long>(item_idx) * kRec;
-  const int seq = it[0], tok0 = it[1] + half * kRowsTokens, page_begin = it[3];
-  const int n_q = min(it[2] - half * kRowsTokens, kRG == 1 ? kRowsNarrowTokens : kRowsTokens);
-  if (n_q <= 0) return;  // the second half of a chunk of up to 32 tokens
-  const int part_row = it[5] < 0 ? -1 : it[5] + half * kRowsTokens * kGroup;
+  const int seq = it[0], tok0 = it[1], n_q = it[2], page_begin = it[3], part_row = it[5];
   const int merge_row = it[7] == 1 ? it[6] : -1;
   const int* sr = a.seqs + static_cast<long long>(seq) * kRec;
   const int flat_start = sr[0], num_cached = sr[2], table_off = sr[4];
-  // Keys after the tile's last token are visible to none of its rows.
-  const int npages = min(it[4], (num_cached + tok0 + n_q + kBlockTokens - 1) / kBlockTokens) - page_begin;
+  const int npages = it[4] - page_begin;
+  if (part_row >= 0 && threadIdx.x == 0) {
+    // What the end of a split needs: its combine record and arrival counter.
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(ra.combines + static_cast<long long>(it[6]) * kRec));
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(ra.arrived + static_cast<long long>(it[6]) * a.num_kv + kvh));
+  }
 
   const int sets = n_q * kGroup > 16 * kRG ? 2 : 1;
   const int phases = kRowsWarps / sets;
@@ -1068,10 +1077,9 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
     // A split of a tile: the last one to arrive merges them all.
     __threadfence();
     asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
-    const int record = kTree ? it[6] : sr[6];
-    const int* cr = ra.combines + static_cast<long long>(record) * kRec;
+    const int* cr = ra.combines + static_cast<long long>(it[6]) * kRec;
     if (threadIdx.x == 0) {
-      int* counter = ra.arrived + (static_cast<long long>(record) * 2 + half) * a.num_kv + kvh;
+      int* counter = ra.arrived + static_cast<long long>(it[6]) * a.num_kv + kvh;
       const bool last = atomicAdd(counter, 1) == cr[4] - 1;
       if (last) *counter = 0;  // ready for the next call
       *last_flag = last ? 1 : 0;
@@ -1079,9 +1087,8 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
     asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
     if (*last_flag) {
       __threadfence();
-      merge_splits<kRG == 1 ? 2 : 8, kRG == 1 ? 8 : 2>(
-          a, cr[3] + half * kRowsTokens * kGroup, cr[5] != 0 ? cr[5] : cr[2] * kGroup, cr[4],
-          n_q * kGroup, kvh, flat_start + tok0, warp, lane);
+      merge_splits<Cfg::kRows>(a, ring, Cfg::kStageBytes, cr[3], cr[4], n_q * kGroup, kvh,
+                               flat_start + tok0);
     }
   }
 }

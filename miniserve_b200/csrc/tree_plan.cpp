@@ -1,13 +1,16 @@
 // Host planners of the 8-bit pool and of drafted token trees (declared in include/msattn.h).
 //
-// ms_kv8_plan_build adds to a packed plan what its tensor-core items need over an 8-bit pool: the
-// pages they read are expanded to bf16 in the workspace, numbered densely, so the part holds the
-// expanded pages' block ids, the identity table the kernel walks instead of the block tables, and the
-// sequence records with their tables' places in it.
+// Both cut the work of kernel F: tiles of at most 32 query tokens of one sequence, split over their
+// pages where that fills the GPU.
 //
-// ms_tree_plan_build cuts every sequence of drafts into tiles of at most 32 tokens (64 query rows),
-// each reading the cached context and the drafts up to its own last one (a parent precedes its
-// children), and splits long tiles over their pages as ms_plan_build does.  Masks are bit rows, one per
+// ms_kv8_plan_build adds to a packed plan those tiles for the sequences of up to 64 new tokens, and
+// what its tensor-core items need over an 8-bit pool: the pages they read are expanded to bf16 in the
+// workspace, numbered densely, so the part holds the expanded pages' block ids, the identity table
+// the kernel walks instead of the block tables, and the sequence records with their tables' places
+// in it.
+//
+// ms_tree_plan_build cuts every sequence of drafts into tiles that read the cached context and the
+// drafts up to the tile's last one (a parent precedes its children).  Masks are bit rows, one per
 // draft, ceil(num_new / 32) words each, at the sequence record's field 6 (length in words in field 7).
 #include <algorithm>
 #include <climits>
@@ -26,10 +29,16 @@ void set_error(const std::string& msg);
 namespace {
 
 constexpr int kRec = 8;
-constexpr int kTileTokens = 32;
-constexpr int kAssumedKvHeads = 4;  // the planner does not see the head count; only speed depends on it
+constexpr int kTileTokens = 32;     // tokens of a wide tile (64 query rows) at most
 constexpr int kNarrowTokens = 16;   // tiles of at most 32 query rows run three CTAs per SM, others two
-constexpr int kMinSplitPages = 8;
+// The planner does not see the head count, and only speed depends on it.  Narrow tiles are sized for two
+// CTAs per SM at 8 KV heads: they are bound by memory, which fewer CTAs still keep busy at 4 heads, and
+// more splits only cost merging (3 rows over 100k tokens: 57 us with 36 splits, 70 with 111; 64 trees
+// of 16 drafts: 101 us, 115 when sized for the three CTAs that fit).  Wide
+// tiles are bound by the SMs, so they are sized for 4 heads, two waves at 8 (16 trees of 63 drafts
+// over 4 heads: 180 us sized for 8 heads, 127 for 4).
+constexpr int kNarrowHeads = 8, kWideHeads = 4;
+constexpr int kMinSplitPages = 8, kMinWideSplitPages = 96;
 constexpr int kMaxSplitPages = 512;
 
 int64_t round4(int64_t x) { return (x + 3) & ~int64_t(3); }
@@ -48,40 +57,177 @@ int guarded(const char* what, F f) {
   }
 }
 
-struct TreeItem {
-  int seq, tok0, n_q, pb, pe, part_row;
-  int record = 0, flag = 0;  // of a split item: its combine record, and 2
+// A tile of at most 32 query tokens and the pages it reads, before splitting; then a work item.
+struct RowsItem {
+  int seq, tok0, n_q, pb, pe;
+  int part_row = -1;
+  // Fields 6 and 7: the combine record and 2 for a split, the shared-prefix partial row and 1 for a
+  // cascade row.
+  int field6 = 0, field7 = 0;
 };
+
+// The items of kernel F: narrow and wide tiles (two launches), split over their pages, and the
+// combine records of the split ones.
+struct RowsPlan {
+  std::vector<RowsItem> narrow, wide, comb;  // comb: pb = first partial row, pe = number of splits
+  int64_t part_rows = 0;                     // from `base` on
+  int split_narrow = 0, split_wide = 0;
+};
+
+// Split size, for the narrow tiles and the wide ones: the smallest multiple of 8 pages whose items fit
+// one resident wave of CTAs; when the tiles alone exceed it, tiles longer than the pages per CTA
+// slot are cut to about that size.
+int choose_split(const std::vector<RowsItem>& tiles, bool narrow, int num_sms) {
+  const int least = narrow ? kMinSplitPages : kMinWideSplitPages;
+  const int64_t target =
+      std::max<int64_t>(1, narrow ? static_cast<int64_t>(num_sms) * 2 / kNarrowHeads
+                                  : static_cast<int64_t>(num_sms) * 2 / kWideHeads);
+  int64_t all = 0;
+  for (const RowsItem& t : tiles)
+    if ((t.n_q <= kNarrowTokens) == narrow) all += t.pe - t.pb;
+  auto items_at = [&](int64_t p) {
+    int64_t items = 0;
+    for (const RowsItem& t : tiles)
+      if ((t.n_q <= kNarrowTokens) == narrow) items += (t.pe - t.pb + p - 1) / p;
+    return items;
+  };
+  if (items_at(kMaxSplitPages) > target) {
+    const int64_t per_slot = (all + target - 1) / target;
+    return static_cast<int>(std::min<int64_t>(
+        kMaxSplitPages, std::max<int64_t>(least, (per_slot + 7) / 8 * 8)));
+  }
+  int lo = least / 8, hi = kMaxSplitPages / 8;
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (items_at(mid * 8) <= target) hi = mid; else lo = mid + 1;
+  }
+  return lo * 8;
+}
+
+// Splits the tiles (cascade rows, field7 == 1, stay whole).  False: too many partial rows.
+bool plan_rows(const std::vector<RowsItem>& tiles, int num_sms, int pages_per_split, int64_t base,
+               RowsPlan* out) {
+  out->split_narrow = pages_per_split > 0 ? pages_per_split : choose_split(tiles, true, num_sms);
+  out->split_wide = pages_per_split > 0 ? pages_per_split : choose_split(tiles, false, num_sms);
+  for (const RowsItem& t : tiles) {
+    const bool narrow = t.n_q <= kNarrowTokens;
+    const int split = narrow ? out->split_narrow : out->split_wide;
+    std::vector<RowsItem>& items = narrow ? out->narrow : out->wide;
+    const int pages = t.pe - t.pb;
+    const int ns = (pages + split - 1) / split;
+    if (ns <= 1 || t.field7 == 1) {
+      items.push_back(t);
+      continue;
+    }
+    const int rows = 2 * t.n_q;
+    const int64_t first = base + out->part_rows;
+    if (first + static_cast<int64_t>(ns) * rows >= INT32_MAX) return false;
+    const int each = pages / ns, rem = pages % ns;
+    int pb = t.pb;
+    for (int s = 0; s < ns; ++s) {
+      const int len = each + (s < rem ? 1 : 0);
+      items.push_back({t.seq, t.tok0, t.n_q, pb, pb + len,
+                       static_cast<int>(first + static_cast<int64_t>(s) * rows),
+                       static_cast<int>(out->comb.size()), 2});
+      pb += len;
+    }
+    out->comb.push_back({t.seq, t.tok0, t.n_q, static_cast<int>(first), ns, 0});
+    out->part_rows += static_cast<int64_t>(ns) * rows;
+  }
+  auto longest_first = [](const RowsItem& x, const RowsItem& y) {
+    return (x.pe - x.pb) > (y.pe - y.pb);
+  };
+  std::stable_sort(out->narrow.begin(), out->narrow.end(), longest_first);
+  std::stable_sort(out->wide.begin(), out->wide.end(), longest_first);
+  return true;
+}
+
+void put_items(int32_t* out, int64_t off, const std::vector<RowsItem>& v) {
+  for (size_t k = 0; k < v.size(); ++k) {
+    int32_t* r = out + off + static_cast<int64_t>(k) * kRec;
+    r[0] = v[k].seq;
+    r[1] = v[k].tok0;
+    r[2] = v[k].n_q;
+    r[3] = v[k].pb;
+    r[4] = v[k].pe;
+    r[5] = v[k].part_row;
+    r[6] = v[k].field6;
+    r[7] = v[k].field7;
+  }
+}
+
+// Combine records have 0 in field 5 (the partial rows of a tile's splits are consecutive).
+void put_combines(int32_t* out, int64_t off, const std::vector<RowsItem>& v) {
+  put_items(out, off, v);
+  for (size_t k = 0; k < v.size(); ++k) out[off + static_cast<int64_t>(k) * kRec + 5] = 0;
+}
+
+int64_t size4(const std::vector<RowsItem>& v) { return round4(static_cast<int64_t>(v.size()) * kRec); }
 
 }  // namespace
 
-extern "C" int64_t ms_kv8_plan_capacity(const MsPlanInfo* plan, int64_t total_table_entries) {
-  if (plan == nullptr || plan->n_tc_items == 0) return 0;
-  return round4(static_cast<int64_t>(plan->num_seqs + plan->n_cascade) * kRec) +
-         2 * round4(total_table_entries);
+extern "C" int64_t ms_kv8_plan_capacity(int32_t num_seqs, int64_t total_table_entries) {
+  if (num_seqs < 0 || total_table_entries < 0) return 0;
+  // At most two tiles of 32 tokens per sequence, each at most one item per page, as many combine
+  // records; the records (one more per cascade group), map and tables of the tensor-core items.
+  const int64_t tiles = 2 * static_cast<int64_t>(num_seqs);
+  return 2 * round4((tiles + 2 * total_table_entries) * kRec) + round4(tiles * kRec) +
+         round4(tiles * kRec) + 2 * round4(total_table_entries) + 16;
 }
 
 static int kv8_plan_build(int32_t* packed, int64_t capacity, const MsPlanInfo* plan,
-                          MsKv8Info* info) {
-  if (packed == nullptr || plan == nullptr || info == nullptr) {
-    ms_host::set_error("ms_kv8_plan_build: null argument");
+                          int32_t num_sms, int32_t pages_per_split, MsKv8Info* info) {
+  if (packed == nullptr || plan == nullptr || info == nullptr || num_sms <= 0 ||
+      pages_per_split < 0) {
+    ms_host::set_error("ms_kv8_plan_build: null argument or bad sizes");
     return MS_ERR_ARG;
   }
   std::memset(info, 0, sizeof(*info));
-  info->total_ints = plan->total_ints;
-  if (plan->n_tc_items == 0) return MS_OK;
-  const int n_rec = plan->num_seqs + plan->n_cascade;
   const int32_t* seqs = packed + plan->off_seqs;
+
+  // Kernel F's tiles: the sequences of up to 64 new tokens, in tiles of up to 32; the rows of
+  // cascade groups read their own pages (their decode items say which) and merge the prefix partial.
+  std::vector<const int32_t*> cascade(plan->num_seqs, nullptr);
+  for (int i = 0; i < plan->n_decode_items; ++i) {
+    const int32_t* it = packed + plan->off_decode + static_cast<int64_t>(i) * kRec;
+    if (it[7] == 1) cascade[it[0]] = it;
+  }
+  std::vector<RowsItem> tiles;
+  for (int i = 0; i < plan->num_seqs; ++i) {
+    const int32_t* r = seqs + static_cast<int64_t>(i) * kRec;
+    const int n = r[1], c = r[2];
+    if (n > 2 * kTileTokens) continue;
+    if (cascade[i] != nullptr) {
+      tiles.push_back({i, 0, n, cascade[i][3], cascade[i][4], -1, cascade[i][6], 1});
+      continue;
+    }
+    for (int t0 = 0; t0 < n; t0 += kTileTokens) {
+      const int nq = std::min(kTileTokens, n - t0);
+      tiles.push_back({i, t0, nq, 0, (c + t0 + nq + 15) / 16});
+    }
+  }
+  RowsPlan rows;
+  if (!plan_rows(tiles, num_sms, pages_per_split, plan->part_rows, &rows)) {
+    ms_host::set_error("ms_kv8_plan_build: too many partial rows");
+    return MS_ERR_PLAN;
+  }
+
   // Pages each record's tensor-core items read (the largest page end).
+  const int n_rec = plan->num_seqs + plan->n_cascade;
   std::vector<int32_t> pages(n_rec, 0);
+  int64_t n_pages = 0;
   for (int i = 0; i < plan->n_tc_items; ++i) {
     const int32_t* it = packed + plan->off_tc + static_cast<int64_t>(i) * kRec;
     pages[it[0]] = std::max(pages[it[0]], it[4]);
   }
-  int64_t n_pages = 0;
   for (int p : pages) n_pages += p;
-  const int64_t off_seqs = plan->total_ints;
-  const int64_t off_map = off_seqs + round4(static_cast<int64_t>(n_rec) * kRec);
+
+  const int64_t off_narrow = round4(plan->total_ints);
+  const int64_t off_wide = off_narrow + size4(rows.narrow);
+  const int64_t off_combine = off_wide + size4(rows.wide);
+  const int64_t off_seqs = off_combine + size4(rows.comb);
+  const int64_t off_map =
+      off_seqs + (n_pages > 0 ? round4(static_cast<int64_t>(n_rec) * kRec) : 0);
   const int64_t off_tables = off_map + round4(n_pages);
   const int64_t total = off_tables + round4(n_pages);
   if (total > capacity) {
@@ -93,9 +239,12 @@ static int kv8_plan_build(int32_t* packed, int64_t capacity, const MsPlanInfo* p
     ms_host::set_error("ms_kv8_plan_build: plan larger than 2^31 ints");
     return MS_ERR_PLAN;
   }
-  std::memset(packed + off_seqs, 0, sizeof(int32_t) * (total - off_seqs));
+  std::memset(packed + plan->total_ints, 0, sizeof(int32_t) * (total - plan->total_ints));
+  put_items(packed, off_narrow, rows.narrow);
+  put_items(packed, off_wide, rows.wide);
+  put_combines(packed, off_combine, rows.comb);
   int32_t at = 0;
-  for (int i = 0; i < n_rec; ++i) {
+  for (int i = 0; n_pages > 0 && i < n_rec; ++i) {
     int32_t* r = packed + off_seqs + static_cast<int64_t>(i) * kRec;
     std::memcpy(r, seqs + static_cast<int64_t>(i) * kRec, sizeof(int32_t) * kRec);
     if (pages[i] == 0) continue;
@@ -112,23 +261,32 @@ static int kv8_plan_build(int32_t* packed, int64_t capacity, const MsPlanInfo* p
   info->off_seqs = static_cast<int32_t>(off_seqs);
   info->off_map = static_cast<int32_t>(off_map);
   info->off_tables = static_cast<int32_t>(off_tables);
+  info->n_narrow = static_cast<int32_t>(rows.narrow.size());
+  info->off_narrow = static_cast<int32_t>(off_narrow);
+  info->n_wide = static_cast<int32_t>(rows.wide.size());
+  info->off_wide = static_cast<int32_t>(off_wide);
+  info->n_combine = static_cast<int32_t>(rows.comb.size());
+  info->off_combine = static_cast<int32_t>(off_combine);
+  info->part_rows = rows.part_rows;
   info->total_ints = static_cast<int32_t>(total);
   return MS_OK;
 }
 
 extern "C" int ms_kv8_plan_build(int32_t* packed, int64_t capacity, const MsPlanInfo* plan,
-                                 MsKv8Info* info) {
-  return guarded("ms_kv8_plan_build",
-                 [&] { return kv8_plan_build(packed, capacity, plan, info); });
+                                 int32_t num_sms, int32_t pages_per_split, MsKv8Info* info) {
+  return guarded("ms_kv8_plan_build", [&] {
+    return kv8_plan_build(packed, capacity, plan, num_sms, pages_per_split, info);
+  });
 }
 
 extern "C" int64_t ms_kv8_workspace_bytes(const MsPlanInfo* plan, const MsKv8Info* info,
                                           int32_t num_kv_heads) {
   if (plan == nullptr || info == nullptr || num_kv_heads <= 0) return 0;
-  // Partials, arrival counters (two per combine record and head), then the expanded pages (8 KiB
-  // per head) on a 1 KiB boundary.
-  const int64_t part =
-      (plan->workspace_bytes_per_kv_head + static_cast<int64_t>(plan->n_combine) * 8) * num_kv_heads;
+  // Partials (the plan's and the 8-bit part's), the arrival counters of kernel F's split tiles, then
+  // the expanded pages (8 KiB per head) on a 1 KiB boundary.
+  const int64_t part = ((plan->part_rows + info->part_rows) * (128 + 1) * 4 +
+                        static_cast<int64_t>(info->n_combine) * 4) *
+                       num_kv_heads;
   if (info->n_pages == 0) return part;
   return (part + 1023) / 1024 * 1024 + static_cast<int64_t>(info->n_pages) * num_kv_heads * 8192;
 }
@@ -178,7 +336,7 @@ static int tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const in
     return MS_ERR_ARG;
   }
 
-  std::vector<TreeItem> tiles;
+  std::vector<RowsItem> tiles;
   int64_t mask_words = 0, total_pages = 0, parent_at = 0;
   std::vector<int64_t> mask_at(num_seqs, 0);
   std::vector<int64_t> parents_at(num_seqs, 0);
@@ -222,79 +380,22 @@ static int tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const in
     for (int64_t t0 = 0; t0 < n; t0 += kTileTokens) {
       const int nq = static_cast<int>(std::min<int64_t>(kTileTokens, n - t0));
       const int pages = static_cast<int>((c + t0 + nq + block_size - 1) / block_size);
-      tiles.push_back({i, static_cast<int>(t0), nq, 0, pages, -1});
+      tiles.push_back({i, static_cast<int>(t0), nq, 0, pages});
       total_pages += pages;
     }
   }
 
-  // Split size, for the narrow tiles and the wide ones (two launches): the smallest multiple of 8
-  // pages whose items fit one resident wave of CTAs; when the tiles alone exceed it, tiles longer
-  // than the pages per CTA slot are cut to about that size.
-  auto choose = [&](bool narrow) {
-    if (pages_per_split > 0) return pages_per_split;
-    const int64_t target =
-        std::max<int64_t>(1, static_cast<int64_t>(num_sms) * (narrow ? 3 : 2) / kAssumedKvHeads);
-    int64_t all = 0;
-    for (const TreeItem& t : tiles)
-      if ((t.n_q <= kNarrowTokens) == narrow) all += t.pe;
-    auto items_at = [&](int64_t p) {
-      int64_t items = 0;
-      for (const TreeItem& t : tiles)
-        if ((t.n_q <= kNarrowTokens) == narrow) items += (t.pe + p - 1) / p;
-      return items;
-    };
-    if (items_at(kMaxSplitPages) > target) {
-      const int64_t per_slot = (all + target - 1) / target;
-      return static_cast<int>(std::min<int64_t>(
-          kMaxSplitPages, std::max<int64_t>(kMinSplitPages, (per_slot + 7) / 8 * 8)));
-    }
-    int lo = kMinSplitPages / 8, hi = kMaxSplitPages / 8;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (items_at(mid * 8) <= target) hi = mid; else lo = mid + 1;
-    }
-    return lo * 8;
-  };
-  const int split_narrow = choose(true), split_wide = choose(false);
-
-  std::vector<TreeItem> narrow, wide, comb;
-  int64_t part_rows = 0;
-  for (const TreeItem& t : tiles) {
-    const int split = t.n_q <= kNarrowTokens ? split_narrow : split_wide;
-    std::vector<TreeItem>& items = t.n_q <= kNarrowTokens ? narrow : wide;
-    const int ns = (t.pe + split - 1) / split;
-    if (ns <= 1) {
-      items.push_back(t);
-      continue;
-    }
-    const int rows = 2 * t.n_q;
-    if (part_rows + static_cast<int64_t>(ns) * rows >= (int64_t(1) << 31)) {
-      ms_host::set_error("ms_tree_plan_build: too many partial rows");
-      return MS_ERR_PLAN;
-    }
-    const int base = t.pe / ns, rem = t.pe % ns;
-    int pb = 0;
-    for (int s = 0; s < ns; ++s) {
-      const int len = base + (s < rem ? 1 : 0);
-      items.push_back({t.seq, t.tok0, t.n_q, pb, pb + len,
-                       static_cast<int>(part_rows + static_cast<int64_t>(s) * rows),
-                       static_cast<int>(comb.size()), 2});
-      pb += len;
-    }
-    comb.push_back({t.seq, t.tok0, t.n_q, static_cast<int>(part_rows), ns, 0});
-    part_rows += static_cast<int64_t>(ns) * rows;
+  RowsPlan rows;
+  if (!plan_rows(tiles, num_sms, pages_per_split, 0, &rows)) {
+    ms_host::set_error("ms_tree_plan_build: too many partial rows");
+    return MS_ERR_PLAN;
   }
-  auto longest_first = [](const TreeItem& x, const TreeItem& y) {
-    return (x.pe - x.pb) > (y.pe - y.pb);
-  };
-  std::stable_sort(narrow.begin(), narrow.end(), longest_first);
-  std::stable_sort(wide.begin(), wide.end(), longest_first);
 
   const int64_t off_tables = round4(static_cast<int64_t>(num_seqs) * kRec);
   const int64_t off_narrow = off_tables + round4(total_entries);
-  const int64_t off_tile = off_narrow + round4(static_cast<int64_t>(narrow.size()) * kRec);
-  const int64_t off_combine = off_tile + round4(static_cast<int64_t>(wide.size()) * kRec);
-  const int64_t off_masks = off_combine + round4(static_cast<int64_t>(comb.size()) * kRec);
+  const int64_t off_tile = off_narrow + size4(rows.narrow);
+  const int64_t off_combine = off_tile + size4(rows.wide);
+  const int64_t off_masks = off_combine + size4(rows.comb);
   const int64_t total = off_masks + round4(mask_words);
   if (total > out_capacity) {
     ms_host::set_error("ms_tree_plan_build: output buffer holds " + std::to_string(out_capacity) +
@@ -328,42 +429,29 @@ static int tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const in
     }
   }
   if (total_entries > 0) std::memcpy(out + off_tables, tables, sizeof(int32_t) * total_entries);
-  auto put = [&](int64_t off, const std::vector<TreeItem>& v) {
-    for (size_t k = 0; k < v.size(); ++k) {
-      int32_t* r = out + off + static_cast<int64_t>(k) * kRec;
-      r[0] = v[k].seq;
-      r[1] = v[k].tok0;
-      r[2] = v[k].n_q;
-      r[3] = v[k].pb;
-      r[4] = v[k].pe;
-      r[5] = v[k].part_row;
-      r[6] = v[k].record;
-      r[7] = v[k].flag;
-    }
-  };
-  put(off_narrow, narrow);
-  put(off_tile, wide);
-  put(off_combine, comb);
+  put_items(out, off_narrow, rows.narrow);
+  put_items(out, off_tile, rows.wide);
+  put_combines(out, off_combine, rows.comb);
 
   info->num_seqs = num_seqs;
   info->num_tokens = num_tokens;
-  info->n_decode_items = static_cast<int32_t>(narrow.size());
-  info->n_tile_items = static_cast<int32_t>(wide.size());
-  info->n_combine = static_cast<int32_t>(comb.size());
+  info->n_decode_items = static_cast<int32_t>(rows.narrow.size());
+  info->n_tile_items = static_cast<int32_t>(rows.wide.size());
+  info->n_combine = static_cast<int32_t>(rows.comb.size());
   info->off_tables = static_cast<int32_t>(off_tables);
   info->off_decode = static_cast<int32_t>(off_narrow);
   info->off_tile = static_cast<int32_t>(off_tile);
   info->off_tc = static_cast<int32_t>(off_combine);
   info->off_combine = static_cast<int32_t>(off_combine);
   info->total_ints = static_cast<int32_t>(total);
-  info->pages_per_split = narrow.empty() ? split_wide : split_narrow;
-  info->part_rows = part_rows;
+  info->pages_per_split = rows.narrow.empty() ? rows.split_wide : rows.split_narrow;
+  info->part_rows = rows.part_rows;
   info->total_pages = total_pages;
-  int combine_tokens_max = 0;
-  for (const TreeItem& c : comb) combine_tokens_max = std::max(combine_tokens_max, c.n_q);
-  info->combine_tokens_max = combine_tokens_max;
-  // Partials and the arrival counters (two per combine record).
-  info->workspace_bytes_per_kv_head = part_rows * (128 + 1) * 4 + static_cast<int64_t>(comb.size()) * 8;
+  for (const RowsItem& c : rows.comb)
+    info->combine_tokens_max = std::max<int32_t>(info->combine_tokens_max, c.n_q);
+  // Partials and the arrival counters of split tiles.
+  info->workspace_bytes_per_kv_head =
+      rows.part_rows * (128 + 1) * 4 + static_cast<int64_t>(rows.comb.size()) * 4;
   return MS_OK;
 }
 

@@ -200,7 +200,7 @@ def test_kv8_part_maps_every_page_of_tensor_core_items() -> None:
         flat += n
     packed, info, kv8 = _plan_with_kv8(chunks, flat, 148, 0)
     assert kv8.n_pages == -(-270 // 16) + -(-65 // 16)
-    assert kv8.off_seqs == info.total_ints and packed.size == kv8.total_ints
+    assert kv8.off_seqs >= info.total_ints and packed.size == kv8.total_ints
     seqs = packed[kv8.off_seqs :][: len(chunks) * 8].reshape(-1, 8)
     plain = packed[info.off_seqs :][: len(chunks) * 8].reshape(-1, 8)
     for i, c in enumerate(chunks):
@@ -212,14 +212,55 @@ def test_kv8_part_maps_every_page_of_tensor_core_items() -> None:
             assert np.array_equal(seqs[i], plain[i])
     lib = _capi.load()
     need = lib.ms_kv8_workspace_bytes(C.byref(info), C.byref(kv8), 8)
-    part = (info.workspace_bytes_per_kv_head + 8 * info.n_combine) * 8
+    part = ((info.part_rows + kv8.part_rows) * 129 * 4 + 4 * kv8.n_combine) * 8
     assert need == -(-part // 1024) * 1024 + kv8.n_pages * 8 * 8192
     _, short, none = _plan_with_kv8(chunks[:1], 1, 148, 0)
     assert none.n_pages == 0 and short.n_tc_items == 0
 
 
 def test_kv8_struct_matches_the_header() -> None:
-    assert C.sizeof(_capi.MsKv8Info) == 32
+    assert C.sizeof(_capi.MsKv8Info) == 56
+
+
+@pytest.mark.parametrize("split", [0, 1, 3])
+def test_kv8_part_covers_every_row_once(split: int) -> None:
+    """Kernel F's items over an 8-bit pool: every tile of up to 32 tokens of the sequences with up to
+    64 new ones reads its pages once, splits name their record; cascade rows read their own pages."""
+    chunks, flat, at = [], 0, 3
+    for n, c in [(1, 0), (1, 4000), (8, 15), (16, 16), (17, 40), (33, 700), (64, 3), (65, 20)]:
+        chunks.append(_chunk(flat, n, c, at))
+        at += len(chunks[-1].block_table)
+        flat += n
+    prefix = list(range(at, at + 20))
+    at += 20
+    for i in range(16):
+        own = list(range(at, at + 3))
+        at += 3
+        chunks.append(SeqChunk(flat, 5, 330 + i, prefix + own))
+        flat += 5
+    packed, info, kv8 = _plan_with_kv8(chunks, flat, 148, split)
+    assert info.n_cascade == 1
+    items = np.concatenate([packed[kv8.off_narrow :][: 8 * kv8.n_narrow].reshape(-1, 8),
+                            packed[kv8.off_wide :][: 8 * kv8.n_wide].reshape(-1, 8)])
+    combine = packed[kv8.off_combine :][: 8 * kv8.n_combine].reshape(-1, 8)
+    pages: dict[tuple[int, int], list[int]] = {}
+    used: set[int] = set()
+    for s, tok0, nq, pb, pe, part, f6, f7 in items.tolist():
+        pages.setdefault((s, tok0), []).extend(range(pb, pe))
+        if f7 == 2:
+            assert combine[f6, :3].tolist() == [s, tok0, nq] and combine[f6, 5] == 0
+            rows = set(range(part, part + 2 * nq))
+            assert min(rows) >= info.part_rows and max(rows) < info.part_rows + kv8.part_rows
+            assert not rows & used
+            used |= rows
+        else:
+            assert part == -1 and f7 == (1 if s >= 8 else 0)
+    want = {}
+    for i, c in enumerate(chunks):
+        for tok0 in range(0, c.num_new if c.num_new <= 64 else 0, 32):
+            last = c.num_cached + min(c.num_new, tok0 + 32)
+            want[(i, tok0)] = list(range(20 if i >= 8 else 0, -(-last // 16)))
+    assert {k: sorted(v) for k, v in pages.items()} == want
 
 
 # ---- refusals, before any CUDA call -----------------------------------------------------------------

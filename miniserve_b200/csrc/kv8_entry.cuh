@@ -114,17 +114,6 @@ cudaError_t launch_rows_attention(const ms::AttnArgs& a, const void* pool, const
   return e;
 }
 
-template <typename K, typename... Args>
-cudaError_t launch_plain(K kernel, unsigned grid, unsigned block, size_t smem, cudaStream_t s,
-                         Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(block);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 }  // namespace
 
 extern "C" int ms_kv_scatter_kv8(const void* k, int64_t k_row_stride, const void* v,
@@ -346,16 +335,15 @@ extern "C" int ms_paged_attention_kv8(const void* q, int64_t q_row_stride, void*
                            256, 0, s, static_cast<const uint8_t*>(pool), plan_dev + info->off_map,
                            num_kv_heads, num_blocks, static_cast<__nv_bfloat16*>(pages), st);
     if (e == cudaSuccess) {
-      // An ordinary launch: this kernel reads earlier steps' pages before it waits for its
-      // predecessor, and here the predecessor writes them.
       ms::AttnArgs t = a;
+      t.pages_fresh = 1;
       t.seqs = plan_dev + info->off_seqs;
       t.tables = plan_dev + info->off_tables;
       t.items = plan_dev + plan->off_tc;
       t.n_items = plan->n_tc_items;
       t.num_blocks = info->n_pages;
-      e = launch_plain(ms::prefill_tc_kernel, plan->n_tc_items * num_kv_heads, ms::TcCfg::kThreads,
-                       ms::TcCfg::kSmemBytes, s, kmap, vmap, t);
+      e = launch(ms::prefill_tc_kernel, plan->n_tc_items * num_kv_heads, ms::TcCfg::kThreads,
+                 ms::TcCfg::kSmemBytes, s, kmap, vmap, t);
     }
     if (e != cudaSuccess) {
       join();
@@ -392,7 +380,7 @@ extern "C" int ms_tree_attention(const void* q, int64_t q_row_stride, void* out,
   const int64_t need = plan != nullptr ? plan->workspace_bytes_per_kv_head * num_kv_heads : 0;
   int rc = check_attention(what, q, q_row_stride, out, out_row_stride, num_heads, num_kv_heads,
                            plan_dev, plan, workspace, workspace_bytes, need,
-                           plan == nullptr ? 0 : std::max(plan->n_decode_items, plan->n_tile_items),
+                           plan == nullptr ? 0 : std::max(std::max(plan->n_decode_items, plan->n_tile_items), plan->n_tc_items),
                            scale);
   if (rc) return rc;
   const bool kv8 = v_cache == nullptr;
@@ -412,9 +400,28 @@ extern "C" int ms_tree_attention(const void* q, int64_t q_row_stride, void* out,
                          plan->off_tile,       plan->off_combine, plan->part_rows};
   const ms::AttnArgs a = attn_args(q, q_row_stride, out, out_row_stride, num_kv_heads, num_blocks,
                                    plan_dev, plan, workspace, work.part_rows, scale);
-  const cudaError_t e =
-      kv8 ? launch_rows_attention<true, true>(a, k_cache, map, plan_dev, work, s)
-          : launch_rows_attention<false, true>(a, nullptr, map, plan_dev, work, s);
+  // The cached blocks of larger trees first (see ms_tree_plan_build); kernel F merges their partials.
+  cudaError_t e = cudaSuccess;
+  if (plan->n_tc_items > 0) {
+    ms::AttnArgs t = a;
+    t.pages_fresh = 1;  // rows moved after a verify step lie below the cached length
+    t.items = plan_dev + plan->off_tc;
+    t.n_items = plan->n_tc_items;
+    const unsigned grid = static_cast<unsigned>(plan->n_tc_items * num_kv_heads);
+    if (kv8) {
+      e = cudaErrorNotSupported;
+    } else {
+      CUtensorMap kmap, vmap;
+      rc = kv_tensor_map(k_cache, num_blocks, num_kv_heads, 1, &kmap);
+      if (rc == MS_OK) rc = kv_tensor_map(k_cache, num_blocks, num_kv_heads, 2, &vmap);
+      if (rc) return rc;
+      e = launch(ms::prefill_tc_kernel, grid, ms::TcCfg::kThreads, ms::TcCfg::kSmemBytes, s, kmap,
+                 vmap, t);
+    }
+  }
+  if (e == cudaSuccess)
+    e = kv8 ? launch_rows_attention<true, true>(a, k_cache, map, plan_dev, work, s)
+            : launch_rows_attention<false, true>(a, nullptr, map, plan_dev, work, s);
   if (e != cudaSuccess) return cuda_fail("tree attention launch", e);
   return MS_OK;
 }

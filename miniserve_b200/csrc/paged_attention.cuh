@@ -50,6 +50,9 @@ struct AttnArgs {
   float* ws_o;    // [part_rows, KVH, 128] fp32 partials
   float* ws_lse;  // [part_rows, KVH]
   float scale_log2;
+  // Tensor-core kernel: the previous kernel may have written the cached pages too (an expanded copy, rows
+  // that were moved), so nothing is read before it has completed.
+  int pages_fresh = 0;
 };
 
 template <int kMode, int kConsumerWarps, int kStages>

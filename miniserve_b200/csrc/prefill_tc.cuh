@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(TcCfg::kThreads, 1)
       auto load = [&](int p, bool is_v, int ids, int j) -> bool {
         // Block j holds a key of this step (written by the previous kernel) unless all its keys
         // are below the cached length.
-        if (key_lo + (j + 1) * TcCfg::kBlockKeys > num_cached) wait_prev();
+        if (a.pages_fresh || key_lo + (j + 1) * TcCfg::kBlockKeys > num_cached) wait_prev();
         const int s = p % NS;
         int ok = 1;
         if (!is_v && lane < 8 && j * 8 + lane < npages &&

@@ -51,7 +51,9 @@ struct RowsArgs {
   AttnArgs a;           // queries, output, plan sections, partials
   const uint8_t* pool;  // 8-bit layer (null for a bf16 pool, which the tensor map describes)
   const int* plan;      // start of the packed plan: tree masks are at sequence record field 6
-  const int* combines;  // combine records of split tiles (an item names its record in field 6)
+  // Combine records {seq, tok0, n_q, first partial row, partials per row, rows between them, CTAs of
+  // this kernel that arrive} of tiles with several partials; an item names its record in field 6.
+  const int* combines;
   int* arrived;         // [record][KVH] splits that have finished: zero between calls
 };
 
@@ -64,9 +66,8 @@ struct RowsCfg {
   static constexpr int kBatch = 4;  // pages the producer's lanes issue side by side
   static_assert(kStages % 8 == 0 && kStages % kBatch == 0, "slots are reused by the same lane, warp");
   static constexpr int kStageBytes = kStages * kPage;
-  // Merge scratch in the ring: per warp 16 column tiles and (m, l) of one row group, a float4 per
-  // lane each.
-  static_assert(kRowsWarps * 17 * 32 * 16 <= kStageBytes, "merge scratch reuses the ring");
+  // Merge scratch in the ring: per warp 16 rows of a row group, padded, and their (m, l).
+  static_assert(kRowsWarps * 16 * (kHeadDim + 4 + 2) * 4 <= kStageBytes, "merge scratch reuses the ring");
   static constexpr int kRows = kRG == 1 ? 32 : 64;
   static constexpr int kQOffset = (kStageBytes + 127) / 128 * 128;
   static constexpr int kScaleOffset = kQOffset + kRows * kHeadDim * 2;  // the rows' query scales
@@ -233,29 +234,45 @@ __device__ __forceinline__ void block_exp(float (&s)[2 * kBlockPages][4], const 
   l[1] += l1;
 }
 
-// Scores of key column col (0..15) of page t that a row does not see become -infinity.
-// vis[g][h]: bit 16 t + k: row (g, h) sees key k of page t.  kCol1: the second column tile's first key.
-template <int kCol1>
+// A thread's keys of a page are key0, key0 + 1, key0 + kNext, key0 + kNext + 1.  Whether row (g, h) sees
+// key i (0..3) of page t; vis[g][h]: bit 16 t + k for key k.
+template <int kNext>
+__device__ __forceinline__ bool sees(uint32_t vis, int t, int key0, int i) {
+  return vis >> (16 * t + key0 + (i >> 1) * kNext + (i & 1)) & 1u;
+}
+
+// Scores a row does not see become -infinity.
+template <int kNext>
 __device__ __forceinline__ void mask_block(float (&s)[2 * kBlockPages][4], const uint32_t (&vis)[2],
-                                           int col0) {
+                                           int key0) {
 #pragma unroll
   for (int t = 0; t < kBlockPages; ++t) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t v = vis[i >> 1] >> (16 * t + col0);
-      if (!(v >> (i & 1) & 1u)) s[2 * t][i] = -INFINITY;
-      if (!(v >> (kCol1 + (i & 1)) & 1u)) s[2 * t + 1][i] = -INFINITY;
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (!sees<kNext>(vis[h], t, key0, i)) s[2 * t + (i >> 1)][2 * h + (i & 1)] = -INFINITY;
     }
   }
 }
 
-// Keys that some row of the warp sees, both pages.
-template <int kRG>
-__device__ __forceinline__ uint32_t seen_by_any(const uint32_t (&vis)[kRG][2]) {
-  uint32_t v = 0;
-#pragma unroll
-  for (int g = 0; g < kRG; ++g) v |= vis[g][0] | vis[g][1];
-  return __reduce_or_sync(0xffffffffu, v);
+// Rows of keys that no row of the tile sees (behind a sequence's end, unused drafts) may hold anything,
+// and 0 times NaN is NaN: their V rows (`dead`: bit k) become zeros in shared memory.  Each warp that
+// reads the page does it for itself, with the same result.  row_bytes of V rows start at v;
+// the 8-bit pool's exponent bytes at `exps` (0: none) go too.
+__device__ __forceinline__ void scrub_keys(uint32_t dead, uint32_t v, bool kv8, uint32_t exps,
+                                           bool refilled, int lane) {
+  // Two lanes per key: half of its 128 (8-bit) or 256 bytes each (a bf16 row lies in two halves).
+  const int k = lane >> 1, h = lane & 1;
+  if (dead >> k & 1u) {
+    const uint32_t row = kv8 ? v + k * kRow8Bytes + h * 64 : v + h * (kBlockTokens * 128) + k * 128;
+    for (int i = 0; i < (kv8 ? 64 : 128); i += 16)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(row + i), "r"(0) : "memory");
+    if (kv8 && h == 0) asm volatile("st.shared.u8 [%0], %1;" ::"r"(exps + k), "r"(0) : "memory");
+  }
+  // A later copy into the slot goes through the async proxy.
+  if (refilled) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
 }
 
 // ---- two pages, 8-bit pool ----------------------------------------------------------------------
@@ -307,7 +324,7 @@ __device__ __forceinline__ void rows_block8(const uint32_t (&page)[kBlockPages],
       }
     }
   }
-  uint32_t vw[kBlockPages], keep[kBlockPages][2];
+  uint32_t vw[kBlockPages];
 #pragma unroll
   for (int t = 0; t < kBlockPages; ++t) {
     const uint32_t kw = lds32(page[t] + kExp8Off + q4);
@@ -324,17 +341,6 @@ __device__ __forceinline__ void rows_block8(const uint32_t (&page)[kBlockPages],
     }
   }
   if constexpr (kMask) {
-    // Rows of keys no row here sees may hold anything (pages of a finished sequence, unused
-    // drafts, a second page that is not there): their values and exponents become zero.
-    const uint32_t any = seen_by_any<kRG>(vis) >> q4;
-#pragma unroll
-    for (int t = 0; t < kBlockPages; ++t) {
-      const uint32_t a = any >> (16 * t);
-      keep[t][0] = (a & 1u ? 0xffffu : 0u) | (a & 2u ? 0xffff0000u : 0u);
-      keep[t][1] = (a & 4u ? 0xffffu : 0u) | (a & 8u ? 0xffff0000u : 0u);
-      vw[t] &= (a & 1u ? 0xffu : 0u) | (a & 2u ? 0xff00u : 0u) | (a & 4u ? 0xff0000u : 0u) |
-               (a & 8u ? 0xff000000u : 0u);
-    }
 #pragma unroll
     for (int g = 0; g < kRG; ++g) mask_block<2>(s[g], vis[g], q4);
   }
@@ -346,31 +352,37 @@ __device__ __forceinline__ void rows_block8(const uint32_t (&page)[kBlockPages],
     mx[g][1] *= c[g][1];
   }
   raise<true, kRG>(st, mx, vw);
-  uint32_t pa[kRG][kBlockPages][4];
 #pragma unroll
   for (int g = 0; g < kRG; ++g) block_exp(s[g], c[g], st.m[g], st.l[g]);
+  // p times the factor of its V row.  A NaN row's factor is infinite, and infinity times its zero
+  // codes NaN; where p is 0 because the row does not see the key, the product is NaN too early and the
+  // maximum makes it 0.  (A NaN p shows in l.)
 #pragma unroll
   for (int t = 0; t < kBlockPages; ++t) {
     const float f[4] = {scale_of_byte<0>(vw[t]) * st.inv_e, scale_of_byte<1>(vw[t]) * st.inv_e,
                         scale_of_byte<2>(vw[t]) * st.inv_e, scale_of_byte<3>(vw[t]) * st.inv_e};
 #pragma unroll
     for (int g = 0; g < kRG; ++g) {
-      float p[2][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p[0][i] = s[g][2 * t][i] * f[i & 1];
-        p[1][i] = s[g][2 * t + 1][i] * f[2 + (i & 1)];
+        s[g][2 * t][i] *= f[i & 1];
+        s[g][2 * t + 1][i] *= f[2 + (i & 1)];
         if constexpr (kMask) {
-          // A key this row does not see contributes nothing, whatever its exponent byte.
-          const uint32_t v = vis[g][i >> 1] >> (16 * t + q4);
-          if (!(v >> (i & 1) & 1u)) p[0][i] = 0.f;
-          if (!(v >> (2 + (i & 1)) & 1u)) p[1][i] = 0.f;
+          s[g][2 * t][i] = fmaxf(s[g][2 * t][i], 0.f);
+          s[g][2 * t + 1][i] = fmaxf(s[g][2 * t + 1][i], 0.f);
         }
       }
-      pa[g][t][0] = pack_f16(p[0][0], p[0][1]);
-      pa[g][t][1] = pack_f16(p[0][2], p[0][3]);
-      pa[g][t][2] = pack_f16(p[1][0], p[1][1]);
-      pa[g][t][3] = pack_f16(p[1][2], p[1][3]);
+    }
+  }
+  uint32_t pa[kRG][kBlockPages][4];
+#pragma unroll
+  for (int g = 0; g < kRG; ++g) {
+#pragma unroll
+    for (int t = 0; t < kBlockPages; ++t) {
+      pa[g][t][0] = pack_f16(s[g][2 * t][0], s[g][2 * t][1]);
+      pa[g][t][1] = pack_f16(s[g][2 * t][2], s[g][2 * t][3]);
+      pa[g][t][2] = pack_f16(s[g][2 * t + 1][0], s[g][2 * t + 1][1]);
+      pa[g][t][3] = pack_f16(s[g][2 * t + 1][2], s[g][2 * t + 1][3]);
     }
   }
   const int vtok = tok + 2 * (mi & 1);
@@ -384,10 +396,6 @@ __device__ __forceinline__ void rows_block8(const uint32_t (&page)[kBlockPages],
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t a = w[2 * h], b = w[2 * h + 1];
-        if constexpr (kMask) {
-          a &= keep[t][0];
-          b &= keep[t][1];
-        }
         // Bytes (token t: columns 2j, 2j + 1; token t + 1: the same) -> column 2j of both tokens
         // in the low half, column 2j + 1 in the high half.
         a = __byte_perm(a, 0, 0x3120);
@@ -405,10 +413,6 @@ __device__ __forceinline__ void rows_block8(const uint32_t (&page)[kBlockPages],
 }
 
 // ---- two pages, bf16 pool -----------------------------------------------------------------------
-
-__device__ __forceinline__ bool bf16_pair_bad(uint32_t w) {
-  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
-}
 
 // A thread's keys of a page are 2q, 2q + 1, 2q + 8, 2q + 9 (q = lane % 4).  Accumulator tile n holds
 // columns 8n + 2q, 8n + 2q + 1.
@@ -444,9 +448,7 @@ __device__ __forceinline__ void rows_block16(const uint32_t (&page)[kBlockPages]
       }
     }
   }
-  uint32_t any = 0;
   if constexpr (kMask) {
-    any = seen_by_any<kRG>(vis) >> q2;
 #pragma unroll
     for (int g = 0; g < kRG; ++g) mask_block<8>(s[g], vis[g], q2);
   }
@@ -474,62 +476,74 @@ __device__ __forceinline__ void rows_block16(const uint32_t (&page)[kBlockPages]
       pa[g][2] = pack_bf16(p1[0], p1[1]);
       pa[g][3] = pack_bf16(p1[2], p1[3]);
     }
-    const uint32_t a = any >> (16 * t);
-    const uint32_t keep0 = (a & 1u ? 0xffffu : 0u) | (a & 2u ? 0xffff0000u : 0u);
-    const uint32_t keep1 = (a & 0x100u ? 0xffffu : 0u) | (a & 0x200u ? 0xffff0000u : 0u);
-    const int key = t8 + (mi & 1) * 8;
-    const uint32_t vbase = page[t] + kPageBytes;
-    bool bad = false;
 #pragma unroll
     for (int np = 0; np < 8; ++np) {
       uint32_t b[4];
-      ldsm_x4_t(vbase + swz_off(key, np * 16 + (mi >> 1) * 8, 16), b[0], b[1], b[2], b[3]);
-      if constexpr (kMask) {
-        // Values of keys no row here sees are dropped; infinities and NaN of the others too, and
-        // added below for the rows that do see them (0 times them would reach every row).
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          b[i] &= (i & 1) ? keep1 : keep0;
-          if (bf16_pair_bad(b[i])) {
-            bad = true;
-            if ((b[i] & 0x7f80u) == 0x7f80u) b[i] &= 0xffff0000u;
-            if ((b[i] & 0x7f800000u) == 0x7f800000u) b[i] &= 0xffffu;
-          }
-        }
-      }
+      ldsm_x4_t(page[t] + kPageBytes + swz_off(t8 + (mi & 1) * 8, np * 16 + (mi >> 1) * 8, 16), b[0],
+                b[1], b[2], b[3]);
 #pragma unroll
       for (int g = 0; g < kRG; ++g) {
         mma_bf16(st.o[g][2 * np], pa[g], b[0], b[1]);
         mma_bf16(st.o[g][2 * np + 1], pa[g], b[2], b[3]);
       }
     }
-    if constexpr (kMask) {
-      if (__any_sync(0xffffffffu, bad)) {
+  }
+}
+
+// Whether a page's V rows hold an infinity or a NaN (all 32 lanes; a page with masked keys only).
+__device__ __forceinline__ bool page_has_special16(uint32_t page, int lane) {
+  bool bad = false;
 #pragma unroll 1
-        for (int k = 0; k < 16; ++k) {
-          const int src = (lane & ~3) | ((k & 7) >> 1);
+  for (int i = 0; i < kPageBytes / (32 * 16); ++i) {
+    uint32_t w[4];
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(page + kPageBytes + (i * 32 + lane) * 16));
 #pragma unroll
-          for (int g = 0; g < kRG; ++g) {
-            const float(&p0)[4] = s[g][2 * t];
-            const float(&p1)[4] = s[g][2 * t + 1];
-            const float a0 = (k & 8) ? ((k & 1) ? p1[1] : p1[0]) : ((k & 1) ? p0[1] : p0[0]);
-            const float a1 = (k & 8) ? ((k & 1) ? p1[3] : p1[2]) : ((k & 1) ? p0[3] : p0[2]);
-            const float w0 = __shfl_sync(0xffffffffu, a0, src);
-            const float w1 = __shfl_sync(0xffffffffu, a1, src);
-            const bool see0 = vis[g][0] >> (16 * t + k) & 1u, see1 = vis[g][1] >> (16 * t + k) & 1u;
+    for (int k = 0; k < 4; ++k)
+      bad = bad || (w[k] & 0x7f80u) == 0x7f80u || (w[k] & 0x7f800000u) == 0x7f800000u;
+  }
+  return __any_sync(0xffffffffu, bad);
+}
+
+// A page whose V rows hold an infinity or a NaN that only some rows see: a product with 0 would bring
+// it to the others, so the page is attended key by key in fp32, each row with the keys it sees.
+template <int kRG>
+__device__ __forceinline__ void rows_page16_special(uint32_t page, int t, uint32_t q_tile,
+                                                    int row00, RowsState<kRG>& st,
+                                                    const float (&c)[kRG][2],
+                                                    const uint32_t (&vis)[kRG][2], int lane) {
+  const int q = lane & 3;
+#pragma unroll 1
+  for (int k = 0; k < kBlockTokens; ++k) {
 #pragma unroll
-            for (int n = 0; n < 16; ++n) {
-              const uint32_t w = lds32(vbase + swz_off(k, n * 8 + q2, 16));
+    for (int g = 0; g < kRG; ++g) {
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const uint32_t bits = i == 0 ? w << 16 : w & 0xffff0000u;
-                if ((bits & 0x7f800000u) != 0x7f800000u) continue;
-                const float v = __uint_as_float(bits);
-                if (see0) st.o[g][n][i] += w0 * v;
-                if (see1) st.o[g][n][2 + i] += w1 * v;
-              }
-            }
-          }
+      for (int h = 0; h < 2; ++h) {
+        const int r = row00 + 16 * g + 8 * h;
+        float s = 0.f;  // a quarter of the dims per lane of the quad
+#pragma unroll 1
+        for (int d = 32 * q; d < 32 * q + 32; d += 2) {
+          const uint32_t a = lds32(q_tile + r * (kHeadDim * 2) + (((d >> 3) ^ (r & 7)) << 4) + (d & 7) * 2);
+          const uint32_t b = lds32(page + swz_off(k, d, 16));
+          s += bf16_lo(a) * bf16_lo(b) + bf16_hi(a) * bf16_hi(b);
+        }
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        s *= c[g][h];
+        const bool see = vis[g][h] >> (16 * t + k) & 1u;
+        float al = 1.f;
+        if (see && s > st.m[g][h]) {
+          al = fast_exp2(st.m[g][h] - s);
+          st.m[g][h] = s;
+        }
+        const float p = see ? fast_exp2(s - (st.m[g][h] == -INFINITY ? 0.f : st.m[g][h])) : 0.f;
+        st.l[g][h] = st.l[g][h] * al + (q == 0 ? p : 0.f);
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          const uint32_t w = lds32(page + kPageBytes + swz_off(k, n * 8 + 2 * q, 16));
+          st.o[g][n][2 * h] = st.o[g][n][2 * h] * al + (see ? p * bf16_lo(w) : 0.f);
+          st.o[g][n][2 * h + 1] = st.o[g][n][2 * h + 1] * al + (see ? p * bf16_hi(w) : 0.f);
         }
       }
     }
@@ -538,79 +552,17 @@ __device__ __forceinline__ void rows_block16(const uint32_t (&page)[kBlockPages]
 
 // ---- the kernel ---------------------------------------------------------------------------------
 
-// Where one row's result goes: bf16 output, or a partial row (normalised O and log2-sum-exp), with
-// the shared-prefix partial of a cascade row merged in.
-struct RowOut {
-  __nv_bfloat16* dst;   // output row (null: partial row)
-  float* part;          // partial row
-  const float* prefix;  // shared-prefix partial row to merge (null: none)
-  float w, wp;          // weights of this item's O and of the prefix partial
-};
-
-__device__ __forceinline__ RowOut row_out(const AttnArgs& a, int r, int tok, bool live, float m,
-                                          float L, int kvh, int part_row, int merge_row,
-                                          int flat_tok, bool first_col) {
-  RowOut o;
-  const float inv = live && L != 0.f ? 1.f / L : 0.f;  // a NaN sum stays NaN
-  o.dst = nullptr;
-  o.part = nullptr;
-  o.prefix = nullptr;
-  o.w = inv;
-  o.wp = 0.f;
-  if (part_row >= 0) {
-    const long long prow = static_cast<long long>(part_row + r) * a.num_kv + kvh;
-    o.part = a.ws_o + prow * kHeadDim;
-    if (first_col) a.ws_lse[prow] = live && L != 0.f ? m + __log2f(L) : -INFINITY;
-    return o;
-  }
-  o.dst = a.out + static_cast<long long>(flat_tok + tok) * a.out_row_stride +
-          (kvh * kGroup + (r & 1)) * kHeadDim;
-  if (merge_row >= 0) {
-    const long long prow = static_cast<long long>(merge_row + r) * a.num_kv + kvh;
-    const float lse_p = a.ws_lse[prow];
-    const float lse_u = L != 0.f ? m + __log2f(L) : -INFINITY;
-    const float M = fmaxf(lse_u, lse_p);
-    const float wu = lse_u == -INFINITY ? 0.f : fast_exp2(lse_u - M);
-    const float wp = lse_p == -INFINITY ? 0.f : fast_exp2(lse_p - M);
-    const float den = wu + wp;
-    const float n = den != 0.f ? 1.f / den : 0.f;
-    o.w = inv * wu * n;
-    o.wp = wp * n;
-    o.prefix = a.ws_o + prow * kHeadDim;
-  }
-  return o;
-}
-
-template <int kN>  // kN neighbouring columns from column d
-__device__ __forceinline__ void put_cols(const RowOut& o, int d, const float (&x)[kN], bool live) {
-  float y[kN];
-#pragma unroll
-  for (int i = 0; i < kN; ++i) {
-    y[i] = live ? x[i] * o.w : 0.f;
-    if (o.prefix != nullptr) y[i] += o.prefix[d + i] * o.wp;
-  }
-  if (o.part != nullptr) {
-    if constexpr (kN == 4)
-      *reinterpret_cast<float4*>(o.part + d) = make_float4(y[0], y[1], y[2], y[3]);
-    else
-      *reinterpret_cast<float2*>(o.part + d) = make_float2(y[0], y[1]);
-  } else {
-    if constexpr (kN == 4)
-      *reinterpret_cast<uint2*>(o.dst + d) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
-    else
-      *reinterpret_cast<uint32_t*>(o.dst + d) = pack_bf16(y[0], y[1]);
-  }
-}
-
 // The last CTA of a split tile merges the splits' partial rows: out = sum_s 2^(lse_s - M) O_s /
 // sum_s 2^(lse_s - M), s in order, so the result does not depend on which CTA came last.  The
 // partial rows come through shared memory (the idle ring, `bytes` of it) by asynchronous copies, as many
-// splits at a time as fit, so that one latency covers them all (through registers the merge took 4-8
-// us of a short call); the rows' M and sums are formed from global memory meanwhile.  A warp
-// takes rows warp, warp + 4, ..., a lane four columns.
+// splits at a time as fit, so that one latency covers them all, and the rows' M and sums are formed from
+// global memory meanwhile.  A warp takes rows warp, warp + 4, ..., a lane four columns.  masks: the
+// tile's first mask row of a tree (a draft that sees nothing writes zeros: the tensor-core kernel
+// does not know it), else null.
 template <int kRows>
 __device__ __forceinline__ void merge_splits(const AttnArgs& a, uint8_t* smem, int bytes, int row0,
-                                             int n_splits, int rows, int kvh, int flat_tok) {
+                                             int n_splits, int stride, int rows, int kvh,
+                                             int flat_tok, const int* masks, int words, int tok0) {
   constexpr int kT = kRowsWarps * 32, kPer = kRows / kRowsWarps, kLanes = kT / kRows;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   float* top = reinterpret_cast<float*>(smem);  // [kRows] M, then [kRows] 1 / sum
@@ -618,23 +570,28 @@ __device__ __forceinline__ void merge_splits(const AttnArgs& a, uint8_t* smem, i
   const int chunk = max(1, min(n_splits, (bytes - 2 * kRows * 4) / (rows * (kHeadDim + 1) * 4 + 16)));
   float* o_s = lse_s + (chunk * rows + 3) / 4 * 4;
   auto at = [&](int s, int r) {
-    return (static_cast<long long>(row0) + static_cast<long long>(s) * rows + r) * a.num_kv + kvh;
+    return (static_cast<long long>(row0) + static_cast<long long>(s) * stride + r) * a.num_kv + kvh;
   };
   float4 acc[kPer];
 #pragma unroll
   for (int k = 0; k < kPer; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
   for (int s0 = 0; s0 < n_splits; s0 += chunk) {
     const int cnt = min(chunk, n_splits - s0);
     if (s0 > 0) asm volatile("bar.sync 1, %0;" ::"r"(kT) : "memory");  // the last chunk was read
-    for (int i = warp; i < cnt * rows; i += kRowsWarps) {
-      const float* src = a.ws_o + at(s0, 0) * kHeadDim +
-                         static_cast<long long>(i) * a.num_kv * kHeadDim + lane * 4;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                       smem_u32(o_s + i * kHeadDim + lane * 4)),
-                   "l"(src)
-                   : "memory");
+#pragma unroll 1
+    for (int s = 0; s < cnt; ++s) {
+      for (int r = warp; r < rows; r += kRowsWarps)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                         smem_u32(o_s + (s * rows + r) * kHeadDim + lane * 4)),
+                     "l"(a.ws_o + at(s0 + s, r) * kHeadDim + lane * 4)
+                     : "memory");
     }
-    for (int i = tid; i < cnt * rows; i += kT) lse_s[i] = __ldcg(a.ws_lse + at(s0, 0) + static_cast<long long>(i) * a.num_kv);
+    // (Past L1, like everything here: its lines may be older than the other CTAs' rows.)
+    for (int i = tid; i < cnt * rows; i += kT) {
+      const int s = i / rows;
+      lse_s[i] = __ldcg(a.ws_lse + at(s0 + s, i - s * rows));
+    }
     if (s0 == 0) {
       // kLanes neighbouring threads per row, over all splits.
       const int r = tid / kLanes;
@@ -669,6 +626,7 @@ __device__ __forceinline__ void merge_splits(const AttnArgs& a, uint8_t* smem, i
       const int r = warp + k * kRowsWarps;
       if (r < rows) {
         const float m = top[r];
+#pragma unroll 2
         for (int i = 0; i < cnt; ++i) {
           const float x = lse_s[i * rows + r];
           const float w = x == -INFINITY ? 0.f : fast_exp2(x - m);
@@ -685,11 +643,16 @@ __device__ __forceinline__ void merge_splits(const AttnArgs& a, uint8_t* smem, i
   for (int k = 0; k < kPer; ++k) {
     const int r = warp + k * kRowsWarps;
     if (r >= rows) break;
-    const float inv = top[kRows + r];
+    const float inv = top[kRows + r];  // a NaN sum stays NaN
+    const int tok = tok0 + (r >> 1);
+    const bool live = masks == nullptr ||
+                      (masks[static_cast<long long>(r >> 1) * words + (tok >> 5)] >> (tok & 31) & 1);
     __nv_bfloat16* dst = a.out + static_cast<long long>(flat_tok + (r >> 1)) * a.out_row_stride +
                          (kvh * kGroup + (r & 1)) * kHeadDim + lane * 4;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc[k].x * inv, acc[k].y * inv),
-                                                pack_bf16(acc[k].z * inv, acc[k].w * inv));
+    *reinterpret_cast<uint2*>(dst) =
+        live ? make_uint2(pack_bf16(acc[k].x * inv, acc[k].y * inv),
+                          pack_bf16(acc[k].z * inv, acc[k].w * inv))
+             : make_uint2(0u, 0u);
   }
 }
 
@@ -879,7 +842,6 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
   // This thread's rows row(g, h) = row_base + 16 g + lane / 4 + 8 h and their facts.
   const int row00 = row_base + (lane >> 2);
   float c[kRG][2];
-  bool live[kRG][2];
   int words = 0;
   const int* masks = nullptr;  // tree: mask rows of the sequence
   if constexpr (kTree) {
@@ -890,17 +852,8 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
   for (int g = 0; g < kRG; ++g) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = row00 + 16 * g + 8 * h;
       c[g][h] = a.scale_log2;
-      if constexpr (kKv8) c[g][h] *= qscale[r];
-      live[g][h] = (r >> 1) < n_q;
-      if constexpr (kTree) {
-        // A token whose mask misses itself sees nothing.
-        if (live[g][h]) {
-          const int k = tok0 + (r >> 1);
-          live[g][h] = masks[static_cast<long long>(k) * words + (k >> 5)] >> (k & 31) & 1;
-        }
-      }
+      if constexpr (kKv8) c[g][h] *= qscale[row00 + 16 * g + 8 * h];
     }
   }
 
@@ -921,64 +874,131 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
   const uint32_t ring_u32 = smem_u32(ring);
   // This lane's ldmatrix row of the query tile.
   const uint32_t q_row = q_u32 + (row_base + (lane & 7) + ((lane >> 3) & 1) * 8) * (kHeadDim * 2);
-  for (int j = phase * kBlockPages; j < npages; j += phases * kBlockPages) {
-    const int cnt = min(kBlockPages, npages - j);
-    uint32_t page[kBlockPages];
+  // Waits for the pages j .. j + cnt - 1 (cnt warp-uniform).  The warp leaves its loop only as a whole: the
+  // tensor-core operations are warp-collective.
+  auto wait_pages = [&](int j, int cnt) -> bool {
     bool ok = true;
 #pragma unroll
-    for (int t = 0; t < kBlockPages; ++t) {
-      // A second page that is not there is masked out; its slot's leftovers are read.
-      const int s = (j + t) % kStages;
-      page[t] = ring_u32 + s * Cfg::kPage;
-      if (t < cnt) ok = ok && mbar_wait_fast(&full[s], ((j + t) / kStages) & 1, abort_flag);
+    for (int t = 0; t < kBlockPages; ++t)
+      if (t < cnt)
+        ok = ok && mbar_wait_fast(&full[(j + t) % kStages], ((j + t) / kStages) & 1, abort_flag);
+    if (__all_sync(0xffffffffu, ok)) return true;
+    if (lane == 0) {
+      atomicOr(&g_status_word, kErrTimeout);
+      *abort_flag = 1;
     }
-    // Leave the loop only as a whole warp: the tensor-core operations are warp-collective.
-    if (!__all_sync(0xffffffffu, ok)) {
-      if (lane == 0) {
-        atomicOr(&g_status_word, kErrTimeout);
-        *abort_flag = 1;
-      }
-      break;
-    }
-    const int key0 = (page_begin + j) * kBlockTokens;
+    return false;
+  };
+  // Whole pairs whose keys every row sees, then the rest (the end of the tile's pages), with masks:
+  // what only the rest needs is kept out of the registers of the first loop.
+  const int n_full = min(npages & ~(kBlockPages - 1),
+                         max(0, first_masked - page_begin * kBlockTokens) / (kBlockPages * kBlockTokens) * kBlockPages);
+  int j = phase * kBlockPages;
+  bool ok = true;
+  for (; j < n_full; j += phases * kBlockPages) {
+    if (!(ok = wait_pages(j, kBlockPages))) break;
     if (warp_active) {
+      const uint32_t page[kBlockPages] = {ring_u32 + (j % kStages) * Cfg::kPage,
+                                          ring_u32 + (j % kStages + 1) * Cfg::kPage};
+      const uint32_t vis[kRG][2] = {};
+      if constexpr (kKv8)
+        rows_block8<kRG, false>(page, q_row, st, c, vis, lane);
+      else
+        rows_block16<kRG, false>(page, q_row, st, c, vis, lane);
+    }
+    __syncwarp();
+    if (lane < kBlockPages) mbar_arrive(&empty[(j + lane) % kStages]);
+  }
+  for (; ok && j < npages; j += phases * kBlockPages) {
+    const int cnt = min(kBlockPages, npages - j);
+    if (!(ok = wait_pages(j, cnt))) break;
+    if (warp_active) {
+      // A second page that is not there is the first one again, with every key masked.
+      uint32_t page[kBlockPages] = {ring_u32 + (j % kStages) * Cfg::kPage,
+                                    ring_u32 + ((j + cnt - 1) % kStages) * Cfg::kPage};
+      // The plan's records again (volatile loads: nothing of them lives through the loop above).
+      auto reload = [](const int* p) {
+        int v;
+        asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p));
+        return v;
+      };
+      const int* itm = a.items + static_cast<long long>(item_idx) * kRec;
+      const int t0 = reload(itm + 1), nq = reload(itm + 2);
+      const int* rec = a.seqs + static_cast<long long>(reload(itm)) * kRec;
+      const int cached = reload(rec + 2);
+      const int* mrows = nullptr;
+      int mwords = 0;
+      if constexpr (kTree) {
+        mwords = reload(rec + 7);
+        mrows = ra.plan + reload(rec + 6);
+      }
+      const int key0 = (reload(itm + 3) + j) * kBlockTokens;
+      // Which of the pages' keys token k of the sequence's new ones sees.
+      auto seen = [&](int k) {
+        uint32_t v = 0;
+#pragma unroll
+        for (int t = 0; t < kBlockPages; ++t) {
+          const int k0 = key0 + t * kBlockTokens;
+          uint32_t bits;
+          if constexpr (kTree) {
+            const int* row = mrows + static_cast<long long>(k) * mwords;
+            bits = 0u;
+            if (row[k >> 5] >> (k & 31) & 1)
+              bits = k0 + kBlockTokens <= cached ? 0xffffu : tree_bits(row, mwords, k0 - cached);
+          } else {
+            bits = causal_bits(cached + k, k0);
+          }
+          if (t < cnt) v |= bits << (16 * t);
+        }
+        return v;
+      };
+      // A lane per token of the tile (at most 32), handed to the rows; and all of them together.
+      const uint32_t mine = lane < nq ? seen(t0 + lane) : 0u;
+      const uint32_t any = __reduce_or_sync(0xffffffffu, mine);
       uint32_t vis[kRG][2];
-      if (cnt < kBlockPages || key0 + kBlockPages * kBlockTokens > first_masked) {
 #pragma unroll
-        for (int g = 0; g < kRG; ++g) {
+      for (int g = 0; g < kRG; ++g) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int k = tok0 + ((row00 + 16 * g + 8 * h) >> 1);  // the row's new token
-            uint32_t v = 0;
-            if (live[g][h]) {
+        for (int h = 0; h < 2; ++h) {
+          const int tok = (row00 + 16 * g + 8 * h) >> 1;  // rows past the last token see nothing
+          vis[g][h] = __shfl_sync(0xffffffffu, mine, tok & 31);
+        }
+      }
+#pragma unroll 1
+      for (int t = 0; t < cnt; ++t) {
+        const uint32_t dead = ~(any >> (16 * t)) & 0xffffu;
+        if (dead != 0)
+          scrub_keys(dead, page[t] + Cfg::kPage / 2 - (kKv8 ? kBlockTokens : 0), kKv8,
+                     kKv8 ? page[t] + kExp8Off + kBlockTokens : 0u, j + t + kStages < npages, lane);
+      }
+      bool run = true;
+      if constexpr (!kKv8) {
+        bool special[kBlockPages];
 #pragma unroll
-              for (int t = 0; t < kBlockPages; ++t) {
-                const int k0 = key0 + t * kBlockTokens;
-                uint32_t bits;
-                if constexpr (kTree) {
-                  bits = k0 + kBlockTokens <= num_cached
-                             ? 0xffffu
-                             : tree_bits(masks + static_cast<long long>(k) * words, words, k0 - num_cached);
-                } else {
-                  bits = causal_bits(num_cached + k, k0);
-                }
-                if (t < cnt) v |= bits << (16 * t);
-              }
-            }
-            vis[g][h] = v;
+        for (int t = 0; t < kBlockPages; ++t)
+          special[t] = t < cnt && page_has_special16(page[t], lane);
+        if (special[0] || special[1]) {
+#pragma unroll 1
+          for (int t = 0; t < kBlockPages; ++t)
+            if (t == 0 ? special[0] : special[1])
+              rows_page16_special<kRG>(page[t], t, q_u32, row00, st, c, vis, lane);
+          // The other page, if it has none, goes the usual way, in both places.
+          const uint32_t keep_bits = (special[0] ? 0u : 0xffffu) | (special[1] ? 0u : 0xffff0000u);
+          run = keep_bits != 0u && !(special[0] && cnt < kBlockPages);
+          if (special[0]) page[0] = page[1];
+          if (special[1]) page[1] = page[0];
+#pragma unroll
+          for (int g = 0; g < kRG; ++g) {
+            vis[g][0] &= keep_bits;
+            vis[g][1] &= keep_bits;
           }
         }
+      }
+      if (run) {
         if constexpr (kKv8)
           rows_block8<kRG, true>(page, q_row, st, c, vis, lane);
         else
           rows_block16<kRG, true>(page, q_row, st, c, vis, lane);
-      } else {
-#pragma unroll
-        for (int g = 0; g < kRG; ++g) vis[g][0] = vis[g][1] = 0xffffffffu;
-        if constexpr (kKv8)
-          rows_block8<kRG, false>(page, q_row, st, c, vis, lane);
-        else
-          rows_block16<kRG, false>(page, q_row, st, c, vis, lane);
       }
     }
     __syncwarp();
@@ -1004,91 +1024,127 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
 
   // Merge of the page phases, one row group at a time: every warp leaves its (O, m, l) in the idle
   // ring (each page has been read once all consumer warps reach the barrier; a copy that was
-  // abandoned on a timeout is drained by the producer before the CTA ends), and each warp merges
-  // and writes 16 / phases of its row set's column tiles.
-  float4* scratch = reinterpret_cast<float4*>(ring);
-  const int per = 16 / phases;
+  // abandoned on a timeout is drained by the producer before the CTA ends), rows of 128 columns, and
+  // the threads share the rows out in chunks of 8 columns.  Loops, not unrolled: this runs once, and
+  // a longer form costs more in instruction fetches than it saves.
+  constexpr int kPitch = kHeadDim + 4;
+  float* so = reinterpret_cast<float*>(ring);                     // [warp][16 rows][kPitch]
+  float* sm = so + kRowsWarps * 16 * kPitch;                      // [warp][16 rows] m, then l
+  float* sl = sm + kRowsWarps * 16;
 #pragma unroll
   for (int g = 0; g < kRG; ++g) {
     asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
 #pragma unroll
-    for (int n = 0; n < 16; ++n)
-      scratch[(warp * 17 + n) * 32 + lane] =
-          make_float4(st.o[g][n][0], st.o[g][n][1], st.o[g][n][2], st.o[g][n][3]);
-    scratch[(warp * 17 + 16) * 32 + lane] =
-        make_float4(st.m[g][0], st.m[g][1], st.l[g][0], st.l[g][1]);
-    asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
-    float mx[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f}, wt[kRowsWarps][2];
-#pragma unroll
-    for (int p = 0; p < kRowsWarps; ++p) {
-      if (p < phases) {
-        const float4 ml = scratch[((p * sets + set) * 17 + 16) * 32 + lane];
-        mx[0] = fmaxf(mx[0], ml.x);
-        mx[1] = fmaxf(mx[1], ml.y);
-      }
-    }
-#pragma unroll
-    for (int p = 0; p < kRowsWarps; ++p) {
-      wt[p][0] = wt[p][1] = 0.f;
-      if (p < phases) {
-        const float4 ml = scratch[((p * sets + set) * 17 + 16) * 32 + lane];
-        wt[p][0] = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mx[0]);
-        wt[p][1] = ml.y == -INFINITY ? 0.f : fast_exp2(ml.y - mx[1]);
-        // A phase whose scores were all NaN never raised its maximum: its sum is kept as it is.
-        if (ml.z != ml.z) wt[p][0] = 1.f;
-        if (ml.w != ml.w) wt[p][1] = 1.f;
-        L[0] += ml.z * wt[p][0];
-        L[1] += ml.w * wt[p][1];
-      }
-    }
-#pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = row00 + 16 * g + 8 * h;
+      const int r = (lane >> 2) + 8 * h;
+      float* row = so + (warp * 16 + r) * kPitch;
+      if constexpr (kKv8) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          *reinterpret_cast<float4*>(row + 16 * u + 2 * q2) =
+              make_float4(st.o[g][2 * u][2 * h], st.o[g][2 * u + 1][2 * h],
+                          st.o[g][2 * u][2 * h + 1], st.o[g][2 * u + 1][2 * h + 1]);
+      } else {
+#pragma unroll
+        for (int n = 0; n < 16; ++n)
+          *reinterpret_cast<float2*>(row + 8 * n + q2) =
+              make_float2(st.o[g][n][2 * h], st.o[g][n][2 * h + 1]);
+      }
+      if (q2 == 0) {
+        sm[warp * 16 + r] = st.m[g][h];
+        sl[warp * 16 + r] = st.l[g][h];
+      }
+    }
+    asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
+#pragma unroll 1
+    for (int e = threadIdx.x; e < sets * 16 * 16; e += kRowsWarps * 32) {
+      const int sr_ = e >> 4, d = (e & 15) * 8;          // row among the sets' rows of this group
+      const int set_ = sr_ >> 4, rr = sr_ & 15;
+      const int r = set_ * 16 * kRG + 16 * g + rr;       // row of the tile
       const int tok = r >> 1;
       if (tok >= n_q) continue;
-      const RowOut out = row_out(a, r, tok, live[g][h], mx[h], L[h], kvh, part_row, merge_row,
-                                 flat_start + tok0, phase == 0 && q2 == 0);
-      for (int n = phase * per; n < (phase + 1) * per; n += 2) {
-        float x0[2] = {0.f, 0.f}, x1[2] = {0.f, 0.f};  // tiles n and n + 1
+      bool alive = true;
+      if constexpr (kTree) {
+        const int k = tok0 + tok;
+        alive = masks[static_cast<long long>(k) * words + (k >> 5)] >> (k & 31) & 1;
+      }
+      float M = -INFINITY, L = 0.f, x[8];
 #pragma unroll
-        for (int p = 0; p < kRowsWarps; ++p) {
-          if (p < phases) {
-            const float2* base = reinterpret_cast<const float2*>(
-                scratch + ((p * sets + set) * 17 + n) * 32 + lane);
-            const float2 y0 = base[h], y1 = base[64 + h];
-            x0[0] += y0.x * wt[p][h];
-            x0[1] += y0.y * wt[p][h];
-            x1[0] += y1.x * wt[p][h];
-            x1[1] += y1.y * wt[p][h];
-          }
-        }
-        if constexpr (kKv8) {
-          const float x[4] = {x0[0], x1[0], x0[1], x1[1]};
-          put_cols<4>(out, 8 * n + 2 * q2, x, live[g][h]);
-        } else {
-          put_cols<2>(out, 8 * n + q2, x0, live[g][h]);
-          put_cols<2>(out, 8 * n + 8 + q2, x1, live[g][h]);
+      for (int i = 0; i < 8; ++i) x[i] = 0.f;
+      for (int p = 0; p < phases; ++p) M = fmaxf(M, sm[(p * sets + set_) * 16 + rr]);
+#pragma unroll 1
+      for (int p = 0; p < phases; ++p) {
+        const int w = (p * sets + set_) * 16 + rr;
+        const float mw = sm[w], lw = sl[w];
+        float f = mw == -INFINITY ? 0.f : fast_exp2(mw - M);
+        if (lw != lw) f = 1.f;  // a phase whose scores were all NaN never raised its maximum
+        L += lw * f;
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(so + w * kPitch + d + i);
+          x[i] += v.x * f;
+          x[i + 1] += v.y * f;
+          x[i + 2] += v.z * f;
+          x[i + 3] += v.w * f;
         }
       }
+      float scale = L != 0.f ? 1.f / L : 0.f;  // a NaN sum stays NaN
+      const float lse = alive && L != 0.f ? M + __log2f(L) : -INFINITY;
+      if (part_row >= 0) {
+        const long long prow = static_cast<long long>(part_row + r) * a.num_kv + kvh;
+        float* dst = a.ws_o + prow * kHeadDim + d;
+#pragma unroll
+        for (int i = 0; i < 8; i += 4)
+          *reinterpret_cast<float4*>(dst + i) =
+              alive ? make_float4(x[i] * scale, x[i + 1] * scale, x[i + 2] * scale, x[i + 3] * scale)
+                    : make_float4(0.f, 0.f, 0.f, 0.f);
+        if (d == 0) a.ws_lse[prow] = lse;
+        continue;
+      }
+      if constexpr (kKv8 && !kTree) {
+        if (merge_row >= 0) {  // a cascade row: with the shared-prefix partial
+          const long long prow = static_cast<long long>(merge_row + r) * a.num_kv + kvh;
+          const float lse_p = a.ws_lse[prow];
+          const float top = fmaxf(lse, lse_p);
+          const float wu = lse == -INFINITY ? 0.f : fast_exp2(lse - top);
+          const float wp = lse_p == -INFINITY ? 0.f : fast_exp2(lse_p - top);
+          const float n = wu + wp != 0.f ? 1.f / (wu + wp) : 0.f;
+          scale *= wu * n;
+          const float* op = a.ws_o + prow * kHeadDim + d;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = x[i] * scale + op[i] * (wp * n);
+          scale = 1.f;
+        }
+      }
+      __nv_bfloat16* dst = a.out + static_cast<long long>(flat_start + tok0 + tok) * a.out_row_stride +
+                           (kvh * kGroup + (r & 1)) * kHeadDim + d;
+      uint4 y = make_uint4(0u, 0u, 0u, 0u);
+      if (alive)
+        y = make_uint4(pack_bf16(x[0] * scale, x[1] * scale), pack_bf16(x[2] * scale, x[3] * scale),
+                       pack_bf16(x[4] * scale, x[5] * scale), pack_bf16(x[6] * scale, x[7] * scale));
+      *reinterpret_cast<uint4*>(dst) = y;
     }
   }
 
   if (part_row >= 0) {
-    // A split of a tile: the last one to arrive merges them all.
+    // A split of a tile, or the last pages of one whose cached blocks the tensor-core kernel read
+    // before this launch: the last one to arrive merges them all.
     __threadfence();
     asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
     const int* cr = ra.combines + static_cast<long long>(it[6]) * kRec;
     if (threadIdx.x == 0) {
       int* counter = ra.arrived + static_cast<long long>(it[6]) * a.num_kv + kvh;
-      const bool last = atomicAdd(counter, 1) == cr[4] - 1;
+      const bool last = atomicAdd(counter, 1) == cr[6] - 1;
       if (last) *counter = 0;  // ready for the next call
       *last_flag = last ? 1 : 0;
     }
     asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
     if (*last_flag) {
       __threadfence();
-      merge_splits<Cfg::kRows>(a, ring, Cfg::kStageBytes, cr[3], cr[4], n_q * kGroup, kvh,
-                               flat_start + tok0);
+      merge_splits<Cfg::kRows>(a, ring, Cfg::kStageBytes, cr[3], cr[4], cr[5], n_q * kGroup, kvh,
+                               flat_start + tok0,
+                               kTree ? masks + static_cast<long long>(tok0) * words : nullptr, words,
+                               tok0);
     }
   }
 }

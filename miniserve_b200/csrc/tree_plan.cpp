@@ -62,33 +62,36 @@ struct RowsItem {
   int seq, tok0, n_q, pb, pe;
   int part_row = -1;
   // Fields 6 and 7: the combine record and 2 for a split, the shared-prefix partial row and 1 for a
-  // cascade row.
+  // cascade row, the combine record and 3 for the last pages of a tile whose cached blocks are read by
+  // tensor-core items (which write the other partial rows of that record).
   int field6 = 0, field7 = 0;
 };
+
+// Cached whole 128-key blocks of the tiles of larger trees run on the tensor cores: tiles of more
+// than 16 drafts are bound by mma.sync (16 trees of 63 drafts over 4000-8100 tokens: 119 us without
+// this), and those blocks need no mask.  kPrefixMinPages: fewer pages are not worth the second launch.
+constexpr int kBlockPages = 8;
+constexpr int kPrefixTileTokens = 64;  // 128 query rows
+constexpr int kPrefixMinPages = 32, kPrefixMinSplitPages = 64;
 
 // The items of kernel F: narrow and wide tiles (two launches), split over their pages, and the
 // combine records of the split ones.
 struct RowsPlan {
-  std::vector<RowsItem> narrow, wide, comb;  // comb: pb = first partial row, pe = number of splits
+  // comb: pb = first partial row, pe = number of partials per row, part_row = rows between them,
+  // field6 = how many of kernel F's CTAs arrive (per head).
+  std::vector<RowsItem> narrow, wide, comb;
   int64_t part_rows = 0;                     // from `base` on
   int split_narrow = 0, split_wide = 0;
 };
 
-// Split size, for the narrow tiles and the wide ones: the smallest multiple of 8 pages whose items fit
-// one resident wave of CTAs; when the tiles alone exceed it, tiles longer than the pages per CTA
-// slot are cut to about that size.
-int choose_split(const std::vector<RowsItem>& tiles, bool narrow, int num_sms) {
-  const int least = narrow ? kMinSplitPages : kMinWideSplitPages;
-  const int64_t target =
-      std::max<int64_t>(1, narrow ? static_cast<int64_t>(num_sms) * 2 / kNarrowHeads
-                                  : static_cast<int64_t>(num_sms) * 2 / kWideHeads);
+// The smallest multiple of 8 pages, at least `least`, whose items number at most `target`; when the
+// tiles alone exceed it, tiles longer than the pages per slot are cut to about that size.
+int fit_split(const std::vector<RowsItem>& tiles, int64_t target, int least) {
   int64_t all = 0;
-  for (const RowsItem& t : tiles)
-    if ((t.n_q <= kNarrowTokens) == narrow) all += t.pe - t.pb;
+  for (const RowsItem& t : tiles) all += t.pe - t.pb;
   auto items_at = [&](int64_t p) {
     int64_t items = 0;
-    for (const RowsItem& t : tiles)
-      if ((t.n_q <= kNarrowTokens) == narrow) items += (t.pe - t.pb + p - 1) / p;
+    for (const RowsItem& t : tiles) items += (t.pe - t.pb + p - 1) / p;
     return items;
   };
   if (items_at(kMaxSplitPages) > target) {
@@ -104,7 +107,18 @@ int choose_split(const std::vector<RowsItem>& tiles, bool narrow, int num_sms) {
   return lo * 8;
 }
 
-// Splits the tiles (cascade rows, field7 == 1, stay whole).  False: too many partial rows.
+// Split size of kernel F's narrow or wide tiles.
+int choose_split(const std::vector<RowsItem>& tiles, bool narrow, int num_sms) {
+  std::vector<RowsItem> mine;
+  for (const RowsItem& t : tiles)
+    if ((t.n_q <= kNarrowTokens) == narrow && t.field7 == 0) mine.push_back(t);
+  const int64_t target = narrow ? static_cast<int64_t>(num_sms) * 2 / kNarrowHeads
+                                : static_cast<int64_t>(num_sms) * 2 / kWideHeads;
+  return fit_split(mine, std::max<int64_t>(1, target), narrow ? kMinSplitPages : kMinWideSplitPages);
+}
+
+// Splits the tiles (cascade rows and the tails of tensor-core prefixes, field7 != 0, stay whole).
+// False: too many partial rows.
 bool plan_rows(const std::vector<RowsItem>& tiles, int num_sms, int pages_per_split, int64_t base,
                RowsPlan* out) {
   out->split_narrow = pages_per_split > 0 ? pages_per_split : choose_split(tiles, true, num_sms);
@@ -115,7 +129,7 @@ bool plan_rows(const std::vector<RowsItem>& tiles, int num_sms, int pages_per_sp
     std::vector<RowsItem>& items = narrow ? out->narrow : out->wide;
     const int pages = t.pe - t.pb;
     const int ns = (pages + split - 1) / split;
-    if (ns <= 1 || t.field7 == 1) {
+    if (ns <= 1 || t.field7 != 0) {
       items.push_back(t);
       continue;
     }
@@ -131,7 +145,7 @@ bool plan_rows(const std::vector<RowsItem>& tiles, int num_sms, int pages_per_sp
                        static_cast<int>(out->comb.size()), 2});
       pb += len;
     }
-    out->comb.push_back({t.seq, t.tok0, t.n_q, static_cast<int>(first), ns, 0});
+    out->comb.push_back({t.seq, t.tok0, t.n_q, static_cast<int>(first), ns, rows, ns, 0});
     out->part_rows += static_cast<int64_t>(ns) * rows;
   }
   auto longest_first = [](const RowsItem& x, const RowsItem& y) {
@@ -154,12 +168,6 @@ void put_items(int32_t* out, int64_t off, const std::vector<RowsItem>& v) {
     r[6] = v[k].field6;
     r[7] = v[k].field7;
   }
-}
-
-// Combine records have 0 in field 5 (the partial rows of a tile's splits are consecutive).
-void put_combines(int32_t* out, int64_t off, const std::vector<RowsItem>& v) {
-  put_items(out, off, v);
-  for (size_t k = 0; k < v.size(); ++k) out[off + static_cast<int64_t>(k) * kRec + 5] = 0;
 }
 
 int64_t size4(const std::vector<RowsItem>& v) { return round4(static_cast<int64_t>(v.size()) * kRec); }
@@ -242,7 +250,7 @@ static int kv8_plan_build(int32_t* packed, int64_t capacity, const MsPlanInfo* p
   std::memset(packed + plan->total_ints, 0, sizeof(int32_t) * (total - plan->total_ints));
   put_items(packed, off_narrow, rows.narrow);
   put_items(packed, off_wide, rows.wide);
-  put_combines(packed, off_combine, rows.comb);
+  put_items(packed, off_combine, rows.comb);
   int32_t at = 0;
   for (int i = 0; n_pages > 0 && i < n_rec; ++i) {
     int32_t* r = packed + off_seqs + static_cast<int64_t>(i) * kRec;
@@ -301,10 +309,11 @@ extern "C" int64_t ms_tree_plan_capacity(int32_t num_seqs, const int32_t* num_ne
     tiles_max = std::max(tiles_max, (n + kTileTokens - 1) / kTileTokens);
     masks += n * ((n + 31) / 32);
   }
-  // A tile has at most one item per page of its sequence.
+  // A tile has at most one item per page of its sequence; narrow, wide and tensor-core items, and a
+  // virtual record per sequence.
   const int64_t items = tiles + tiles_max * total_table_entries;
-  return round4(static_cast<int64_t>(num_seqs) * kRec) + round4(total_table_entries) +
-         2 * round4(items * kRec) + round4(tiles * kRec) + round4(masks) + 16;
+  return round4(2 * static_cast<int64_t>(num_seqs) * kRec) + round4(total_table_entries) +
+         3 * round4(items * kRec) + round4(tiles * kRec) + round4(masks) + 16;
 }
 
 static int tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const int32_t* num_new,
@@ -385,16 +394,66 @@ static int tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const in
     }
   }
 
+  // The cached blocks of larger trees: tensor-core items over virtual sequences (records after the
+  // real ones) whose cached context is those blocks, one tile of up to 64 drafts each, split over the
+  // pages; the drafts' tiles keep the pages after them.
   RowsPlan rows;
+  std::vector<RowsItem> prefix, tc;
+  std::vector<int> vseq_of(num_seqs, -1);
+  int n_vseq = 0;
+  for (int i = 0; i < num_seqs; ++i) {
+    const int pages = num_cached[i] / (kBlockPages * 16) * kBlockPages;
+    if (num_new[i] <= kNarrowTokens || pages < kPrefixMinPages) continue;
+    vseq_of[i] = n_vseq++;
+    for (int t0 = 0; t0 < num_new[i]; t0 += kPrefixTileTokens)
+      prefix.push_back({i, t0, std::min(kPrefixTileTokens, num_new[i] - t0), 0, pages});
+  }
+  if (!prefix.empty()) {
+    const int split =
+        pages_per_split > 0
+            ? (pages_per_split + kBlockPages - 1) / kBlockPages * kBlockPages
+            : fit_split(prefix, std::max(1, num_sms / kWideHeads), kPrefixMinSplitPages);
+    std::vector<RowsItem> rest;
+    for (const RowsItem& t : tiles)
+      if (vseq_of[t.seq] < 0) rest.push_back(t);
+    for (const RowsItem& p : prefix) {
+      const int blocks = p.pe / kBlockPages, ns = (p.pe + split - 1) / split, stride = 2 * p.n_q;
+      const int64_t first = rows.part_rows;
+      rows.part_rows += static_cast<int64_t>(ns + 1) * stride;
+      if (rows.part_rows >= INT32_MAX) {
+        ms_host::set_error("ms_tree_plan_build: too many partial rows");
+        return MS_ERR_PLAN;
+      }
+      int pb = 0;
+      for (int s = 0; s < ns; ++s) {
+        const int len = (blocks / ns + (s < blocks % ns ? 1 : 0)) * kBlockPages;
+        tc.push_back({num_seqs + vseq_of[p.seq], p.tok0, p.n_q, pb, pb + len,
+                      static_cast<int>(first + static_cast<int64_t>(s) * stride)});
+        pb += len;
+      }
+      for (int t0 = p.tok0; t0 < p.tok0 + p.n_q; t0 += kTileTokens) {
+        const int nq = std::min(kTileTokens, p.tok0 + p.n_q - t0);
+        const int row0 = static_cast<int>(first) + 2 * (t0 - p.tok0);
+        rest.push_back({p.seq, t0, nq, p.pe, (num_cached[p.seq] + t0 + nq + 15) / 16,
+                        row0 + ns * stride, static_cast<int>(rows.comb.size()), 3});
+        rows.comb.push_back({p.seq, t0, nq, row0, ns + 1, stride, 1, 0});
+      }
+    }
+    tiles.swap(rest);
+    std::stable_sort(tc.begin(), tc.end(), [](const RowsItem& x, const RowsItem& y) {
+      return (x.pe - x.pb) > (y.pe - y.pb);
+    });
+  }
   if (!plan_rows(tiles, num_sms, pages_per_split, 0, &rows)) {
     ms_host::set_error("ms_tree_plan_build: too many partial rows");
     return MS_ERR_PLAN;
   }
 
-  const int64_t off_tables = round4(static_cast<int64_t>(num_seqs) * kRec);
+  const int64_t off_tables = round4((static_cast<int64_t>(num_seqs) + n_vseq) * kRec);
   const int64_t off_narrow = off_tables + round4(total_entries);
   const int64_t off_tile = off_narrow + size4(rows.narrow);
-  const int64_t off_combine = off_tile + size4(rows.wide);
+  const int64_t off_tc = off_tile + size4(rows.wide);
+  const int64_t off_combine = off_tc + size4(tc);
   const int64_t off_masks = off_combine + size4(rows.comb);
   const int64_t total = off_masks + round4(mask_words);
   if (total > out_capacity) {
@@ -418,6 +477,16 @@ static int tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const in
     r[5] = static_cast<int32_t>(table_offsets[i + 1] - table_offsets[i]);
     r[6] = static_cast<int32_t>(off_masks + mask_at[i]);
     r[7] = words;
+    if (vseq_of[i] >= 0) {
+      const int pages = num_cached[i] / (kBlockPages * 16) * kBlockPages;
+      int32_t* v = out + (static_cast<int64_t>(num_seqs) + vseq_of[i]) * kRec;
+      v[0] = flat_start[i];
+      v[1] = n;
+      v[2] = pages * 16;
+      v[3] = pages * 16 + n;
+      v[4] = r[4];
+      v[5] = pages;
+    }
     const int32_t* par = parents + parents_at[i];
     uint32_t* mask = reinterpret_cast<uint32_t*>(out + off_masks + mask_at[i]);
     for (int k = 0; k < n; ++k) {
@@ -431,7 +500,8 @@ static int tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const in
   if (total_entries > 0) std::memcpy(out + off_tables, tables, sizeof(int32_t) * total_entries);
   put_items(out, off_narrow, rows.narrow);
   put_items(out, off_tile, rows.wide);
-  put_combines(out, off_combine, rows.comb);
+  put_items(out, off_tc, tc);
+  put_items(out, off_combine, rows.comb);
 
   info->num_seqs = num_seqs;
   info->num_tokens = num_tokens;
@@ -441,7 +511,8 @@ static int tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const in
   info->off_tables = static_cast<int32_t>(off_tables);
   info->off_decode = static_cast<int32_t>(off_narrow);
   info->off_tile = static_cast<int32_t>(off_tile);
-  info->off_tc = static_cast<int32_t>(off_combine);
+  info->n_tc_items = static_cast<int32_t>(tc.size());
+  info->off_tc = static_cast<int32_t>(off_tc);
   info->off_combine = static_cast<int32_t>(off_combine);
   info->total_ints = static_cast<int32_t>(total);
   info->pages_per_split = rows.narrow.empty() ? rows.split_wide : rows.split_narrow;

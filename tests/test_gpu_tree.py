@@ -60,13 +60,13 @@ def check(views, chunks, q, u: float, split: int = 0) -> torch.Tensor:
 @pytest.mark.parametrize("split", [0, 1, 5])
 @pytest.mark.parametrize("n", [1, 2, 7, 8, 9, 15, 16, 17, 24, 31, 32, 33, 63, 64, 65, 100])
 def test_random_trees(n: int, split: int, pool: str, cuda_device) -> None:
-    """Tile and page borders: trees over 0, 1, 15, 16, 17 and 500 cached tokens, some positions
-    unused."""
+    """Tile and page borders: trees over 0, 1, 15, 16, 17 and 500 cached tokens (and 512, 645 and 1535,
+    whose whole blocks larger trees read on the tensor cores), some positions unused."""
     rng = random.Random(n)
     seqs = [(n, c, random_tree(rng, n, unused=rng.choice([0, 0, n // 4])))
-            for c in (0, 1, 15, 16, 17, 500)]
+            for c in (0, 1, 15, 16, 17, 500, 512, 645, 1535)]
     views, chunks, q = batch(cuda_device, seqs, 2, pool, seed=n)
-    check(views, chunks, q, POOLS[pool][1], split)
+    check(views, chunks, q, U_BF16 if n > 16 else POOLS[pool][1], split)
 
 
 @pytest.mark.parametrize("pool", POOLS)
@@ -111,9 +111,10 @@ def test_unused_positions_may_hold_anything(pool: str, cuda_device) -> None:
     dev = cuda_device
     rng = random.Random(2)
     seqs = [(16, 40, random_tree(rng, 16, unused=5)), (8, 0, [-2] * 8), (3, 9, [-2, -1, -2]),
-            (33, 3, random_tree(rng, 33, unused=20))]
+            (33, 3, random_tree(rng, 33, unused=20)), (40, 700, random_tree(rng, 40, unused=30)),
+            (20, 600, [-2] * 20)]
     views, chunks, q = batch(dev, seqs, 2, pool, seed=6)
-    clean = check(views, chunks, q, POOLS[pool][1])
+    clean = check(views, chunks, q, U_BF16)
     ks, vs = layer_as_slots(views[0]), layer_as_slots(views[1])
     live = torch.zeros(ks.shape[0], dtype=torch.bool)
     for c in chunks:
@@ -129,8 +130,8 @@ def test_unused_positions_may_hold_anything(pool: str, cuda_device) -> None:
     vs[dead[::2]] = float("nan")
     slots_into_layer(views[0], ks)
     slots_into_layer(views[1], vs)
-    assert torch.equal(check(views, chunks, q, POOLS[pool][1]), clean)
-    assert torch.equal(check(views, chunks, q, POOLS[pool][1], split=1).isnan(), clean.isnan())
+    assert torch.equal(check(views, chunks, q, U_BF16), clean)
+    assert torch.equal(check(views, chunks, q, U_BF16, split=1).isnan(), clean.isnan())
 
 
 @pytest.mark.parametrize("pool", POOLS)
@@ -164,8 +165,8 @@ def test_long_context_is_split(pool: str, cuda_device) -> None:
                                            (50, 6001, random_tree(rng, 50))], 2, pool, seed=8)
     meta = build_attention_metadata(chunks, slots_of(chunks, cuda_device), 16)
     assert meta.tree.info.n_combine > 0
-    first = check(views, chunks, q, POOLS[pool][1])
-    assert torch.equal(check(views, chunks, q, POOLS[pool][1]), first)
+    first = check(views, chunks, q, U_BF16)
+    assert torch.equal(check(views, chunks, q, U_BF16), first)
 
 
 @pytest.mark.parametrize("pool", POOLS)

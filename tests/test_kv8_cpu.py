@@ -105,12 +105,15 @@ def _random_parents(rng: random.Random, n: int, unused: int = 0) -> list[int]:
     return [rng.randint(max(-1, i - 6), i - 1) for i in range(n - unused)] + [-2] * unused
 
 
-@pytest.mark.parametrize("n", [1, 8, 31, 32, 33, 64, 100, 256])
-@pytest.mark.parametrize("split", [0, 1, 3])
+@pytest.mark.parametrize("n", [1, 8, 16, 17, 31, 32, 33, 64, 100, 256])
+@pytest.mark.parametrize("split", [0, 1, 3, 40])
 def test_tree_plan_covers_every_page_once(n: int, split: int) -> None:
+    """Every tile's pages are read once, by kernel F's items or (the cached whole 128-key blocks of trees
+    of more than 16 drafts over 512 tokens and more) by tensor-core items; the partial rows of a
+    combine record are those its items write."""
     rng = random.Random(n)
     chunks, flat, at = [], 0, 7
-    for cached in (0, 15, 16, 700):
+    for cached in (0, 15, 16, 511, 512, 700, 5000):
         parents = _random_parents(rng, n, unused=n // 5)
         c = _chunk(flat, n, cached, at, parents)
         at += len(c.block_table)
@@ -118,32 +121,49 @@ def test_tree_plan_covers_every_page_once(n: int, split: int) -> None:
         chunks.append(c)
     packed, info = plan_tree_batch(chunks, flat, 16, 148, split)
     assert packed.size == info.total_ints
-    seqs = packed[: 4 * 8].reshape(4, 8)
-    pages: dict[tuple[int, int], set[int]] = {}
-    parts = set()
+    count = len(chunks)
+    has_prefix = [n > 16 and c.num_cached >= 512 for c in chunks]
+    seqs = packed[: (count + sum(has_prefix)) * 8].reshape(-1, 8)
     narrow = packed[info.off_decode :][: 8 * info.n_decode_items].reshape(-1, 8)
     wide = packed[info.off_tile :][: 8 * info.n_tile_items].reshape(-1, 8)
-    assert all(it[2] <= 16 for it in narrow) and all(16 < it[2] <= 32 for it in wide)
+    tcs = packed[info.off_tc :][: 8 * info.n_tc_items].reshape(-1, 8)
     combine = packed[info.off_combine :][: 8 * info.n_combine].reshape(-1, 8)
-    for it in np.concatenate([narrow, wide]):
-        s, tok0, nq, pb, pe, part, rec, flag = (int(v) for v in it)
-        assert tok0 % 32 == 0 and pb < pe
-        if part >= 0:  # its combine record names its tile
-            assert flag == 2 and combine[rec, :3].tolist() == [s, tok0, nq]
-            assert (part - combine[rec, 3]) % (2 * nq) == 0
-            assert 0 <= (part - combine[rec, 3]) // (2 * nq) < combine[rec, 4]
-        seen = pages.setdefault((s, tok0), set())
-        assert not seen & set(range(pb, pe))
-        seen |= set(range(pb, pe))
+    assert all(it[2] <= 16 for it in narrow) and all(16 < it[2] <= 32 for it in wide)
+    pages: dict[tuple[int, int], list[int]] = {}
+    written: dict[int, int] = {}  # partial row -> how often
+    arrive = [0] * info.n_combine
+    for s, tok0, nq, pb, pe, part, rec, flag in np.concatenate([narrow, wide]).tolist():
+        assert tok0 % 32 == 0 and pb < pe and (part >= 0) == (flag != 0)
+        pages.setdefault((s, tok0), []).extend(range(pb, pe))
         if part >= 0:
-            rows = set(range(part, part + 2 * nq))
-            assert not parts & rows and max(rows) < info.part_rows
-            parts |= rows
+            assert flag == (3 if has_prefix[s] else 2)
+            assert combine[rec, :3].tolist() == [s, tok0, nq]
+            arrive[rec] += 1
+            for r in range(2 * nq):
+                written[part + r] = written.get(part + r, 0) + 1
+    for vs, tok0, nq, pb, pe, part, tok_b, n_b in tcs.tolist():
+        s = [i for i in range(count) if has_prefix[i]][vs - count]
+        assert seqs[vs, 0] == chunks[s].flat_start and seqs[vs, 4] == seqs[s, 4]
+        assert seqs[vs, 2] == chunks[s].num_cached // 128 * 128
+        assert n_b == 0 and tok0 % 64 == 0 and nq == min(64, n - tok0)
+        assert pb % 8 == 0 and pe % 8 == 0 and pb < pe and pe * 16 <= chunks[s].num_cached
+        for t0 in range(tok0, tok0 + nq, 32):
+            pages.setdefault((s, t0), []).extend(range(pb, pe))
+        for r in range(2 * nq):
+            written[part + r] = written.get(part + r, 0) + 1
+    assert set(written.values()) <= {1} and len(written) == info.part_rows
+    merged: dict[int, int] = {}
+    for k, (s, tok0, nq, row0, parts, stride, arrivals, _) in enumerate(combine.tolist()):
+        assert arrivals == arrive[k] and (parts == arrivals or has_prefix[s])
+        for p in range(parts):
+            for r in range(2 * nq):
+                merged[row0 + p * stride + r] = 1
+    assert merged == written
     for i, c in enumerate(chunks):
         assert seqs[i, 0] == c.flat_start and seqs[i, 2] == c.num_cached
         for tok0 in range(0, n, 32):
             last = c.num_cached + min(n, tok0 + 32)
-            assert pages[(i, tok0)] == set(range(-(-last // 16)))
+            assert sorted(pages[(i, tok0)]) == list(range(-(-last // 16)))
         words = int(seqs[i, 7])
         mask = packed[seqs[i, 6] : seqs[i, 6] + n * words].view(np.uint32).reshape(n, words)
         bits = np.unpackbits(mask.view(np.uint8), axis=1, bitorder="little")[:, :n].astype(bool)
@@ -248,7 +268,7 @@ def test_kv8_part_covers_every_row_once(split: int) -> None:
     for s, tok0, nq, pb, pe, part, f6, f7 in items.tolist():
         pages.setdefault((s, tok0), []).extend(range(pb, pe))
         if f7 == 2:
-            assert combine[f6, :3].tolist() == [s, tok0, nq] and combine[f6, 5] == 0
+            assert combine[f6, :3].tolist() == [s, tok0, nq] and combine[f6, 5] == 2 * nq
             rows = set(range(part, part + 2 * nq))
             assert min(rows) >= info.part_rows and max(rows) < info.part_rows + kv8.part_rows
             assert not rows & used

@@ -98,7 +98,8 @@ typedef struct MsPlanInfo {
   int32_t decode_pages;    /* pages (per KV head) the decode / verify items read, in total */
   int32_t combine_tokens_max; /* most query tokens of one combine record (sizes its grid) */
   int32_t n_tc_combine;       /* combine records of tensor-core items: the last ones */
-  int32_t reserved[2];
+  int32_t is_tree;            /* 1: a plan of ms_tree_plan_build, for ms_tree_attention(_kv8) */
+  int32_t reserved;
 } MsPlanInfo;
 
 /* Upper bound on the packed buffer length (int32 elements) for a batch of this size. */
@@ -253,9 +254,11 @@ MS_API int ms_paged_attention_kv8(const void* q, int64_t q_row_stride, void* out
  * depth.
  *
  * The plan is a packed int32 buffer described by MsPlanInfo, as ms_plan_build's (masks included);
- * ms_tree_attention launches it over a bf16 pool, or over an 8-bit pool when v_cache is NULL (k_cache is then
- * the 8-bit layer).  Its workspace of plan->workspace_bytes_per_kv_head * num_kv_heads bytes is
- * zero-filled before its first use, as ms_paged_attention_kv8's.  Sequences of at most MS_MAX_TREE_TOKENS drafts. */
+ * ms_tree_attention launches it over a bf16 pool; its workspace of plan->workspace_bytes_per_kv_head *
+ * num_kv_heads bytes is zero-filled before its first use, as ms_paged_attention_kv8's.  Over an 8-bit
+ * pool ms_kv8_plan_build appends its part to the plan (the capacity below has room for it) and
+ * ms_tree_attention_kv8 launches that, with a workspace of ms_kv8_workspace_bytes.  Sequences of at most
+ * MS_MAX_TREE_TOKENS drafts. */
 #define MS_MAX_TREE_TOKENS 1024
 MS_API int64_t ms_tree_plan_capacity(int32_t num_seqs, const int32_t* num_new,
                                      int64_t total_table_entries);
@@ -269,6 +272,11 @@ MS_API int ms_tree_attention(const void* q, int64_t q_row_stride, void* out, int
                              const void* v_cache, int32_t num_blocks, const int32_t* plan_dev,
                              const MsPlanInfo* plan, void* workspace, int64_t workspace_bytes,
                              float scale, void* stream);
+MS_API int ms_tree_attention_kv8(const void* q, int64_t q_row_stride, void* out,
+                                 int64_t out_row_stride, int32_t num_heads, int32_t num_kv_heads,
+                                 const void* pool, int32_t num_blocks, const int32_t* plan_dev,
+                                 const MsPlanInfo* plan, const MsKv8Info* info, void* workspace,
+                                 int64_t workspace_bytes, float scale, void* stream);
 
 /* ---- Attention for callers that cannot allocate device memory -------------------------------
  * No counterpart in the reference (MiniServe allocates everything through PyTorch).

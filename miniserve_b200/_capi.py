@@ -47,6 +47,7 @@ EXPORTED = (
     "ms_tree_plan_capacity",
     "ms_tree_plan_build",
     "ms_tree_attention",
+    "ms_tree_attention_kv8",
     "ms_paged_attention",
     "ms_paged_attention_noalloc",
 )
@@ -75,7 +76,8 @@ class MsPlanInfo(C.Structure):
         ("decode_pages", C.c_int32),
         ("combine_tokens_max", C.c_int32),
         ("n_tc_combine", C.c_int32),
-        ("reserved", C.c_int32 * 2),
+        ("is_tree", C.c_int32),
+        ("reserved", C.c_int32),
     ]
 
 
@@ -149,6 +151,11 @@ _SIGNATURES = {
         C.c_int,
         [_P, _I64, _P, _I64, _I32, _I32, _P, _P, _I32, _P, C.POINTER(MsPlanInfo), _P, _I64,
          C.c_float, _P],
+    ),
+    "ms_tree_attention_kv8": (
+        C.c_int,
+        [_P, _I64, _P, _I64, _I32, _I32, _P, _I32, _P, C.POINTER(MsPlanInfo),
+         C.POINTER(MsKv8Info), _P, _I64, C.c_float, _P],
     ),
     "ms_paged_attention": (
         C.c_int,

@@ -107,9 +107,9 @@ class AttentionMetadata:
         if bool(trees) != (self.tree is not None):
             return False
         if self.tree is not None:
-            tpacked, tinfo = plan_tree_batch(trees, self.num_tokens, BLOCK_SIZE, self._num_sms,
-                                             self._pages_per_split)
-            if not same_launch_shape(tinfo, self.tree.info) or tpacked.size != self.tree.plan.numel():
+            tpacked, tinfo, tkv8 = _plan_trees(trees, self.num_tokens, self._num_sms,
+                                               self._pages_per_split, _capi.MsKv8Info())
+            if not same_launch_shape(tinfo, self.tree.info) or bytes(tkv8) != bytes(self.tree.kv8):
                 return False
             self.tree.plan.copy_(torch.from_numpy(tpacked).pin_memory(), non_blocking=True)
         self.plan.copy_(torch.from_numpy(packed).pin_memory(), non_blocking=True)
@@ -215,6 +215,14 @@ def plan_tree_batch(
 ) -> tuple[np.ndarray, _capi.MsPlanInfo]:
     """Run the native planner of draft trees on the host (every chunk has ``parents``); returns
     ``(packed int32 plan, info)``."""
+    if block_size != BLOCK_SIZE:
+        raise ValueError(f"block_size must be {BLOCK_SIZE}")
+    packed, info, _ = _plan_trees(chunks, num_tokens, num_sms, pages_per_split, None)
+    return packed, info
+
+
+def _plan_trees(chunks: list[SeqChunk], num_tokens: int, num_sms: int, pages_per_split: int,
+                kv8: _capi.MsKv8Info | None):
     lib = _capi.load()
     n = len(chunks)
     for i, c in enumerate(chunks):
@@ -236,11 +244,16 @@ def plan_tree_batch(
     info = _capi.MsPlanInfo()
     rc = lib.ms_tree_plan_build(
         n, flat.ctypes.data, new.ctypes.data, cached.ctypes.data, offsets.ctypes.data,
-        tables.ctypes.data if total else None, parents.ctypes.data, num_tokens, block_size,
+        tables.ctypes.data if total else None, parents.ctypes.data, num_tokens, BLOCK_SIZE,
         num_sms, pages_per_split, out.ctypes.data, cap, C.byref(info),
     )
     _capi.check(rc, "build_attention_metadata")
-    return out[: info.total_ints], info
+    if kv8 is None:
+        return out[: info.total_ints], info, None
+    rc = lib.ms_kv8_plan_build(out.ctypes.data, cap, C.byref(info), num_sms, pages_per_split,
+                               C.byref(kv8))
+    _capi.check(rc, "build_attention_metadata")
+    return out[: kv8.total_ints], info, kv8
 
 
 def _split_trees(chunks: list[SeqChunk]) -> tuple[list[SeqChunk], list[SeqChunk]]:
@@ -326,9 +339,10 @@ def build_attention_metadata(
     slots = slots.contiguous()
     tree = None
     if trees:
-        tpacked, tinfo = plan_tree_batch(trees, num_tokens, block_size, num_sms, pages_per_split)
+        tpacked, tinfo, tkv8 = _plan_trees(trees, num_tokens, num_sms, pages_per_split,
+                                           _capi.MsKv8Info())
         tree = AttentionMetadata(slots, _upload_plan(tpacked, device), tinfo, num_tokens,
-                                 _num_sms=num_sms, _pages_per_split=pages_per_split)
+                                 _num_sms=num_sms, _pages_per_split=pages_per_split, kv8=tkv8)
     return AttentionMetadata(slots, _upload_plan(packed, device), info, num_tokens,
                              _num_sms=num_sms, _pages_per_split=pages_per_split, kv8=kv8,
                              tree=tree)
@@ -499,12 +513,16 @@ def _attend_parts(lib, q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: Attent
                 meta.plan.data_ptr(), C.byref(info), *ws_args, scale, stream)
         _capi.check(rc, "paged_attention")
     if tree is not None:
-        ws = tree.workspace(kvh, dev, counters=True)
+        ws = tree.workspace(kvh, dev, kv8, True)
         ws_args = (0, 0) if ws is None else (ws.data_ptr(), ws.numel())
-        rc = _on_own_device(
-            lib.ms_tree_attention, dev, *q_args, k_cache.data_ptr(),
-            None if kv8 else v_cache.data_ptr(), nb, tree.plan.data_ptr(), C.byref(tree.info),
-            *ws_args, scale, stream)
+        if kv8:
+            rc = _on_own_device(
+                lib.ms_tree_attention_kv8, dev, *q_args, k_cache.data_ptr(), nb,
+                tree.plan.data_ptr(), C.byref(tree.info), C.byref(tree.kv8), *ws_args, scale, stream)
+        else:
+            rc = _on_own_device(
+                lib.ms_tree_attention, dev, *q_args, k_cache.data_ptr(), v_cache.data_ptr(), nb,
+                tree.plan.data_ptr(), C.byref(tree.info), *ws_args, scale, stream)
         _capi.check(rc, "paged_attention")
 
 

@@ -59,6 +59,13 @@ int check_attention(const char* what, const void* q, int64_t q_row_stride, const
   return MS_OK;
 }
 
+// A plan of ms_tree_plan_build.
+int check_tree_plan(const char* what, const MsPlanInfo* plan) {
+  if (plan != nullptr && plan->is_tree) return MS_OK;
+  set_error(std::string(what) + ": need a plan of ms_tree_plan_build");
+  return MS_ERR_ARG;
+}
+
 ms::AttnArgs attn_args(const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride,
                        int num_kv, int num_blocks, const int32_t* plan_dev, const MsPlanInfo* plan,
                        void* workspace, int64_t part_rows, float scale) {
@@ -269,6 +276,10 @@ extern "C" int ms_paged_attention_kv8(const void* q, int64_t q_row_stride, void*
                                       const MsKv8Info* info, void* workspace,
                                       int64_t workspace_bytes, float scale, void* stream) {
   const char* what = "ms_paged_attention_kv8";
+  if (plan != nullptr && plan->is_tree) {
+    set_error("ms_paged_attention_kv8: a plan of ms_tree_plan_build is for ms_tree_attention_kv8");
+    return MS_ERR_ARG;
+  }
   if (plan != nullptr &&
       static_cast<int64_t>(plan->n_decode_items) + plan->n_tile_items + plan->n_tc_items == 0)
     return MS_OK;
@@ -376,25 +387,22 @@ extern "C" int ms_tree_attention(const void* q, int64_t q_row_stride, void* out,
                                  const int32_t* plan_dev, const MsPlanInfo* plan, void* workspace,
                                  int64_t workspace_bytes, float scale, void* stream) {
   const char* what = "ms_tree_attention";
-  if (plan != nullptr && plan->n_decode_items + plan->n_tile_items == 0) return MS_OK;
-  const int64_t need = plan != nullptr ? plan->workspace_bytes_per_kv_head * num_kv_heads : 0;
-  int rc = check_attention(what, q, q_row_stride, out, out_row_stride, num_heads, num_kv_heads,
-                           plan_dev, plan, workspace, workspace_bytes, need,
-                           plan == nullptr ? 0 : std::max(std::max(plan->n_decode_items, plan->n_tile_items), plan->n_tc_items),
-                           scale);
+  int rc = check_tree_plan(what, plan);
   if (rc) return rc;
-  const bool kv8 = v_cache == nullptr;
-  rc = kv8 ? check_pool8(what, k_cache, num_blocks, num_kv_heads)
-           : check_pool(k_cache, v_cache, num_blocks, num_kv_heads);
+  if (plan->n_decode_items + plan->n_tile_items == 0) return MS_OK;
+  rc = check_attention(what, q, q_row_stride, out, out_row_stride, num_heads, num_kv_heads, plan_dev,
+                       plan, workspace, workspace_bytes,
+                       plan->workspace_bytes_per_kv_head * num_kv_heads,
+                       std::max(std::max(plan->n_decode_items, plan->n_tile_items), plan->n_tc_items),
+                       scale);
+  if (rc) return rc;
+  rc = check_pool(k_cache, v_cache, num_blocks, num_kv_heads);
   if (rc) return rc;
   rc = ensure_smem_attrs();
   if (rc) return rc;
-  CUtensorMap map;
-  std::memset(&map, 0, sizeof(map));
-  if (!kv8) {
-    rc = kv_tensor_map(k_cache, num_blocks, num_kv_heads, 0, &map);
-    if (rc) return rc;
-  }
+  CUtensorMap map, kmap, vmap;
+  rc = kv_tensor_map(k_cache, num_blocks, num_kv_heads, 0, &map);
+  if (rc) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const RowsWork work = {plan->n_decode_items, plan->off_decode,  plan->n_tile_items,
                          plan->off_tile,       plan->off_combine, plan->part_rows};
@@ -403,25 +411,54 @@ extern "C" int ms_tree_attention(const void* q, int64_t q_row_stride, void* out,
   // The cached blocks of larger trees first (see ms_tree_plan_build); kernel F merges their partials.
   cudaError_t e = cudaSuccess;
   if (plan->n_tc_items > 0) {
+    rc = kv_tensor_map(k_cache, num_blocks, num_kv_heads, 1, &kmap);
+    if (rc == MS_OK) rc = kv_tensor_map(k_cache, num_blocks, num_kv_heads, 2, &vmap);
+    if (rc) return rc;
     ms::AttnArgs t = a;
     t.pages_fresh = 1;  // rows moved after a verify step lie below the cached length
     t.items = plan_dev + plan->off_tc;
     t.n_items = plan->n_tc_items;
-    const unsigned grid = static_cast<unsigned>(plan->n_tc_items * num_kv_heads);
-    if (kv8) {
-      e = cudaErrorNotSupported;
-    } else {
-      CUtensorMap kmap, vmap;
-      rc = kv_tensor_map(k_cache, num_blocks, num_kv_heads, 1, &kmap);
-      if (rc == MS_OK) rc = kv_tensor_map(k_cache, num_blocks, num_kv_heads, 2, &vmap);
-      if (rc) return rc;
-      e = launch(ms::prefill_tc_kernel, grid, ms::TcCfg::kThreads, ms::TcCfg::kSmemBytes, s, kmap,
-                 vmap, t);
-    }
+    e = launch(ms::prefill_tc_kernel, plan->n_tc_items * num_kv_heads, ms::TcCfg::kThreads,
+               ms::TcCfg::kSmemBytes, s, kmap, vmap, t);
   }
   if (e == cudaSuccess)
-    e = kv8 ? launch_rows_attention<true, true>(a, k_cache, map, plan_dev, work, s)
-            : launch_rows_attention<false, true>(a, nullptr, map, plan_dev, work, s);
+    e = launch_rows_attention<false, true>(a, nullptr, map, plan_dev, work, s);
   if (e != cudaSuccess) return cuda_fail("tree attention launch", e);
+  return MS_OK;
+}
+
+extern "C" int ms_tree_attention_kv8(const void* q, int64_t q_row_stride, void* out,
+                                     int64_t out_row_stride, int32_t num_heads,
+                                     int32_t num_kv_heads, const void* pool, int32_t num_blocks,
+                                     const int32_t* plan_dev, const MsPlanInfo* plan,
+                                     const MsKv8Info* info, void* workspace,
+                                     int64_t workspace_bytes, float scale, void* stream) {
+  const char* what = "ms_tree_attention_kv8";
+  int rc = check_tree_plan(what, plan);
+  if (rc) return rc;
+  if (plan->n_decode_items + plan->n_tile_items == 0) return MS_OK;
+  if (info == nullptr || info->total_ints < plan->total_ints ||
+      info->n_narrow + info->n_wide == 0) {
+    set_error("ms_tree_attention_kv8: the plan has no 8-bit part (ms_kv8_plan_build)");
+    return MS_ERR_ARG;
+  }
+  rc = check_attention(what, q, q_row_stride, out, out_row_stride, num_heads, num_kv_heads, plan_dev,
+                       plan, workspace, workspace_bytes,
+                       ms_kv8_workspace_bytes(plan, info, num_kv_heads),
+                       std::max(info->n_narrow, info->n_wide), scale);
+  if (rc) return rc;
+  rc = check_pool8(what, pool, num_blocks, num_kv_heads);
+  if (rc) return rc;
+  rc = ensure_smem_attrs();
+  if (rc) return rc;
+  CUtensorMap none;
+  std::memset(&none, 0, sizeof(none));
+  const RowsWork work = {info->n_narrow,    info->off_narrow,  info->n_wide, info->off_wide,
+                         info->off_combine, plan->part_rows + info->part_rows};
+  const ms::AttnArgs a = attn_args(q, q_row_stride, out, out_row_stride, num_kv_heads, num_blocks,
+                                   plan_dev, plan, workspace, work.part_rows, scale);
+  const cudaError_t e = launch_rows_attention<true, true>(a, pool, none, plan_dev, work,
+                                                          static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail("8-bit tree attention launch", e);
   return MS_OK;
 }

@@ -662,6 +662,10 @@ extern "C" int ms_paged_attention(const void* q, int64_t q_row_stride, void* out
     set_error("ms_paged_attention: need a plan and num_heads == 2 * num_kv_heads > 0");
     return MS_ERR_ARG;
   }
+  if (plan->is_tree) {
+    set_error("ms_paged_attention: a plan of ms_tree_plan_build is for ms_tree_attention");
+    return MS_ERR_ARG;
+  }
   const int64_t n_items = static_cast<int64_t>(plan->n_decode_items) + plan->n_tile_items +
                           plan->n_tc_items;
   if (n_items == 0) return MS_OK;

@@ -7,7 +7,9 @@
 // what its tensor-core items need over an 8-bit pool: the pages they read are expanded to bf16 in the
 // workspace, numbered densely, so the part holds the expanded pages' block ids, the identity table
 // the kernel walks instead of the block tables, and the sequence records with their tables' places
-// in it.
+// in it.  To a plan of trees with tensor-core items it adds the tiles that kernel F reads whole in
+// their place: expanding pages that one sequence reads once would write and read four times their
+// bytes (48 trees of 32 drafts over 500-2700 tokens: 145 us with kernel F).
 //
 // ms_tree_plan_build cuts every sequence of drafts into tiles that read the cached context and the
 // drafts up to the tile's last one (a parent precedes its children).  Masks are bit rows, one per
@@ -191,6 +193,16 @@ static int kv8_plan_build(int32_t* packed, int64_t capacity, const MsPlanInfo* p
     return MS_ERR_ARG;
   }
   std::memset(info, 0, sizeof(*info));
+  if (plan->is_tree && plan->n_tc_items == 0) {  // kernel F's items serve either pool
+    info->n_narrow = plan->n_decode_items;
+    info->off_narrow = plan->off_decode;
+    info->n_wide = plan->n_tile_items;
+    info->off_wide = plan->off_tile;
+    info->n_combine = plan->n_combine;
+    info->off_combine = plan->off_combine;
+    info->total_ints = plan->total_ints;
+    return MS_OK;
+  }
   const int32_t* seqs = packed + plan->off_seqs;
 
   // Kernel F's tiles: the sequences of up to 64 new tokens, in tiles of up to 32; the rows of
@@ -204,7 +216,7 @@ static int kv8_plan_build(int32_t* packed, int64_t capacity, const MsPlanInfo* p
   for (int i = 0; i < plan->num_seqs; ++i) {
     const int32_t* r = seqs + static_cast<int64_t>(i) * kRec;
     const int n = r[1], c = r[2];
-    if (n > 2 * kTileTokens) continue;
+    if (n > 2 * kTileTokens && !plan->is_tree) continue;
     if (cascade[i] != nullptr) {
       tiles.push_back({i, 0, n, cascade[i][3], cascade[i][4], -1, cascade[i][6], 1});
       continue;
@@ -224,7 +236,7 @@ static int kv8_plan_build(int32_t* packed, int64_t capacity, const MsPlanInfo* p
   const int n_rec = plan->num_seqs + plan->n_cascade;
   std::vector<int32_t> pages(n_rec, 0);
   int64_t n_pages = 0;
-  for (int i = 0; i < plan->n_tc_items; ++i) {
+  for (int i = 0; i < plan->n_tc_items && !plan->is_tree; ++i) {
     const int32_t* it = packed + plan->off_tc + static_cast<int64_t>(i) * kRec;
     pages[it[0]] = std::max(pages[it[0]], it[4]);
   }
@@ -309,11 +321,11 @@ extern "C" int64_t ms_tree_plan_capacity(int32_t num_seqs, const int32_t* num_ne
     tiles_max = std::max(tiles_max, (n + kTileTokens - 1) / kTileTokens);
     masks += n * ((n + 31) / 32);
   }
-  // A tile has at most one item per page of its sequence; narrow, wide and tensor-core items, and a
-  // virtual record per sequence.
+  // A tile has at most one item per page of its sequence; narrow, wide and tensor-core items, a
+  // virtual record per sequence, and the 8-bit part's items and combine records.
   const int64_t items = tiles + tiles_max * total_table_entries;
   return round4(2 * static_cast<int64_t>(num_seqs) * kRec) + round4(total_table_entries) +
-         3 * round4(items * kRec) + round4(tiles * kRec) + round4(masks) + 16;
+         5 * round4(items * kRec) + 2 * round4(tiles * kRec) + round4(masks) + 16;
 }
 
 static int tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const int32_t* num_new,
@@ -503,6 +515,7 @@ static int tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const in
   put_items(out, off_tc, tc);
   put_items(out, off_combine, rows.comb);
 
+  info->is_tree = 1;
   info->num_seqs = num_seqs;
   info->num_tokens = num_tokens;
   info->n_decode_items = static_cast<int32_t>(rows.narrow.size());

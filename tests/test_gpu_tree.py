@@ -66,7 +66,7 @@ def test_random_trees(n: int, split: int, pool: str, cuda_device) -> None:
     seqs = [(n, c, random_tree(rng, n, unused=rng.choice([0, 0, n // 4])))
             for c in (0, 1, 15, 16, 17, 500, 512, 645, 1535)]
     views, chunks, q = batch(cuda_device, seqs, 2, pool, seed=n)
-    check(views, chunks, q, U_BF16 if n > 16 else POOLS[pool][1], split)
+    check(views, chunks, q, POOLS[pool][1], split)
 
 
 @pytest.mark.parametrize("pool", POOLS)

@@ -11,8 +11,8 @@ import pytest
 import torch
 
 from miniserve_b200 import _capi, tree_positions
-from miniserve_b200.attention import (SeqChunk, _plan_with_kv8, attend, kv_gather, kv_scatter,
-                                      plan_tree_batch)
+from miniserve_b200.attention import (SeqChunk, _plan_trees, _plan_with_kv8, attend, kv_gather,
+                                      kv_scatter, plan_tree_batch)
 from miniserve_b200.kv_pool import (KV8, KV8_PAGE_BYTES, _kv8_parts, allocate_kv_cache,
                                     check_layer_views, kv8_bytes_per_token, layer_as_slots,
                                     quantise_rows, slots_into_layer)
@@ -172,6 +172,43 @@ def test_tree_plan_covers_every_page_once(n: int, split: int) -> None:
         assert tab.tolist() == c.block_table
 
 
+@pytest.mark.parametrize("n", [1, 16, 17, 48, 100])
+@pytest.mark.parametrize("split", [0, 1, 3, 40])
+def test_tree_plans_kv8_part_covers_every_page_once(n: int, split: int) -> None:
+    """Over an 8-bit pool kernel F reads every page of a tile itself, larger trees' cached blocks too."""
+    chunks, flat, at = [], 0, 7
+    for cached in (0, 15, 511, 512, 5000):
+        chunks.append(_chunk(flat, n, cached, at, list(range(-1, n - 1))))
+        at += len(chunks[-1].block_table)
+        flat += n
+    packed, info, kv8 = _plan_trees(chunks, flat, 148, split, _capi.MsKv8Info())
+    assert packed.size == kv8.total_ints >= info.total_ints and kv8.n_pages == 0
+    items = [packed[off:][: 8 * count].reshape(-1, 8)
+             for off, count in ((kv8.off_narrow, kv8.n_narrow), (kv8.off_wide, kv8.n_wide))]
+    assert all(it[2] <= 16 for it in items[0]) and all(16 < it[2] <= 32 for it in items[1])
+    combine = packed[kv8.off_combine :][: 8 * kv8.n_combine].reshape(-1, 8)
+    pages: dict[tuple[int, int], list[int]] = {}
+    used: set[int] = set()
+    arrive = [0] * kv8.n_combine
+    for s, tok0, nq, pb, pe, part, rec, flag in np.concatenate(items).tolist():
+        pages.setdefault((s, tok0), []).extend(range(pb, pe))
+        assert (part >= 0) == (flag == 2) and flag in (0, 2)
+        if part >= 0:
+            k = (part - combine[rec, 3]) // (2 * nq)
+            assert combine[rec, :3].tolist() == [s, tok0, nq] and combine[rec, 5] == 2 * nq
+            assert 0 <= k < combine[rec, 4] and (part - combine[rec, 3]) % (2 * nq) == 0
+            rows = set(range(part, part + 2 * nq))
+            assert not rows & used and max(rows) < info.part_rows + kv8.part_rows
+            used |= rows
+            arrive[rec] += 1
+    assert arrive == combine[:, 4].tolist() == combine[:, 6].tolist()
+    for i, c in enumerate(chunks):
+        for tok0 in range(0, n, 32):
+            last = c.num_cached + min(n, tok0 + 32)
+            assert sorted(pages.pop((i, tok0))) == list(range(-(-last // 16)))
+    assert not pages
+
+
 @pytest.mark.parametrize("parents,what", [
     ([-1, 1, 0], "draft 1 has parent 1"), ([0, -1], "draft 0 has parent 0"),
     ([-1, -3], "draft 1 has parent -3"), ([-2, 0], "draft 1 has parent 0"), ([-1, 2, -1], "draft 1"),
@@ -302,13 +339,22 @@ def test_entry_points_refuse_bad_arguments() -> None:
                                            0, None, None, 0, None, 0, None) == _capi.MS_ERR_ARG
     _, info = plan_tree_batch([_chunk(0, 2, 4, 0, [-1, 0])], 2)
     for scale in (0.0, -1.0, float("nan"), float("inf")):
-        rc = lib.ms_tree_attention(p, 256, p, 256, 2, 1, p, None, 1, p, C.byref(info), None, 0, scale,
+        rc = lib.ms_tree_attention(p, 256, p, 256, 2, 1, p, p, 1, p, C.byref(info), None, 0, scale,
                                    None)
         assert rc == _capi.MS_ERR_ARG and b"scale" in lib.ms_last_error()
-    rc = lib.ms_tree_attention(p, 256, p, 256, 3, 1, p, None, 1, p, C.byref(info), None, 0, 1.0, None)
+    rc = lib.ms_tree_attention(p, 256, p, 256, 3, 1, p, p, 1, p, C.byref(info), None, 0, 1.0, None)
     assert rc == _capi.MS_ERR_ARG and b"num_heads" in lib.ms_last_error()
+    args = (p, 256, p, 256, 2, 1, p, 1, p, C.byref(info))
+    rc = lib.ms_tree_attention_kv8(*args, None, None, 0, 1.0, None)
+    assert rc == _capi.MS_ERR_ARG and b"8-bit part" in lib.ms_last_error()
+    rc = lib.ms_paged_attention_kv8(*args, None, None, 0, 1.0, None)
+    assert rc == _capi.MS_ERR_ARG and b"ms_tree_plan_build" in lib.ms_last_error()
+    rc = lib.ms_paged_attention(p, 256, p, 256, 2, 1, p, p, 1, p, C.byref(info), None, 0, 1.0, None)
+    assert rc == _capi.MS_ERR_ARG and b"ms_tree_plan_build" in lib.ms_last_error()
     _, info, kv8 = _plan_with_kv8([_chunk(0, 100, 4, 0)], 100, 148, 0)
     args = (p, 256, p, 256, 2, 1, p, 1, p, C.byref(info))
+    rc = lib.ms_tree_attention_kv8(*args, C.byref(kv8), None, 0, 1.0, None)
+    assert rc == _capi.MS_ERR_ARG and b"ms_tree_plan_build" in lib.ms_last_error()
     rc = lib.ms_paged_attention_kv8(*args, None, None, 0, 1.0, None)
     assert rc == _capi.MS_ERR_ARG and b"8-bit part" in lib.ms_last_error()
     rc = lib.ms_paged_attention_kv8(*args, C.byref(kv8), None, 0, 1.0, None)

@@ -553,106 +553,98 @@ __device__ __forceinline__ void rows_page16_special(uint32_t page, int t, uint32
 // ---- the kernel ---------------------------------------------------------------------------------
 
 // The last CTA of a split tile merges the splits' partial rows: out = sum_s 2^(lse_s - M) O_s /
-// sum_s 2^(lse_s - M), s in order, so the result does not depend on which CTA came last.  The
-// partial rows come through shared memory (the idle ring, `bytes` of it) by asynchronous copies, as many
-// splits at a time as fit, so that one latency covers them all, and the rows' M and sums are formed from
-// global memory meanwhile.  A warp takes rows warp, warp + 4, ..., a lane four columns.  masks: the
-// tile's first mask row of a tree (a draft that sees nothing writes zeros: the tensor-core kernel
-// does not know it), else null.
-template <int kRows>
-__device__ __forceinline__ void merge_splits(const AttnArgs& a, uint8_t* smem, int bytes, int row0,
-                                             int n_splits, int stride, int rows, int kvh,
-                                             int flat_tok, const int* masks, int words, int tok0) {
-  constexpr int kT = kRowsWarps * 32, kPer = kRows / kRowsWarps, kLanes = kT / kRows;
+// sum_s 2^(lse_s - M), s in order, so the result does not depend on which CTA came last.  It runs alone
+// and is bound by latencies, so it has few of them: first L neighbouring threads per row form its M and
+// sum, then each warp takes rows warp, warp + 4, ..., two at a time, a lane four columns, and fetches
+// eight splits of both rows at once, their weights with them.  (3 rows over 100k tokens in 36 splits:
+// 51 us; 57 with the partial rows copied to shared memory first.)  Every load goes past L1, whose lines
+// may be older than the other CTAs' rows.  masks: the tile's first mask row of a tree (a draft that sees
+// nothing writes zeros: the tensor-core kernel does not know it), else null.  top: 2 x rows floats.
+__device__ __forceinline__ void merge_splits(const AttnArgs& a, float* top, int row0, int n_splits,
+                                             int stride, int rows, int kvh, int flat_tok,
+                                             const int* masks, int words, int tok0) {
+  constexpr int kStep = 8;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  float* top = reinterpret_cast<float*>(smem);  // [kRows] M, then [kRows] 1 / sum
-  float* lse_s = top + 2 * kRows;               // [splits of a chunk][rows], then their O rows
-  const int chunk = max(1, min(n_splits, (bytes - 2 * kRows * 4) / (rows * (kHeadDim + 1) * 4 + 16)));
-  float* o_s = lse_s + (chunk * rows + 3) / 4 * 4;
-  auto at = [&](int s, int r) {
-    return (static_cast<long long>(row0) + static_cast<long long>(s) * stride + r) * a.num_kv + kvh;
-  };
-  float4 acc[kPer];
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-  for (int s0 = 0; s0 < n_splits; s0 += chunk) {
-    const int cnt = min(chunk, n_splits - s0);
-    if (s0 > 0) asm volatile("bar.sync 1, %0;" ::"r"(kT) : "memory");  // the last chunk was read
-#pragma unroll 1
-    for (int s = 0; s < cnt; ++s) {
-      for (int r = warp; r < rows; r += kRowsWarps)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                         smem_u32(o_s + (s * rows + r) * kHeadDim + lane * 4)),
-                     "l"(a.ws_o + at(s0 + s, r) * kHeadDim + lane * 4)
-                     : "memory");
-    }
-    // (Past L1, like everything here: its lines may be older than the other CTAs' rows.)
-    for (int i = tid; i < cnt * rows; i += kT) {
-      const int s = i / rows;
-      lse_s[i] = __ldcg(a.ws_lse + at(s0 + s, i - s * rows));
-    }
-    if (s0 == 0) {
-      // kLanes neighbouring threads per row, over all splits.
-      const int r = tid / kLanes;
-      float m = -INFINITY, l = 0.f;
-      if (r < rows) {
+  const long long split_rows = static_cast<long long>(stride) * a.num_kv;
+  {
+    const int log_l = min(5, 7 - (32 - __clz(rows - 1)));  // 128 threads over the rows, L <= 32
+    const int r = tid >> log_l, l_step = 1 << log_l;
+    const float* lse = a.ws_lse + static_cast<long long>(row0 + r) * a.num_kv + kvh;
+    float m = -INFINITY, l = 0.f;
+    if (r < rows) {
 #pragma unroll 4
-        for (int s = tid % kLanes; s < n_splits; s += kLanes) {
-          const float x = __ldcg(a.ws_lse + at(s, r));
-          if (x == -INFINITY) continue;
-          const float mn = fmaxf(m, x);
-          l = l * fast_exp2(m - mn) + fast_exp2(x - mn);  // a NaN stays in l
-          m = mn;
-        }
-      }
-#pragma unroll
-      for (int off = 1; off < kLanes; off <<= 1) {
-        const float mo = __shfl_xor_sync(0xffffffffu, m, off);
-        const float lo = __shfl_xor_sync(0xffffffffu, l, off);
-        const float mn = fmaxf(m, mo);
-        l = (m == -INFINITY ? l : l * fast_exp2(m - mn)) + (mo == -INFINITY ? lo : lo * fast_exp2(mo - mn));
+      for (int s = tid & (l_step - 1); s < n_splits; s += l_step) {
+        const float x = __ldcg(lse + s * split_rows);
+        if (x == -INFINITY) continue;
+        const float mn = fmaxf(m, x);
+        l = l * fast_exp2(m - mn) + fast_exp2(x - mn);  // a NaN stays in l
         m = mn;
       }
-      if (r < kRows && tid % kLanes == 0) {
-        top[r] = m;
-        top[kRows + r] = l != 0.f ? 1.f / l : 0.f;
-      }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    asm volatile("bar.sync 1, %0;" ::"r"(kT) : "memory");
+    for (int off = 1; off < l_step; off <<= 1) {
+      const float mo = __shfl_xor_sync(0xffffffffu, m, off);
+      const float lo = __shfl_xor_sync(0xffffffffu, l, off);
+      const float mn = fmaxf(m, mo);
+      l = (m == -INFINITY ? l : l * fast_exp2(m - mn)) + (mo == -INFINITY ? lo : lo * fast_exp2(mo - mn));
+      m = mn;
+    }
+    if (r < rows && (tid & (l_step - 1)) == 0) {
+      top[r] = m;
+      top[rows + r] = l != 0.f ? 1.f / l : 0.f;  // a NaN sum stays NaN
+    }
+  }
+  asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
+#pragma unroll 1
+  for (int r0 = warp; r0 < rows; r0 += 2 * kRowsWarps) {
+    const int n_r = r0 + kRowsWarps < rows ? 2 : 1;
+    const long long first = static_cast<long long>(row0 + r0) * a.num_kv + kvh;
+    const long long second = (n_r == 2 ? kRowsWarps : 0) * static_cast<long long>(a.num_kv);
+    const float* o = a.ws_o + first * kHeadDim + lane * 4;
+    // Lane 8 h + i (h < 2) forms the weight of split s + i of row h.
+    const int wh = lane >> 3 & 1, wi = lane & (kStep - 1);
+    const float* lse = a.ws_lse + first + wh * second;
+    const float m = top[r0 + (wh && n_r == 2 ? kRowsWarps : 0)];
+    float4 acc[2] = {};
+#pragma unroll 1
+    for (int s = 0; s < n_splits; s += kStep) {
+      float4 x[2][kStep];
+      const float w_lse = s + wi < n_splits ? __ldcg(lse + (s + wi) * split_rows) : -INFINITY;
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int r = warp + k * kRowsWarps;
-      if (r < rows) {
-        const float m = top[r];
-#pragma unroll 2
-        for (int i = 0; i < cnt; ++i) {
-          const float x = lse_s[i * rows + r];
-          const float w = x == -INFINITY ? 0.f : fast_exp2(x - m);
-          const float4 v = *reinterpret_cast<const float4*>(o_s + (i * rows + r) * kHeadDim + lane * 4);
-          acc[k].x += w * v.x;
-          acc[k].y += w * v.y;
-          acc[k].z += w * v.z;
-          acc[k].w += w * v.w;
+      for (int i = 0; i < kStep; ++i) {
+        x[0][i] = x[1][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (s + i < n_splits) {
+          const float* at = o + (s + i) * split_rows * kHeadDim;
+          x[0][i] = __ldcg(reinterpret_cast<const float4*>(at));
+          if (n_r == 2) x[1][i] = __ldcg(reinterpret_cast<const float4*>(at + second * kHeadDim));
+        }
+      }
+      const float w = w_lse == -INFINITY ? 0.f : fast_exp2(w_lse - m);
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float u = __shfl_sync(0xffffffffu, w, 8 * h + i);
+          acc[h].x += u * x[h][i].x;
+          acc[h].y += u * x[h][i].y;
+          acc[h].z += u * x[h][i].z;
+          acc[h].w += u * x[h][i].w;
         }
       }
     }
-  }
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const int r = warp + k * kRowsWarps;
-    if (r >= rows) break;
-    const float inv = top[kRows + r];  // a NaN sum stays NaN
-    const int tok = tok0 + (r >> 1);
-    const bool live = masks == nullptr ||
-                      (masks[static_cast<long long>(r >> 1) * words + (tok >> 5)] >> (tok & 31) & 1);
-    __nv_bfloat16* dst = a.out + static_cast<long long>(flat_tok + (r >> 1)) * a.out_row_stride +
-                         (kvh * kGroup + (r & 1)) * kHeadDim + lane * 4;
-    *reinterpret_cast<uint2*>(dst) =
-        live ? make_uint2(pack_bf16(acc[k].x * inv, acc[k].y * inv),
-                          pack_bf16(acc[k].z * inv, acc[k].w * inv))
-             : make_uint2(0u, 0u);
+    for (int h = 0; h < 2; ++h) {
+      if (h >= n_r) break;
+      const int r = r0 + h * kRowsWarps, tok = tok0 + (r >> 1);
+      const float inv = top[rows + r];
+      const bool live = masks == nullptr ||
+                        (masks[static_cast<long long>(r >> 1) * words + (tok >> 5)] >> (tok & 31) & 1);
+      __nv_bfloat16* dst = a.out + static_cast<long long>(flat_tok + (r >> 1)) * a.out_row_stride +
+                           (kvh * kGroup + (r & 1)) * kHeadDim + lane * 4;
+      *reinterpret_cast<uint2*>(dst) =
+          live ? make_uint2(pack_bf16(acc[h].x * inv, acc[h].y * inv),
+                            pack_bf16(acc[h].z * inv, acc[h].w * inv))
+               : make_uint2(0u, 0u);
+    }
   }
 }
 
@@ -1141,10 +1133,9 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
     asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
     if (*last_flag) {
       __threadfence();
-      merge_splits<Cfg::kRows>(a, ring, Cfg::kStageBytes, cr[3], cr[4], cr[5], n_q * kGroup, kvh,
-                               flat_start + tok0,
-                               kTree ? masks + static_cast<long long>(tok0) * words : nullptr, words,
-                               tok0);
+      merge_splits(a, reinterpret_cast<float*>(ring), cr[3], cr[4], cr[5], n_q * kGroup, kvh,
+                   flat_start + tok0,
+                   kTree ? masks + static_cast<long long>(tok0) * words : nullptr, words, tok0);
     }
   }
 }

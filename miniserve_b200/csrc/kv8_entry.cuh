@@ -16,13 +16,14 @@ int check_pool8(const char* what, const void* pool, int num_blocks, int num_kv) 
   return MS_OK;
 }
 
-// Grid of the row-copy kernels (see row_pair): a warp takes 4 tokens where that leaves every SM enough
+// Grid of the row-copy kernels (see row_group): a warp takes 4 tokens where that leaves every SM enough
 // warps, else one, so that a decode step's few rows spread over more SMs.
 constexpr int kCopyWarps = 8;
 constexpr int64_t kMaxCopyWarps = int64_t(1) << 31;  // warp indices are 32-bit
 template <typename Few, typename Many>
 cudaError_t launch_rows(int64_t tokens, int num_kv, int sms, Few few, Many many) {
-  const int64_t w4 = (tokens + 3) / 4 * num_kv, w1 = tokens * num_kv;
+  const int64_t groups = (2 * static_cast<int64_t>(num_kv) + 3) / 4;
+  const int64_t w4 = (tokens + 3) / 4 * groups, w1 = tokens * groups;
   if (w4 >= static_cast<int64_t>(16) * sms)
     return many(static_cast<unsigned>((w4 + kCopyWarps - 1) / kCopyWarps));
   return few(static_cast<unsigned>((w1 + kCopyWarps - 1) / kCopyWarps));

@@ -94,16 +94,19 @@ struct RowsWork {
   int64_t part_rows;  // of all partials in the workspace; the arrival counters lie behind them
 };
 
-// Kernel F over the narrow tiles and the wide ones.
+// Kernel F over the narrow tiles and the wide ones.  behind: see RowsArgs; the wide tiles never depend on
+// the narrow ones.
 template <bool kKv8, bool kTree>
 cudaError_t launch_rows_attention(const ms::AttnArgs& a, const void* pool, const CUtensorMap& map,
-                                  const int32_t* plan_dev, const RowsWork& w, cudaStream_t s) {
+                                  const int32_t* plan_dev, const RowsWork& w, bool behind,
+                                  cudaStream_t s) {
   ms::RowsArgs r;
   r.a = a;
   r.pool = static_cast<const uint8_t*>(pool);
   r.plan = plan_dev;
   r.combines = plan_dev + w.off_combine;
   r.arrived = a.ws_lse != nullptr ? reinterpret_cast<int*>(a.ws_lse + w.part_rows * a.num_kv) : nullptr;
+  r.behind = behind;
   cudaError_t e = cudaSuccess;
   if (w.n_narrow > 0) {
     using Cfg = ms::RowsCfg<kKv8, 1>;
@@ -111,6 +114,7 @@ cudaError_t launch_rows_attention(const ms::AttnArgs& a, const void* pool, const
     r.a.n_items = w.n_narrow;
     e = launch(ms::rows_attn_kernel<kKv8, kTree, 1>, static_cast<unsigned>(w.n_narrow * a.num_kv),
                Cfg::kThreads, Cfg::kSmemBytes, s, map, r);
+    r.behind = 1;
   }
   if (e == cudaSuccess && w.n_wide > 0) {
     using Cfg = ms::RowsCfg<kKv8, 2>;
@@ -365,7 +369,7 @@ extern "C" int ms_paged_attention_kv8(const void* q, int64_t q_row_stride, void*
   if (n_rows > 0) {
     CUtensorMap none;
     std::memset(&none, 0, sizeof(none));
-    const cudaError_t e = launch_rows_attention<true, false>(a, pool, none, plan_dev, work, ds);
+    const cudaError_t e = launch_rows_attention<true, false>(a, pool, none, plan_dev, work, false, ds);
     if (e != cudaSuccess) {
       join();
       return cuda_fail("8-bit rows launch", e);
@@ -423,7 +427,7 @@ extern "C" int ms_tree_attention(const void* q, int64_t q_row_stride, void* out,
                ms::TcCfg::kSmemBytes, s, kmap, vmap, t);
   }
   if (e == cudaSuccess)
-    e = launch_rows_attention<false, true>(a, nullptr, map, plan_dev, work, s);
+    e = launch_rows_attention<false, true>(a, nullptr, map, plan_dev, work, plan->n_tc_items > 0, s);
   if (e != cudaSuccess) return cuda_fail("tree attention launch", e);
   return MS_OK;
 }
@@ -459,7 +463,7 @@ extern "C" int ms_tree_attention_kv8(const void* q, int64_t q_row_stride, void* 
   const ms::AttnArgs a = attn_args(q, q_row_stride, out, out_row_stride, num_kv_heads, num_blocks,
                                    plan_dev, plan, workspace, work.part_rows, scale);
   const cudaError_t e = launch_rows_attention<true, true>(a, pool, none, plan_dev, work,
-                                                          static_cast<cudaStream_t>(stream));
+                                                          false, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail("8-bit tree attention launch", e);
   return MS_OK;
 }

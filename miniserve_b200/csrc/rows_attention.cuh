@@ -55,6 +55,12 @@ struct RowsArgs {
   // this kernel that arrive} of tiles with several partials; an item names its record in field 6.
   const int* combines;
   int* arrived;         // [record][KVH] splits that have finished: zero between calls
+  // The kernel before this one belongs to the same call and lets this one start only once its own
+  // predecessor has completed (every CTA of it waits before it triggers), and nothing before the merge
+  // reads what it writes: the wait for it moves from the start to the merge, so this kernel's pages fill the SMs
+  // that its longest CTAs leave idle.  Every CTA still waits, so that whoever waits for this kernel has
+  // waited for that one too.
+  int behind;
 };
 
 template <bool kKv8, int kRG>
@@ -552,19 +558,84 @@ __device__ __forceinline__ void rows_page16_special(uint32_t page, int t, uint32
 
 // ---- the kernel ---------------------------------------------------------------------------------
 
+// Rows of a split tile from their M and 1 / sum in `top`: warp w takes rows w, w + 4, ..., kR at a time, a
+// lane four columns; the partial rows of kS splits are fetched at once, their weights with them (lane
+// kS h + i forms that of split i of row h).
+template <int kR, int kS>
+__device__ __forceinline__ void merge_rows(const AttnArgs& a, const float* top, int row0,
+                                           int n_splits, int stride, int rows, int kvh, int flat_tok,
+                                           const int* masks, int words, int tok0) {
+  static_assert(kR * kS <= 32 && (kS & (kS - 1)) == 0 && (kR & (kR - 1)) == 0, "a lane per weight");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long split_rows = static_cast<long long>(stride) * a.num_kv;
+  const long long row_step = static_cast<long long>(kRowsWarps) * a.num_kv;
+  const int wh = lane / kS & (kR - 1), wi = lane & (kS - 1);
+#pragma unroll 1
+  for (int r0 = warp; r0 < rows; r0 += kR * kRowsWarps) {
+    const int n_r = min(kR, (rows - r0 + kRowsWarps - 1) / kRowsWarps);
+    const long long first = static_cast<long long>(row0 + r0) * a.num_kv + kvh;
+    const float* o = a.ws_o + first * kHeadDim + lane * 4;
+    const int my_h = min(wh, n_r - 1);
+    const float* lse = a.ws_lse + first + my_h * row_step;
+    const float m = top[r0 + my_h * kRowsWarps];
+    float4 acc[kR] = {};
+#pragma unroll 1
+    for (int s = 0; s < n_splits; s += kS) {
+      float4 x[kR][kS];
+      const float w_lse = s + wi < n_splits ? __ldcg(lse + (s + wi) * split_rows) : -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kS; ++i) {
+#pragma unroll
+        for (int h = 0; h < kR; ++h) {
+          x[h][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (s + i < n_splits && h < n_r)
+            x[h][i] = __ldcg(reinterpret_cast<const float4*>(
+                o + ((s + i) * split_rows + h * row_step) * kHeadDim));
+        }
+      }
+      const float w = w_lse == -INFINITY ? 0.f : fast_exp2(w_lse - m);
+#pragma unroll
+      for (int i = 0; i < kS; ++i) {
+#pragma unroll
+        for (int h = 0; h < kR; ++h) {
+          const float u = __shfl_sync(0xffffffffu, w, kS * h + i);
+          acc[h].x += u * x[h][i].x;
+          acc[h].y += u * x[h][i].y;
+          acc[h].z += u * x[h][i].z;
+          acc[h].w += u * x[h][i].w;
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < kR; ++h) {
+      if (h >= n_r) break;
+      const int r = r0 + h * kRowsWarps, tok = tok0 + (r >> 1);
+      const float inv = top[rows + r];
+      const bool live = masks == nullptr ||
+                        (masks[static_cast<long long>(r >> 1) * words + (tok >> 5)] >> (tok & 31) & 1);
+      __nv_bfloat16* dst = a.out + static_cast<long long>(flat_tok + (r >> 1)) * a.out_row_stride +
+                           (kvh * kGroup + (r & 1)) * kHeadDim + lane * 4;
+      *reinterpret_cast<uint2*>(dst) =
+          live ? make_uint2(pack_bf16(acc[h].x * inv, acc[h].y * inv),
+                            pack_bf16(acc[h].z * inv, acc[h].w * inv))
+               : make_uint2(0u, 0u);
+    }
+  }
+}
+
 // The last CTA of a split tile merges the splits' partial rows: out = sum_s 2^(lse_s - M) O_s /
 // sum_s 2^(lse_s - M), s in order, so the result does not depend on which CTA came last.  It runs alone
-// and is bound by latencies, so it has few of them: first L neighbouring threads per row form its M and
-// sum, then each warp takes rows warp, warp + 4, ..., two at a time, a lane four columns, and fetches
-// eight splits of both rows at once, their weights with them.  (3 rows over 100k tokens in 36 splits:
-// 51 us; 57 with the partial rows copied to shared memory first.)  Every load goes past L1, whose lines
-// may be older than the other CTAs' rows.  masks: the tile's first mask row of a tree (a draft that sees
-// nothing writes zeros: the tensor-core kernel does not know it), else null.  top: 2 x rows floats.
+// and is bound by latencies, so it has few of them: L neighbouring threads per row form its M and sum,
+// then the rows are merged with 16 loads in flight per lane (3 rows over 100k tokens in 36 splits: 51 us;
+// 57 with the partial rows copied to shared memory first), spread over the splits where there are many,
+// else over the rows (48 trees of 32 drafts: 131 us, 135 with two rows at a time).  Every load
+// goes past L1, whose lines may be older than the other CTAs' rows.  masks: the tile's first mask row of
+// a tree (a draft that sees nothing writes zeros: the tensor-core kernel does not know it), else null.
+// top: 2 x rows floats.
 __device__ __forceinline__ void merge_splits(const AttnArgs& a, float* top, int row0, int n_splits,
                                              int stride, int rows, int kvh, int flat_tok,
                                              const int* masks, int words, int tok0) {
-  constexpr int kStep = 8;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x;
   const long long split_rows = static_cast<long long>(stride) * a.num_kv;
   {
     const int log_l = min(5, 7 - (32 - __clz(rows - 1)));  // 128 threads over the rows, L <= 32
@@ -594,58 +665,10 @@ __device__ __forceinline__ void merge_splits(const AttnArgs& a, float* top, int 
     }
   }
   asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
-#pragma unroll 1
-  for (int r0 = warp; r0 < rows; r0 += 2 * kRowsWarps) {
-    const int n_r = r0 + kRowsWarps < rows ? 2 : 1;
-    const long long first = static_cast<long long>(row0 + r0) * a.num_kv + kvh;
-    const long long second = (n_r == 2 ? kRowsWarps : 0) * static_cast<long long>(a.num_kv);
-    const float* o = a.ws_o + first * kHeadDim + lane * 4;
-    // Lane 8 h + i (h < 2) forms the weight of split s + i of row h.
-    const int wh = lane >> 3 & 1, wi = lane & (kStep - 1);
-    const float* lse = a.ws_lse + first + wh * second;
-    const float m = top[r0 + (wh && n_r == 2 ? kRowsWarps : 0)];
-    float4 acc[2] = {};
-#pragma unroll 1
-    for (int s = 0; s < n_splits; s += kStep) {
-      float4 x[2][kStep];
-      const float w_lse = s + wi < n_splits ? __ldcg(lse + (s + wi) * split_rows) : -INFINITY;
-#pragma unroll
-      for (int i = 0; i < kStep; ++i) {
-        x[0][i] = x[1][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (s + i < n_splits) {
-          const float* at = o + (s + i) * split_rows * kHeadDim;
-          x[0][i] = __ldcg(reinterpret_cast<const float4*>(at));
-          if (n_r == 2) x[1][i] = __ldcg(reinterpret_cast<const float4*>(at + second * kHeadDim));
-        }
-      }
-      const float w = w_lse == -INFINITY ? 0.f : fast_exp2(w_lse - m);
-#pragma unroll
-      for (int i = 0; i < kStep; ++i) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float u = __shfl_sync(0xffffffffu, w, 8 * h + i);
-          acc[h].x += u * x[h][i].x;
-          acc[h].y += u * x[h][i].y;
-          acc[h].z += u * x[h][i].z;
-          acc[h].w += u * x[h][i].w;
-        }
-      }
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (h >= n_r) break;
-      const int r = r0 + h * kRowsWarps, tok = tok0 + (r >> 1);
-      const float inv = top[rows + r];
-      const bool live = masks == nullptr ||
-                        (masks[static_cast<long long>(r >> 1) * words + (tok >> 5)] >> (tok & 31) & 1);
-      __nv_bfloat16* dst = a.out + static_cast<long long>(flat_tok + (r >> 1)) * a.out_row_stride +
-                           (kvh * kGroup + (r & 1)) * kHeadDim + lane * 4;
-      *reinterpret_cast<uint2*>(dst) =
-          live ? make_uint2(pack_bf16(acc[h].x * inv, acc[h].y * inv),
-                            pack_bf16(acc[h].z * inv, acc[h].w * inv))
-               : make_uint2(0u, 0u);
-    }
-  }
+  if (n_splits <= 4)
+    merge_rows<4, 4>(a, top, row0, n_splits, stride, rows, kvh, flat_tok, masks, words, tok0);
+  else
+    merge_rows<2, 8>(a, top, row0, n_splits, stride, rows, kvh, flat_tok, masks, words, tok0);
 }
 
 template <bool kKv8, bool kTree, int kRG>
@@ -700,7 +723,7 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
     if constexpr (kRG == 2) setmaxnreg_dec<Cfg::kProducerRegs>();
     const int* table = a.tables + table_off + page_begin;
     int mine = lane < npages ? table[lane] : 0;
-    pdl_wait();
+    if (!ra.behind) pdl_wait();
     pdl_trigger();
     if (warp != kRowsWarps) return;
     // ---------------- producer warp ----------------
@@ -772,7 +795,7 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
 
   // ---------------- consumer warps ----------------
   if constexpr (kRG == 2) setmaxnreg_inc<Cfg::kConsumerRegs>();
-  pdl_wait();
+  if (!ra.behind) pdl_wait();
   pdl_trigger();
   // Query rows to shared memory, half a warp per row: bf16 as they are; for an 8-bit pool scaled
   // into f16 and in the order of dims that rows_block8 wants.  Rows without a token are zeros.
@@ -1118,6 +1141,7 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
     }
   }
 
+  if (ra.behind) pdl_wait();
   if (part_row >= 0) {
     // A split of a tile, or the last pages of one whose cached blocks the tensor-core kernel read
     // before this launch: the last one to arrive merges them all.

@@ -121,7 +121,9 @@ class AttentionMetadata:
                   counters: bool = False) -> Tensor | None:
         """Scratch for this step (allocated once, reused by every layer): split-KV partials, with
         ``counters`` the arrival counters of split tiles behind them (zeroed here, left at zero by
-        every call), and for an 8-bit pool the expanded pages of tensor-core items."""
+        every call), and for an 8-bit pool the expanded pages of tensor-core items.  Allocated while
+        the stream is captured, a workspace with counters is that call's own: its zeroing is a node
+        of the graph, which runs only when that graph does."""
         key = (device, -num_kv_heads if kv8 else num_kv_heads)  # a tensor's device has its index
         ws = self._workspace.get(key)
         if ws is not None:
@@ -138,7 +140,10 @@ class AttentionMetadata:
             rows = int(self.info.part_rows) + (int(self.kv8.part_rows) if kv8 else 0)
             n = int(self.kv8.n_combine if kv8 else self.info.n_combine)
             at = rows * (HEAD_DIM + 1) * 4 * num_kv_heads
-            ws[at : at + n * 4 * num_kv_heads].zero_()
+            if n:
+                ws[at : at + n * 4 * num_kv_heads].zero_()
+                if torch.cuda.is_current_stream_capturing():
+                    return ws
         self._workspace[key] = ws
         return ws
 
@@ -381,7 +386,13 @@ def _rows(t: Tensor, name: str) -> int:
 
 def kv_scatter(k: Tensor, v: Tensor, slot_mapping: Tensor, k_cache: Tensor, v_cache: Tensor) -> None:
     """Write this step's K/V rows into their slots (backends.py:159-160).  Into an 8-bit pool each
-    row is quantised as it is written (see ``kv_pool``)."""
+    row is quantised as it is written (see ``kv_pool``).
+
+    The slots of one call differ from each other, as for ``index_copy_``: what a slot named twice
+    holds afterwards is undefined (an 8-bit one may pair one row's codes with the other's exponent).
+    ``attend`` over a bf16 pool may read rows below a sequence's ``num_cached`` while the call before it
+    on the stream still runs: they are written by an earlier call than the one right before it (a step that
+    moves accepted drafts does so before it writes its own rows)."""
     nb, kvh = check_layer_views(k_cache, v_cache, kv8=True)
     t = int(k.shape[0])
     lib = _capi.load()

@@ -105,7 +105,7 @@ cudaError_t launch_rows_attention(const ms::AttnArgs& a, const void* pool, const
   r.pool = static_cast<const uint8_t*>(pool);
   r.plan = plan_dev;
   r.combines = plan_dev + w.off_combine;
-  r.arrived = a.ws_lse != nullptr ? reinterpret_cast<int*>(a.ws_lse + w.part_rows * a.num_kv) : nullptr;
+  r.arrived = a.ws_lse != nullptr ? reinterpret_cast<unsigned*>(a.ws_lse + w.part_rows * a.num_kv) : nullptr;
   r.behind = behind;
   cudaError_t e = cudaSuccess;
   if (w.n_narrow > 0) {

@@ -54,7 +54,7 @@ struct RowsArgs {
   // Combine records {seq, tok0, n_q, first partial row, partials per row, rows between them, CTAs of
   // this kernel that arrive} of tiles with several partials; an item names its record in field 6.
   const int* combines;
-  int* arrived;         // [record][KVH] splits that have finished: zero between calls
+  unsigned* arrived;    // [record][KVH] splits that have finished: zero between calls
   // The kernel before this one belongs to the same call and lets this one start only once its own
   // predecessor has completed (every CTA of it waits before it triggers), and nothing before the merge
   // reads what it writes: the wait for it moves from the start to the merge, so this kernel's pages fill the SMs
@@ -809,7 +809,7 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
       const int r = (i * kRowsWarps + warp) * 2 + (lane >> 4);
       x[i] = make_uint4(0u, 0u, 0u, 0u);
       if ((r >> 1) < n_q)
-        x[i] = __ldg(reinterpret_cast<const uint4*>(
+        x[i] = __ldcg(reinterpret_cast<const uint4*>(
             a.q + static_cast<long long>(flat_start + tok0 + (r >> 1)) * a.q_row_stride +
             (kvh * kGroup + (r & 1)) * kHeadDim + l16 * 8));
     }
@@ -1149,10 +1149,9 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
     asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
     const int* cr = ra.combines + static_cast<long long>(it[6]) * kRec;
     if (threadIdx.x == 0) {
-      int* counter = ra.arrived + static_cast<long long>(it[6]) * a.num_kv + kvh;
-      const bool last = atomicAdd(counter, 1) == cr[6] - 1;
-      if (last) *counter = 0;  // ready for the next call
-      *last_flag = last ? 1 : 0;
+      unsigned* counter = ra.arrived + static_cast<long long>(it[6]) * a.num_kv + kvh;
+      // Wraps to 0 with the last arrival: ready for the next call.
+      *last_flag = atomicInc(counter, static_cast<unsigned>(cr[6] - 1)) == static_cast<unsigned>(cr[6] - 1);
     }
     asm volatile("bar.sync 1, %0;" ::"r"(kRowsWarps * 32) : "memory");
     if (*last_flag) {

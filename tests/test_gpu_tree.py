@@ -263,3 +263,55 @@ def test_a_speculative_loop(pool: str, cuda_device) -> None:
         ref, bound, covered = attention64(q, *views, chunks, U_BF16)
         assert_close(out, ref, bound, covered)
         cached = [c + 1 for c in cached]
+
+
+@pytest.mark.parametrize("pool", POOLS)
+def test_graphs_captured_first_and_eager_calls_between(pool: str, cuda_device) -> None:
+    """Split tiles count their arrivals in the workspace: graphs captured before any eager call, an eager
+    call before their first replay, and replays in any order all find the counters at zero."""
+    dev = cuda_device
+    rng = random.Random(5)
+    warm_views, warm_chunks, warm_q = batch(dev, [(3, 20, [-1, 0, 0])], 2, pool, seed=1)
+    check(warm_views, warm_chunks, warm_q, U_BF16)  # loads the kernels
+    seqs = [(8, 2500, random_tree(rng, 8)), (40, 1100, random_tree(rng, 40)), (2, 3000, None)]
+    views, chunks, q = batch(dev, seqs, 2, pool, seed=11)
+    meta = build_attention_metadata(chunks, slots_of(chunks, dev), 16, pages_per_split=24)
+    assert meta.tree.info.n_combine > 0
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = attend(q, *views, meta, SCALE)
+            out2 = attend(q, *views, meta, SCALE)
+        graphs.append((g, out, out2))
+    eager = attend(q, *views, meta, SCALE).clone()
+    ref, bound, covered = attention64(q, *views, chunks, U_BF16)
+    assert_close(eager, ref, bound, covered)
+    for k in (1, 0, 0, 1):
+        g, out, out2 = graphs[k]
+        out.fill_(7.0)
+        out2.fill_(7.0)
+        g.replay()
+        assert torch.equal(out, eager) and torch.equal(out2, eager)
+        assert torch.equal(attend(q, *views, meta, SCALE), eager)
+
+
+@pytest.mark.parametrize("pool", POOLS)
+def test_two_steps_at_once(pool: str, cuda_device) -> None:
+    """Two steps with metadata of their own, on two streams over one pool."""
+    dev = cuda_device
+    rng = random.Random(6)
+    seqs = [(16, 1500, random_tree(rng, 16)), (50, 900, random_tree(rng, 50)), (4, 2000, None)] * 3
+    views, chunks, q = batch(dev, seqs, 4, pool, seed=12)
+    want = check(views, chunks, q, U_BF16, split=16)
+    metas = [build_attention_metadata(chunks, slots_of(chunks, dev), 16, pages_per_split=16)
+             for _ in range(2)]
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    torch.cuda.synchronize(dev)
+    outs = []
+    for _ in range(5):
+        for meta, stream in zip(metas, streams):
+            with torch.cuda.stream(stream):
+                outs.append(attend(q, *views, meta, SCALE))
+    torch.cuda.synchronize(dev)
+    assert all(torch.equal(out, want) for out in outs)

@@ -448,9 +448,9 @@ def kv_gather(slots: Tensor, k_cache: Tensor, v_cache: Tensor, k_out: Tensor | N
     values again.  A slot outside the pool reads as zeros (and sets the device status bit).
     """
     nb, kvh = check_layer_views(k_cache, v_cache, kv8=True)
-    n = int(slots.shape[0]) if slots.dim() == 1 else 0
+    n = slots.shape[0] if slots.dim() == 1 else 0
     if k_out is None:
-        k_out = torch.empty((n, kvh, HEAD_DIM), dtype=torch.bfloat16, device=slots.device)
+        k_out = k_cache.new_empty((n, kvh, HEAD_DIM), dtype=torch.bfloat16)
     if v_out is None:
         v_out = torch.empty_like(k_out)
     dev = _check_rows_args(k_out, v_out, slots, k_cache, kvh)
@@ -499,13 +499,13 @@ def _attend_parts(lib, q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: Attent
     dev = k_cache.device
     if dev.type != "cuda":
         raise RuntimeError("miniserve_b200 attention runs on CUDA only (no CPU fallback)")
-    if q.device != dev or out.device != dev or meta.plan.device != dev:
+    if not (q.device == out.device == meta.plan.device == dev):
         raise ValueError(f"q, out and meta are on {q.device}, {out.device} and {meta.plan.device}, "
                          f"the pool on {dev}")
-    shape = q.shape
-    if shape != out.shape and shape[1:] != out.shape[1:]:
+    shape, oshape = q.shape, out.shape
+    if shape != oshape and shape[1:] != oshape[1:]:
         raise ValueError("out must have q's heads")
-    if shape[0] < meta.num_tokens or out.shape[0] < meta.num_tokens:
+    if shape[0] < meta.num_tokens or oshape[0] < meta.num_tokens:
         raise ValueError(f"q and out must have the step's {meta.num_tokens} rows")
     kv8 = is_kv8(k_cache)
     stream = _stream(dev)

@@ -94,7 +94,7 @@ def _check_kv8_views(k_cache: Tensor, v_cache: Tensor) -> tuple[int, int]:
             "k_cache must be a layer view of miniserve_b200.kv_pool.allocate_kv_cache "
             f"([blocks, kv_heads, 16, 128] of an 8-bit pool); got shape {tuple(shape)}"
         )
-    nb, kvh = int(shape[0]), int(shape[1])
+    nb, kvh = shape[0], shape[1]
     want = (kvh * KV8_PAGE_BYTES, KV8_PAGE_BYTES, HEAD_DIM, 1)
     if k_cache.stride() != want or v_cache.stride() != want:
         raise ValueError(f"KV pool views have strides {k_cache.stride()}, expected {want}")
@@ -111,17 +111,18 @@ def check_layer_views(k_cache: Tensor, v_cache: Tensor, kv8: bool = False) -> tu
         return _check_kv8_views(k_cache, v_cache)
     if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
         raise ValueError("KV pool views must be bf16")
-    if k_cache.dim() != 5 or tuple(k_cache.shape[2:]) != (2, BLOCK_SIZE, HEAD_DIM // 2):
+    shape = k_cache.shape
+    if len(shape) != 5 or shape[2:] != (2, BLOCK_SIZE, HEAD_DIM // 2):
         raise ValueError(
             "k_cache must be a layer view of miniserve_b200.kv_pool.allocate_kv_cache "
-            f"([blocks, kv_heads, 2, 16, 64]); got shape {tuple(k_cache.shape)}"
+            f"([blocks, kv_heads, 2, 16, 64]); got shape {tuple(shape)}"
         )
-    nb, kvh = int(k_cache.shape[0]), int(k_cache.shape[1])
+    nb, kvh = shape[0], shape[1]
     page = BLOCK_SIZE * HEAD_DIM  # elements of one K (or V) page
     want = (kvh * 2 * page, 2 * page, page // 2, HEAD_DIM // 2, 1)
-    if tuple(k_cache.stride()) != want or tuple(v_cache.stride()) != want:
-        raise ValueError(f"KV pool views have strides {tuple(k_cache.stride())}, expected {want}")
-    if v_cache.shape != k_cache.shape or v_cache.data_ptr() != k_cache.data_ptr() + 2 * page:
+    if k_cache.stride() != want or v_cache.stride() != want:
+        raise ValueError(f"KV pool views have strides {k_cache.stride()}, expected {want}")
+    if v_cache.shape != shape or v_cache.data_ptr() != k_cache.data_ptr() + 2 * page:
         raise ValueError("v_cache must be the V half of the same pool as k_cache")
     return nb, kvh
 

@@ -9,7 +9,7 @@
 // the kernel walks instead of the block tables, and the sequence records with their tables' places
 // in it.  To a plan of trees with tensor-core items it adds the tiles that kernel F reads whole in
 // their place: expanding pages that one sequence reads once would write and read four times their
-// bytes (48 trees of 32 drafts over 500-2700 tokens: 145 us with kernel F).
+// bytes (48 trees of 32 drafts over 256-4096 tokens: 131 us with kernel F).
 //
 // ms_tree_plan_build cuts every sequence of drafts into tiles that read the cached context and the
 // drafts up to the tile's last one (a parent precedes its children).  Masks are bit rows, one per
@@ -35,10 +35,12 @@ constexpr int kTileTokens = 32;     // tokens of a wide tile (64 query rows) at 
 constexpr int kNarrowTokens = 16;   // tiles of at most 32 query rows run three CTAs per SM, others two
 // The planner does not see the head count, and only speed depends on it.  Narrow tiles are sized for two
 // CTAs per SM at 8 KV heads: they are bound by memory, which fewer CTAs still keep busy at 4 heads, and
-// more splits only cost merging (3 rows over 100k tokens: 57 us with 36 splits, 70 with 111; 64 trees
-// of 16 drafts: 101 us, 115 when sized for the three CTAs that fit).  Wide
-// tiles are bound by the SMs, so they are sized for 4 heads, two waves at 8 (16 trees of 63 drafts
-// over 4 heads: 180 us sized for 8 heads, 127 for 4).
+// more splits only cost merging (3 rows over 100k tokens: 51 us with 36 splits, 64 with 108; 64 trees
+// of 16 drafts: 98 us, 107 in splits of 128 pages).  Wide tiles are bound by the SMs, so they are sized
+// for 4 heads, two waves at 8 (16 trees of 63 drafts over 4 heads, all of them on wide tiles: 180 us
+// sized for 8 heads, 127 for 4).  Shorter splits than the least ones cost more than they fill (8 decode
+// rows: 16 us in splits of 4 pages, 14 in 8; 48 trees of 32 drafts: 143 us in splits of 80 pages, 139 in
+// 96, 133 in the 128 that the rule takes).
 constexpr int kNarrowHeads = 8, kWideHeads = 4;
 constexpr int kMinSplitPages = 8, kMinWideSplitPages = 96;
 constexpr int kMaxSplitPages = 512;
@@ -69,9 +71,10 @@ struct RowsItem {
   int field6 = 0, field7 = 0;
 };
 
-// Cached whole 128-key blocks of the tiles of larger trees run on the tensor cores: tiles of more
-// than 16 drafts are bound by mma.sync (16 trees of 63 drafts over 4000-8100 tokens: 119 us without
-// this), and those blocks need no mask.  kPrefixMinPages: fewer pages are not worth the second launch.
+// Cached whole 128-key blocks of the tiles of larger trees run on the tensor cores over a bf16 pool: tiles
+// of more than 16 drafts are bound by mma.sync, and those blocks need no mask (16 trees of 63 drafts over
+// 4000-8100 tokens: 117 us without this, 76 with it).  Fewer pages than kPrefixMinPages are not worth the
+// second launch.
 constexpr int kBlockPages = 8;
 constexpr int kPrefixTileTokens = 64;  // 128 query rows
 constexpr int kPrefixMinPages = 32, kPrefixMinSplitPages = 64;

@@ -19,6 +19,7 @@
 #include <cstdint>
 #include <cstring>
 #include <exception>
+#include <functional>
 #include <string>
 #include <vector>
 
@@ -36,14 +37,25 @@ constexpr int kNarrowTokens = 16;   // tiles of at most 32 query rows run three 
 // The planner does not see the head count, and only speed depends on it.  Narrow tiles are sized for two
 // CTAs per SM at 8 KV heads: they are bound by memory, which fewer CTAs still keep busy at 4 heads, and
 // more splits only cost merging (3 rows over 100k tokens: 51 us with 36 splits, 64 with 108; 64 trees
-// of 16 drafts: 98 us, 107 in splits of 128 pages).  Wide tiles are bound by the SMs, so they are sized
-// for 4 heads, two waves at 8 (16 trees of 63 drafts over 4 heads, all of them on wide tiles: 180 us
-// sized for 8 heads, 127 for 4).  Shorter splits than the least ones cost more than they fill (8 decode
-// rows: 16 us in splits of 4 pages, 14 in 8; 48 trees of 32 drafts: 143 us in splits of 80 pages, 139 in
-// 96, 133 in the 128 that the rule takes).
-constexpr int kNarrowHeads = 8, kWideHeads = 4;
-constexpr int kMinSplitPages = 8, kMinWideSplitPages = 96;
+// of 16 drafts: 98 us, 107 in splits of 128 pages; the costs below instead of this rule: 36 trees of 12
+// drafts at 8 heads 81 -> 107 us, 19 of 13 at 4 heads 55 -> 37).  Splits of less than 8 pages cost more than
+// they fill (8 decode rows: 16 us in splits of 4 pages, 14 in 8).  The tiles of tensor-core items are sized
+// for one CTA per SM at 4 heads.
+constexpr int kNarrowHeads = 8, kTensorHeads = 4;
+constexpr int kMinSplitPages = 8;
 constexpr int kMaxSplitPages = 512;
+
+// What wide tiles cost, in microseconds (measured with 1 and 2 CTAs per SM over 64 to 256 pages): a page for a
+// CTA that has its SM to itself, a page of the SM's throughput, and a work item's fixed part (start, first
+// pages, epilogue); an SM holds two.
+constexpr double kWidePageAlone = 0.35, kWidePageSm = 0.26, kWideItem = 9;
+constexpr int kWideCtas = 2;
+// The merge of n splits of `rows` rows: latencies of L2, see merge_splits.
+double merge_cost(int n, int rows) {
+  if (n <= 1) return 0;
+  const int per_warp = (rows + 3) / 4;
+  return 2 + 0.8 * (n <= 4 ? (per_warp + 3) / 4 : (per_warp + 1) / 2 * ((n + 7) / 8));
+}
 
 int64_t round4(int64_t x) { return (x + 3) & ~int64_t(3); }
 
@@ -112,14 +124,83 @@ int fit_split(const std::vector<RowsItem>& tiles, int64_t target, int least) {
   return lo * 8;
 }
 
+// Time of pieces of `len` wide pages (longest first) of h heads each: every SM shares its throughput among
+// the CTAs that it holds, so they are dealt to SMs, the least loaded one next, and no piece is faster than
+// alone.
+double wide_time(const std::vector<int>& len, int h, int num_sms) {
+  const size_t sms = std::max(1, num_sms / h);
+  const double item = kWideItem / kWideCtas;
+  std::vector<double> load;  // a heap, the least loaded SM first
+  load.reserve(sms);
+  double end = len[0] * kWidePageAlone;
+  for (int p : len) {
+    double t = item + p * kWidePageSm;
+    if (load.size() == sms) {
+      std::pop_heap(load.begin(), load.end(), std::greater<double>());
+      t += load.back();
+      load.pop_back();
+    }
+    load.push_back(t);
+    std::push_heap(load.begin(), load.end(), std::greater<double>());
+    end = std::max(end, t);
+  }
+  return end + kWideItem - item;
+}
+
+// Pages per split of wide tiles, which are bound by the SMs.  Many tiles (two waves of 8 heads and more) fill
+// the GPU whole; only those longer than a CTA's share of the pages are cut to about that.  With fewer,
+// the longest tile cut into 1, 2, 3 ... parts, and all others into parts as long, whichever the costs above
+// put first: splits shorten the run, but the last CTA of a tile merges them alone (one tree of 24 drafts
+// over 4000 tokens: 55 us in 3 splits, 35 as chosen here; 48 trees of 32 drafts: 143 us in
+// splits of 80 pages, 133 in the 128 chosen).  4 and 8 heads are weighed, each against its own best.
+int wide_split(const std::vector<RowsItem>& tiles, int num_sms) {
+  constexpr int kHeads[2] = {8, 4};
+  const int64_t slots = static_cast<int64_t>(num_sms) * kWideCtas;
+  int64_t all = 0;
+  int longest = 0;
+  for (const RowsItem& t : tiles) {
+    all += t.pe - t.pb;
+    longest = std::max(longest, t.pe - t.pb);
+  }
+  if (static_cast<int64_t>(tiles.size()) * kHeads[0] >= 2 * slots) {
+    const int64_t share = all * kHeads[1] / slots;
+    return static_cast<int>(std::min<int64_t>(kMaxSplitPages, std::max<int64_t>(96, (share + 7) / 8 * 8)));
+  }
+  constexpr int kParts[] = {1,  2,  3,  4,  5,  6,  7,  8,  10, 12, 14, 16,
+                            20, 24, 28, 32, 36, 40, 48, 56, 64, 96, 128};
+  std::vector<int> split, len;
+  std::vector<double> time[2];
+  for (int parts : kParts) {
+    const int p = std::max(kMinSplitPages, ((longest + parts - 1) / parts + 7) / 8 * 8);
+    if (!split.empty() && p == split.back()) continue;
+    len.clear();
+    double merge = 0;
+    for (const RowsItem& t : tiles) {
+      const int pages = t.pe - t.pb, n = (pages + p - 1) / p;
+      for (int k = 0; k < n; ++k) len.push_back(pages / n + (k < pages % n ? 1 : 0));
+      merge = std::max(merge, merge_cost(n, 2 * t.n_q));
+    }
+    if (!split.empty() && static_cast<int64_t>(len.size()) * kHeads[1] > 2 * slots) break;
+    std::sort(len.begin(), len.end(), std::greater<int>());
+    split.push_back(p);
+    for (int h = 0; h < 2; ++h) time[h].push_back(wide_time(len, kHeads[h], num_sms) + merge);
+  }
+  const double best0 = *std::min_element(time[0].begin(), time[0].end());
+  const double best1 = *std::min_element(time[1].begin(), time[1].end());
+  size_t at = 0;
+  for (size_t i = 1; i < split.size(); ++i)
+    if (time[0][i] / best0 + time[1][i] / best1 < time[0][at] / best0 + time[1][at] / best1) at = i;
+  return split[at];
+}
+
 // Split size of kernel F's narrow or wide tiles.
 int choose_split(const std::vector<RowsItem>& tiles, bool narrow, int num_sms) {
   std::vector<RowsItem> mine;
   for (const RowsItem& t : tiles)
     if ((t.n_q <= kNarrowTokens) == narrow && t.field7 == 0) mine.push_back(t);
-  const int64_t target = narrow ? static_cast<int64_t>(num_sms) * 2 / kNarrowHeads
-                                : static_cast<int64_t>(num_sms) * 2 / kWideHeads;
-  return fit_split(mine, std::max<int64_t>(1, target), narrow ? kMinSplitPages : kMinWideSplitPages);
+  if (mine.empty()) return kMaxSplitPages;
+  if (!narrow) return wide_split(mine, num_sms);
+  return fit_split(mine, std::max(1, num_sms * 2 / kNarrowHeads), kMinSplitPages);
 }
 
 // Splits the tiles (cascade rows and the tails of tensor-core prefixes, field7 != 0, stay whole).
@@ -427,7 +508,7 @@ static int tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const in
     const int split =
         pages_per_split > 0
             ? (pages_per_split + kBlockPages - 1) / kBlockPages * kBlockPages
-            : fit_split(prefix, std::max(1, num_sms / kWideHeads), kPrefixMinSplitPages);
+            : fit_split(prefix, std::max(1, num_sms / kTensorHeads), kPrefixMinSplitPages);
     std::vector<RowsItem> rest;
     for (const RowsItem& t : tiles)
       if (vseq_of[t.seq] < 0) rest.push_back(t);

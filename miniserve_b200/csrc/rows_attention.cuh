@@ -304,6 +304,11 @@ __device__ __forceinline__ void rows_block8(const uint32_t (&page)[kBlockPages],
   const int mi = lane >> 3, t8 = lane & 7, q4 = 4 * (lane & 3);
   const int tok = 4 * (t8 >> 1) + (t8 & 1);  // this lane's ldmatrix row in tile 0
   const int sw = code_swizzle8(tok);         // the same for tok + 2
+  // Unmasked pairs lie side by side in the ring: the second page is an offset in the load.
+  auto at_page = [&](uint32_t addr, int t) {
+    return t == 0 ? addr : addr + (kMask ? page[1] - page[0] : static_cast<uint32_t>(kPage8Bytes));
+  };
+  const uint32_t k_row = page[0] + (tok + 2 * (mi >> 1)) * kRow8Bytes;
   float s[kRG][2 * kBlockPages][4];
 #pragma unroll
   for (int g = 0; g < kRG; ++g) {
@@ -320,15 +325,14 @@ __device__ __forceinline__ void rows_block8(const uint32_t (&page)[kBlockPages],
     for (int g = 0; g < kRG; ++g) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        ldsm_x4(q + g * (16 * kHeadDim * 2) + (((2 * (2 * u + i) + (mi >> 1)) ^ t8) << 4),
+        ldsm_x4((q + (((2 * (2 * u + i) + (mi >> 1)) ^ t8) << 4)) + g * (16 * kHeadDim * 2),
                 qa[g][i][0], qa[g][i][1], qa[g][i][2], qa[g][i][3]);
     }
 #pragma unroll
     for (int t = 0; t < kBlockPages; ++t) {
       // Both key tiles of the page, chunks 2u and 2u + 1.
       uint32_t b[4];
-      ldsm_x4(page[t] + (tok + 2 * (mi >> 1)) * kRow8Bytes + (((2 * u + (mi & 1)) ^ sw) << 4), b[0],
-              b[1], b[2], b[3]);
+      ldsm_x4(at_page(k_row + (((2 * u + (mi & 1)) ^ sw) << 4), t), b[0], b[1], b[2], b[3]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t b0 = e4m3x2_to_f16x2<0>(b[i]), b1 = e4m3x2_to_f16x2<1>(b[i]);
@@ -340,8 +344,8 @@ __device__ __forceinline__ void rows_block8(const uint32_t (&page)[kBlockPages],
   uint32_t vw[kBlockPages];
 #pragma unroll
   for (int t = 0; t < kBlockPages; ++t) {
-    const uint32_t kw = lds32(page[t] + kExp8Off + q4);
-    vw[t] = lds32(page[t] + kExp8Off + kBlockTokens + q4);
+    const uint32_t kw = lds32(at_page(page[0] + kExp8Off + q4, t));
+    vw[t] = lds32(at_page(page[0] + kExp8Off + kBlockTokens + q4, t));
     const float f[4] = {scale_of_byte<0>(kw), scale_of_byte<1>(kw), scale_of_byte<2>(kw),
                         scale_of_byte<3>(kw)};
 #pragma unroll
@@ -398,14 +402,13 @@ __device__ __forceinline__ void rows_block8(const uint32_t (&page)[kBlockPages],
       pa[g][t][3] = pack_f16(s[g][2 * t + 1][2], s[g][2 * t + 1][3]);
     }
   }
-  const int vtok = tok + 2 * (mi & 1);
+  const uint32_t v_row = page[0] + kCodes8Bytes + (tok + 2 * (mi & 1)) * kRow8Bytes;
 #pragma unroll
   for (int t = 0; t < kBlockPages; ++t) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       uint32_t w[4];
-      ldsm_x4_t(page[t] + kCodes8Bytes + vtok * kRow8Bytes + (((2 * u + (mi >> 1)) ^ sw) << 4), w[0],
-                w[1], w[2], w[3]);
+      ldsm_x4_t(at_page(v_row + (((2 * u + (mi >> 1)) ^ sw) << 4), t), w[0], w[1], w[2], w[3]);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t a = w[2 * h], b = w[2 * h + 1];

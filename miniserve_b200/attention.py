@@ -423,17 +423,24 @@ def _check_rows_args(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, kvh: 
     shape = k.shape
     if len(shape) != 3 or shape != v.shape or shape[1] != kvh:
         raise ValueError(f"k and v must both be [T, {kvh}, {HEAD_DIM}]")
-    if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
-        raise ValueError("slots must be a contiguous int64 vector")
-    if slots.shape[0] != shape[0]:
-        raise ValueError(f"{shape[0]} rows but {slots.shape[0]} slots")
+    n = _check_slots(slots)
+    if n != shape[0]:
+        raise ValueError(f"{shape[0]} rows but {n} slots")
     dev = k_cache.device
     if dev.type != "cuda":
         raise RuntimeError("miniserve_b200 attention runs on CUDA only (no CPU fallback)")
-    if k.device != dev or v.device != dev or slots.device != dev:
+    if not (k.device == v.device == slots.device == dev):
         raise ValueError(f"k, v and slots are on {k.device}, {v.device} and {slots.device}, "
                          f"the pool on {dev}")
     return dev
+
+
+def _check_slots(slots: Tensor) -> int:
+    """The length of a vector of slots."""
+    shape = slots.shape
+    if slots.dtype != torch.int64 or len(shape) != 1 or not slots.is_contiguous():
+        raise ValueError("slots must be a contiguous int64 vector")
+    return shape[0]
 
 
 def kv_gather(slots: Tensor, k_cache: Tensor, v_cache: Tensor, k_out: Tensor | None = None,
@@ -448,14 +455,19 @@ def kv_gather(slots: Tensor, k_cache: Tensor, v_cache: Tensor, k_out: Tensor | N
     values again.  A slot outside the pool reads as zeros (and sets the device status bit).
     """
     nb, kvh = check_layer_views(k_cache, v_cache, kv8=True)
-    n = slots.shape[0] if slots.dim() == 1 else 0
+    n = _check_slots(slots)
+    ours = k_out is None and v_out is None
     if k_out is None:
         k_out = k_cache.new_empty((n, kvh, HEAD_DIM), dtype=torch.bfloat16)
     if v_out is None:
         v_out = torch.empty_like(k_out)
-    dev = _check_rows_args(k_out, v_out, slots, k_cache, kvh)
-    outs = (k_out.data_ptr(), _rows(k_out, "k_out"), v_out.data_ptr(), _rows(v_out, "v_out"),
-            _stream(dev))
+    if ours and k_cache.is_cuda and slots.device == k_cache.device:  # rows that need no checking
+        dev = k_cache.device
+        k_stride = v_stride = kvh * HEAD_DIM
+    else:
+        dev = _check_rows_args(k_out, v_out, slots, k_cache, kvh)
+        k_stride, v_stride = _rows(k_out, "k_out"), _rows(v_out, "v_out")
+    outs = (k_out.data_ptr(), k_stride, v_out.data_ptr(), v_stride, _stream(dev))
     lib = _capi.load()
     if is_kv8(k_cache):
         rc = _on_own_device(lib.ms_kv_gather_kv8, dev, slots.data_ptr(), n, kvh, k_cache.data_ptr(),
@@ -475,13 +487,12 @@ def attend(q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: AttentionMetadata,
     Rows not covered by ``meta`` are left untouched (undefined, like ``torch.empty_like``).
     """
     nb, kvh = check_layer_views(k_cache, v_cache, kv8=True)
+    lib = _capi.load()
+    if meta.tree is not None or is_kv8(k_cache):
+        return _attend_parts(lib, q, k_cache, v_cache, meta, float(scale), out, nb, kvh)
     if out is None:
         out = torch.empty_like(q)
     h = int(q.shape[1])
-    lib = _capi.load()
-    if is_kv8(k_cache) or meta.tree is not None:
-        _attend_parts(lib, q, k_cache, v_cache, meta, float(scale), out, nb, kvh)
-        return out
     ws = meta.workspace(kvh, q.device)
     rc = lib.ms_paged_attention(
         q.data_ptr(), _rows(q, "q"), out.data_ptr(), _rows(out, "out"), h, kvh,
@@ -494,22 +505,29 @@ def attend(q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: AttentionMetadata,
 
 
 def _attend_parts(lib, q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: AttentionMetadata,
-                  scale: float, out: Tensor, nb: int, kvh: int) -> None:
+                  scale: float, out: Tensor | None, nb: int, kvh: int) -> Tensor:
     """The causal part and the draft trees of a step, over either kind of pool."""
     dev = k_cache.device
     if dev.type != "cuda":
         raise RuntimeError("miniserve_b200 attention runs on CUDA only (no CPU fallback)")
-    if not (q.device == out.device == meta.plan.device == dev):
-        raise ValueError(f"q, out and meta are on {q.device}, {out.device} and {meta.plan.device}, "
-                         f"the pool on {dev}")
-    shape, oshape = q.shape, out.shape
-    if shape != oshape and shape[1:] != oshape[1:]:
-        raise ValueError("out must have q's heads")
-    if shape[0] < meta.num_tokens or oshape[0] < meta.num_tokens:
-        raise ValueError(f"q and out must have the step's {meta.num_tokens} rows")
+    shape = q.shape
+    q_stride = _rows(q, "q")
+    if not (q.device == meta.plan.device == dev):
+        raise ValueError(f"q and meta are on {q.device} and {meta.plan.device}, the pool on {dev}")
+    if shape[0] < meta.num_tokens:
+        raise ValueError(f"q must have the step's {meta.num_tokens} rows")
+    if out is None:
+        out = torch.empty_like(q)
+        out_stride = out.stride(0)
+    else:
+        out_stride = _rows(out, "out")
+        if out.device != dev:
+            raise ValueError(f"out is on {out.device}, the pool on {dev}")
+        if out.shape[1:] != shape[1:] or out.shape[0] < meta.num_tokens:
+            raise ValueError(f"out must have q's heads and the step's {meta.num_tokens} rows")
     kv8 = is_kv8(k_cache)
     stream = _stream(dev)
-    q_args = (q.data_ptr(), _rows(q, "q"), out.data_ptr(), _rows(out, "out"), int(shape[1]), kvh)
+    q_args = (q.data_ptr(), q_stride, out.data_ptr(), out_stride, shape[1], kvh)
     info, tree = meta.info, meta.tree
     if tree is None or info.n_decode_items or info.n_tile_items or info.n_tc_items:
         ws = meta.workspace(kvh, dev, kv8, kv8)
@@ -535,6 +553,7 @@ def _attend_parts(lib, q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: Attent
                 lib.ms_tree_attention, dev, *q_args, k_cache.data_ptr(), v_cache.data_ptr(), nb,
                 tree.plan.data_ptr(), C.byref(tree.info), *ws_args, scale, stream)
         _capi.check(rc, "paged_attention")
+    return out
 
 
 def paged_attention(

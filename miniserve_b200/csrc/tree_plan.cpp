@@ -50,6 +50,9 @@ constexpr int kMaxSplitPages = 512;
 // pages, epilogue); an SM holds two.
 constexpr double kWidePageAlone = 0.35, kWidePageSm = 0.26, kWideItem = 9;
 constexpr int kWideCtas = 2;
+// Tensor-core items, one per SM, and what follows them: kernel F's last pages and the merge.
+constexpr double kTensorPage = 0.21, kTensorItem = 10, kTensorTail = 18;
+constexpr int kHeads[2] = {8, 4};  // the head counts that times are weighed for
 // The merge of n splits of `rows` rows: latencies of L2, see merge_splits.
 double merge_cost(int n, int rows) {
   if (n <= 1) return 0;
@@ -124,17 +127,15 @@ int fit_split(const std::vector<RowsItem>& tiles, int64_t target, int least) {
   return lo * 8;
 }
 
-// Time of pieces of `len` wide pages (longest first) of h heads each: every SM shares its throughput among
-// the CTAs that it holds, so they are dealt to SMs, the least loaded one next, and no piece is faster than
-// alone.
-double wide_time(const std::vector<int>& len, int h, int num_sms) {
+// Time of pieces of `len` pages (longest first) of h heads each: every SM shares its throughput among the
+// CTAs that it holds, so they are dealt to SMs, the least loaded one next.
+double deal(const std::vector<int>& len, int h, double item, double page, int num_sms) {
   const size_t sms = std::max(1, num_sms / h);
-  const double item = kWideItem / kWideCtas;
   std::vector<double> load;  // a heap, the least loaded SM first
   load.reserve(sms);
-  double end = len[0] * kWidePageAlone;
+  double end = 0;
   for (int p : len) {
-    double t = item + p * kWidePageSm;
+    double t = item + p * page;
     if (load.size() == sms) {
       std::pop_heap(load.begin(), load.end(), std::greater<double>());
       t += load.back();
@@ -144,7 +145,11 @@ double wide_time(const std::vector<int>& len, int h, int num_sms) {
     std::push_heap(load.begin(), load.end(), std::greater<double>());
     end = std::max(end, t);
   }
-  return end + kWideItem - item;
+  return end;
+}
+double wide_time(const std::vector<int>& len, int h, int num_sms) {
+  const double item = kWideItem / kWideCtas;
+  return std::max(len[0] * kWidePageAlone, deal(len, h, item, kWidePageSm, num_sms)) + kWideItem - item;
 }
 
 // Pages per split of wide tiles, which are bound by the SMs.  Many tiles (two waves of 8 heads and more) fill
@@ -153,8 +158,9 @@ double wide_time(const std::vector<int>& len, int h, int num_sms) {
 // put first: splits shorten the run, but the last CTA of a tile merges them alone (one tree of 24 drafts
 // over 4000 tokens: 55 us in 3 splits, 35 as chosen here; 48 trees of 32 drafts: 143 us in
 // splits of 80 pages, 133 in the 128 chosen).  4 and 8 heads are weighed, each against its own best.
-int wide_split(const std::vector<RowsItem>& tiles, int num_sms) {
-  constexpr int kHeads[2] = {8, 4};
+// best: the times of that choice (0 where the tiles are many).
+int wide_split(const std::vector<RowsItem>& tiles, int num_sms, double (&best)[2]) {
+  best[0] = best[1] = 0;
   const int64_t slots = static_cast<int64_t>(num_sms) * kWideCtas;
   int64_t all = 0;
   int longest = 0;
@@ -190,6 +196,8 @@ int wide_split(const std::vector<RowsItem>& tiles, int num_sms) {
   size_t at = 0;
   for (size_t i = 1; i < split.size(); ++i)
     if (time[0][i] / best0 + time[1][i] / best1 < time[0][at] / best0 + time[1][at] / best1) at = i;
+  best[0] = time[0][at];
+  best[1] = time[1][at];
   return split[at];
 }
 
@@ -199,8 +207,34 @@ int choose_split(const std::vector<RowsItem>& tiles, bool narrow, int num_sms) {
   for (const RowsItem& t : tiles)
     if ((t.n_q <= kNarrowTokens) == narrow && t.field7 == 0) mine.push_back(t);
   if (mine.empty()) return kMaxSplitPages;
-  if (!narrow) return wide_split(mine, num_sms);
+  double unused[2];
+  if (!narrow) return wide_split(mine, num_sms, unused);
   return fit_split(mine, std::max(1, num_sms * 2 / kNarrowHeads), kMinSplitPages);
+}
+
+// Whether kernel F alone is faster over trees that could have their cached blocks on the tensor cores: not for
+// trees of more than 32 drafts, whose tiles read the pages twice, but for smaller ones unless they are
+// many or long, since it cuts them into short pieces while the tensor-core kernel is followed by a second one
+// (2 trees of 23 drafts over 1800 tokens: 29 us, 35 with tensor-core items; 51 of 17 over 900: 41 and 57;
+// 61 of 17 over 4000: 86 with them).
+bool wide_is_faster(const std::vector<RowsItem>& tiles, const std::vector<RowsItem>& prefix, int split,
+                    int num_sms) {
+  std::vector<RowsItem> wide;
+  for (const RowsItem& t : tiles)
+    if (t.n_q > kNarrowTokens) wide.push_back(t);
+  std::vector<int> len;
+  for (const RowsItem& t : prefix) {
+    if (t.n_q > kTileTokens || t.tok0 > 0) return false;
+    const int n = (t.pe + split - 1) / split;
+    for (int k = 0; k < n; ++k) len.push_back(t.pe / n);
+  }
+  std::sort(len.begin(), len.end(), std::greater<int>());
+  double best[2], ratio = 0;
+  wide_split(wide, num_sms, best);
+  if (best[0] == 0) return false;
+  for (int h = 0; h < 2; ++h)
+    ratio += best[h] / (deal(len, kHeads[h], kTensorItem, kTensorPage, num_sms) + kTensorTail);
+  return ratio < 2;
 }
 
 // Splits the tiles (cascade rows and the tails of tensor-core prefixes, field7 != 0, stay whole).
@@ -504,11 +538,17 @@ static int tree_plan_build(int32_t num_seqs, const int32_t* flat_start, const in
     for (int t0 = 0; t0 < num_new[i]; t0 += kPrefixTileTokens)
       prefix.push_back({i, t0, std::min(kPrefixTileTokens, num_new[i] - t0), 0, pages});
   }
+  const int split =
+      prefix.empty() ? 0
+      : pages_per_split > 0
+          ? (pages_per_split + kBlockPages - 1) / kBlockPages * kBlockPages
+          : fit_split(prefix, std::max(1, num_sms / kTensorHeads), kPrefixMinSplitPages);
+  if (!prefix.empty() && pages_per_split == 0 && wide_is_faster(tiles, prefix, split, num_sms)) {
+    prefix.clear();
+    vseq_of.assign(num_seqs, -1);
+    n_vseq = 0;
+  }
   if (!prefix.empty()) {
-    const int split =
-        pages_per_split > 0
-            ? (pages_per_split + kBlockPages - 1) / kBlockPages * kBlockPages
-            : fit_split(prefix, std::max(1, num_sms / kTensorHeads), kPrefixMinSplitPages);
     std::vector<RowsItem> rest;
     for (const RowsItem& t : tiles)
       if (vseq_of[t.seq] < 0) rest.push_back(t);

@@ -109,7 +109,7 @@ def _random_parents(rng: random.Random, n: int, unused: int = 0) -> list[int]:
 @pytest.mark.parametrize("split", [0, 1, 3, 40])
 def test_tree_plan_covers_every_page_once(n: int, split: int) -> None:
     """Every tile's pages are read once, by kernel F's items or (the cached whole 128-key blocks of trees
-    of more than 16 drafts over 512 tokens and more) by tensor-core items; the partial rows of a
+    of more than 16 drafts over 512 tokens and more, as the planner chooses) by tensor-core items; the partial rows of a
     combine record are those its items write."""
     rng = random.Random(n)
     chunks, flat, at = [], 0, 7
@@ -122,7 +122,9 @@ def test_tree_plan_covers_every_page_once(n: int, split: int) -> None:
     packed, info = plan_tree_batch(chunks, flat, 16, 148, split)
     assert packed.size == info.total_ints
     count = len(chunks)
-    has_prefix = [n > 16 and c.num_cached >= 512 for c in chunks]
+    # (Without a given split, trees of up to 32 drafts keep their cached blocks where that is faster.)
+    could = n > 16 and (n > 32 or split > 0 or info.n_tc_items > 0)
+    has_prefix = [could and c.num_cached >= 512 for c in chunks]
     seqs = packed[: (count + sum(has_prefix)) * 8].reshape(-1, 8)
     narrow = packed[info.off_decode :][: 8 * info.n_decode_items].reshape(-1, 8)
     wide = packed[info.off_tile :][: 8 * info.n_tile_items].reshape(-1, 8)

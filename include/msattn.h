@@ -161,7 +161,10 @@ MS_API int ms_qkv_proj_norm_rope_scatter(const void* x, int64_t x_row_stride, in
                                   int64_t q_out_row_stride, void* k_cache, void* v_cache,
                                   int32_t num_blocks, void* stream);
 
-/* Scatter only (backends.py:159-160): k, v [T, KVH, 128] with the given row strides. */
+/* Scatter only (backends.py:159-160): k, v [T, KVH, 128] with the given row strides.  The slots of one call
+ * differ from each other.  ms_paged_attention may read rows below a sequence's cached length while the call
+ * before it on the stream still runs, so those are written by an earlier call than the one right before it
+ * (a step that moves accepted drafts does so before it writes its own rows). */
 MS_API int ms_kv_scatter(const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride,
                   int32_t num_tokens, int32_t num_kv_heads, const int64_t* slot_mapping,
                   void* k_cache, void* v_cache, int32_t num_blocks, void* stream);

@@ -315,3 +315,65 @@ def test_two_steps_at_once(pool: str, cuda_device) -> None:
                 outs.append(attend(q, *views, meta, SCALE))
     torch.cuda.synchronize(dev)
     assert all(torch.equal(out, want) for out in outs)
+
+
+@pytest.mark.parametrize("pool", POOLS)
+@pytest.mark.parametrize("n,cached", [(1024, 3), (1024, 530), (1000, 515)])
+def test_the_largest_trees(n: int, cached: int, pool: str, cuda_device) -> None:
+    rng = random.Random(n + cached)
+    seqs = [(n, cached, random_tree(rng, n, unused=rng.choice([0, 9]), back=40)), (3, 40, [-1, 0, 0])]
+    views, chunks, q = batch(cuda_device, seqs, 1, pool, seed=n)
+    check(views, chunks, q, POOLS[pool][1])
+
+
+@pytest.mark.parametrize("pool", POOLS)
+def test_pools_beyond_32_bit_offsets(pool: str, cuda_device) -> None:
+    """The same rows in the first and in the last blocks of a pool of more than 4 GiB: read back and
+    attended (decode, a short and a long chunk, small and larger trees), the results are the same."""
+    dev = cuda_device
+    kvh, rng = 8, random.Random(13)
+    page = 4128 if pool == "e4m3" else 8192
+    blocks = (1 << 32) // (page * kvh) + 200
+    _, layers = allocate_kv_cache(1, blocks, kvh, dev, dtype=POOLS[pool][0])
+    views = layers[0]
+    seqs = [(1, 300, None), (20, 30, None), (90, 40, None), (9, 100, random_tree(rng, 9)),
+            (40, 700, random_tree(rng, 40))]
+    outs, rows = [], []
+    g = torch.Generator(device=dev).manual_seed(13)
+    tokens = sum(n + c for n, c, _ in seqs)
+    k = torch.randn(tokens, kvh, 128, device=dev, generator=g).bfloat16()
+    v = torch.randn(tokens, kvh, 128, device=dev, generator=g).bfloat16()
+    q = torch.randn(sum(n for n, _, _ in seqs), 2 * kvh, 128, device=dev, generator=g).bfloat16()
+    need = sum(-(-(n + c) // 16) for n, c, _ in seqs)
+    assert blocks * page * kvh > 1 << 32 and need < 150
+    for first in (0, blocks - need):
+        at, flat, chunks = first, 0, []
+        for n, c, parents in seqs:
+            nb = -(-(n + c) // 16)
+            chunks.append(SeqChunk(flat, n, c, list(range(at, at + nb)), parents=parents))
+            at += nb
+            flat += n
+        slots = torch.tensor([c.block_table[p // 16] * 16 + p % 16 for c in chunks
+                              for p in range(c.context_len)], device=dev)
+        kv_scatter(k, v, slots, *views)
+        torch.cuda.synchronize(dev)
+        rows.append(kv_gather(slots, *views))
+        meta = build_attention_metadata(chunks, slots_of(chunks, dev), 16)
+        outs.append(attend(q, *views, meta, SCALE))
+    assert torch.equal(outs[0], outs[1]) and not bool(outs[0].isnan().any())
+    assert torch.equal(rows[0][0], rows[1][0]) and torch.equal(rows[0][1], rows[1][1])
+    if pool == "bf16":
+        assert torch.equal(rows[1][0], k) and torch.equal(rows[1][1], v)
+
+
+@pytest.mark.parametrize("pool", POOLS)
+def test_empty_calls(pool: str, cuda_device) -> None:
+    dev = cuda_device
+    _, layers = allocate_kv_cache(1, 2, 2, dev, dtype=POOLS[pool][0])
+    none = torch.empty(0, 2, 128, dtype=torch.bfloat16, device=dev)
+    slots = torch.empty(0, dtype=torch.int64, device=dev)
+    kv_scatter(none, none, slots, *layers[0])
+    assert kv_gather(slots, *layers[0])[0].shape == (0, 2, 128)
+    meta = build_attention_metadata([], slots, 16)
+    q = torch.empty(0, 4, 128, dtype=torch.bfloat16, device=dev)
+    assert attend(q, *layers[0], meta, SCALE).shape == q.shape

@@ -25,10 +25,13 @@
 // largest value.  (mma.sync on e4m3 operands would need no conversion, but it runs at less than
 // half the rate per product here: 256 decode rows took 431 us with K multiplied that way.)
 // The row exponents of K multiply S's columns in fp32; those of V multiply p before it is rounded
-// to f16: p 2^(b - E), with E the largest exponent byte this warp has met (raised only when a page
-// exceeds it by more than 7, as the running maximum is raised only beyond 2^8, so a product stays
-// below 2^15).  f16 keeps 11 bits of p, three more than the bf16 form; what it drops lies 2^-40
-// below the largest p 2^b.
+// to f16, which keeps 11 bits of a product, three more than the bf16 form, as long as it lies between
+// 2^-14 and 2^16.  So O needs a reference of its own.  While the V exponents that a warp meets lie within
+// 10 of each other, it is the running maximum of the scores times one power of two, placed so that
+// p 2^e is at most 2^15 and a row's largest at least 2.  A warp that meets others gives every row a power of
+// two of its own from there on, from the largest s c + e over the keys that the row sees, which holds the
+// row's largest product between 1 and 2^15 whatever the values are (see raise8).  Either way f16's range
+// costs a key at most 2^-25 in units in which the row's largest p 2^e is at least 1.
 //
 // Why this shape.  A decode row needs its bytes and little else: up to 32 rows per CTA, three CTAs per SM
 // at 128 registers (the query rows stay in shared memory and are read again for every pair of pages).
@@ -84,7 +87,8 @@ struct RowsCfg {
   static constexpr int kRows = kRG == 1 ? 32 : 64;
   static constexpr int kQOffset = (kStageBytes + 127) / 128 * 128;
   static constexpr int kScaleOffset = kQOffset + kRows * kHeadDim * 2;  // the rows' query scales
-  static constexpr int kBarOffset = kScaleOffset + kRows * 4;
+  static constexpr int kFactorOffset = kScaleOffset + kRows * 4;  // 8-bit pool: the rows' factors, per warp
+  static constexpr int kBarOffset = kFactorOffset + (kKv8 ? kRowsWarps * 16 * kRG * 4 : 0);
   static constexpr int kSmemBytes = 1024 + kBarOffset + 2 * kStages * 8 + 16;
   // kRG == 1: four consumer warps and a producer warp, three CTAs per SM.  kRG == 2: a consumer
   // warpgroup and a producer warpgroup (one warp of it works), two CTAs per SM launched with 128
@@ -151,64 +155,170 @@ template <int kRG>
 struct RowsState {
   float o[kRG][16][4];
   float m[kRG][2], l[kRG][2];
-  int eb;        // 8-bit pool: the exponent byte E that O is held against
-  float inv_e;   // 2^(127 - E)
-  uint32_t hot;  // E + 7 in every byte (0 while E is unset)
+  // 8-bit pool: what p 2^e is multiplied by before it is rounded, for all rows of the warp, and the middle
+  // of the V exponent bytes that this serves, in every byte (see raise8).
+  float unit;
+  uint32_t mid;
 };
 
-// Raises the running maxima to the block's (mx, in exp2 units) where they exceed them by 2^8, and,
-// for an 8-bit pool, E to the block's largest exponent byte (vw: this thread's exponent words,
-// invisible keys as 0) where that exceeds it by 7; O and l follow.
-template <bool kKv8, int kRG>
-__device__ __forceinline__ void raise(RowsState<kRG>& st, const float (&mx)[kRG][2],
-                                      const uint32_t (&vw)[kBlockPages]) {
+// Multiplies a row's O.
+template <int kRG>
+__device__ __forceinline__ void scale_o(RowsState<kRG>& st, int g, const float (&f)[2]) {
+#pragma unroll
+  for (int n = 0; n < 16; ++n) {
+    st.o[g][n][0] *= f[0];
+    st.o[g][n][1] *= f[0];
+    st.o[g][n][2] *= f[1];
+    st.o[g][n][3] *= f[1];
+  }
+}
+
+// 8-bit pool.  p 2^e is multiplied by a power of two, x = 2^-d, before it is rounded, so O stands for O 2^d.
+// The rows of a warp share x (`unit`) while its V exponent bytes lie within kReach of a middle: p is at
+// most 2^kSlack8 and 2^(e - d) between 2 and 2^(2 kReach + 1), so a product is at most 2^kTop8 and a
+// row's largest at least 2.
+constexpr float kSlack8 = 4.f;
+constexpr int kReach = 5;
+constexpr int kTop8 = 15;
+static_assert(kSlack8 + 2 * kReach + 1 == kTop8, "largest product");
+// Values of `mid` before the first V row that is not zero (unit 0), and once the bytes have spread.
+constexpr uint32_t kUnset = 0, kSpread = 1;
+constexpr int kLeastMid = kReach + 1;
+constexpr int kFirstProduct = 8;  // log2 of what a row's largest product is when its own d is set
+
+// 2^k: 0 below fp32's normal range.
+__device__ __forceinline__ float pow2i(int k) {
+  return k < -126 ? 0.f : __int_as_float((min(k, 127) + kExpBias) << 23);
+}
+
+// Whether one of this thread's V exponent bytes (vw) lies further than kReach from the middle (a carry out
+// of a byte above 133 only adds to what is found).
+template <int kRG>
+__device__ __forceinline__ bool bytes_out(const RowsState<kRG>& st, const uint32_t (&vw)[kBlockPages]) {
+  constexpr uint32_t kOver = (127 - kReach) * 0x01010101u;
+  const uint32_t far0 = __vabsdiffu4(vw[0], st.mid), far1 = __vabsdiffu4(vw[1], st.mid);
+  return st.mid <= kSpread || ((far0 + kOver | far0 | far1 + kOver | far1) & 0x80808080u) != 0;
+}
+template <int kRG>
+__device__ __forceinline__ bool max_up(const RowsState<kRG>& st, const float (&mx)[kRG][2], float slack) {
   bool up = false;
 #pragma unroll
-  for (int g = 0; g < kRG; ++g) up = up || mx[g][0] > st.m[g][0] + 8.f || mx[g][1] > st.m[g][1] + 8.f;
-  // Any byte above E + 7 (an unset E lets everything through).
-  if constexpr (kKv8) up = up || __vcmpgtu4(__vmaxu4(vw[0], vw[1]), st.hot) != 0;
-  if (!__any_sync(0xffffffffu, up)) return;
-  float f = 1.f;
-  if constexpr (kKv8) {
-    // The largest exponent of a finite row (a NaN row's 255 does not move E: it acts through its
-    // infinite factor, and only on the rows that see it).
-    int top = 0;
+  for (int g = 0; g < kRG; ++g) up = up || mx[g][0] > st.m[g][0] + slack || mx[g][1] > st.m[g][1] + slack;
+  return up;
+}
+
+// Sets the middle for a warp that has none, around the block's bytes (but zeros, which any middle serves) with
+// room for 4 larger ones if there is.  False: they have spread already.
+template <int kRG>
+__device__ __forceinline__ bool set_mid(RowsState<kRG>& st, const uint32_t (&vw)[kBlockPages]) {
+  int top = 0, bottom = 255;
 #pragma unroll
-    for (int t = 0; t < kBlockPages; ++t) {
+  for (int t = 0; t < kBlockPages; ++t) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int e = static_cast<int>(vw[t] >> (8 * i) & 255u);
-        top = max(top, e == static_cast<int>(kExpNan) ? 0 : e);
-      }
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (top > st.eb + 7 || st.eb < 0) {
-      const int d = st.eb - top + kExpBias;  // 2^(E_old - E_new); O is still zero when E was unset
-      f = d <= 0 ? 0.f : __int_as_float(d << 23);
-      st.eb = top;
-      st.inv_e = __int_as_float((2 * kExpBias - top) << 23);
-      st.hot = static_cast<uint32_t>(min(top + 7, 255)) * 0x01010101u;
+    for (int i = 0; i < 4; ++i) {
+      const int b = static_cast<int>(vw[t] >> (8 * i) & 255u);
+      top = max(top, b);
+      if (b != 0) bottom = min(bottom, b);
     }
   }
+  top = __reduce_max_sync(0xffffffffu, top);
+  bottom = __reduce_min_sync(0xffffffffu, bottom);
+  if (st.mid != kUnset || top == static_cast<int>(kExpNan) || top - bottom > 2 * kReach) return false;
+  if (top > 0) {
+    const int mid = max(top + min(4, 2 * kReach - (top - bottom)) - kReach, kLeastMid);
+    st.mid = static_cast<uint32_t>(mid) * 0x01010101u;
+    st.unit = pow2i(kExpBias + kReach + 1 - mid);
+  }
+  return true;
+}
+
+// Brings the running maxima up to a block (mx, in exp2 units) where it exceeds them by `slack`; O and l
+// follow.
+template <int kRG>
+__device__ __forceinline__ void raise(RowsState<kRG>& st, const float (&mx)[kRG][2], float slack) {
 #pragma unroll
   for (int g = 0; g < kRG; ++g) {
     float al[2] = {1.f, 1.f};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      if (mx[g][h] > st.m[g][h] + 8.f) {
+      if (mx[g][h] > st.m[g][h] + slack) {
         al[h] = fast_exp2(st.m[g][h] - mx[g][h]);
         st.m[g][h] = mx[g][h];
       }
       st.l[g][h] *= al[h];
-      al[h] *= f;
     }
+    scale_o(st, g, al);
+  }
+}
+
+// The same for a block of an 8-bit pool in the form that serves any bytes: s its scores (invisible keys
+// -infinity), vw this thread's V exponent words, x this thread's first row among its warp's factors in
+// shared memory (all lanes of a quad hold, read and write the same; 0 until a row has one).
+//
+// Once the bytes have spread, every row has a d of its own.  It grows where the block's largest
+// s c - m + e over the keys that the row sees exceeds d + 15, to 8 below it; when m is raised by y, it
+// falls by y rounded up and O keeps its size.  So products stay below 2^15, and a row's largest at least 1.
+// d is whole: values that are held with another exponent, or beside other rows, round alike.  Zero rows
+// (byte 0) and NaN rows (255) are left out: the one adds nothing, the other is NaN at any d.
+template <int kRG>
+__device__ __forceinline__ void raise8(RowsState<kRG>& st, const float (&s)[kRG][2 * kBlockPages][4],
+                                       const float (&c)[kRG][2], const float (&mx)[kRG][2],
+                                       const uint32_t (&vw)[kBlockPages], float* x, int lane) {
+  // Zero bytes, those of scrubbed rows among them, are inside.
+  const uint32_t in[kBlockPages] = {vw[0] | (__vcmpeq4(vw[0], 0u) & st.mid),
+                                    vw[1] | (__vcmpeq4(vw[1], 0u) & st.mid)};
+  const bool out = bytes_out(st, in);
+  if (!__any_sync(0xffffffffu, out || max_up(st, mx, kSlack8))) return;
+  if (st.mid != kSpread && __any_sync(0xffffffffu, out) && !set_mid(st, vw)) {
+    st.mid = kSpread;
 #pragma unroll
-    for (int n = 0; n < 16; ++n) {
-      st.o[g][n][0] *= al[0];
-      st.o[g][n][1] *= al[0];
-      st.o[g][n][2] *= al[1];
-      st.o[g][n][3] *= al[1];
+    for (int g = 0; g < kRG; ++g) x[16 * g] = x[16 * g + 8] = st.unit;
+  }
+  if (st.mid != kSpread) {
+    raise(st, mx, kSlack8);
+    return;
+  }
+#pragma unroll
+  for (int g = 0; g < kRG; ++g) {
+    float al[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float by = mx[g][h] - st.m[g][h];
+      const float old = x[16 * g + 8 * h];
+      int d = kExpBias - (__float_as_int(old) >> 23);
+      al[h] = 1.f;
+      if (by > kSlack8) {
+        st.m[g][h] = mx[g][h];
+        st.l[g][h] *= fast_exp2(-by);
+        const int y = min(static_cast<int>(ceilf(fminf(by, 500.f))), d + 126);
+        al[h] = fast_exp2(static_cast<float>(y) - by);
+        d -= y;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < kBlockPages; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t b = vw[t] >> (8 * i) & 255u;
+          // b - 127 as a float: b in the low bits of 2^23.
+          const float e = b - 1u < kExpNan - 1u ? __uint_as_float(0x4b000000u | b) - (8388608.f + kExpBias)
+                                                : -INFINITY;
+          top = fmaxf(top, __fmaf_rn(s[g][2 * t + (i >> 1)][2 * h + (i & 1)], c[g][h], e));
+        }
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      top -= st.m[g][h];
+      if (old == 0.f ? top > -INFINITY : top > static_cast<float>(d + kTop8)) {
+        const int grown = static_cast<int>(ceilf(fminf(top, 200.f))) - kFirstProduct;
+        al[h] = old == 0.f ? 1.f : al[h] * pow2i(d - grown);
+        d = grown;
+        x[16 * g + 8 * h] = pow2i(-d);
+      } else if (old != 0.f) {
+        x[16 * g + 8 * h] = pow2i(-d);
+      }
     }
+    scale_o(st, g, al);
   }
 }
 
@@ -297,10 +407,12 @@ __device__ __forceinline__ void scrub_keys(uint32_t dead, uint32_t v, bool kv8, 
 // keys of a page are neighbours (4 (lane % 4) .. + 3) and their exponent bytes one word.  Accumulator
 // tile 2u + p holds columns 16u + 2j + p, so a thread's o[2u][0], o[2u + 1][0], o[2u][1],
 // o[2u + 1][1] are four neighbouring columns.
+// The unmasked form serves the common unit only: it returns false, with nothing done, for a block whose V
+// exponents leave it.
 template <int kRG, bool kMask>
-__device__ __forceinline__ void rows_block8(const uint32_t (&page)[kBlockPages], uint32_t q,
+__device__ __forceinline__ bool rows_block8(const uint32_t (&page)[kBlockPages], uint32_t q,
                                             RowsState<kRG>& st, const float (&c)[kRG][2],
-                                            const uint32_t (&vis)[kRG][2], int lane) {
+                                            const uint32_t (&vis)[kRG][2], float* x_rows, int lane) {
   const int mi = lane >> 3, t8 = lane & 7, q4 = 4 * (lane & 3);
   const int tok = 4 * (t8 >> 1) + (t8 & 1);  // this lane's ldmatrix row in tile 0
   const int sw = code_swizzle8(tok);         // the same for tok + 2
@@ -368,25 +480,46 @@ __device__ __forceinline__ void rows_block8(const uint32_t (&page)[kBlockPages],
     mx[g][0] *= c[g][0];
     mx[g][1] *= c[g][1];
   }
-  raise<true, kRG>(st, mx, vw);
+  if constexpr (kMask) {
+    raise8(st, s, c, mx, vw, x_rows, lane);
+  } else {
+    const bool out = bytes_out(st, vw);
+    if (__any_sync(0xffffffffu, out || max_up(st, mx, kSlack8))) {
+      if (__any_sync(0xffffffffu, out) && !set_mid(st, vw)) return false;
+      raise(st, mx, kSlack8);
+    }
+  }
 #pragma unroll
   for (int g = 0; g < kRG; ++g) block_exp(s[g], c[g], st.m[g], st.l[g]);
-  // p times the factor of its V row.  A NaN row's factor is infinite, and infinity times its zero
-  // codes NaN; where p is 0 because the row does not see the key, the product is NaN too early and the
-  // maximum makes it 0.  (A NaN p shows in l.)
+  // p times the scale of its V row and the row's factor.  A NaN row's scale is infinite, and infinity
+  // times its zero codes NaN; what a row does not see is 0 whatever the scale.
 #pragma unroll
   for (int t = 0; t < kBlockPages; ++t) {
-    const float f[4] = {scale_of_byte<0>(vw[t]) * st.inv_e, scale_of_byte<1>(vw[t]) * st.inv_e,
-                        scale_of_byte<2>(vw[t]) * st.inv_e, scale_of_byte<3>(vw[t]) * st.inv_e};
+    const float unit = kMask ? 1.f : st.unit;
+    const float f[4] = {scale_of_byte<0>(vw[t]) * unit, scale_of_byte<1>(vw[t]) * unit,
+                        scale_of_byte<2>(vw[t]) * unit, scale_of_byte<3>(vw[t]) * unit};
 #pragma unroll
     for (int g = 0; g < kRG; ++g) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         s[g][2 * t][i] *= f[i & 1];
         s[g][2 * t + 1][i] *= f[2 + (i & 1)];
-        if constexpr (kMask) {
-          s[g][2 * t][i] = fmaxf(s[g][2 * t][i], 0.f);
-          s[g][2 * t + 1][i] = fmaxf(s[g][2 * t + 1][i], 0.f);
+      }
+    }
+  }
+  if constexpr (kMask) {
+#pragma unroll
+    for (int g = 0; g < kRG; ++g) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float x = st.mid == kSpread ? x_rows[16 * g + 8 * h] : st.unit;
+#pragma unroll
+        for (int t = 0; t < kBlockPages; ++t) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float& w = s[g][2 * t + (i >> 1)][2 * h + (i & 1)];
+            w = sees<2>(vis[g][h], t, q4, i) ? w * x : 0.f;
+          }
         }
       }
     }
@@ -426,6 +559,7 @@ __device__ __forceinline__ void rows_block8(const uint32_t (&page)[kBlockPages],
       }
     }
   }
+  return true;
 }
 
 // ---- two pages, bf16 pool -----------------------------------------------------------------------
@@ -475,8 +609,7 @@ __device__ __forceinline__ void rows_block16(const uint32_t (&page)[kBlockPages]
     mx[g][0] *= c[g][0];
     mx[g][1] *= c[g][1];
   }
-  const uint32_t none[kBlockPages] = {};
-  raise<false, kRG>(st, mx, none);
+  if (__any_sync(0xffffffffu, max_up(st, mx, 8.f))) raise(st, mx, 8.f);
 #pragma unroll
   for (int g = 0; g < kRG; ++g) block_exp(s[g], c[g], st.m[g], st.l[g]);
 #pragma unroll
@@ -891,9 +1024,10 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
     st.m[g][0] = st.m[g][1] = -INFINITY;
     st.l[g][0] = st.l[g][1] = 0.f;
   }
-  st.eb = -1000;
-  st.inv_e = 0.f;
-  st.hot = 0;
+  st.unit = 0.f;
+  st.mid = kUnset;
+  // This thread's first row among its warp's factors (see raise8).
+  float* const x_rows = reinterpret_cast<float*>(smem + Cfg::kFactorOffset) + warp * 16 * kRG + (lane >> 2);
   // First key position that some row of the warp may not see.
   const int first_masked = kTree ? num_cached : num_cached + tok0 + (row_base >> 1) + 1;
   const uint32_t ring_u32 = smem_u32(ring);
@@ -914,8 +1048,9 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
     }
     return false;
   };
-  // Whole pairs whose keys every row sees, then the rest (the end of the tile's pages), with masks:
-  // what only the rest needs is kept out of the registers of the first loop.
+  // Whole pairs whose keys every row sees, then the rest (the end of the tile's pages, and in an 8-bit pool
+  // everything from a pair on whose V exponents spread), with masks: what only the rest needs is kept out
+  // of the registers of the first loop.
   const int n_full = min(npages & ~(kBlockPages - 1),
                          max(0, first_masked - page_begin * kBlockTokens) / (kBlockPages * kBlockTokens) * kBlockPages);
   int j = phase * kBlockPages;
@@ -926,10 +1061,11 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
       const uint32_t page[kBlockPages] = {ring_u32 + (j % kStages) * Cfg::kPage,
                                           ring_u32 + (j % kStages + 1) * Cfg::kPage};
       const uint32_t vis[kRG][2] = {};
-      if constexpr (kKv8)
-        rows_block8<kRG, false>(page, q_row, st, c, vis, lane);
-      else
+      if constexpr (kKv8) {
+        if (!rows_block8<kRG, false>(page, q_row, st, c, vis, x_rows, lane)) break;
+      } else {
         rows_block16<kRG, false>(page, q_row, st, c, vis, lane);
+      }
     }
     __syncwarp();
     if (lane < kBlockPages) mbar_arrive(&empty[(j + lane) % kStages]);
@@ -1021,7 +1157,7 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
       }
       if (run) {
         if constexpr (kKv8)
-          rows_block8<kRG, true>(page, q_row, st, c, vis, lane);
+          rows_block8<kRG, true>(page, q_row, st, c, vis, x_rows, lane);
         else
           rows_block16<kRG, true>(page, q_row, st, c, vis, lane);
       }
@@ -1030,7 +1166,6 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
     if (lane < cnt) mbar_arrive(&empty[(j + lane) % kStages]);
   }
 
-  const float fe = st.eb < 0 ? 0.f : scale8(st.eb);  // O back to the values the codes stand for
 #pragma unroll
   for (int g = 0; g < kRG; ++g) {
 #pragma unroll
@@ -1038,12 +1173,14 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
       st.l[g][h] += __shfl_xor_sync(0xffffffffu, st.l[g][h], 1);
       st.l[g][h] += __shfl_xor_sync(0xffffffffu, st.l[g][h], 2);
     }
-    if constexpr (kKv8) {
+    if constexpr (kKv8) {  // O back to the values the codes stand for
+      float back[2];
 #pragma unroll
-      for (int n = 0; n < 16; ++n) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) st.o[g][n][i] *= fe;
+      for (int h = 0; h < 2; ++h) {
+        const float x = st.mid == kSpread ? x_rows[16 * g + 8 * h] : st.unit;
+        back[h] = x == 0.f ? 0.f : __int_as_float((2 * kExpBias << 23) - __float_as_int(x));
       }
+      scale_o(st, g, back);
     }
   }
 

@@ -80,7 +80,12 @@ class AttentionMetadata:
     _workspace: dict[tuple[torch.device, int], Tensor] = field(default_factory=dict, repr=False)
     _num_sms: int = field(default=148, repr=False)
     _pages_per_split: int = field(default=0, repr=False)
-    kv8: _capi.MsKv8Info = field(default_factory=_capi.MsKv8Info, repr=False)  # 8-bit pool part
+    # The plan's part for 8-bit pools: its description, and the device plan with it behind (None: not
+    # built for the present step).  Once a call has used it, a captured graph may hold it.
+    kv8: _capi.MsKv8Info | None = field(default=None, repr=False)
+    _plan8: Tensor | None = field(default=None, repr=False)
+    _kv8_used: bool = field(default=False, repr=False)
+    _packed: np.ndarray | None = field(default=None, repr=False)  # the plan on the host, without it
     # The sequences whose new tokens are trees of drafts, planned apart (None: there are none).
     tree: AttentionMetadata | None = field(default=None, repr=False)
 
@@ -94,28 +99,69 @@ class AttentionMetadata:
         last pages), its plan and, if given, its slot mapping are copied into the existing buffers
         on the current stream (after the work already queued there, so no kernel of the previous
         step sees them) and True is returned.  Otherwise nothing changes and False is returned:
-        build new metadata and capture again.  No reference counterpart (MiniServe captures no
-        graphs).
+        build new metadata and capture again.  What a launch over an 8-bit pool adds to the shape
+        (the pages that its tensor-core items read) counts once this metadata has been used for one.
+        No reference counterpart (MiniServe captures no graphs).
         """
         if slot_mapping is not None and tuple(slot_mapping.shape) != tuple(self.slot_mapping.shape):
             return False
         plain, trees = _split_trees(chunks)
-        packed, info, kv8 = _plan_with_kv8(plain, self.num_tokens, self._num_sms,
-                                           self._pages_per_split)
-        if not same_launch_shape(info, self.info) or bytes(kv8) != bytes(self.kv8):
-            return False
         if bool(trees) != (self.tree is not None):
             return False
+        new = [(self, self._replan(plain))]
         if self.tree is not None:
-            tpacked, tinfo, tkv8 = _plan_trees(trees, self.num_tokens, self._num_sms,
-                                               self._pages_per_split, _capi.MsKv8Info())
-            if not same_launch_shape(tinfo, self.tree.info) or bytes(tkv8) != bytes(self.tree.kv8):
-                return False
-            self.tree.plan.copy_(torch.from_numpy(tpacked).pin_memory(), non_blocking=True)
-        self.plan.copy_(torch.from_numpy(packed).pin_memory(), non_blocking=True)
+            new.append((self.tree, self.tree._replan(trees)))
+        if any(plan is None for _, plan in new):
+            return False
+        for meta, plan in new:
+            meta._write(*plan)
         if slot_mapping is not None and slot_mapping.data_ptr() != self.slot_mapping.data_ptr():
             self.slot_mapping.copy_(slot_mapping, non_blocking=True)
         return True
+
+    def _replan(self, chunks: list[SeqChunk]
+                ) -> tuple[np.ndarray, _capi.MsPlanInfo, _capi.MsKv8Info | None] | None:
+        """The plan of a new step, or None if it launches differently.  A part for 8-bit pools that
+        launches differently is left out where no call has used it: the next one builds it anew."""
+        kv8 = None if self.kv8 is None else _capi.MsKv8Info()
+        if self.info.is_tree:
+            packed, info, kv8 = _plan_trees(chunks, self.num_tokens, self._num_sms,
+                                            self._pages_per_split, kv8)
+        else:
+            packed, info, kv8 = _plan(chunks, self.num_tokens, BLOCK_SIZE, self._num_sms,
+                                      self._pages_per_split, kv8)
+        if not same_launch_shape(info, self.info):
+            return None
+        if kv8 is not None and (bytes(kv8) != bytes(self.kv8)
+                                or info.n_tc_combine != self.info.n_tc_combine):
+            if self._kv8_used:
+                return None
+            packed, kv8 = packed[: info.total_ints], None
+        return packed, info, kv8
+
+    def _write(self, packed: np.ndarray, info: _capi.MsPlanInfo, kv8: _capi.MsKv8Info | None) -> None:
+        """A plan of the same launch shape into this metadata's buffers."""
+        base = int(info.total_ints)
+        host = torch.from_numpy(packed).pin_memory()
+        if kv8 is not None:
+            self._plan8.copy_(host, non_blocking=True)
+        if self._plan8 is not self.plan or kv8 is None:
+            self.plan[:base].copy_(host[:base], non_blocking=True)
+        if kv8 is None:
+            self._plan8 = None
+        self.info, self.kv8, self._packed = info, kv8, packed[:base]
+
+    def for_kv8(self) -> tuple[Tensor, _capi.MsKv8Info]:
+        """The device plan with its part for 8-bit pools, and that part's description."""
+        if self.kv8 is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the step has no plan for 8-bit pools since it was updated: call it "
+                                   "once before it is captured")
+            packed, self.kv8 = _add_kv8(self._packed, self.info, self._num_sms,
+                                        self._pages_per_split)
+            self._plan8 = _upload_plan(packed, self.plan.device)
+        self._kv8_used = True
+        return self._plan8, self.kv8
 
     def workspace(self, num_kv_heads: int, device: torch.device, kv8: bool = False,
                   counters: bool = False) -> Tensor | None:
@@ -129,8 +175,8 @@ class AttentionMetadata:
         if ws is not None:
             return ws
         if kv8:
-            need = int(_capi.load().ms_kv8_workspace_bytes(C.byref(self.info), C.byref(self.kv8),
-                                                           num_kv_heads))
+            need = int(_capi.load().ms_kv8_workspace_bytes(
+                C.byref(self.info), C.byref(self.for_kv8()[1]), num_kv_heads))
         else:
             need = int(self.info.workspace_bytes_per_kv_head) * num_kv_heads
         if need == 0:
@@ -209,6 +255,25 @@ def _plan(chunks: list[SeqChunk], num_tokens: int, block_size: int, num_sms: int
                                C.byref(kv8))
     _capi.check(rc, "build_attention_metadata")
     return out[: kv8.total_ints], info, kv8
+
+
+def _add_kv8(packed: np.ndarray, info: _capi.MsPlanInfo, num_sms: int, pages_per_split: int
+             ) -> tuple[np.ndarray, _capi.MsKv8Info]:
+    """A packed plan with the part for 8-bit pools behind it."""
+    lib = _capi.load()
+    n = int(info.num_seqs)
+    seqs = packed[info.off_seqs :][: 8 * n].reshape(n, 8)  # fields 1 and 5: new tokens, table length
+    new = np.ascontiguousarray(seqs[:, 1])
+    entries = int(seqs[:, 5].sum(dtype=np.int64))
+    more = (lib.ms_tree_plan_capacity(n, new.ctypes.data, entries) if info.is_tree
+            else lib.ms_kv8_plan_capacity(n, entries))
+    out = np.empty(packed.size + int(more), dtype=np.int32)
+    out[: packed.size] = packed
+    kv8 = _capi.MsKv8Info()
+    rc = lib.ms_kv8_plan_build(out.ctypes.data, out.size, C.byref(info), num_sms, pages_per_split,
+                               C.byref(kv8))
+    _capi.check(rc, "build_attention_metadata")
+    return out[: kv8.total_ints], kv8
 
 
 def plan_tree_batch(
@@ -339,27 +404,31 @@ def build_attention_metadata(
         raise ValueError(f"block_size must be {BLOCK_SIZE}")
     num_tokens = int(slot_mapping.shape[0])
     plain, trees = _split_trees(chunks)
-    packed, info, kv8 = _plan_with_kv8(plain, num_tokens, num_sms, pages_per_split)
     slots = slot_mapping if slot_mapping.dtype == torch.int64 else slot_mapping.to(torch.int64)
     slots = slots.contiguous()
-    tree = None
+
+    def metadata(packed: np.ndarray, info: _capi.MsPlanInfo, kv8: _capi.MsKv8Info
+                 ) -> AttentionMetadata:
+        plan = _upload_plan(packed, device)
+        return AttentionMetadata(slots, plan, info, num_tokens, _num_sms=num_sms,
+                                 _pages_per_split=pages_per_split, kv8=kv8, _plan8=plan,
+                                 _packed=packed[: info.total_ints])
+
+    meta = metadata(*_plan_with_kv8(plain, num_tokens, num_sms, pages_per_split))
     if trees:
-        tpacked, tinfo, tkv8 = _plan_trees(trees, num_tokens, num_sms, pages_per_split,
-                                           _capi.MsKv8Info())
-        tree = AttentionMetadata(slots, _upload_plan(tpacked, device), tinfo, num_tokens,
-                                 _num_sms=num_sms, _pages_per_split=pages_per_split, kv8=tkv8)
-    return AttentionMetadata(slots, _upload_plan(packed, device), info, num_tokens,
-                             _num_sms=num_sms, _pages_per_split=pages_per_split, kv8=kv8,
-                             tree=tree)
+        meta.tree = metadata(*_plan_trees(trees, num_tokens, num_sms, pages_per_split,
+                                          _capi.MsKv8Info()))
+    return meta
 
 
 def same_launch_shape(a: _capi.MsPlanInfo, b: _capi.MsPlanInfo) -> bool:
     """Whether two plans launch the same kernels with the same arguments apart from the plan's
     contents: every field of the plan description is equal except the total page count (a
-    statistic no launch reads)."""
+    statistic no launch reads) and the count of tensor-core combine records, which only a launch
+    over an 8-bit pool reads (``AttentionMetadata.update`` compares it for those)."""
     return all(getattr(a, name) == getattr(b, name)
                for name, _ in _capi.MsPlanInfo._fields_
-               if name not in ("total_pages", "reserved"))
+               if name not in ("total_pages", "n_tc_combine", "reserved"))
 
 
 def _upload_plan(packed: np.ndarray, device: torch.device) -> Tensor:
@@ -530,24 +599,28 @@ def _attend_parts(lib, q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: Attent
     q_args = (q.data_ptr(), q_stride, out.data_ptr(), out_stride, shape[1], kvh)
     info, tree = meta.info, meta.tree
     if tree is None or info.n_decode_items or info.n_tile_items or info.n_tc_items:
+        if kv8:
+            plan8, info8 = meta.for_kv8()
         ws = meta.workspace(kvh, dev, kv8, kv8)
         ws_args = (0, 0) if ws is None else (ws.data_ptr(), ws.numel())
         if kv8:
             rc = _on_own_device(
                 lib.ms_paged_attention_kv8, dev, *q_args, k_cache.data_ptr(), nb,
-                meta.plan.data_ptr(), C.byref(info), C.byref(meta.kv8), *ws_args, scale, stream)
+                plan8.data_ptr(), C.byref(info), C.byref(info8), *ws_args, scale, stream)
         else:
             rc = _on_own_device(
                 lib.ms_paged_attention, dev, *q_args, k_cache.data_ptr(), v_cache.data_ptr(), nb,
                 meta.plan.data_ptr(), C.byref(info), *ws_args, scale, stream)
         _capi.check(rc, "paged_attention")
     if tree is not None:
+        if kv8:
+            plan8, info8 = tree.for_kv8()
         ws = tree.workspace(kvh, dev, kv8, True)
         ws_args = (0, 0) if ws is None else (ws.data_ptr(), ws.numel())
         if kv8:
             rc = _on_own_device(
                 lib.ms_tree_attention_kv8, dev, *q_args, k_cache.data_ptr(), nb,
-                tree.plan.data_ptr(), C.byref(tree.info), C.byref(tree.kv8), *ws_args, scale, stream)
+                plan8.data_ptr(), C.byref(tree.info), C.byref(info8), *ws_args, scale, stream)
         else:
             rc = _on_own_device(
                 lib.ms_tree_attention, dev, *q_args, k_cache.data_ptr(), v_cache.data_ptr(), nb,

@@ -32,7 +32,7 @@ import torch
 from torch import Tensor
 
 from . import _capi
-from .kv_pool import BLOCK_SIZE, HEAD_DIM, check_layer_views, is_kv8
+from .kv_pool import BLOCK_SIZE, HEAD_DIM, check_layer_views, is_kv8, kv8_in_use
 
 SHORT_QUERY = 8  # rows with at most this many new tokens take the decode kernel
 MAX_GATHER_TOKENS = 16384  # kept for the runner's profiler; nothing is gathered here
@@ -155,8 +155,9 @@ class AttentionMetadata:
         """The device plan with its part for 8-bit pools, and that part's description."""
         if self.kv8 is None:
             if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("the step has no plan for 8-bit pools since it was updated: call it "
-                                   "once before it is captured")
+                raise RuntimeError("the step has no plan for 8-bit pools (it was planned before the "
+                                   "process had one, or updated since): call it once before it is "
+                                   "captured")
             packed, self.kv8 = _add_kv8(self._packed, self.info, self._num_sms,
                                         self._pages_per_split)
             self._plan8 = _upload_plan(packed, self.plan.device)
@@ -397,7 +398,10 @@ def build_attention_metadata(
     *,
     pages_per_split: int = 0,
 ) -> AttentionMetadata:
-    """Plan one step and upload it (one pinned H2D copy, no sync).  backends.py:80-98."""
+    """Plan one step and upload it (one pinned H2D copy, no sync).  backends.py:80-98.
+
+    The plan serves bf16 pools, and 8-bit ones once the process has allocated one; a step planned before
+    that gets their part with its first call over one."""
     device = slot_mapping.device
     num_sms = _num_sms(device)  # raises for a non-CUDA device: there is no CPU path
     if block_size != BLOCK_SIZE:
@@ -407,17 +411,20 @@ def build_attention_metadata(
     slots = slot_mapping if slot_mapping.dtype == torch.int64 else slot_mapping.to(torch.int64)
     slots = slots.contiguous()
 
-    def metadata(packed: np.ndarray, info: _capi.MsPlanInfo, kv8: _capi.MsKv8Info
+    def part() -> _capi.MsKv8Info | None:
+        return _capi.MsKv8Info() if kv8_in_use() else None
+
+    def metadata(packed: np.ndarray, info: _capi.MsPlanInfo, kv8: _capi.MsKv8Info | None
                  ) -> AttentionMetadata:
         plan = _upload_plan(packed, device)
         return AttentionMetadata(slots, plan, info, num_tokens, _num_sms=num_sms,
-                                 _pages_per_split=pages_per_split, kv8=kv8, _plan8=plan,
+                                 _pages_per_split=pages_per_split, kv8=kv8,
+                                 _plan8=None if kv8 is None else plan,
                                  _packed=packed[: info.total_ints])
 
-    meta = metadata(*_plan_with_kv8(plain, num_tokens, num_sms, pages_per_split))
+    meta = metadata(*_plan(plain, num_tokens, BLOCK_SIZE, num_sms, pages_per_split, part()))
     if trees:
-        meta.tree = metadata(*_plan_trees(trees, num_tokens, num_sms, pages_per_split,
-                                          _capi.MsKv8Info()))
+        meta.tree = metadata(*_plan_trees(trees, num_tokens, num_sms, pages_per_split, part()))
     return meta
 
 

@@ -47,6 +47,15 @@ def kv8_bytes_per_token(num_layers: int, num_kv_heads: int) -> int:
     return 2 * num_layers * num_kv_heads * (HEAD_DIM + 1)
 
 
+_kv8_allocated = False
+
+
+def kv8_in_use() -> bool:
+    """Whether this process has allocated an 8-bit pool: steps are then planned for both kinds of
+    pool, else for bf16 ones only (a step of cascade groups takes a tenth less to plan and upload)."""
+    return _kv8_allocated
+
+
 def allocate_kv_cache(
     num_layers: int,
     num_blocks: int,
@@ -64,6 +73,8 @@ def allocate_kv_cache(
     every function that takes a layer's views takes either kind, except the fused projection.
     """
     if dtype == KV8:
+        global _kv8_allocated
+        _kv8_allocated = True
         raw = (torch.zeros if zero else torch.empty)(
             (num_layers, num_blocks, num_kv_heads, KV8_PAGE_BYTES), dtype=torch.uint8,
             device=device)

@@ -136,3 +136,46 @@ def test_trees_follow_the_same_rule(cuda_device) -> None:
     check(q, bf16, step(780), meta)
     assert meta.update(step(781))
     check(q, kv8, step(781), meta)
+
+
+@pytest.mark.parametrize("trees", [False, True])
+def test_a_process_without_8_bit_pools_plans_none(trees: bool, cuda_device, monkeypatch) -> None:
+    """Neither planned nor uploaded, nor added by an update; the first 8-bit call adds it, which a capture
+    cannot."""
+    from miniserve_b200 import kv_pool
+
+    dev = cuda_device
+    bf16, kv8 = pools(dev)
+    monkeypatch.setattr(kv_pool, "_kv8_allocated", False)
+    parents = [-1] + [i // 2 for i in range(39)]
+
+    def step(i: int) -> list[SeqChunk]:
+        if not trees:
+            return prefill(i, 3)
+        return [SeqChunk(0, 40, 780 + i, list(range(60)), parents=parents),
+                SeqChunk(40, 1, 3000, [i % 7] * 188)]
+
+    n = sum(c.num_new for c in step(1))
+    q = queries(dev, n)
+    slots = torch.zeros(n, dtype=torch.int64, device=dev)
+    meta = build_attention_metadata(step(1), slots, 16)
+    metas = [meta] if meta.tree is None else [meta, meta.tree]
+    assert all(m.kv8 is None and m.plan.numel() == m.info.total_ints for m in metas)
+    check(q, bf16, step(1), meta)
+    assert meta.update(step(2)) and all(m.kv8 is None for m in metas)
+    torch.cuda.synchronize(dev)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before it is captured"):
+        with torch.cuda.graph(graph):
+            attend(q, *kv8, meta, SCALE)
+    check(q, kv8, step(2), meta)
+    torch.cuda.synchronize(dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attend(q, *kv8, meta, SCALE)
+    swapped = [SeqChunk(c.flat_start, c.num_new, c.num_cached, c.block_table[::-1], c.parents)
+               for c in step(2)]
+    assert meta.update(swapped)
+    graph.replay()
+    check(q, kv8, swapped, meta, out)
+    check(q, bf16, swapped, meta)

@@ -184,6 +184,8 @@ static_assert(kSlack8 + 2 * kReach + 1 == kTop8, "largest product");
 // Values of `mid` before the first V row that is not zero (unit 0), and once the bytes have spread.
 constexpr uint32_t kUnset = 0, kSpread = 1;
 constexpr int kLeastMid = kReach + 1;
+// Beyond this 2^d a row's sums may leave fp32 (products below 2^15, codes below 2^9, up to 2^30 keys).
+constexpr float kLargeBack = 9.223372036854775808e18f;  // 2^63
 constexpr int kFirstProduct = 8;  // log2 of what a row's largest product is when its own d is set
 
 // 2^k: 0 below fp32's normal range.
@@ -720,7 +722,7 @@ __device__ __forceinline__ void merge_rows(const AttnArgs& a, const float* top, 
     const float* o = a.ws_o + first * kHeadDim + lane * 4;
     const int my_h = min(wh, n_r - 1);
     const float* lse = a.ws_lse + first + my_h * row_step;
-    const float m = top[r0 + my_h * kRowsWarps];
+    const float m = top[r0 + my_h * kRowsWarps], inv = top[rows + r0 + my_h * kRowsWarps];
     float4 acc[kR] = {};
 #pragma unroll 1
     for (int s = 0; s < n_splits; s += kS) {
@@ -736,7 +738,7 @@ __device__ __forceinline__ void merge_rows(const AttnArgs& a, const float* top, 
                 o + ((s + i) * split_rows + h * row_step) * kHeadDim));
         }
       }
-      const float w = w_lse == -INFINITY ? 0.f : fast_exp2(w_lse - m);
+      const float w = (w_lse == -INFINITY ? 0.f : fast_exp2(w_lse - m)) * inv;
 #pragma unroll
       for (int i = 0; i < kS; ++i) {
 #pragma unroll
@@ -753,21 +755,19 @@ __device__ __forceinline__ void merge_rows(const AttnArgs& a, const float* top, 
     for (int h = 0; h < kR; ++h) {
       if (h >= n_r) break;
       const int r = r0 + h * kRowsWarps, tok = tok0 + (r >> 1);
-      const float inv = top[rows + r];
       const bool live = masks == nullptr ||
                         (masks[static_cast<long long>(r >> 1) * words + (tok >> 5)] >> (tok & 31) & 1);
       __nv_bfloat16* dst = a.out + static_cast<long long>(flat_tok + (r >> 1)) * a.out_row_stride +
                            (kvh * kGroup + (r & 1)) * kHeadDim + lane * 4;
       *reinterpret_cast<uint2*>(dst) =
-          live ? make_uint2(pack_bf16(acc[h].x * inv, acc[h].y * inv),
-                            pack_bf16(acc[h].z * inv, acc[h].w * inv))
+          live ? make_uint2(pack_bf16(acc[h].x, acc[h].y), pack_bf16(acc[h].z, acc[h].w))
                : make_uint2(0u, 0u);
     }
   }
 }
 
-// The last CTA of a split tile merges the splits' partial rows: out = sum_s 2^(lse_s - M) O_s /
-// sum_s 2^(lse_s - M), s in order, so the result does not depend on which CTA came last.  It runs alone
+// The last CTA of a split tile merges the splits' partial rows: out = sum_s (2^(lse_s - M) /
+// sum_t 2^(lse_t - M)) O_s, s in order, so the result does not depend on which CTA came last.  It runs alone
 // and is bound by latencies, so it has few of them: L neighbouring threads per row form its M and sum,
 // then the rows are merged with 16 loads in flight per lane (3 rows over 100k tokens in 36 splits: 51 us;
 // 57 with the partial rows copied to shared memory first), spread over the splits where there are many,
@@ -1175,10 +1175,25 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
     }
     if constexpr (kKv8) {  // O back to the values the codes stand for
       float back[2];
+      bool large = false;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float x = st.mid == kSpread ? x_rows[16 * g + 8 * h] : st.unit;
         back[h] = x == 0.f ? 0.f : __int_as_float((2 * kExpBias << 23) - __float_as_int(x));
+        large = large || back[h] > kLargeBack;
+      }
+      if (__any_sync(0xffffffffu, large)) {
+        // Rows near the end of the range have finite means, but no finite sums: a quarter of their mean
+        // (four of them are added), with the weight in m.
+        float inv[2] = {1.f, 1.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (!(back[h] > kLargeBack && st.l[g][h] > 0.f)) continue;
+          inv[h] = 0.25f / st.l[g][h];
+          st.m[g][h] += __log2f(4.f * st.l[g][h]);
+          st.l[g][h] = 0.25f;
+        }
+        scale_o(st, g, inv);
       }
       scale_o(st, g, back);
     }

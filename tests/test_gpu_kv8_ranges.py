@@ -191,3 +191,19 @@ def test_zero_and_unwritten_rows_beside_others(cuda_device) -> None:
         got = attend(qb, *views[0], meta, SCALE)
         ref, bound, rows = attention64(qb, *views[0], [chunk], U_F16)
         assert_close(got, ref, bound + lost(qb, views[0], chunk), rows)
+
+
+@pytest.mark.parametrize("split", [0, 2])
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_at_the_end_of_the_range(kind: str, split: int, cuda_device) -> None:
+    """V rows of 2e38 and 3e38, one and all of them: every weighted mean is finite, though sums of rows
+    are not."""
+    dev = cuda_device
+    for every in (False, True):
+        chunk, slots, k, v, q = setup(dev, kind, 200, seed=11)
+        if every:
+            v = torch.where(v < 0, -2e38, 2e38)
+        else:
+            v[slots[[5, 199, 200]]] = 3e38
+        got = check(dev, chunk, slots, k, v, q * 0.3, split)
+        assert bool(torch.isfinite(got).all())

@@ -175,6 +175,8 @@ _lib: C.CDLL | None = None
 def load(path: str | os.PathLike[str] | None = None) -> C.CDLL:
     """Load (once) and return the library; raises if it is missing."""
     global _lib
+    if _lib is not None and path is None:
+        return _lib
     with _lock:
         if _lib is not None and path is None:
             return _lib

@@ -164,6 +164,13 @@ class AttentionMetadata:
         self._kv8_used = True
         return self._plan8, self.kv8
 
+    def rows_needed(self) -> int:
+        """Rows of q and out that the planned sequences reach (``num_tokens`` counts the slots)."""
+        n = int(self.info.num_seqs)
+        seqs = self._packed[self.info.off_seqs :][: 8 * n].reshape(n, 8)  # first row, new tokens
+        last = int((seqs[:, 0] + seqs[:, 1]).max()) if n else 0
+        return last if self.tree is None else max(last, self.tree.rows_needed())
+
     def workspace(self, num_kv_heads: int, device: torch.device, kv8: bool = False,
                   counters: bool = False) -> Tensor | None:
         """Scratch for this step (allocated once, reused by every layer): split-KV partials, with
@@ -447,7 +454,10 @@ def _upload_plan(packed: np.ndarray, device: torch.device) -> Tensor:
 def _stream(device: torch.device) -> int:
     """The current stream of a tensor's device, as the library takes it (torch's own accessor of the
     raw handle: a Stream object per call costs two microseconds)."""
-    return int(torch._C._cuda_getCurrentRawStream(device.index))
+    index = device.index  # a CUDA tensor's device always has one
+    if index is None:
+        raise RuntimeError("miniserve_b200 attention runs on CUDA only (no CPU fallback)")
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _rows(t: Tensor, name: str) -> int:
@@ -470,42 +480,41 @@ def kv_scatter(k: Tensor, v: Tensor, slot_mapping: Tensor, k_cache: Tensor, v_ca
     on the stream still runs: they are written by an earlier call than the one right before it (a step that
     moves accepted drafts does so before it writes its own rows)."""
     nb, kvh = check_layer_views(k_cache, v_cache, kv8=True)
-    t = int(k.shape[0])
+    kv8 = is_kv8(k_cache)
+    dev = _check_rows_args(k, v, slot_mapping, k_cache, kvh, spare_slots=not kv8)
+    t = k.shape[0]
+    rows = (k.data_ptr(), _rows(k, "k"), v.data_ptr(), _rows(v, "v"), t, kvh,
+            slot_mapping.data_ptr(), k_cache.data_ptr())
     lib = _capi.load()
-    if is_kv8(k_cache):
-        dev = _check_rows_args(k, v, slot_mapping, k_cache, kvh)
-        rc = _on_own_device(
-            lib.ms_kv_scatter_kv8, dev, k.data_ptr(), _rows(k, "k"), v.data_ptr(), _rows(v, "v"), t,
-            kvh, slot_mapping.data_ptr(), k_cache.data_ptr(), nb, _stream(dev),
-        )
+    if kv8:
+        rc = _on_own_device(lib.ms_kv_scatter_kv8, dev, *rows, nb, _stream(dev))
     else:
-        rc = lib.ms_kv_scatter(
-            k.data_ptr(), _rows(k, "k"), v.data_ptr(), _rows(v, "v"), t, kvh,
-            slot_mapping.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), nb, _stream(k.device),
-        )
+        rc = _on_own_device(lib.ms_kv_scatter, dev, *rows, v_cache.data_ptr(), nb, _stream(dev))
     _capi.check(rc, "kv_scatter")
 
 
 def _on_own_device(fn, device: torch.device, *args) -> int:
     """Call the library, which launches on the current device, with the tensors' own device current."""
-    if torch.cuda.current_device() == device.index:
+    index = device.index
+    if index is None or torch._C._cuda_getDevice() == index:
         return fn(*args)
     with torch.cuda.device(device):
         return fn(*args)
 
 
-def _check_rows_args(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, kvh: int) -> torch.device:
-    """Rows and their slots fit each other and the pool; returns the pool's device."""
+def _check_rows_args(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, kvh: int,
+                     spare_slots: bool = False) -> torch.device:
+    """Rows and their slots fit each other and the pool (with ``spare_slots`` slots behind the last row
+    are ignored); returns the pool's device."""
     shape = k.shape
     if len(shape) != 3 or shape != v.shape or shape[1] != kvh:
         raise ValueError(f"k and v must both be [T, {kvh}, {HEAD_DIM}]")
     n = _check_slots(slots)
-    if n != shape[0]:
+    if n != shape[0] and (n < shape[0] or not spare_slots):
         raise ValueError(f"{shape[0]} rows but {n} slots")
     dev = k_cache.device
-    if dev.type != "cuda":
-        raise RuntimeError("miniserve_b200 attention runs on CUDA only (no CPU fallback)")
-    if not (k.device == v.device == slots.device == dev):
+    index = k_cache.get_device()
+    if not (k.get_device() == index and v.get_device() == index and slots.get_device() == index):
         raise ValueError(f"k, v and slots are on {k.device}, {v.device} and {slots.device}, "
                          f"the pool on {dev}")
     return dev
@@ -563,45 +572,27 @@ def attend(q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: AttentionMetadata,
     Rows not covered by ``meta`` are left untouched (undefined, like ``torch.empty_like``).
     """
     nb, kvh = check_layer_views(k_cache, v_cache, kv8=True)
-    lib = _capi.load()
-    if meta.tree is not None or is_kv8(k_cache):
-        return _attend_parts(lib, q, k_cache, v_cache, meta, float(scale), out, nb, kvh)
-    if out is None:
-        out = torch.empty_like(q)
-    h = int(q.shape[1])
-    ws = meta.workspace(kvh, q.device)
-    rc = lib.ms_paged_attention(
-        q.data_ptr(), _rows(q, "q"), out.data_ptr(), _rows(out, "out"), h, kvh,
-        k_cache.data_ptr(), v_cache.data_ptr(), nb, meta.plan.data_ptr(), C.byref(meta.info),
-        ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
-        float(scale), _stream(q.device),
-    )
-    _capi.check(rc, "paged_attention")
-    return out
-
-
-def _attend_parts(lib, q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: AttentionMetadata,
-                  scale: float, out: Tensor | None, nb: int, kvh: int) -> Tensor:
-    """The causal part and the draft trees of a step, over either kind of pool."""
     dev = k_cache.device
-    if dev.type != "cuda":
-        raise RuntimeError("miniserve_b200 attention runs on CUDA only (no CPU fallback)")
     shape = q.shape
     q_stride = _rows(q, "q")
-    if not (q.device == meta.plan.device == dev):
+    index = k_cache.get_device()
+    if q.get_device() != index or meta.plan.get_device() != index:
         raise ValueError(f"q and meta are on {q.device} and {meta.plan.device}, the pool on {dev}")
-    if shape[0] < meta.num_tokens:
-        raise ValueError(f"q must have the step's {meta.num_tokens} rows")
+    need = meta.num_tokens
+    if shape[0] < need and shape[0] < (need := meta.rows_needed()):
+        raise ValueError(f"q must have the step's {need} rows")
     if out is None:
         out = torch.empty_like(q)
         out_stride = out.stride(0)
     else:
         out_stride = _rows(out, "out")
-        if out.device != dev:
+        if out.get_device() != index:
             raise ValueError(f"out is on {out.device}, the pool on {dev}")
-        if out.shape[1:] != shape[1:] or out.shape[0] < meta.num_tokens:
-            raise ValueError(f"out must have q's heads and the step's {meta.num_tokens} rows")
+        if out.shape[1:] != shape[1:] or (out.shape[0] < need and out.shape[0] < meta.rows_needed()):
+            raise ValueError(f"out must have q's heads and the step's {meta.rows_needed()} rows")
     kv8 = is_kv8(k_cache)
+    scale = float(scale)
+    lib = _capi.load()
     stream = _stream(dev)
     q_args = (q.data_ptr(), q_stride, out.data_ptr(), out_stride, shape[1], kvh)
     info, tree = meta.info, meta.tree

@@ -16,7 +16,7 @@ import torch
 from torch import Tensor, nn
 
 from . import _capi
-from .attention import AttentionMetadata, _rows, _stream, attend
+from .attention import AttentionMetadata, _on_own_device, _rows, _stream, attend
 from .kv_pool import HEAD_DIM, check_layer_views, is_kv8
 
 # Smallest step (tokens) for which ``fused_qkv="auto"`` takes kernel E: measured on a B200 against
@@ -32,6 +32,38 @@ class HeadNorm(nn.Module):
         super().__init__()
         self.weight = nn.Parameter(torch.ones(dim))
         self.eps = eps
+
+
+def _check_step(t: int, x: Tensor, k_cache: Tensor, num_heads: int, q_weight: Tensor, k_weight: Tensor,
+                cos: Tensor, sin: Tensor, slot_mapping: Tensor, positions: Tensor | None,
+                q_out: Tensor | None) -> None:
+    """What kernels A and E read and write beside x's t rows fits them, on the pool's device."""
+    _check_index(slot_mapping, "slot_mapping", t)
+    if q_weight.numel() < HEAD_DIM or k_weight.numel() < HEAD_DIM:
+        raise ValueError(f"q_norm / k_norm weights must have {HEAD_DIM} values")
+    shape, sin_shape = cos.shape, sin.shape
+    if shape[-1] < HEAD_DIM or sin_shape[-1] < HEAD_DIM or sin_shape[0] < shape[0]:
+        raise ValueError(f"cos and sin must have rows of {HEAD_DIM} for the same positions")
+    dev = k_cache.get_device()
+    ok = (x.get_device() == dev and slot_mapping.get_device() == dev and q_weight.get_device() == dev
+          and k_weight.get_device() == dev and cos.get_device() == dev and sin.get_device() == dev)
+    if positions is not None:
+        _check_index(positions, "positions", t)
+        ok = ok and positions.get_device() == dev
+    if q_out is not None:
+        shape = q_out.shape
+        if len(shape) != 3 or shape[0] < t or shape[1] != num_heads:
+            raise ValueError(f"q_out must be [{t}, {num_heads}, {HEAD_DIM}]")
+        ok = ok and q_out.get_device() == dev
+    if not ok:
+        raise ValueError(f"every argument must be on the pool's device, {k_cache.device}")
+
+
+def _check_index(index: Tensor, name: str, rows: int) -> None:
+    if index.dtype != torch.int64 or not index.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int64")
+    if index.numel() < rows:
+        raise ValueError(f"{rows} rows but {name} has {index.numel()} entries")
 
 
 def qk_norm_rope_scatter(
@@ -65,12 +97,11 @@ def qk_norm_rope_scatter(
         raise ValueError("cos and sin must share a row stride")
     if positions is None and cos.shape[0] < t:
         raise ValueError("per-token cos/sin rows must cover every token")
+    _check_step(t, qkv, k_cache, num_heads, q_weight, k_weight, cos, sin, slot_mapping, positions, q_out)
     if q_out is None:
         q_out = torch.empty((t, num_heads, HEAD_DIM), dtype=torch.bfloat16, device=qkv.device)
     pos_ptr, max_pos = None, 0
     if positions is not None:
-        if positions.dtype != torch.int64:
-            raise ValueError("positions must be int64")
         pos_ptr, max_pos = positions.data_ptr(), int(cos.shape[0])
     lib = _capi.load()
     args = (
@@ -78,12 +109,13 @@ def qk_norm_rope_scatter(
         k_weight.data_ptr(), float(eps), cos.data_ptr(), sin.data_ptr(), int(cos.stride(0)),
         pos_ptr, max_pos, slot_mapping.data_ptr(), q_out.data_ptr(), _rows(q_out, "q_out"),
     )
+    dev = qkv.device
     if is_kv8(k_cache):
-        with torch.cuda.device(k_cache.device):
-            rc = lib.ms_qk_norm_rope_scatter_kv8(*args, k_cache.data_ptr(), nb, _stream(qkv.device))
+        rc = _on_own_device(lib.ms_qk_norm_rope_scatter_kv8, dev, *args, k_cache.data_ptr(), nb,
+                            _stream(dev))
     else:
-        rc = lib.ms_qk_norm_rope_scatter(*args, k_cache.data_ptr(), v_cache.data_ptr(), nb,
-                                         _stream(qkv.device))
+        rc = _on_own_device(lib.ms_qk_norm_rope_scatter, dev, *args, k_cache.data_ptr(),
+                            v_cache.data_ptr(), nb, _stream(dev))
     _capi.check(rc, "qk_norm_rope_scatter")
     return q_out
 
@@ -123,16 +155,15 @@ def qkv_proj_norm_rope_scatter(
         raise ValueError("cos and sin must share a row stride")
     if positions is None and cos.shape[0] < t:
         raise ValueError("per-token cos/sin rows must cover every token")
+    _check_step(t, x, k_cache, num_heads, q_weight, k_weight, cos, sin, slot_mapping, positions, q_out)
     if q_out is None:
         q_out = torch.empty((t, num_heads, HEAD_DIM), dtype=torch.bfloat16, device=x.device)
     pos_ptr, max_pos = None, 0
     if positions is not None:
-        if positions.dtype != torch.int64:
-            raise ValueError("positions must be int64")
         pos_ptr, max_pos = positions.data_ptr(), int(cos.shape[0])
     lib = _capi.load()
-    rc = lib.ms_qkv_proj_norm_rope_scatter(
-        x.data_ptr(), int(x.stride(0)), t, hidden, w_qkv.data_ptr(), int(w_qkv.stride(0)),
+    rc = _on_own_device(
+        lib.ms_qkv_proj_norm_rope_scatter, x.device, x.data_ptr(), int(x.stride(0)), t, hidden, w_qkv.data_ptr(), int(w_qkv.stride(0)),
         num_heads, kvh, q_weight.data_ptr(), k_weight.data_ptr(), float(eps), cos.data_ptr(),
         sin.data_ptr(), int(cos.stride(0)), pos_ptr, max_pos, slot_mapping.data_ptr(),
         q_out.data_ptr(), _rows(q_out, "q_out"), k_cache.data_ptr(), v_cache.data_ptr(), nb,

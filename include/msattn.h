@@ -163,8 +163,8 @@ MS_API int ms_qkv_proj_norm_rope_scatter(const void* x, int64_t x_row_stride, in
 
 /* Scatter only (backends.py:159-160): k, v [T, KVH, 128] with the given row strides.  The slots of one call
  * differ from each other.  ms_paged_attention may read rows below a sequence's cached length while the call
- * before it on the stream still runs, so those are written by an earlier call than the one right before it
- * (a step that moves accepted drafts does so before it writes its own rows). */
+ * before it on the stream still runs: rows that are moved below it (accepted drafts) are followed by another
+ * call of the step, such as the write of its own rows, or by ms_kv_moved. */
 MS_API int ms_kv_scatter(const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride,
                   int32_t num_tokens, int32_t num_kv_heads, const int64_t* slot_mapping,
                   void* k_cache, void* v_cache, int32_t num_blocks, void* stream);
@@ -179,6 +179,9 @@ MS_API int ms_paged_attention(const void* q, int64_t q_row_stride, void* out, in
                        const void* v_cache, int32_t num_blocks, const int32_t* plan_dev,
                        const MsPlanInfo* plan, void* workspace, int64_t workspace_bytes,
                        float scale, void* stream);
+
+/* After rows were moved by the calls before: the next call on the stream starts when they have completed. */
+MS_API int ms_kv_moved(void* stream);
 
 /* ---- Rows of a pool by slot -------------------------------------------------------------------
  * No counterpart in the reference.  k_out, v_out [num_tokens, KVH, 128] bf16 (row strides in

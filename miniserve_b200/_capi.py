@@ -36,6 +36,7 @@ EXPORTED = (
     "ms_qk_norm_rope_scatter",
     "ms_qkv_proj_norm_rope_scatter",
     "ms_kv_scatter",
+    "ms_kv_moved",
     "ms_kv_scatter_kv8",
     "ms_qk_norm_rope_scatter_kv8",
     "ms_kv_gather",
@@ -124,6 +125,7 @@ _SIGNATURES = {
          _P, _P, _I64, _P, _P, _I32, _P],
     ),
     "ms_kv_scatter": (C.c_int, [_P, _I64, _P, _I64, _I32, _I32, _P, _P, _P, _I32, _P]),
+    "ms_kv_moved": (C.c_int, [_P]),
     "ms_kv_scatter_kv8": (C.c_int, [_P, _I64, _P, _I64, _I32, _I32, _P, _P, _I32, _P]),
     "ms_qk_norm_rope_scatter_kv8": (
         C.c_int,

@@ -470,15 +470,17 @@ def _rows(t: Tensor, name: str) -> int:
     return stride[0]
 
 
-def kv_scatter(k: Tensor, v: Tensor, slot_mapping: Tensor, k_cache: Tensor, v_cache: Tensor) -> None:
+def kv_scatter(k: Tensor, v: Tensor, slot_mapping: Tensor, k_cache: Tensor, v_cache: Tensor,
+               moved: bool = False) -> None:
     """Write this step's K/V rows into their slots (backends.py:159-160).  Into an 8-bit pool each
-    row is quantised as it is written (see ``kv_pool``).
+    row is quantised as it is written (see ``kv_pool``).  ``moved``: the rows are not the step's own but lie
+    below the cached length of sequences that the next call may attend over.
 
     The slots of one call differ from each other, as for ``index_copy_``: what a slot named twice
     holds afterwards is undefined (an 8-bit one may pair one row's codes with the other's exponent).
     ``attend`` over a bf16 pool may read rows below a sequence's ``num_cached`` while the call before it
-    on the stream still runs: they are written by an earlier call than the one right before it (a step that
-    moves accepted drafts does so before it writes its own rows)."""
+    on the stream still runs: it waits for rows that are written with ``moved`` (a launch more), and a step
+    that writes its own rows in between needs no flag."""
     nb, kvh = check_layer_views(k_cache, v_cache, kv8=True)
     kv8 = is_kv8(k_cache)
     dev = _check_rows_args(k, v, slot_mapping, k_cache, kvh, spare_slots=not kv8)
@@ -489,7 +491,10 @@ def kv_scatter(k: Tensor, v: Tensor, slot_mapping: Tensor, k_cache: Tensor, v_ca
     if kv8:
         rc = _on_own_device(lib.ms_kv_scatter_kv8, dev, *rows, nb, _stream(dev))
     else:
-        rc = _on_own_device(lib.ms_kv_scatter, dev, *rows, v_cache.data_ptr(), nb, _stream(dev))
+        stream = _stream(dev)
+        rc = _on_own_device(lib.ms_kv_scatter, dev, *rows, v_cache.data_ptr(), nb, stream)
+        if moved and rc == _capi.MS_OK:
+            rc = _on_own_device(lib.ms_kv_moved, dev, stream)
     _capi.check(rc, "kv_scatter")
 
 
@@ -534,9 +539,9 @@ def kv_gather(slots: Tensor, k_cache: Tensor, v_cache: Tensor, k_out: Tensor | N
     ``(k, v)``, each ``[len(slots), kv_heads, 128]``.  No reference counterpart.
 
     What it is for: after a verify step the accepted drafts' rows are read and written to the
-    positions they take in the sequence (``kv_scatter(*kv_gather(from_slots, ...), to_slots, ...)``; the
-    rows are read before any is written, so the two sets may overlap), or a sequence's rows are handed
-    to another cache.  From an 8-bit pool the values are exact, and writing them back stores the same
+    positions they take in the sequence (``kv_scatter(*kv_gather(from_slots, ...), to_slots, ...,
+    moved=True)``; the rows are read before any is written, so the two sets may overlap), or a sequence's
+    rows are handed to another cache.  From an 8-bit pool the values are exact, and writing them back stores the same
     values again.  A slot outside the pool reads as zeros (and sets the device status bit).
     """
     nb, kvh = check_layer_views(k_cache, v_cache, kv8=True)

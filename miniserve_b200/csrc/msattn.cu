@@ -629,6 +629,19 @@ extern "C" int ms_kv_scatter(const void* k, int64_t k_row_stride, const void* v,
   return MS_OK;
 }
 
+namespace {
+__global__ void order_kernel() {}
+}  // namespace
+
+// Launched without programmatic serialization, so it starts when the work before it has completed and its
+// writes are visible; a kernel that starts early behind it starts after that.
+extern "C" int ms_kv_moved(void* stream) {
+  order_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>();
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail("ms_kv_moved launch", e);
+  return MS_OK;
+}
+
 // Merge of the split items' partials (kernel C), after every launch that writes them.
 static int launch_combine(const ms::AttnArgs& a, const MsPlanInfo* plan, const int32_t* plan_dev,
                           cudaStream_t s) {

@@ -849,6 +849,7 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
     asm volatile("prefetch.global.L2 [%0];" ::"l"(ra.arrived + static_cast<long long>(it[6]) * a.num_kv + kvh));
   }
 
+  // Row sets of 16 kRG rows; each holds at least one token (two only where the rows exceed one).
   const int sets = n_q * kGroup > 16 * kRG ? 2 : 1;
   const int phases = kRowsWarps / sets;
   if (threadIdx.x == 0) {
@@ -995,7 +996,6 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
 
   const int set = warp % sets, phase = warp / sets;
   const int row_base = set * 16 * kRG;  // of this warp's rows
-  const bool warp_active = (row_base >> 1) < n_q;
   const int q2 = 2 * (lane & 3);
   // This thread's rows row(g, h) = row_base + 16 g + lane / 4 + 8 h and their facts.
   const int row00 = row_base + (lane >> 2);
@@ -1057,15 +1057,13 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
   bool ok = true;
   for (; j < n_full; j += phases * kBlockPages) {
     if (!(ok = wait_pages(j, kBlockPages))) break;
-    if (warp_active) {
-      const uint32_t page[kBlockPages] = {ring_u32 + (j % kStages) * Cfg::kPage,
-                                          ring_u32 + (j % kStages + 1) * Cfg::kPage};
-      const uint32_t vis[kRG][2] = {};
-      if constexpr (kKv8) {
-        if (!rows_block8<kRG, false>(page, q_row, st, c, vis, x_rows, lane)) break;
-      } else {
-        rows_block16<kRG, false>(page, q_row, st, c, vis, lane);
-      }
+    const uint32_t page[kBlockPages] = {ring_u32 + (j % kStages) * Cfg::kPage,
+                                        ring_u32 + (j % kStages + 1) * Cfg::kPage};
+    const uint32_t vis[kRG][2] = {};
+    if constexpr (kKv8) {
+      if (!rows_block8<kRG, false>(page, q_row, st, c, vis, x_rows, lane)) break;
+    } else {
+      rows_block16<kRG, false>(page, q_row, st, c, vis, lane);
     }
     __syncwarp();
     if (lane < kBlockPages) mbar_arrive(&empty[(j + lane) % kStages]);
@@ -1073,94 +1071,92 @@ __global__ void __launch_bounds__(RowsCfg<kKv8, kRG>::kThreads, RowsCfg<kKv8, kR
   for (; ok && j < npages; j += phases * kBlockPages) {
     const int cnt = min(kBlockPages, npages - j);
     if (!(ok = wait_pages(j, cnt))) break;
-    if (warp_active) {
-      // A second page that is not there is the first one again, with every key masked.
-      uint32_t page[kBlockPages] = {ring_u32 + (j % kStages) * Cfg::kPage,
-                                    ring_u32 + ((j + cnt - 1) % kStages) * Cfg::kPage};
-      // The plan's records again (volatile loads: nothing of them lives through the loop above).
-      auto reload = [](const int* p) {
-        int v;
-        asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p));
-        return v;
-      };
-      const int* itm = a.items + static_cast<long long>(item_idx) * kRec;
-      const int t0 = reload(itm + 1), nq = reload(itm + 2);
-      const int* rec = a.seqs + static_cast<long long>(reload(itm)) * kRec;
-      const int cached = reload(rec + 2);
-      const int* mrows = nullptr;
-      int mwords = 0;
-      if constexpr (kTree) {
-        mwords = reload(rec + 7);
-        mrows = ra.plan + reload(rec + 6);
-      }
-      const int key0 = (reload(itm + 3) + j) * kBlockTokens;
-      // Which of the pages' keys token k of the sequence's new ones sees.
-      auto seen = [&](int k) {
-        uint32_t v = 0;
+    // A second page that is not there is the first one again, with every key masked.
+    uint32_t page[kBlockPages] = {ring_u32 + (j % kStages) * Cfg::kPage,
+                                  ring_u32 + ((j + cnt - 1) % kStages) * Cfg::kPage};
+    // The plan's records again (volatile loads: nothing of them lives through the loop above).
+    auto reload = [](const int* p) {
+      int v;
+      asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p));
+      return v;
+    };
+    const int* itm = a.items + static_cast<long long>(item_idx) * kRec;
+    const int t0 = reload(itm + 1), nq = reload(itm + 2);
+    const int* rec = a.seqs + static_cast<long long>(reload(itm)) * kRec;
+    const int cached = reload(rec + 2);
+    const int* mrows = nullptr;
+    int mwords = 0;
+    if constexpr (kTree) {
+      mwords = reload(rec + 7);
+      mrows = ra.plan + reload(rec + 6);
+    }
+    const int key0 = (reload(itm + 3) + j) * kBlockTokens;
+    // Which of the pages' keys token k of the sequence's new ones sees.
+    auto seen = [&](int k) {
+      uint32_t v = 0;
 #pragma unroll
-        for (int t = 0; t < kBlockPages; ++t) {
-          const int k0 = key0 + t * kBlockTokens;
-          uint32_t bits;
-          if constexpr (kTree) {
-            const int* row = mrows + static_cast<long long>(k) * mwords;
-            bits = 0u;
-            if (row[k >> 5] >> (k & 31) & 1)
-              bits = k0 + kBlockTokens <= cached ? 0xffffu : tree_bits(row, mwords, k0 - cached);
-          } else {
-            bits = causal_bits(cached + k, k0);
-          }
-          if (t < cnt) v |= bits << (16 * t);
+      for (int t = 0; t < kBlockPages; ++t) {
+        const int k0 = key0 + t * kBlockTokens;
+        uint32_t bits;
+        if constexpr (kTree) {
+          const int* row = mrows + static_cast<long long>(k) * mwords;
+          bits = 0u;
+          if (row[k >> 5] >> (k & 31) & 1)
+            bits = k0 + kBlockTokens <= cached ? 0xffffu : tree_bits(row, mwords, k0 - cached);
+        } else {
+          bits = causal_bits(cached + k, k0);
         }
-        return v;
-      };
-      // A lane per token of the tile (at most 32), handed to the rows; and all of them together.
-      const uint32_t mine = lane < nq ? seen(t0 + lane) : 0u;
-      const uint32_t any = __reduce_or_sync(0xffffffffu, mine);
-      uint32_t vis[kRG][2];
-#pragma unroll
-      for (int g = 0; g < kRG; ++g) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int tok = (row00 + 16 * g + 8 * h) >> 1;  // rows past the last token see nothing
-          vis[g][h] = __shfl_sync(0xffffffffu, mine, tok & 31);
-        }
+        if (t < cnt) v |= bits << (16 * t);
       }
+      return v;
+    };
+    // A lane per token of the tile (at most 32), handed to the rows; and all of them together.
+    const uint32_t mine = lane < nq ? seen(t0 + lane) : 0u;
+    const uint32_t any = __reduce_or_sync(0xffffffffu, mine);
+    uint32_t vis[kRG][2];
+#pragma unroll
+    for (int g = 0; g < kRG; ++g) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int tok = (row00 + 16 * g + 8 * h) >> 1;  // rows past the last token see nothing
+        vis[g][h] = __shfl_sync(0xffffffffu, mine, tok & 31);
+      }
+    }
 #pragma unroll 1
-      for (int t = 0; t < cnt; ++t) {
-        const uint32_t dead = ~(any >> (16 * t)) & 0xffffu;
-        if (dead != 0)
-          scrub_keys(dead, page[t] + Cfg::kPage / 2 - (kKv8 ? kBlockTokens : 0), kKv8,
-                     kKv8 ? page[t] + kExp8Off + kBlockTokens : 0u, j + t + kStages < npages, lane);
-      }
-      bool run = true;
-      if constexpr (!kKv8) {
-        bool special[kBlockPages];
+    for (int t = 0; t < cnt; ++t) {
+      const uint32_t dead = ~(any >> (16 * t)) & 0xffffu;
+      if (dead != 0)
+        scrub_keys(dead, page[t] + Cfg::kPage / 2 - (kKv8 ? kBlockTokens : 0), kKv8,
+                   kKv8 ? page[t] + kExp8Off + kBlockTokens : 0u, j + t + kStages < npages, lane);
+    }
+    bool run = true;
+    if constexpr (!kKv8) {
+      bool special[kBlockPages];
 #pragma unroll
+      for (int t = 0; t < kBlockPages; ++t)
+        special[t] = t < cnt && page_has_special16(page[t], lane);
+      if (special[0] || special[1]) {
+#pragma unroll 1
         for (int t = 0; t < kBlockPages; ++t)
-          special[t] = t < cnt && page_has_special16(page[t], lane);
-        if (special[0] || special[1]) {
-#pragma unroll 1
-          for (int t = 0; t < kBlockPages; ++t)
-            if (t == 0 ? special[0] : special[1])
-              rows_page16_special<kRG>(page[t], t, q_u32, row00, st, c, vis, lane);
-          // The other page, if it has none, goes the usual way, in both places.
-          const uint32_t keep_bits = (special[0] ? 0u : 0xffffu) | (special[1] ? 0u : 0xffff0000u);
-          run = keep_bits != 0u && !(special[0] && cnt < kBlockPages);
-          if (special[0]) page[0] = page[1];
-          if (special[1]) page[1] = page[0];
+          if (t == 0 ? special[0] : special[1])
+            rows_page16_special<kRG>(page[t], t, q_u32, row00, st, c, vis, lane);
+        // The other page, if it has none, goes the usual way, in both places.
+        const uint32_t keep_bits = (special[0] ? 0u : 0xffffu) | (special[1] ? 0u : 0xffff0000u);
+        run = keep_bits != 0u && !(special[0] && cnt < kBlockPages);
+        if (special[0]) page[0] = page[1];
+        if (special[1]) page[1] = page[0];
 #pragma unroll
-          for (int g = 0; g < kRG; ++g) {
-            vis[g][0] &= keep_bits;
-            vis[g][1] &= keep_bits;
-          }
+        for (int g = 0; g < kRG; ++g) {
+          vis[g][0] &= keep_bits;
+          vis[g][1] &= keep_bits;
         }
       }
-      if (run) {
-        if constexpr (kKv8)
-          rows_block8<kRG, true>(page, q_row, st, c, vis, x_rows, lane);
-        else
-          rows_block16<kRG, true>(page, q_row, st, c, vis, lane);
-      }
+    }
+    if (run) {
+      if constexpr (kKv8)
+        rows_block8<kRG, true>(page, q_row, st, c, vis, x_rows, lane);
+      else
+        rows_block16<kRG, true>(page, q_row, st, c, vis, lane);
     }
     __syncwarp();
     if (lane < cnt) mbar_arrive(&empty[(j + lane) % kStages]);

@@ -64,7 +64,10 @@ def tree_positions(num_cached: int, parents: list[int]) -> list[int]:
     """RoPE position of each draft of a tree: ``num_cached`` plus its depth (unused positions get
     ``num_cached``)."""
     depth: list[int] = []
-    for p in parents:
+    for k, p in enumerate(parents):
+        if not UNUSED_DRAFT <= p < k or (p >= 0 and parents[p] == UNUSED_DRAFT):
+            raise ValueError(f"draft {k} has parent {p} (want an earlier draft in use, -1 for the last "
+                             f"cached token, or {UNUSED_DRAFT} for an unused position)")
         depth.append(depth[p] + 1 if p >= 0 else 0)
     return [num_cached + d for d in depth]
 

@@ -21,8 +21,8 @@
 // memory in that order of dims, so two conversions give a B operand.  V: ldmatrix.trans
 // leaves two neighbouring columns of two neighbouring tokens in a word; one byte permute and two
 // conversions give the operands of two column tiles (even and odd columns).  The query row (bf16, 8
-// significant bits) is scaled by a power of two into f16's range: exact down to 2^-33 of its
-// largest value.  (mma.sync on e4m3 operands would need no conversion, but it runs at less than
+// significant bits) is scaled by a power of two into f16's range: exact down to 2^-25 of its
+// largest value, and below that off by at most 2^-32 of it.  (mma.sync on e4m3 operands would need no conversion, but it runs at less than
 // half the rate per product here: 256 decode rows took 431 us with K multiplied that way.)
 // The row exponents of K multiply S's columns in fp32; those of V multiply p before it is rounded
 // to f16, which keeps 11 bits of a product, three more than the bf16 form, as long as it lies between
@@ -39,12 +39,15 @@
 // groups (kRG = 2) and uses each converted operand twice; that takes more than 168 registers, which
 // two CTAs of two warpgroups have once the producer's warpgroup hands its share to the consumers.
 //
-// What it measures (cold L2, 8 KV heads unless said): 256 decode rows over 1.2 GB of 8-bit pages 199 us
-// (0.93 of the copy rate), 64 trees of 16 drafts over 562 MB of bf16 pages 98 us (0.88), 3 rows over
-// 100k tokens 51 us (0.62; 8 us of it merge 36 splits); the short forms, 8 decode rows or one tree of 8
-// drafts, 14 to 18 us, which is latency.  48 trees of 32 drafts (wide tiles, 8-bit pages) 131 us (0.26):
-// mma.sync keeps the tensor pipe 47 % busy, and two warps per scheduler at 232 registers do not cover
-// their own latencies; another order of the products changes nothing.
+// What it measures (cold L2, 8 KV heads unless said): 256 decode rows over 1.2 GB of 8-bit pages 196 to
+// 219 us by GPU and by where the pool lies (0.94 to 0.85 of the copy rate), 64 trees of 16 drafts over 562 MB
+// of bf16 pages 102 to 109 us (0.84 to 0.79), 3 rows over 100k tokens 50 to 52 us (0.62; 8 us of it merge
+// 36 splits); the short forms, 8 decode rows or one tree of 8 drafts, 15 to 18 us, which is latency.  48
+// trees of 32 drafts (wide tiles, 8-bit pages) 123 to 130 us (0.27): mma.sync keeps the tensor pipe 48 %
+// busy, and two warps per scheduler at 232 registers do not cover their own latencies; another order of the
+// products changes nothing.  Where V rows spread over 2^24 in size, so that rows have factors of their own
+// and every pair of pages takes the masked loop: 256 decode rows 292 us (219 beside it), 3 rows 73 (50), 48
+// trees 215 (130).
 #pragma once
 
 #include "kv8.cuh"

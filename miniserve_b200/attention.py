@@ -543,9 +543,10 @@ def kv_gather(slots: Tensor, k_cache: Tensor, v_cache: Tensor, k_out: Tensor | N
 
     What it is for: after a verify step the accepted drafts' rows are read and written to the
     positions they take in the sequence (``kv_scatter(*kv_gather(from_slots, ...), to_slots, ...,
-    moved=True)``; the rows are read before any is written, so the two sets may overlap), or a sequence's
-    rows are handed to another cache.  From an 8-bit pool the values are exact, and writing them back stores the same
-    values again.  A slot outside the pool reads as zeros (and sets the device status bit).
+    moved=True)``; the rows are read before any is written, so the two sets may overlap), or a
+    sequence's rows are handed to another cache.  From an 8-bit pool the values are exact, and writing
+    them back stores the same values again.  A slot outside the pool reads as zeros (and sets the device
+    status bit).
     """
     nb, kvh = check_layer_views(k_cache, v_cache, kv8=True)
     n = _check_slots(slots)

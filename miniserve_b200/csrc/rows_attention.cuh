@@ -13,7 +13,8 @@
 // A tree token sees the cached context and the drafts its mask names (ancestors and itself); a row
 // that sees nothing writes zeros.
 //
-// bf16 pool: mma.sync m16n8k16 with bf16 operands, as in kernel B.
+// bf16 pool: mma.sync m16n8k16 with bf16 operands, as in kernel B.  As there, p reaches 2^8 before the
+// maximum follows, so V rows beyond 2^119 may overflow where they are seen.
 //
 // 8-bit pool: mma.sync m16n8k16 with f16 operands.  e4m3 codes are f16 values, so they are converted
 // exactly, two codes per instruction, after ldmatrix has brought them (16-bit units of two codes)
@@ -31,7 +32,8 @@
 // p 2^e is at most 2^15 and a row's largest at least 2.  A warp that meets others gives every row a power of
 // two of its own from there on, from the largest s c + e over the keys that the row sees, which holds the
 // row's largest product between 1 and 2^15 whatever the values are (see raise8).  Either way f16's range
-// costs a key at most 2^-25 in units in which the row's largest p 2^e is at least 1.
+// costs a key at most 2^-25 in units in which the row's largest p 2^e is at least 1.  (Scores are formed in
+// fp32 from a query row scaled to at most 448: K rows beyond 2^100 may overflow there.)
 //
 // Why this shape.  A decode row needs its bytes and little else: up to 32 rows per CTA, three CTAs per SM
 // at 128 registers (the query rows stay in shared memory and are read again for every pair of pages).

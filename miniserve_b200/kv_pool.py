@@ -21,9 +21,10 @@ e4m3 codes and one exponent byte, 129 bytes instead of 256:
 A row with exponent byte b stands for its codes times 2^(b - 127); b is chosen when the row is written
 (``kv_scatter``, kernel A), from the row's largest magnitude.  The 16-byte chunks of row t are stored
 at chunk ^ (t % 2 + 2 (t // 4)), which the kernels read without bank conflicts; ``layer_as_slots`` gives the
-values a layer stands for.  Attention takes rows of any finite sizes side by side: a key's share is lost
+values a layer stands for.  Attention takes V rows of any finite sizes side by side: a key's share is lost
 only where its softmax weight is below fp32's range (2^-126 of the row's largest), or where it adds less than
-2^-25 of the row's largest share.
+2^-25 of the row's largest share.  (Chunks of more than 64 tokens, which run over bf16 copies of the pages,
+may overflow where they see V rows beyond 2^119, as over a bf16 pool.)
 """
 
 from __future__ import annotations

@@ -349,8 +349,8 @@ MS_API int ms_attend_pages_kv8(const void* q, int64_t q_row_stride, void* out, i
  * The lists are host memory, read before the call returns; a captured call keeps them.
  *
  * ms_copy_pages copies block src[i] to block dst[i] in every layer.  No block is written twice, or both
- * written and read, by one call (one block may go to several).  Attention that follows waits for it.
- * ms_clear_pages fills blocks with zeros. */
+ * written and read, by one call (one block may go to several).
+ * ms_clear_pages fills blocks with zeros.  Attention that follows either waits for it. */
 MS_API int ms_copy_pages(void* base, int64_t layer_stride, int64_t page_bytes, int32_t num_layers,
                          int32_t num_blocks, const int32_t* src, const int32_t* dst, int32_t count,
                          void* stream);

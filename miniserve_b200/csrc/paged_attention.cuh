@@ -359,9 +359,10 @@ __global__ void __launch_bounds__(AttnCfg<kMode, kConsumerWarps, kStages>::kThre
   // and streams the pool pages holding only tokens cached in earlier steps before pdl_wait(),
   // and the consumers wait before loading the queries; this step's K/V rows (written by the
   // previous kernel) and every write come after the wait.  Only kernels of this library run as
-  // a programmatic predecessor, and none of them writes an earlier step's pages.  Any other
-  // launch waits at once: for a bandwidth-bound launch the early start only competes with the
-  // kernel it overlaps (measured 1-2 % slower on config 2).
+  // a programmatic predecessor.  Those that write an earlier step's pages are followed by an ordered
+  // launch: ms_copy_pages and ms_clear_pages make it, a caller of ms_kv_scatter does with ms_kv_moved.
+  // Any other launch waits at once: for a bandwidth-bound launch the early start only competes with
+  // the kernel it overlaps (measured 1-2 % slower on config 2).
   if constexpr (!kEarly) pdl_wait();
   pdl_trigger();
   using Cfg = AttnCfg<kMode, kConsumerWarps, kStages>;

@@ -428,7 +428,9 @@ int move_pages(const char* what, void* base, int64_t layer_stride, int64_t page_
                                              : launch_pages<kCopy, kMany>(a, layers, from, dst + at, s);
     if (e != cudaSuccess) return cuda_fail((std::string(what) + " launch").c_str(), e);
   }
-  return MS_OK;
+  // Attention that starts early reads cached rows before the launch in front of it has ended, and the pages' launch
+  // lets the next one start before its stores.
+  return ms_kv_moved(stream);
 }
 
 }  // namespace
@@ -436,10 +438,8 @@ int move_pages(const char* what, void* base, int64_t layer_stride, int64_t page_
 extern "C" int ms_copy_pages(void* base, int64_t layer_stride, int64_t page_bytes, int32_t num_layers,
                              int32_t num_blocks, const int32_t* src, const int32_t* dst, int32_t count,
                              void* stream) {
-  const int rc = move_pages<true>("ms_copy_pages", base, layer_stride, page_bytes, num_layers, num_blocks,
-                                  src, dst, count, stream);
-  // Attention that starts early reads cached rows before the launch in front of it has ended.
-  return rc != MS_OK || count == 0 || num_layers == 0 ? rc : ms_kv_moved(stream);
+  return move_pages<true>("ms_copy_pages", base, layer_stride, page_bytes, num_layers, num_blocks, src, dst,
+                          count, stream);
 }
 
 extern "C" int ms_clear_pages(void* base, int64_t layer_stride, int64_t page_bytes, int32_t num_layers,

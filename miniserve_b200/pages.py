@@ -68,7 +68,7 @@ def copy_pages(pool: Tensor, src: Sequence[int] | np.ndarray, dst: Sequence[int]
 
 def clear_pages(pool: Tensor, blocks: Sequence[int] | np.ndarray) -> None:
     """Fill the listed blocks of every layer with zeros: a page that held an infinity or a NaN passes
-    neither on to the next sequence that is given it."""
+    neither on to the next sequence that is given it.  ``attend`` waits for it."""
     layers, num_blocks, page = _paged(pool)
     b, n = _block_list(blocks, "blocks")
     if n == 0 or layers == 0:

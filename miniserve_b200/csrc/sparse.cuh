@@ -973,11 +973,13 @@ constexpr int kMaxPageStages = 4;
 
 // Queries as A: the channels of a lane's key pieces, of head r % 2.  For an 8-bit pool in f16, times 2^-shift
 // so that the row's largest value is near 2^13: exact but for values 2^-27 of it (and in rows below 2^-87, which are
-// scaled by 2^100).
+// scaled by 2^100).  2^shift goes to the score before the key row's scale where it is below 1 and after it where it is
+// above: the two may be near opposite ends of fp32's range.
 template <bool kKv8>
 struct PageQuery {
   uint32_t x[16];
   float unit;  // of a score, in the exponent of 2
+  float after;
   __device__ __forceinline__ void load(const __nv_bfloat16* q, float scale_log2, int lane) {
     const int c = lane & 3;
     q += ((lane >> 2) & 1) * kHeadDim;
@@ -1001,9 +1003,10 @@ struct PageQuery {
       top = max(top & 0xffffu, top >> 16);
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int shift = min(max(static_cast<int>(top >> 7) - 127 - 13, -100), 100);
+      const int shift = min(max(static_cast<int>(top >> 7) - 127 - 13, -100), 254 - 127 - 13);
       const float down = __int_as_float((127 - shift) << 23);
-      unit *= __int_as_float((127 + shift) << 23);
+      unit *= __int_as_float((127 + min(shift, 0)) << 23);
+      after = __int_as_float((127 + max(shift, 0)) << 23);
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -1072,7 +1075,7 @@ __device__ __forceinline__ void page_scores(const PageQuery<kKv8>& q, const uint
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     s[i] = (acc[i >> 1][0][i & 1] + acc[i >> 1][1][i & 1]) * q.unit;
-    if constexpr (kKv8) s[i] *= row_scale8(page[kExp8Off + page_key<kKv8>(i, c)]);
+    if constexpr (kKv8) s[i] = s[i] * row_scale8(page[kExp8Off + page_key<kKv8>(i, c)]) * q.after;
   }
 }
 

@@ -1022,17 +1022,18 @@ struct PageQuery {
   }
 };
 
-// One warp's share of a row, for head r % 2: running maximum m of the scores and sum of 2^(s - m); reference
-// `ref` of the shares, and the sum of 2^(s + e - ref) c over keys with values c 2^e.
-// * bf16 (e = 0): ref = m + 24, so that the sum of 2^16 values of any size stays in fp32's range (the shares of values
+// One warp's share of a row, for head r % 2: running maximum m of the scores, sum of 2^(s - m), and the sum of
+// 2^(s - m + e - lead) c over keys with values c 2^e.
+// * bf16 (e = 0): lead = 24, so that the sum of 2^16 values of any size stays in fp32's range (the shares of values
 //   below 2^-100 reach its smallest numbers).
-// * 8-bit: codes c, and ref follows the largest s + e, so that no row's size changes what others give.
-// Both move only when they grow by more than 8 (weights up to 2^8), which few pages do.
+// * 8-bit: codes c, and lead follows the largest s - m + e, so that no row's size changes what others give.
+// Both move only when they grow by more than 8 (weights up to 2^8), which few pages do.  Scores enter as differences
+// from m alone: beside a score beyond 2^24, fp32 does not hold the 24 or an e that is added to it.
 // A weight is two bf16 or f16 numbers, itself and what its rounding lost (f16: times 2^12), in columns 0-1
 // and 2-3 of B, which a product with eight columns has room for: weights are exact to 2^-17 (f16 2^-22).
 template <bool kKv8>
 struct RowState {
-  float m, ref, sum;
+  float m, lead, sum;  // lead: 8-bit
   float acc[8][4];  // product t: channels of rows r and r + 8, columns 2 c and 2 c + 1
 };
 // Channel of acc[t][0] (head 0) and acc[t][1] (head 1); acc[t][2], [3] are the next one's.
@@ -1085,33 +1086,48 @@ template <bool kKv8>
 __device__ __forceinline__ void page_update(const uint8_t* page, float (&s)[4], int visible, int lane,
                                             RowState<kKv8>& st) {
   const int r = lane >> 2, c = lane & 3;
-  float e[4], top = -INFINITY, most = -INFINITY;
+  // Exponent of a key's share over 2^m, from d = s - m.
+  auto share = [&](int i, float d) {
+    const int key = page_key<kKv8>(i, c), b = page[kExp8Off + kBlockTokens + key];
+    if (key >= visible) return -INFINITY;
+    return d + (b == static_cast<int>(kExpNan) ? __int_as_float(0x7fc00000) : static_cast<float>(b - kExpBias));
+  };
+  float m = st.m == -INFINITY ? 0.f : st.m;
+  float d[4], e[4], top = -INFINITY, most = -INFINITY;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int key = page_key<kKv8>(i, c);
-    if (key >= visible) s[i] = -INFINITY;
-    e[i] = s[i];
-    if constexpr (kKv8) {
-      const int b = page[kExp8Off + kBlockTokens + key];
-      if (key < visible)
-        e[i] += b == static_cast<int>(kExpNan) ? __int_as_float(0x7fc00000) : static_cast<float>(b - kExpBias);
-      most = fmaxf(most, e[i]);
-    }
+    if (page_key<kKv8>(i, c) >= visible) s[i] = -INFINITY;
     top = fmaxf(top, s[i]);
+    d[i] = s[i] - m;
+    if constexpr (kKv8) most = fmaxf(most, e[i] = share(i, d[i]));
   }
 #pragma unroll
   for (int off = 1; off <= 2; off <<= 1) {
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
     if constexpr (kKv8) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
   }
-  bool grow = top > st.m + 8.f;
-  if constexpr (kKv8) grow = grow || most > st.ref + 8.f;
+  bool grow = top - st.m > 8.f;
+  if constexpr (kKv8) grow = grow || most - st.lead > 8.f;
   if (__any_sync(0xffffffffu, grow)) {
-    const float m = fmaxf(st.m, top), old = st.ref;
-    st.sum *= st.m == -INFINITY ? 0.f : fast_exp2(st.m - m);
-    st.m = m;
-    st.ref = kKv8 ? fmaxf(st.ref, most) : m + 24.f;
-    const float fix = old == -INFINITY ? 0.f : fast_exp2(old - st.ref);
+    const float old = st.m;
+    st.m = fmaxf(old, top);
+    m = st.m == -INFINITY ? 0.f : st.m;
+    const float down = old == -INFINITY ? -INFINITY : old - st.m;
+    st.sum *= fast_exp2(down);
+    most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      d[i] = s[i] - m;
+      if constexpr (kKv8) most = fmaxf(most, e[i] = share(i, d[i]));
+    }
+    float fix = fast_exp2(down);
+    if constexpr (kKv8) {
+#pragma unroll
+      for (int off = 1; off <= 2; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+      const float was = st.lead == -INFINITY ? -INFINITY : st.lead + down;
+      st.lead = fmaxf(was, most);
+      fix = was == -INFINITY ? 0.f : fast_exp2(was - st.lead);
+    }
     const float other = __shfl_xor_sync(0xffffffffu, fix, 4);
     const float f0 = lane & 4 ? other : fix, f1 = lane & 4 ? fix : other;
 #pragma unroll
@@ -1120,15 +1136,18 @@ __device__ __forceinline__ void page_update(const uint8_t* page, float (&s)[4], 
       st.acc[t][1] *= f1, st.acc[t][3] *= f1;
     }
   }
-  const float m = st.m == -INFINITY ? 0.f : st.m, ref = st.ref == -INFINITY ? 0.f : st.ref;
+  const float lead = st.lead == -INFINITY ? 0.f : st.lead;
   const bool rest = lane & 8;  // columns 2 and 3, and what nobody reads
   uint32_t b[2];
   float w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float x = fast_exp2(s[i] - m);
+    const float x = fast_exp2(d[i]);
     st.sum += x;
-    w[i] = kKv8 ? fast_exp2(e[i] - ref) : x * 0x1p-24f;
+    if constexpr (kKv8)
+      w[i] = fast_exp2(e[i] - lead);
+    else
+      w[i] = x * 0x1p-24f;
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -1177,7 +1196,7 @@ __device__ __forceinline__ void page_update(const uint8_t* page, float (&s)[4], 
 
 // What warps and CTAs pass on of their share of a row.
 struct RowPart {
-  float m[kGroup], ref[kGroup], sum[kGroup];
+  float m[kGroup], lead[kGroup], sum[kGroup];
   float pad[2];
   float acc[kGroup][kHeadDim];
 };
@@ -1193,8 +1212,8 @@ __device__ __forceinline__ bool mbar_wait_nohint(uint64_t* bar, uint32_t parity)
 
 // One cluster of CTAs (or one CTA) per (sequence, new token, KV head); their warps take the listed pages in
 // turn, each through its own ring, and the first CTA merges.  Memory bounds it where the CTAs fill the GPU: 256
-// rows of 64 bf16 pages 145 us (6.7 TB/s, the copy rate), of 64 8-bit pages 82 (0.81 of it); 48 rows of 128 8-bit
-// pages are two or three CTAs per SM, 41 us (0.75).  Four warps share one row and head: with one or two each 166 and
+// rows of 64 bf16 pages 145 us (6.9 TB/s, the copy rate), of 64 8-bit pages 85 (0.78 of it); 48 rows of 128 8-bit
+// pages are two or three CTAs per SM, 43 us (0.73).  Four warps share one row and head: with one or two each 166 and
 // 150 us, 88 and 57.  Few rows are a chain of latencies: 8 rows of 16 pages 5.3 us.
 template <bool kKv8>
 __global__ void __launch_bounds__(kPagesWarps * 32, kKv8 ? 4 : 3)
@@ -1225,7 +1244,7 @@ __global__ void __launch_bounds__(kPagesWarps * 32, kKv8 ? 4 : 3)
   const int position = seq.num_cached + tok;
   const int n = live ? position / kBlockTokens + 1 : 0;
   RowState<kKv8> st;
-  st.m = st.ref = -INFINITY;
+  st.m = st.lead = -INFINITY;
   st.sum = 0.f;
 #pragma unroll
   for (int t = 0; t < 8; ++t)
@@ -1303,7 +1322,7 @@ __global__ void __launch_bounds__(kPagesWarps * 32, kKv8 ? 4 : 3)
   for (int off = 1; off <= 2; off <<= 1) st.sum += __shfl_xor_sync(0xffffffffu, st.sum, off);
   __syncwarp();
   RowPart& mine = *part_of(warp);
-  if ((lane & ~4) == 0) mine.m[lane >> 2] = st.m, mine.ref[lane >> 2] = st.ref, mine.sum[lane >> 2] = st.sum;
+  if ((lane & ~4) == 0) mine.m[lane >> 2] = st.m, mine.lead[lane >> 2] = st.lead, mine.sum[lane >> 2] = st.sum;
 #pragma unroll
   for (int t = 0; t < 8; ++t)
 #pragma unroll
@@ -1317,16 +1336,19 @@ __global__ void __launch_bounds__(kPagesWarps * 32, kKv8 ? 4 : 3)
   // Merges `count` parts: a thread has two neighbouring channels of a head.
   constexpr int kPer = kGroup * kHeadDim / (kPagesWarps * 32);
   const int at = threadIdx.x * kPer, g = at / kHeadDim, d = at % kHeadDim;
-  float m, ref, sum, acc[kPer];
+  float m, lead, sum, acc[kPer];
   auto merge = [&](auto of, int count) {
-    m = ref = -INFINITY, sum = 0.f;
+    m = lead = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-    for (int w = 0; w < count; ++w) m = fmaxf(m, of(w)->m[g]), ref = fmaxf(ref, of(w)->ref[g]);
+    for (int w = 0; w < count; ++w) m = fmaxf(m, of(w)->m[g]);
+    if constexpr (kKv8)  // without keys neither: minus infinity less itself is NaN, which fmaxf passes over
+      for (int w = 0; w < count; ++w) lead = fmaxf(lead, of(w)->lead[g] + (of(w)->m[g] - m));
     for (int w = 0; w < count; ++w) {
       const RowPart* p = of(w);
-      sum += p->m[g] == -INFINITY ? p->sum[g] : p->sum[g] * fast_exp2(p->m[g] - m);
-      const float f = p->ref[g] == -INFINITY ? 1.f : fast_exp2(p->ref[g] - ref);
+      float f = p->m[g] == -INFINITY ? 1.f : fast_exp2(p->m[g] - m);
+      sum += p->sum[g] * f;
+      if constexpr (kKv8) f = p->lead[g] == -INFINITY ? 1.f : fast_exp2(p->lead[g] + (p->m[g] - m) - lead);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) acc[i] += p->acc[g][d + i] * f;
     }
@@ -1340,7 +1362,7 @@ __global__ void __launch_bounds__(kPagesWarps * 32, kKv8 ? 4 : 3)
       store_cluster(to + offsetof(RowPart, acc) + (at + i) * 4, __float_as_uint(acc[i]));
     if (d == 0) {
       store_cluster(to + offsetof(RowPart, m) + g * 4, __float_as_uint(m));
-      store_cluster(to + offsetof(RowPart, ref) + g * 4, __float_as_uint(ref));
+      store_cluster(to + offsetof(RowPart, lead) + g * 4, __float_as_uint(lead));
       store_cluster(to + offsetof(RowPart, sum) + g * 4, __float_as_uint(sum));
     }
     __syncwarp();
@@ -1350,9 +1372,9 @@ __global__ void __launch_bounds__(kPagesWarps * 32, kKv8 ? 4 : 3)
     merge([&](int w) { return peers + w; }, a.cluster);
   }
   if (!live) return;
-  // 2^(ref - m) in two steps: it may be beyond fp32 where the values are near the end of their range.  No key
-  // at all: zero; NaN goes through.
-  const float half = fast_exp2(0.5f * (ref - m)), part = half / sum;
+  // 2^lead in two steps: it may be beyond fp32 where the values are near the end of their range.  No key at all:
+  // zero; NaN goes through.
+  const float half = fast_exp2(0.5f * (kKv8 ? lead : 24.f)), part = half / sum;
   *reinterpret_cast<uint32_t*>(a.out + row * a.out_row_stride + head * kGroup * kHeadDim + at) =
       sum == 0.f ? 0u : pack_bf16(acc[0] * part * half, acc[1] * part * half);
 }

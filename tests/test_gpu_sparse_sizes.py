@@ -8,9 +8,9 @@ import torch
 
 from miniserve_b200 import attend_pages, build_attention_metadata, kv_scatter
 from miniserve_b200.attention import SeqChunk
-from miniserve_b200.kv_pool import KV8, allocate_kv_cache
+from miniserve_b200.kv_pool import KV8, allocate_kv_cache, layer_as_slots
 from paged_reference import assert_close
-from sparse_reference import attend_pages64
+from sparse_reference import SCALE, attend_pages64
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,22 @@ def test_queries_of_any_size(exponent: int, dtype, cuda_device) -> None:
     ref, bound, rows = attend_pages64(q, *views, CHUNKS, pages, scale)
     assert bool(torch.isfinite(out[rows]).all())
     assert_close(out, ref, bound, rows)
+
+
+@POOLS
+@pytest.mark.parametrize("scale", [SCALE, 1.0, 2.0**20])
+@pytest.mark.parametrize("exponent", [100, 115, 128])
+def test_one_key_has_all_the_weight(exponent: int, scale: float, dtype, cuda_device) -> None:
+    """Every key but one is zero, and that one's scores are far above 0: the rows are its values, exactly."""
+    dev = cuda_device
+    q = queries(exponent, dev)
+    k = torch.zeros(BLOCKS * 16, KVH, 128, dtype=torch.bfloat16, device=dev)
+    at = [17, 19 * 16 + 40]  # one in each sequence, for the first head of the pair
+    for slot, row in zip(at, (0, 1)):
+        k[slot] = q[row, ::2].sign() * 2.0**-90
+    views = pool(k, dtype, dev)
+    pages = torch.arange(19, dtype=torch.int32, device=dev).repeat(4, KVH, 1)
+    out = attend_pages(q, *views, metadata(dev), pages, scale)
+    v = layer_as_slots(views[1])
+    for slot, row in zip(at, (0, 1)):
+        assert torch.equal(out[row, ::2], v[slot])

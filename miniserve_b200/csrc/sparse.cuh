@@ -5,7 +5,10 @@
 // the largest key value lo_d, hi_d over its tokens (bf16 values, or what 8-bit rows stand for, which are
 // bf16 values too: nothing is rounded).  For a query q no key within the bounds has a product above
 //   sum_d max(q_d lo_d, q_d hi_d) = sum_d max(q_d, 0) hi_d + min(q_d, 0) lo_d,
-// and a page's score is the larger one of that for the two query heads of the KV head.
+// and a page's score is the larger one of that for the two query heads of the KV head.  The two sums are the same
+// where the bounds are finite.  The second one, which is computed, is infinite or NaN for every q where a bound is
+// not finite (0 times infinity on the side that q_d rules out): such a page holds a key that is not finite, and
+// counts as one of infinite score.
 #pragma once
 
 #include <cstddef>

@@ -124,7 +124,8 @@ def select_pages(q: Tensor, bounds: Tensor, meta: AttentionMetadata, budget: int
     A token that sees at most ``budget`` pages keeps them all.  Else it keeps the ``first`` first and the
     ``last`` last ones (its own page is the last) and of those between the ones with the highest scores,
     max over the KV head's two query heads of sum_d max(q_d lo_d, q_d hi_d), compared as exactly as 64 bits
-    give them; equal scores go to the lower page, and a score that is not finite counts as infinite.
+    give them; equal scores go to the lower page, and a score that is not finite counts as infinite, as does
+    that of any page with a bound that is not finite.
     Rows of longer chunks and of trees are left untouched (undefined).  Calls that use one metadata share its
     scratch, so they are ordered on the GPU (one stream, or events)."""
     nb, kvh = _check_bounds(bounds)

@@ -8,6 +8,7 @@ has no block manager of its own, or wants forks and compaction beside it.
 
 from __future__ import annotations
 
+import math
 import struct
 from collections import Counter
 from collections.abc import Sequence
@@ -26,7 +27,8 @@ def _paged(pool: Tensor) -> tuple[int, int, int]:
     shape = pool.shape
     if len(shape) < 3 or not pool.is_contiguous():
         raise ValueError("pool must be a contiguous paged tensor [layers, num_blocks, ...]")
-    return shape[0], shape[1], pool.stride(1) * pool.element_size()
+    # Not the stride of a block: where there is one block, a contiguous tensor may have any.
+    return shape[0], shape[1], math.prod(shape[2:]) * pool.element_size()
 
 
 def _block_list(blocks: Sequence[int] | np.ndarray, name: str) -> tuple[bytes, int]:

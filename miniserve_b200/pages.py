@@ -91,6 +91,15 @@ class CachePages:
         sizes = {_paged(t)[1] for t in tensors}
         if len(sizes) != 1:
             raise ValueError(f"paged tensors of different numbers of blocks: {sorted(sizes)}")
+        # What a copy would refuse, or do to a page that another tensor's copy still reads, is refused here: the
+        # counts change before the copies are queued.
+        for t in tensors:
+            if _paged(t)[2] % 16 or t.data_ptr() % 16:
+                raise ValueError("paged tensors need pages of whole multiples of 16 bytes on 16-byte boundaries")
+        spans = sorted((str(t.device), t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+                       for t in tensors)
+        if any(a[0] == b[0] and b[1] < a[2] for a, b in zip(spans, spans[1:])):
+            raise ValueError("paged tensors must not share memory")
         self.tensors = tensors
         self.num_blocks = sizes.pop()
         self._free = list(range(self.num_blocks - 1, -1, -1))  # the lowest is taken first

@@ -109,6 +109,9 @@ class AttentionMetadata:
         step sees them) and True is returned.  Otherwise nothing changes and False is returned:
         build new metadata and capture again.  What a launch over an 8-bit pool adds to the shape
         (the pages that its tensor-core items read) counts once this metadata has been used for one.
+        A launch over selected pages takes the most new tokens of the step's short rows and a bound of the
+        pages that they see (``short_rows``): once this metadata has been used for one, the first has to be
+        the same and the second is not to grow past the bound.
         No reference counterpart (MiniServe captures no graphs).
         """
         if slot_mapping is not None and tuple(slot_mapping.shape) != tuple(self.slot_mapping.shape):
@@ -123,8 +126,10 @@ class AttentionMetadata:
             new.append((self._rest, self._rest._replan([c for c in plain if c.num_new > SHORT_QUERY])))
         if any(plan is None for _, plan in new):
             return False
-        if self._short is not None and _short_rows(*new[0][1][:2]) != self._short:
-            return False
+        if self._short is not None:
+            most_new, most_pages = _short_rows(*new[0][1][:2])
+            if most_new != self._short[0] or most_pages > self._short[1]:
+                return False
         if self._no_rest and any(c.num_new > SHORT_QUERY for c in plain):
             return False
         for meta, plan in new:
@@ -179,8 +184,9 @@ class AttentionMetadata:
         return self._plan8, self.kv8
 
     def short_rows(self) -> tuple[int, int]:
-        """Most new tokens of the sequences of at most SHORT_QUERY of them (0: there are none), and most
-        pages that one of them sees, in steps of 64: what a launch over their selected pages depends on."""
+        """Most new tokens of the sequences of at most SHORT_QUERY of them (0: there are none), and a bound of
+        the pages that one of them sees (the most of them in steps of 64, of the step that first asked): what
+        a launch over their selected pages depends on."""
         if self._short is None:
             self._short = _short_rows(self._packed, self.info)
         return self._short

@@ -331,7 +331,9 @@ MS_API int ms_select_pages(const void* q, int64_t q_row_stride, int32_t num_head
 /* Attention of those query tokens over the keys of their pages, up to the token's own position.  Entries of
  * `pages` that the token does not see (negative, or behind its own page) are skipped, in any place; a page
  * named twice counts twice; a row without pages gives zeros.  Other rows of out are left as they are.  A
- * block outside the pool is left out and sets MS_DEV_BAD_BLOCK. */
+ * block outside the pool is left out and sets MS_DEV_BAD_BLOCK.  Over an 8-bit pool a key adds nothing where
+ * its weight times its value row's size is below 2^-36 of the largest such product of the query token, and a
+ * query's channels below 2^-27 of its largest one lose bits. */
 MS_API int ms_attend_pages(const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride,
                            int32_t num_heads, int32_t num_kv_heads, const void* k_cache,
                            const void* v_cache, int32_t num_blocks, const int32_t* plan_dev,

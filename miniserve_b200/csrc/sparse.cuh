@@ -1029,7 +1029,9 @@ struct PageQuery {
 // 2^(s - m + e - lead) c over keys with values c 2^e.
 // * bf16 (e = 0): lead = 24, so that the sum of 2^16 values of any size stays in fp32's range (the shares of values
 //   below 2^-100 reach its smallest numbers).
-// * 8-bit: codes c, and lead follows the largest s - m + e, so that no row's size changes what others give.
+// * 8-bit: codes c, and lead follows the largest s - m + e, so that values of any size do not overflow, and rows whose
+//   2^(s + e) is within 2^-14 of the largest one keep their weight; below that it loses bits, and a share below 2^-36 of
+//   the largest 2^(s + e) is lost (f16's smallest number, 2^-24, of a second part that is held 2^12 larger).
 // Both move only when they grow by more than 8 (weights up to 2^8), which few pages do.  Scores enter as differences
 // from m alone: beside a score beyond 2^24, fp32 does not hold the 24 or an e that is added to it.
 // A weight is two bf16 or f16 numbers, itself and what its rounding lost (f16: times 2^12), in columns 0-1

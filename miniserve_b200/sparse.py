@@ -166,7 +166,10 @@ def attend_pages(q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: AttentionMet
 
     Entries that the token does not see (negative, or behind its own page) are skipped in any place; a page
     named twice counts twice; a row without pages gives zeros.  Longer chunks and trees see all that they
-    see in ``attend``.  Rows not covered by ``meta`` are left untouched."""
+    see in ``attend``.  Rows not covered by ``meta`` are left untouched.
+
+    Over an 8-bit pool a key adds nothing where its weight times its value row's size is below 2^-36 of the
+    largest such product of the query token, and a query's channels below 2^-27 of its largest one lose bits."""
     nb, kvh = check_layer_views(k_cache, v_cache, kv8=True)
     dev, index, plan = k_cache.device, k_cache.get_device(), meta.plan
     q_stride, shape = _rows(q, "q"), q.shape

@@ -34,10 +34,10 @@ constexpr unsigned kExpNan = 255;
 
 // What the chunk positions of token `tok` are XORed with: distinct over the tokens 0, 1, 4, 5, 8, 9,
 // 12, 13 that one ldmatrix reads, and the same for tok and tok + 2 there.
-__device__ __forceinline__ int code_swizzle8(int tok) { return (tok & 1) | ((tok >> 1) & 6); }
+__host__ __device__ constexpr int code_swizzle8(int tok) { return (tok & 1) | ((tok >> 1) & 6); }
 
 // Byte offset of 16-byte chunk `chunk` of token `tok` inside one K or V code block.
-__device__ __forceinline__ int code_off8(int tok, int chunk) {
+__host__ __device__ constexpr int code_off8(int tok, int chunk) {
   return tok * kRow8Bytes + ((chunk ^ code_swizzle8(tok)) << 4);
 }
 

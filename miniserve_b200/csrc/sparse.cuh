@@ -959,15 +959,42 @@ __device__ __forceinline__ void store_cluster(uint32_t addr, uint32_t x) {
 //
 // Key of column n of the g-th product of eight keys.
 template <bool kKv8>
-__device__ __forceinline__ int column_key(int n, int g) {
+__host__ __device__ constexpr int column_key(int n, int g) {
   if constexpr (kKv8) return n + 8 * ((g ^ (n >> 1) ^ n) & 1);
   return ((n & 1) ? ((n - 1) ^ 4) + 1 : n) + 8 * g;
 }
 // Key of a lane's i-th score.
 template <bool kKv8>
-__device__ __forceinline__ int page_key(int i, int c) {
+__host__ __device__ constexpr int page_key(int i, int c) {
   return column_key<kKv8>(2 * c + (i & 1), i >> 1);
 }
+// Byte offset in K (or V) of 16-byte piece `piece` of a key: of its 8 (8-bit), or of its 16 in two halves.
+template <bool kKv8>
+__host__ __device__ constexpr int piece_off(int key, int piece) {
+  if constexpr (kKv8) return code_off8(key, piece);
+  return (piece >> 3) * (kPageBytes / 2) + key * 128 + (((piece & 7) ^ (key & 7)) << 4);
+}
+// What the above has to hold: every key is met once, and the loads of eight lanes meet eight different 16 bytes of
+// the 128 that the banks serve at a time.
+template <bool kKv8>
+constexpr bool page_layout_holds() {
+  unsigned columns = 0, scores = 0;
+  for (int i = 0; i < 16; ++i) columns |= 1u << column_key<kKv8>(i & 7, i >> 3), scores |= 1u << page_key<kKv8>(i & 3, i >> 2);
+  bool apart = true;
+  for (int first = 0; first < 32; first += 8)
+    for (int i = 0; i < 4; ++i)
+      for (int g = 0; g < 2; ++g) {
+        unsigned keys = 0, values = 0;
+        for (int lane = first; lane < first + 8; ++lane) {
+          const int r = lane >> 2, c = lane & 3;
+          keys |= 1u << (piece_off<kKv8>(column_key<kKv8>(r, g), kKv8 ? 4 * (i & 1) + c : 4 * i + c) >> 4 & 7);
+          values |= 1u << (piece_off<kKv8>(page_key<kKv8>(i, c), kKv8 ? r : 8 * g + r) >> 4 & 7);
+        }
+        apart = apart && keys == 0xffu && values == 0xffu;
+      }
+  return columns == 0xffffu && scores == 0xffffu && apart;
+}
+static_assert(page_layout_holds<false>() && page_layout_holds<true>(), "layout of the products over a page");
 
 // A warp's ring: `stages` pages in flight.
 template <bool kKv8>
@@ -1059,9 +1086,7 @@ __device__ __forceinline__ void page_scores(const PageQuery<kKv8>& q, const uint
     const int key = column_key<kKv8>(r, g);
 #pragma unroll
     for (int j = 0; j < (kKv8 ? 2 : 4); ++j) {
-      const uint4 x = *reinterpret_cast<const uint4*>(
-          page + (kKv8 ? code_off8(key, 4 * j + c)
-                       : (j >> 1) * (kPageBytes / 2) + key * 128 + (((4 * (j & 1) + c) ^ (key & 7)) << 4)));
+      const uint4 x = *reinterpret_cast<const uint4*>(page + piece_off<kKv8>(key, 4 * j + c));
       const uint32_t w[4] = {x.x, x.y, x.z, x.w};
       if constexpr (kKv8) {
 #pragma unroll
@@ -1174,8 +1199,7 @@ __device__ __forceinline__ void page_update(const uint8_t* page, float (&s)[4], 
     for (int i = 0; i < 4; ++i) {
       const int key = page_key<kKv8>(i, c);
       uint4 x = *reinterpret_cast<const uint4*>(
-          page + (kKv8 ? kCodes8Bytes + code_off8(key, r)
-                       : kPageBytes + h * (kPageBytes / 2) + key * 128 + ((r ^ (key & 7)) << 4)));
+          page + (kKv8 ? kCodes8Bytes : kPageBytes) + piece_off<kKv8>(key, 8 * h + r));
       if (key >= visible) x = make_uint4(0u, 0u, 0u, 0u);
       y[i][0] = x.x, y[i][1] = x.y, y[i][2] = x.z, y[i][3] = x.w;
     }

@@ -4,7 +4,8 @@
 // The lists come as kernel arguments (a launch carries up to 32 KiB of them), since a host that manages
 // pages has them at hand: no copy to the device, nothing that a captured graph would have to keep alive.
 // Memory bounds both: a page is read once and written once (1000 bf16 pages of 8 layers and 8 heads, 1.05 GB: 162 us, 0.99
-// of the copy rate; 2000 8-bit pages cleared, 0.53 GB: 74 us).  One page copied three times in 28 layers takes 3.3 us.
+// of the copy rate; 2000 8-bit pages cleared, 0.53 GB: 75 us).  One page copied three times in 28 layers takes 3.3 us.
+// Either with the ordered launch that follows it, about 1 us of it.
 #pragma once
 
 #include "ms_common.cuh"

@@ -60,7 +60,7 @@ __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
   return *reinterpret_cast<uint32_t*>(&r);
 }
 
-// Launch latency bounds a decode step (61 rows: 2.2 us), memory a prompt (16384 tokens of an 8-bit pool: 6.9 us of
+// Launch latency bounds a decode step (61 rows: 2.3 us), memory a prompt (16384 tokens of an 8-bit pool: 7.0 us of
 // which 21 MB take 3.2).
 //
 // Bounds of the first `rows` tokens of one page, by one warp.  Lane l reads 16-byte pieces: piece l % 8 of
@@ -1243,7 +1243,7 @@ __device__ __forceinline__ bool mbar_wait_nohint(uint64_t* bar, uint32_t parity)
 // turn, each through its own ring, and the first CTA merges.  Memory bounds it where the CTAs fill the GPU: 256
 // rows of 64 bf16 pages 145 us (6.9 TB/s, the copy rate), of 64 8-bit pages 85 (0.78 of it); 48 rows of 128 8-bit
 // pages are two or three CTAs per SM, 43 us (0.73).  Four warps share one row and head: with one or two each 166 and
-// 150 us, 88 and 57.  Few rows are a chain of latencies: 8 rows of 16 pages 5.3 us.
+// 150 us, 88 and 57.  Few rows are a chain of latencies: 8 rows of 16 pages 5.0 us.
 template <bool kKv8>
 __global__ void __launch_bounds__(kPagesWarps * 32, kKv8 ? 4 : 3)
     attend_pages_kernel(const __grid_constant__ PagesArgs a, const __grid_constant__ CUtensorMap map,

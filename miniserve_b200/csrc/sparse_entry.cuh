@@ -163,15 +163,15 @@ int attend_selected(const char* what, bool kv8, const void* q, int64_t q_row_str
   rc = sm_count(&sms);
   if (rc) return rc;
   // A row and head is shared by more CTAs, as a cluster, while they all fit two per SM and a warp has two pages
-  // (measured: 24 of 128 bf16 pages 21 us with one CTA each, 8.0 with eight; 64 of 300 8-bit pages 57 and 27
-  // with four; 128 of 64 bf16 pages 14.5 and 14.8 with two).
+  // (measured: 24 of 128 bf16 pages 21 us with one CTA each, 8.4 with eight; 64 of 300 8-bit pages 57 and 28
+  // with four; 128 of 64 bf16 pages 14.4 and 15.4 with two).
   const int64_t units = static_cast<int64_t>(plan->num_seqs) * max_new * num_kv;
   a.cluster = 1;
   while (a.cluster < ms::kMaxCluster && units * a.cluster * 2 <= 2 * sms &&
          budget >= 2 * 2 * a.cluster * ms::kPagesWarps)
     a.cluster *= 2;
   // 8-bit: rings of four pages leave room for three CTAs per SM, of three for four.  CTAs that three per SM hold
-  // spread better (384 of 128 pages: 41 us, 50 with four per SM); more of them want four (2048 of 64: 86 and 83).
+  // spread better (384 of 128 pages: 43 us, 51 with four per SM); more of them want four (2048 of 64: 92 and 85).
   const int64_t ctas = units * a.cluster;
   a.stages = !kv8 ? 2 : ctas <= 3 * sms ? 4 : 3;
   const size_t smem = ms::kPagesWarps * a.stages * (kv8 ? ms::kStageBytes<true> : ms::kStageBytes<false>) +
@@ -285,9 +285,9 @@ extern "C" int ms_select_pages(const void* q, int64_t q_row_stride, int32_t num_
   };
   cudaError_t e = cudaSuccess;
   if (max_pages > budget && max_pages <= 256 && grid <= 256) {
-    // Few rows of few pages in one launch (measured on the device and on the host: 64 rows and heads of 128
-    // pages 6.7 and 11.4 us instead of 9.4 and 13.8, 256 of 256 pages 14.9 and 15.8 on the device; 1024 of 128
-    // pages 37 and 23, 128 of 512 pages 22 and 16).
+    // Few rows of few pages in one launch.  Measured with one launch and with two, on the device: 64 rows and heads of
+    // 128 pages 5.7 and 9.4 us (on the host 10.7 and 13.0), 256 of 256 pages 11.8 and 15.2; beyond the border 512 of
+    // 256 pages 23.0 and 21.8, 1024 of 128 29.4 and 22.9, 128 of 512 15.0 and 15.2.
     e = select(Threads<256>(), std::true_type());
     if (e != cudaSuccess) return cuda_fail("select_pages launch", e);
     return MS_OK;

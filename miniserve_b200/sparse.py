@@ -127,7 +127,9 @@ def select_pages(q: Tensor, bounds: Tensor, meta: AttentionMetadata, budget: int
     give them; equal scores go to the lower page, and a score that is not finite counts as infinite, as does
     that of any page with a bound that is not finite.
     Rows of longer chunks and of trees are left untouched (undefined).  Calls that use one metadata share its
-    scratch, so they are ordered on the GPU (one stream, or events)."""
+    scratch, so they are ordered on the GPU (one stream, or events).  The scratch is the product of the step's
+    sequences, the most new tokens of a short row (up to 8), the KV heads and the most pages that a short row
+    sees, 4.25 bytes each: one very long row makes it large for every row of its step."""
     nb, kvh = _check_bounds(bounds)
     q_stride, (t, heads, _) = _rows(q, "q"), q.shape
     if heads != 2 * kvh:

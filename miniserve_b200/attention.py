@@ -654,7 +654,8 @@ def attend(q: Tensor, k_cache: Tensor, v_cache: Tensor, meta: AttentionMetadata,
     """Attention of every planned query row through the pool (backends.py:161-197); draft trees
     and an 8-bit pool included.
 
-    Rows not covered by ``meta`` are left untouched (undefined, like ``torch.empty_like``).
+    Rows not covered by ``meta`` are left untouched (undefined, like ``torch.empty_like``).  Scores are held
+    in fp32: rows that see any beyond 2^29 in magnitude may come out wrong or NaN.
     """
     nb, kvh = check_layer_views(k_cache, v_cache, kv8=True)
     dev = k_cache.device

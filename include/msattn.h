@@ -316,11 +316,12 @@ MS_API int ms_key_bounds_kv8(const void* pool, int32_t num_blocks, int32_t num_k
  * page), and of those between the ones with the highest scores,
  *   score(page) = max over the KV head's two query heads of sum_d max(q_d lo_d, q_d hi_d),
  * equal scores by the lower page, one that is not finite as infinity, and so any score of a page with a bound
- * that is not finite.  Scores are compared as exactly as 64 bits give them.  max_new (1 .. 8) and max_pages (at most 49152) bound the new tokens and the pages of those
- * sequences; budget is at most 4096.  Bounds of the pages between are read: they have to be up to date.  A block
- * outside the pool is scored by the bounds of block 0 and sets MS_DEV_BAD_BLOCK.
- * workspace: ms_select_workspace_bytes of scratch (num_seqs * max_new * num_kv_heads * max_pages * 4.25, max_pages in
- * steps of 64), 16-byte aligned; nothing is kept in it between calls. */
+ * that is not finite.  Scores are compared as exactly as 64 bits give them.  max_new (1 .. 8) and max_pages (at
+ * most 49152) bound the new tokens and the pages of those sequences; budget is at most 4096.  Bounds of the pages
+ * between are read: they have to be up to date.  A block outside the pool is scored by the bounds of block 0 and
+ * sets MS_DEV_BAD_BLOCK.
+ * workspace: ms_select_workspace_bytes of scratch (num_seqs * max_new * num_kv_heads * max_pages * 4.25, max_pages
+ * in steps of 64), 16-byte aligned; nothing is kept in it between calls. */
 MS_API int64_t ms_select_workspace_bytes(int32_t num_seqs, int32_t max_new, int32_t max_pages,
                                          int32_t num_kv_heads);
 MS_API int ms_select_pages(const void* q, int64_t q_row_stride, int32_t num_heads, int32_t num_kv_heads,

@@ -979,7 +979,10 @@ __host__ __device__ constexpr int piece_off(int key, int piece) {
 template <bool kKv8>
 constexpr bool page_layout_holds() {
   unsigned columns = 0, scores = 0;
-  for (int i = 0; i < 16; ++i) columns |= 1u << column_key<kKv8>(i & 7, i >> 3), scores |= 1u << page_key<kKv8>(i & 3, i >> 2);
+  for (int i = 0; i < 16; ++i) {
+    columns |= 1u << column_key<kKv8>(i & 7, i >> 3);
+    scores |= 1u << page_key<kKv8>(i & 3, i >> 2);
+  }
   bool apart = true;
   for (int first = 0; first < 32; first += 8)
     for (int i = 0; i < 4; ++i)
